@@ -148,8 +148,8 @@ def _normal(gen, *shape):
 def _quantised(x, store):
     """Codes and scales of the rows of x."""
     most = x.abs().amax(-1, keepdim=True)
-    big = LARGEST[store]
-    code = torch.where(most > 0, x * (big / most), 0.0).clamp(-big, big)
+    big = torch.full_like(most, LARGEST[store])  # a tensor: torch divides by a number by way of its reciprocal
+    code = torch.where(most > 0, x * (big / most), 0.0).clamp(-LARGEST[store], LARGEST[store])
     code = code.round().to(torch.int8) if store == "i8" else code.to(torch.float8_e4m3fn)
     return code, (most / big).squeeze(-1)
 

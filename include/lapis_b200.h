@@ -278,6 +278,78 @@ int lapis_b200_mht_f64(lapis_b200_csr_t h, const double *d_mask, const double *d
 /* d_out[i] = sqrt(d_mom2[i] - d_mom1[i]^2)  (examples/hitting_times.py:196-218). */
 int lapis_b200_normalize_mom2_f64(int64_t n, const double *d_mom1, const double *d_mom2, double *d_out, void *stream);
 
+/* ---- attention: norms with rotation, a paged cache, attention of one new token ---------------------------- */
+
+/* Types of the rows and of the cache. */
+enum { LAPIS_F32 = 0, LAPIS_F16 = 1, LAPIS_BF16 = 2, LAPIS_I8 = 3, LAPIS_E4M3 = 4 };
+
+/* Heads of tokens, [tokens, heads, dim], strides in elements; the values of a head lie next to one another (a view of the
+ * queries in the output of one projection for queries, keys and values will do). */
+typedef struct { const void *d; int64_t heads, token_stride, head_stride; } lapis_b200_heads;
+
+/* Norms of queries and keys and the rotation: weights [dim], float32 or of the rows' type; tables [places, rot / 2] of the
+ * cosines and sines of the angles.  The first rot (even, at most dim) values of a head are turned, in pairs (i, i + rot/2),
+ * or (2i, 2i + 1) with interleaved != 0.  A token whose place is outside the tables is padding: zeros come out of it
+ * (outputs and gradients) and nothing of it is written to a cache. */
+typedef struct {
+  const void *d_q_weight, *d_k_weight;
+  int weight_type;
+  const float *d_cos, *d_sin;
+  int64_t places, rot;
+  int interleaved;
+  double eps;
+} lapis_b200_norm_rope;
+
+/* Keys and values in pages, [pages, heads, page_size, dim], of the rows' type, int8 or e4m3.  A quantised cache has a scale
+ * for each head of each token, [pages, heads, page_size]: amax / 127 (448 for e4m3), and holds value * (127 / amax) to the
+ * nearest code, ties to even; a row that holds a NaN or an infinity reads as NaN.  At most 256 values a head and 2^32 - 1
+ * rows (pages * heads * page_size). */
+typedef struct {
+  int type;
+  int64_t pages, heads, page_size, dim;
+  void *d_k, *d_v;
+  float *d_k_scale, *d_v_scale;
+} lapis_b200_kv_cache;
+
+/* Which pages hold a request's tokens, as the rows of a CSR pattern: place p of request r is in page
+ * crd[pos[r] + p / page_size], slot p % page_size.  pos has rows + 1 entries, crd `entries`.  A place that the lists do not
+ * cover, a request outside [0, rows) and a page outside the cache are never accessed: nothing is written there, and zeros
+ * are read. */
+typedef struct {
+  int idx_bytes;
+  int64_t rows, entries;
+  const void *d_pos, *d_crd;
+} lapis_b200_page_lists;
+
+/* q, k -> w x / sqrt(mean x^2 + eps), rotated; q_out, k_out [tokens, heads, dim] contiguous.  d_place: a place for each token,
+ * idx_bytes wide. */
+int lapis_b200_qk_norm_rope(int type, int64_t tokens, int64_t dim, const lapis_b200_heads *q, const lapis_b200_heads *k,
+                            const lapis_b200_norm_rope *how, int idx_bytes, const void *d_place, void *d_q_out, void *d_k_out,
+                            void *stream);
+/* Its gradients: dq, dk of the outputs; q, k and `how` as they went in; contiguous gradients of q and k, of their type, and of
+ * the weights in 32 bits (sums over all tokens and heads in a fixed order). */
+int lapis_b200_qk_norm_rope_backward(int type, int64_t tokens, int64_t dim, const lapis_b200_heads *dq, const lapis_b200_heads *dk,
+                                     const lapis_b200_heads *q, const lapis_b200_heads *k, const lapis_b200_norm_rope *how,
+                                     int idx_bytes, const void *d_place, void *d_q_grad, void *d_k_grad, float *d_q_weight_grad,
+                                     float *d_k_weight_grad, void *stream);
+/* Writes k and v of new tokens into the cache, token t at place d_place[t] of request d_row[t].  With `how` the keys are
+ * normalised and rotated on their way (and quantised from 32 bits), and q comes out in d_q_out, all in one launch; without,
+ * q and d_q_out are not looked at.  Two tokens for one place: either may stay. */
+int lapis_b200_kv_append(int type, int64_t tokens, const lapis_b200_heads *q, const lapis_b200_heads *k, const lapis_b200_heads *v,
+                         const lapis_b200_norm_rope *how, const lapis_b200_kv_cache *cache, const lapis_b200_page_lists *lists,
+                         const void *d_row, const void *d_place, void *d_q_out, void *stream);
+/* Reads tokens back: code * scale in 32 bits, rounded to `type`; d_k, d_v [tokens, heads, dim] contiguous. */
+int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_b200_page_lists *lists, int64_t tokens, const void *d_row,
+                       const void *d_place, int type, void *d_k, void *d_v, void *stream);
+/* One new token of each request over the first d_length[r] places of its list (of these the last `window`, where that is not
+ * 0), which hold its own key and value too: softmax(scale q.k) v for each query head, query heads h with h / (q heads / cache
+ * heads) sharing a key head.  q [requests, heads, dim]; out the same, contiguous; d_lse (may be null) [requests, heads] gets
+ * the natural logarithm of the sum of the exponentials.  A request of length 0 gets zeros and -infinity.  A length beyond the
+ * listed pages counts as their end.  At most 65,535 requests. */
+int lapis_b200_paged_attention(int type, int64_t requests, const lapis_b200_heads *q, const lapis_b200_kv_cache *cache,
+                               const lapis_b200_page_lists *lists, const void *d_length, double scale, int64_t window, void *d_out,
+                               float *d_lse, void *stream);
+
 /* Step-level PCG entry points: the three passes of one iteration, for callers that
  * put an exchange between them (row-block partitioned solves put a halo copy of p in
  * front of pass A and an allreduce of the scalar block behind passes A and B).

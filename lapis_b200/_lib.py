@@ -85,6 +85,12 @@ _PROTOS = {
                                               ctypes.POINTER(c_vp)]),
     "lapis_b200_mm_free": (None, [c_vp]),
     "lapis_b200_partition_rows": (c_int, [c_int, c_i64, c_vp, c_int, c_vp]),
+    "lapis_b200_qk_norm_rope": (c_int, [c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_qk_norm_rope_backward": (c_int, [c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_vp,
+                                                 c_vp, c_vp]),
+    "lapis_b200_kv_append": (c_int, [c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_kv_read": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
+    "lapis_b200_paged_attention": (c_int, [c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_dbl, c_i64, c_vp, c_vp, c_vp]),
     "lapis_b200_validate_csr_host": (c_int, [c_int, c_i64, c_i64, c_i64, c_vp, c_vp]),
 }
 
@@ -94,6 +100,12 @@ class PcgExchange(ctypes.Structure):
     """``lapis_b200_pcg_exchange`` of include/lapis_b200.h."""
     _fields_ = [("me", c_int), ("world", c_int), ("d_mbox", c_vp), ("d_peer_mbox", c_vp), ("d_halo_srcs", c_vp),
                 ("nsrc", c_int), ("d_z_pieces", c_vp), ("nzpieces", c_int), ("d_halo_ranges", c_vp), ("nranges", c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """``lapis_b200_kv_cache`` of include/lapis_b200.h."""
+    _fields_ = [("type", c_int), ("pages", c_i64), ("heads", c_i64), ("page_size", c_i64), ("dim", c_i64), ("d_k", c_vp), ("d_v", c_vp),
+                ("d_k_scale", c_vp), ("d_v_scale", c_vp)]
 
 
 _LIB = None

@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -128,12 +129,193 @@ PyObject *py_bgemm(PyObject *const *a) {
   return call(lapis_b200_bgemm_f32, batch, M, N, K, addr_of<float>(A), addr_of<float>(B), addr_of<float>(C), stream());
 }
 
+// ---- attention (lapis_b200/attention.py) ----
+
+// LAPIS_F32 ... of a tensor's elements, or -1.
+int type_of(const at::Tensor *t) {
+  switch (t->scalar_type()) {
+    case at::kFloat: return LAPIS_F32;
+    case at::kHalf: return LAPIS_F16;
+    case at::kBFloat16: return LAPIS_BF16;
+    default: return -1;
+  }
+}
+bool on_device(const at::Tensor *t) { return t->is_cuda() && t->device().index() == c10::cuda::current_device(); }
+// Heads of tokens, [tokens, heads, dim], whose values lie next to one another.
+bool heads_of(PyObject *o, int type, int64_t tokens, int64_t dim, lapis_b200_heads *h) {
+  const at::Tensor *t = tensor(o);
+  if (t == nullptr || t->dim() != 3 || !on_device(t) || type_of(t) != type || t->size(0) != tokens || t->size(2) != dim) return false;
+  if (dim > 1 && t->stride(2) != 1 && t->numel() > 0) return false;
+  *h = {addr(t), t->size(1), t->stride(0), t->stride(1)};
+  return true;
+}
+// A contiguous result [tokens, heads, dim].
+bool result_of(PyObject *o, int type, int64_t tokens, int64_t heads, int64_t dim, void **p) {
+  const at::Tensor *t = tensor(o);
+  if (t == nullptr || t->dim() != 3 || !on_device(t) || type_of(t) != type || !t->is_contiguous()) return false;
+  if (t->size(0) != tokens || t->size(1) != heads || t->size(2) != dim) return false;
+  *p = addr(t);
+  return true;
+}
+bool indices_of(PyObject *o, int64_t count, int *idx_bytes, const void **p) {
+  const at::Tensor *t = tensor(o);
+  if (!is_index(t) || !on_device(t) || t->dim() != 1 || (count >= 0 && t->numel() != count)) return false;
+  if (*idx_bytes != 0 && *idx_bytes != (int)t->element_size()) return false;
+  *idx_bytes = (int)t->element_size();
+  *p = addr(t);
+  return true;
+}
+bool lists_of(PyObject *pos, PyObject *crd, lapis_b200_page_lists *l) {
+  *l = {};
+  if (!indices_of(pos, -1, &l->idx_bytes, &l->d_pos) || !indices_of(crd, -1, &l->idx_bytes, &l->d_crd)) return false;
+  l->rows = tensor(pos)->numel() - 1;
+  l->entries = tensor(crd)->numel();
+  return l->rows >= 0;
+}
+// a: q_weight, k_weight, cos, sin, eps, interleaved
+bool norm_rope_of(PyObject *const *a, int type, int64_t dim, lapis_b200_norm_rope *how) {
+  const at::Tensor *w[2] = {tensor(a[0]), tensor(a[1])}, *cos = tensor(a[2]), *sin = tensor(a[3]);
+  for (const at::Tensor *t : w)
+    if (t == nullptr || !on_device(t) || !t->is_contiguous() || t->dim() != 1 || t->numel() != dim || t->scalar_type() != w[0]->scalar_type())
+      return false;
+  for (const at::Tensor *t : {cos, sin})
+    if (!is(t, at::kFloat) || !on_device(t) || t->dim() != 2 || t->size(0) != cos->size(0) || t->size(1) != cos->size(1)) return false;
+  const int weight_type = type_of(w[0]);
+  if (weight_type != LAPIS_F32 && weight_type != type) return false;
+  if (2 * cos->size(1) > dim) return false;
+  const double eps = PyFloat_AsDouble(a[4]);
+  const int interleaved = PyObject_IsTrue(a[5]);
+  *how = {addr(w[0]), addr(w[1]), weight_type, addr_of<float>(cos), addr_of<float>(sin), cos->size(0), 2 * cos->size(1), interleaved, eps};
+  return true;
+}
+const lapis_b200_kv_cache *cache_of(PyObject *o) { return static_cast<const lapis_b200_kv_cache *>(PyLong_AsVoidPtr(o)); }
+
+// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_out, k_out)
+PyObject *py_qk_norm_rope(PyObject *const *a) {
+  const at::Tensor *q = tensor(a[0]);
+  if (q == nullptr || q->dim() != 3) return status(-1);
+  const int64_t tokens = q->size(0), dim = q->size(2);
+  const int type = type_of(q);
+  lapis_b200_heads hq, hk;
+  lapis_b200_norm_rope how;
+  int idx_bytes = 0;
+  const void *place;
+  void *q_out, *k_out;
+  if (type < 0 || !heads_of(a[0], type, tokens, dim, &hq) || !heads_of(a[1], type, tokens, dim, &hk) || !norm_rope_of(a + 2, type, dim, &how) ||
+      !indices_of(a[8], tokens, &idx_bytes, &place) || !result_of(a[9], type, tokens, hq.heads, dim, &q_out) ||
+      !result_of(a[10], type, tokens, hk.heads, dim, &k_out))
+    return status(-1);
+  if (PyErr_Occurred()) return nullptr;
+  return call(lapis_b200_qk_norm_rope, type, tokens, dim, &hq, &hk, &how, idx_bytes, place, q_out, k_out, stream());
+}
+
+// qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_grad, k_grad, weight_grads [2, dim])
+PyObject *py_qk_norm_rope_backward(PyObject *const *a) {
+  const at::Tensor *q = tensor(a[2]), *dw = tensor(a[13]);
+  if (q == nullptr || q->dim() != 3) return status(-1);
+  const int64_t tokens = q->size(0), dim = q->size(2);
+  const int type = type_of(q);
+  lapis_b200_heads hdq, hdk, hq, hk;
+  lapis_b200_norm_rope how;
+  int idx_bytes = 0;
+  const void *place;
+  void *q_grad, *k_grad;
+  if (type < 0 || !heads_of(a[0], type, tokens, dim, &hdq) || !heads_of(a[1], type, tokens, dim, &hdk) ||
+      !heads_of(a[2], type, tokens, dim, &hq) || !heads_of(a[3], type, tokens, dim, &hk) || !norm_rope_of(a + 4, type, dim, &how) ||
+      !indices_of(a[10], tokens, &idx_bytes, &place) || !result_of(a[11], type, tokens, hq.heads, dim, &q_grad) ||
+      !result_of(a[12], type, tokens, hk.heads, dim, &k_grad) || !is(dw, at::kFloat) || !on_device(dw) || dw->numel() != 2 * dim)
+    return status(-1);
+  if (PyErr_Occurred()) return nullptr;
+  float *const dqw = addr_of<float>(dw);
+  return call(lapis_b200_qk_norm_rope_backward, type, tokens, dim, &hdq, &hdk, &hq, &hk, &how, idx_bytes, place, q_grad, k_grad, dqw,
+              dqw == nullptr ? nullptr : dqw + dim, stream());
+}
+
+// kv_append(cache, k, v, pos, crd, row, place)
+PyObject *py_kv_append(PyObject *const *a) {
+  const lapis_b200_kv_cache *cache = cache_of(a[0]);
+  const at::Tensor *k = tensor(a[1]);
+  if (cache == nullptr || k == nullptr || k->dim() != 3) return status(-1);
+  const int64_t tokens = k->size(0);
+  const int type = type_of(k);
+  lapis_b200_heads hk, hv;
+  lapis_b200_page_lists lists;
+  const void *row, *place;
+  if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hk) || !heads_of(a[2], type, tokens, cache->dim, &hv) || !lists_of(a[3], a[4], &lists) ||
+      !indices_of(a[5], tokens, &lists.idx_bytes, &row) || !indices_of(a[6], tokens, &lists.idx_bytes, &place))
+    return status(-1);
+  return call(lapis_b200_kv_append, type, tokens, nullptr, &hk, &hv, nullptr, cache, &lists, row, place, nullptr, stream());
+}
+
+// kv_append_norm_rope(cache, q, k, v, q_weight, k_weight, cos, sin, eps, interleaved, pos, crd, row, place, q_out)
+PyObject *py_kv_append_norm_rope(PyObject *const *a) {
+  const lapis_b200_kv_cache *cache = cache_of(a[0]);
+  const at::Tensor *k = tensor(a[2]);
+  if (cache == nullptr || k == nullptr || k->dim() != 3) return status(-1);
+  const int64_t tokens = k->size(0);
+  const int type = type_of(k);
+  lapis_b200_heads hq, hk, hv;
+  lapis_b200_norm_rope how;
+  lapis_b200_page_lists lists;
+  const void *row, *place;
+  void *q_out;
+  if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hq) || !heads_of(a[2], type, tokens, cache->dim, &hk) ||
+      !heads_of(a[3], type, tokens, cache->dim, &hv) || !norm_rope_of(a + 4, type, cache->dim, &how) || !lists_of(a[10], a[11], &lists) ||
+      !indices_of(a[12], tokens, &lists.idx_bytes, &row) || !indices_of(a[13], tokens, &lists.idx_bytes, &place) ||
+      !result_of(a[14], type, tokens, hq.heads, cache->dim, &q_out))
+    return status(-1);
+  if (PyErr_Occurred()) return nullptr;
+  return call(lapis_b200_kv_append, type, tokens, &hq, &hk, &hv, &how, cache, &lists, row, place, q_out, stream());
+}
+
+// kv_read(cache, pos, crd, row, place, k_out, v_out)
+PyObject *py_kv_read(PyObject *const *a) {
+  const lapis_b200_kv_cache *cache = cache_of(a[0]);
+  const at::Tensor *k = tensor(a[5]), *row_of = tensor(a[3]);
+  if (cache == nullptr || k == nullptr || row_of == nullptr) return status(-1);
+  const int64_t tokens = row_of->numel();
+  const int type = type_of(k);
+  lapis_b200_page_lists lists;
+  const void *row, *place;
+  void *k_out, *v_out;
+  if (type < 0 || !lists_of(a[1], a[2], &lists) || !indices_of(a[3], tokens, &lists.idx_bytes, &row) ||
+      !indices_of(a[4], tokens, &lists.idx_bytes, &place) || !result_of(a[5], type, tokens, cache->heads, cache->dim, &k_out) ||
+      !result_of(a[6], type, tokens, cache->heads, cache->dim, &v_out))
+    return status(-1);
+  return call(lapis_b200_kv_read, cache, &lists, tokens, row, place, type, k_out, v_out, stream());
+}
+
+// paged_attention(cache, q, pos, crd, length, scale, window, out, lse or None)
+PyObject *py_paged_attention(PyObject *const *a) {
+  const lapis_b200_kv_cache *cache = cache_of(a[0]);
+  const at::Tensor *q = tensor(a[1]), *lse = tensor(a[8]);
+  if (cache == nullptr || q == nullptr || q->dim() != 3) return status(-1);
+  const int64_t requests = q->size(0);
+  const int type = type_of(q);
+  lapis_b200_heads hq;
+  lapis_b200_page_lists lists;
+  const void *length;
+  void *out;
+  const double scale = PyFloat_AsDouble(a[5]);
+  const long long window = PyLong_AsLongLong(a[6]);
+  if (type < 0 || !heads_of(a[1], type, requests, cache->dim, &hq) || !lists_of(a[2], a[3], &lists) ||
+      !indices_of(a[4], requests, &lists.idx_bytes, &length) || !result_of(a[7], type, requests, hq.heads, cache->dim, &out))
+    return status(-1);
+  if (a[8] != Py_None && (!is(lse, at::kFloat) || !on_device(lse) || lse->numel() != requests * hq.heads)) return status(-1);
+  if (PyErr_Occurred()) return nullptr;
+  return call(lapis_b200_paged_attention, type, requests, &hq, cache, &lists, length, scale, window, out,
+              lse == nullptr ? nullptr : addr_of<float>(lse), stream());
+}
+
 template <PyObject *(*CALL)(PyObject *const *), Py_ssize_t ARGS>
 PyMethodDef method(const char *name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<CALL, ARGS>)), METH_FASTCALL, nullptr};
 }
 PyMethodDef methods[] = {method<py_spmv, 6>("spmv"),   method<py_spmm, 6>("spmm"),   method<py_spmm_dcsr, 7>("spmm_dcsr"),
-                         method<py_bspmm, 7>("bspmm"), method<py_bgemm, 3>("bgemm"), {nullptr, nullptr, 0, nullptr}};
+                         method<py_bspmm, 7>("bspmm"), method<py_bgemm, 3>("bgemm"),
+                         method<py_qk_norm_rope, 11>("qk_norm_rope"), method<py_qk_norm_rope_backward, 14>("qk_norm_rope_backward"),
+                         method<py_kv_append, 7>("kv_append"), method<py_kv_append_norm_rope, 15>("kv_append_norm_rope"),
+                         method<py_kv_read, 7>("kv_read"), method<py_paged_attention, 9>("paged_attention"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -15,6 +15,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv.h"
 
@@ -37,7 +38,11 @@ struct AttendArgs {
   float *lse;
   float *partial;  // [blocks][2][HEADS][dim + 2]
   int blocks, min_tiles;
+  int page_shift;  // log2 of the slots of a page, or -1
 };
+
+// A request's tokens beyond these are not looked at: places are 32-bit numbers in the kernels.
+constexpr int MOST_TOKENS = 0x7fff0000;
 
 // Keys [lo, hi) of request b that are attended.
 struct Span {
@@ -47,7 +52,7 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int64_t b) {
   const int64_t first = load_index(a.lists.d_pos, b, a.lists.idx_bytes), last = load_index(a.lists.d_pos, b + 1, a.lists.idx_bytes);
   const int64_t room = (last - first) * a.cache.page_size, n = load_index(a.length, b, a.lists.idx_bytes);
   Span s;
-  s.hi = max((int64_t)0, min(n, room));
+  s.hi = max((int64_t)0, min(min(n, room), (int64_t)MOST_TOKENS));
   s.lo = a.window > 0 ? max((int64_t)0, s.hi - a.window) : 0;
   return s;
 }
@@ -61,6 +66,7 @@ struct Share {
   int64_t from, to;    // this block's tiles
   int64_t request, in_request;  // the request of the first one, and its number among the request's
 };
+__device__ __forceinline__ int64_t shares_of(const AttendArgs &a, int64_t all) { return max((int64_t)1, min((int64_t)a.blocks, all / a.min_tiles)); }
 __device__ __forceinline__ int64_t share_start(int64_t i, int64_t all, int64_t shares) { return i * all / shares; }
 
 // Sums the tiles of all requests (a thread takes a run of them), and finds the request of tile `at(all, shares)`.
@@ -85,7 +91,7 @@ __device__ __forceinline__ Share find_share(const AttendArgs &a, int tile, At at
     if (w < warp) upto += warp_sums[w];
     s.all += warp_sums[w];
   }
-  s.shares = max((int64_t)1, min((int64_t)a.blocks, s.all / a.min_tiles));
+  s.shares = shares_of(a, s.all);
   s.from = at(s);
   s.to = s.from;
   if (s.from >= upto - sum && s.from < upto) {
@@ -105,6 +111,43 @@ __device__ __forceinline__ Share find_share(const AttendArgs &a, int tile, At at
   s.in_request = found[1];
   __syncthreads();
   return s;
+}
+
+// Which shares hold the tiles of a unit, and where the first of them left its part (0: its first piece, 1: its last).
+struct Cut {
+  int64_t first, last;
+  int first_slot;
+};
+__device__ __forceinline__ Cut cut_of(const AttendArgs &a, int64_t request, int unit, int tile) {
+  __shared__ int64_t sums[2][ATT_THREADS / 32];
+  const int units = (int)a.cache.heads * a.head_blocks;
+  int64_t front = 0, all = 0;
+  for (int b = threadIdx.x; b < a.requests; b += ATT_THREADS) {
+    const int64_t n = tiles_of(span_of(a, b), tile) * units;
+    all += n;
+    if (b < request) front += n;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) {
+    all += __shfl_xor_sync(0xffffffffu, all, d);
+    front += __shfl_xor_sync(0xffffffffu, front, d);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sums[0][threadIdx.x / 32] = front;
+    sums[1][threadIdx.x / 32] = all;
+  }
+  __syncthreads();
+  front = all = 0;
+  for (int w = 0; w < ATT_THREADS / 32; ++w) {
+    front += sums[0][w];
+    all += sums[1][w];
+  }
+  const int64_t tiles = tiles_of(span_of(a, request), tile), shares = shares_of(a, all), from = front + unit * tiles, to = from + tiles;
+  Cut c;  // the share of tile t is the largest i with i * all / shares < t + 1
+  c.first = ((from + 1) * shares + all - 1) / all - 1;
+  c.last = (to * shares + all - 1) / all - 1;
+  c.first_slot = share_start(c.first, all, shares) == from ? 0 : 1;
+  return c;
 }
 
 // ---- any type, width, stride and alignment --------------------------------------
@@ -198,7 +241,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
       if (lane != 0) continue;
       total[h] = sum;
       if (whole && a.lse != nullptr)
-        a.lse[request * a.q_heads + kv_head * a.group + head0 + h] = sum > 0.0f || sum != sum ? m[u] * LN2 + logf(sum) : -INFINITY;
+        a.lse[request * a.q_heads + kv_head * a.group + head0 + h] = sum == 0.0f ? -INFINITY : m[u] * LN2 + logf(sum);
       if (!whole) {
         slot[h * (dim + 2)] = m[u];
         slot[h * (dim + 2) + 1] = sum;
@@ -230,50 +273,18 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
 
 // Adds up what the blocks left of the units that were cut: block (unit, request), a thread a dimension or two of each head.
 template <typename T>
-__global__ void __launch_bounds__(ATT_THREADS) attend_join_kernel(const __grid_constant__ AttendArgs a, int tile_keys, int heads_of_unit) {
+__global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_constant__ AttendArgs a) {
   const int64_t request = blockIdx.y;
   const int unit = blockIdx.x, dim = a.dim;
-  int64_t before = 0;  // tiles of the requests in front
-  const Span span = span_of(a, request);
-  const int64_t tiles = tiles_of(span, tile_keys);
-  const int units = (int)a.cache.heads * a.head_blocks;
-  __shared__ int64_t sums[2][ATT_THREADS / 32];
-  int64_t front = 0, all = 0;
-  for (int b = threadIdx.x; b < a.requests; b += ATT_THREADS) {
-    const int64_t n = tiles_of(span_of(a, b), tile_keys) * units;
-    all += n;
-    if (b < request) front += n;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    all += __shfl_xor_sync(0xffffffffu, all, d);
-    front += __shfl_xor_sync(0xffffffffu, front, d);
-  }
-  if (threadIdx.x % 32 == 0) {
-    sums[0][threadIdx.x / 32] = front;
-    sums[1][threadIdx.x / 32] = all;
-  }
-  __syncthreads();
-  all = 0;
-  for (int w = 0; w < ATT_THREADS / 32; ++w) {
-    before += sums[0][w];
-    all += sums[1][w];
-  }
-  const int64_t shares = max((int64_t)1, min((int64_t)a.blocks, all / a.min_tiles));
-  const int64_t from = before + unit * tiles, to = from + tiles;
-  // the last share that begins at or in front of a tile t: the largest i with i * all / shares < t + 1
-  const int64_t first = ((from + 1) * shares + all - 1) / all - 1, last = (to * shares + all - 1) / all - 1;
-  if (first == last) return;
-  const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * heads_of_unit, heads = min(heads_of_unit, a.group - head0);
+  const Cut cut = cut_of(a, request, unit, ANY_TILE);
+  if (cut.first == cut.last) return;
+  const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
   for (int h = 0; h < heads; ++h) {
-    auto slot = [&](int64_t i) {
-      const int which = i > first || share_start(first, all, shares) == from ? 0 : 1;
-      return a.partial + ((i * 2 + which) * heads_of_unit + h) * (dim + 2);
-    };
+    auto slot = [&](int64_t i) { return a.partial + ((i * 2 + (i > cut.first ? 0 : cut.first_slot)) * ANY_HEADS + h) * (dim + 2); };
     float most = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int64_t i = first; i <= last; ++i) most = fmaxf(most, slot(i)[0]);
+    for (int64_t i = cut.first; i <= cut.last; ++i) most = fmaxf(most, slot(i)[0]);
     const float base = most == -INFINITY ? 0.0f : most;
-    for (int64_t i = first; i <= last; ++i) {
+    for (int64_t i = cut.first; i <= cut.last; ++i) {
       const float *p = slot(i);
       const float f = exp2f(p[0] - base);
       sum = fmaf(p[1], f, sum);
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_join_kernel(const __grid_c
       const int d = threadIdx.x + e * ATT_THREADS;
       if (d < dim) static_cast<T *>(a.out)[head * dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
     }
-    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[head] = sum > 0.0f || sum != sum ? most * LN2 + logf(sum) : -INFINITY;
+    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : most * LN2 + logf(sum);
   }
 }
 
@@ -308,9 +319,631 @@ static int launch_any(AttendArgs a, int dev, cudaStream_t st) {
   a.partial = static_cast<float *>(partial.p);
   attend_any_kernel<T><<<a.blocks, ATT_THREADS, any_smem(a.dim), st>>>(a);
   LAPIS_CUDA_TRY(cudaGetLastError());
-  attend_join_kernel<T><<<dim3((unsigned)(a.cache.heads * a.head_blocks), (unsigned)a.requests), ATT_THREADS, 0, st>>>(a, ANY_TILE, ANY_HEADS);
+  join_any_kernel<T><<<dim3((unsigned)(a.cache.heads * a.head_blocks), (unsigned)a.requests), ATT_THREADS, 0, st>>>(a);
   LAPIS_CUDA_TRY(cudaGetLastError());
   return LAPIS_OK;
+}
+
+// ---- 16-bit queries: products on the tensor cores ----------------------------------
+//
+// Bound by the cache coming from memory, so the products only have to keep out of its way: mma.sync of 16 keys by 8 heads by
+// 16 values, whose smallest shape fits the few query heads of a key head (tcgen05 has 64 or 128 rows, of which one to sixteen
+// would be heads or, turned round, needs the weights to go through shared memory once more).  S^T = K Q^T has the keys in rows
+// and the heads in columns, O^T = V^T P^T the values in rows: keys and values are the A operands, which shared memory gives
+// by ldmatrix without a copy, and P^T is S^T's accumulator after a movmatrix.
+// A warp is a pipeline of its own: it copies the KEYS keys that are its part of a tile by cp.async, STAGES deep, keeps its own
+// m, l and O, and meets the other three only where a unit ends.
+// Weights go into the product with the values as a 16-bit number, and where that would show in the result (all but bf16
+// results from a quantised cache, whose own 8 bits are 2^-8 and the weights' 11 here) as two, high and low part, whose sum has
+// at least 16 bits.  Quantised caches: codes are exact in fp16, so are queries after a power of two is taken out of each; a
+// key's scale is multiplied to its score in 32 bits, a value's scale to its weight, relative to the largest power of two so
+// far.  Weights in fp16 are times 2^14, so that they are subnormal only below 2^-28.
+
+constexpr int MMA_WARPS = ATT_THREADS / 32;
+
+template <typename T_, int STORE_, int DP_, int NT_>
+struct MmaConfig {
+  using T = T_;                                             // type of q and of the result
+  static constexpr int STORE = STORE_;                      // LAPIS_I8, LAPIS_E4M3, or anything else: T
+  static constexpr bool CODES = STORE == LAPIS_I8 || STORE == LAPIS_E4M3;
+  static constexpr bool HALF = CODES || std::is_same<T, __half>::value;  // fp16 products, or bf16
+  static constexpr bool TWO_PARTS = !(CODES && std::is_same<T, __nv_bfloat16>::value);
+  static constexpr int DP = DP_, NT = NT_;                  // padded head, and eights of query heads
+  static constexpr int ROW = DP * (CODES ? 1 : 2);          // bytes of a key in shared memory
+  static constexpr int KEYS = ROW == 64 ? 64 : ROW == 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
+  static constexpr int CHUNKS = ROW / 16;
+  static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
+  static constexpr int STAGES = DP <= 128 ? 3 : CODES ? 5 : 3;
+  static constexpr int BLOCKS = DP <= 128 ? 2 : 1;          // an SM
+  static constexpr int DT = DP / 16, REGS = DT * 4 + 4;     // values a lane leaves of eight heads: O, m and l
+  static constexpr int EXCHANGE = 2 * REGS * 32 * 4;
+  static constexpr int SMEM = MMA_WARPS * STAGES * STAGE + EXCHANGE;
+  static constexpr float OFFSET = HALF ? 14.0f : 0.0f;
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool real) {  // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0));
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 load8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ float load4(uint32_t at) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (HALF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two numbers of 32 bits as two of 16, the first in the low half; `back`: the 16-bit numbers in 32 bits.
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t r;
+  if (HALF) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <bool HALF>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if (HALF) return __half22float2(*reinterpret_cast<const __half2 *>(&x));
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+// Two codes, in the low or the high half of x, as two fp16 numbers.  int8: 0x6400 + (code + 128) is 1024 + 128 + code.
+template <int STORE, bool HIGH>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) {
+  if (STORE == LAPIS_I8) {
+    const uint32_t biased = __byte_perm(x, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t *>(&r);
+  }
+  uint32_t r;
+  const uint16_t two = (uint16_t)(HIGH ? x >> 16 : x);
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
+  return r;
+}
+
+// Position in a block's share of the tiles.
+struct Cursor {
+  int request, unit, tile, tiles, lo, hi;
+};
+__device__ __forceinline__ void enter(const AttendArgs &a, Cursor &c, int request, int tile_keys) {
+  const Span s = span_of(a, request);
+  c.request = request;
+  c.lo = (int)s.lo;
+  c.hi = (int)s.hi;
+  c.tiles = (int)tiles_of(s, tile_keys);
+}
+__device__ __forceinline__ void next_unit(const AttendArgs &a, Cursor &c, int units, int tile_keys) {
+  c.tile = 0;
+  if (++c.unit < units) return;
+  c.unit = 0;
+  if (c.request + 1 < a.requests) enter(a, c, c.request + 1, tile_keys);
+}
+
+// What a warp has summed of eight heads: lane (g, c), g = lane / 4, c = lane % 4, holds dimensions by g of heads 2c and 2c + 1.
+template <int DT>
+struct Sums {
+  float o[DT][4], m[2], l[2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.0f;
+  }
+  __device__ __forceinline__ void store(float *p) const {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) reinterpret_cast<float4 *>(p)[t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
+    reinterpret_cast<float4 *>(p)[DT * 32 + lane] = make_float4(m[0], m[1], l[0], l[1]);
+  }
+  __device__ __forceinline__ void add(const float *p) {
+    const int lane = threadIdx.x % 32;
+    const float4 x = reinterpret_cast<const float4 *>(p)[DT * 32 + lane];
+    float f[2], e[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float om = i == 0 ? x.x : x.y, ol = i == 0 ? x.z : x.w, most = fmaxf(m[i], om), base = most == -INFINITY ? 0.0f : most;
+      f[i] = exp2f(m[i] - base);
+      e[i] = exp2f(om - base);
+      m[i] = most;
+      l[i] = l[i] * f[i] + ol * e[i];
+    }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const float4 y = reinterpret_cast<const float4 *>(p)[t * 32 + lane];
+      o[t][0] = o[t][0] * f[0] + y.x * e[0];
+      o[t][1] = o[t][1] * f[1] + y.y * e[1];
+      o[t][2] = o[t][2] * f[0] + y.z * e[0];
+      o[t][3] = o[t][3] * f[1] + y.w * e[1];
+    }
+  }
+};
+
+// Dimension of o[t][0] of group g; that of o[t][2] is the one 8 further (16-bit caches) or the next (codes).
+template <typename C>
+__device__ __forceinline__ int dimension(int t, int g) {
+  if (!C::CODES) return t * 16 + g;
+  return C::DP == 64 ? g * 8 + 2 * t : (g + 8 * (t / 8)) * 16 + 2 * (t % 8);
+}
+
+// Adds up the warps of the block and gives eight heads out: as results, or to `slot` where the unit was cut.
+template <typename C>
+__device__ __forceinline__ void give(const AttendArgs &a, Sums<C::DT> &s, float *exchange, int request, int first_head, int heads, float *slot) {
+  using T = typename C::T;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  constexpr int PART = C::REGS * 32;
+  __syncthreads();
+  if (warp >= 2) s.store(exchange + (warp - 2) * PART);
+  __syncthreads();
+  if (warp < 2) s.add(exchange + warp * PART);
+  __syncthreads();
+  if (warp == 1) s.store(exchange);
+  __syncthreads();
+  if (warp != 0) return;
+  s.add(exchange);
+  if (slot != nullptr) {
+    s.store(slot);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (2 * c + i >= heads) continue;
+    const int64_t head = (int64_t)request * a.q_heads + first_head + 2 * c + i;
+    const float by = s.l[i] == 0.0f ? 0.0f : 1.0f / s.l[i];
+    if (g == 0 && a.lse != nullptr) a.lse[head] = s.l[i] == 0.0f ? -INFINITY : (s.m[i] - C::OFFSET) * LN2 + logf(s.l[i]);
+    T *const out = static_cast<T *>(a.out) + head * a.dim;
+#pragma unroll
+    for (int t = 0; t < C::DT; ++t) {
+      const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
+      if (d0 < a.dim) out[d0] = from_f32<T>(s.o[t][i] * by);
+      if (d1 < a.dim) out[d1] = from_f32<T>(s.o[t][2 + i] * by);
+    }
+  }
+}
+
+template <typename C>
+__global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(const __grid_constant__ AttendArgs a) {
+  using T = typename C::T;
+  constexpr int KEYS = C::KEYS, MT = C::MT, NT = C::NT, DT = C::DT, STAGES = C::STAGES;
+  extern __shared__ __align__(128) unsigned char stages[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
+  float *const exchange = reinterpret_cast<float *>(stages + MMA_WARPS * STAGES * C::STAGE);
+  unsigned char *const mine = stages + warp * STAGES * C::STAGE;
+  const uint32_t ring = shared_address(mine);
+  const int units = (int)a.cache.heads * a.head_blocks;
+  Share share = find_share(a, C::TILE, [&](const Share &x) { return share_start(min((int64_t)blockIdx.x, x.shares - 1), x.all, x.shares); });
+  if (blockIdx.x >= share.shares) return;
+  const int64_t steps = share_start(blockIdx.x + 1, share.all, share.shares) - share.from;
+  if (a.dim != C::DP)  // what is beyond the head is never copied
+    for (int i = lane; i < STAGES * C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
+
+  Cursor in, out;  // of the copies and of the products
+  enter(a, in, (int)share.request, C::TILE);
+  in.unit = (int)(share.in_request / in.tiles);
+  in.tile = (int)(share.in_request % in.tiles);
+  out = in;
+
+  // Pages of the next step to copy: a lane looks up key `lane` (and lane + 32) of it one step ahead.
+  constexpr int LOOK = KEYS == 64 ? 2 : 1;
+  int64_t page[LOOK];
+  int slot_in_page[LOOK];
+  auto look_up = [&]() {
+#pragma unroll
+    for (int u = 0; u < LOOK; ++u) {
+      const int key = in.lo + in.tile * C::TILE + warp * KEYS + (KEYS == 16 ? lane % 16 : lane) + 32 * u;
+      page[u] = -1;
+      slot_in_page[u] = 0;
+      if (key < in.hi) {
+        const int nth = a.page_shift >= 0 ? key >> a.page_shift : key / (int)a.cache.page_size;
+        slot_in_page[u] = key - nth * (int)a.cache.page_size;
+        const int64_t entry = load_index(a.lists.d_pos, in.request, a.lists.idx_bytes) + nth;
+        if (entry >= 0 && entry < a.lists.entries) page[u] = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
+      }
+    }
+  };
+  const int row_bytes = a.dim * (C::CODES ? 1 : 2);
+  auto fetch = [&](int stage) {
+    const uint32_t to = ring + stage * C::STAGE;
+    uint32_t row[LOOK];
+    const int kv_head = in.unit / a.head_blocks;
+#pragma unroll
+    for (int u = 0; u < LOOK; ++u)
+      row[u] = page[u] < 0 || page[u] >= a.cache.pages
+                   ? 0xffffffffu
+                   : (uint32_t)((page[u] * a.cache.heads + kv_head) * a.cache.page_size + slot_in_page[u]);
+#pragma unroll
+    for (int i = 0; i < KEYS * C::CHUNKS / 32; ++i) {
+      const int at = i * 32 + lane, r = at / C::CHUNKS, ch = at % C::CHUNKS;
+      const uint32_t from_row = __shfl_sync(0xffffffffu, row[LOOK == 2 && i >= KEYS * C::CHUNKS / 64 ? 1 : 0], r % 32);
+      if (ch * 16 >= row_bytes) continue;
+      const bool real = from_row != 0xffffffffu;
+      const int64_t offset = real ? (int64_t)from_row * row_bytes + ch * 16 : 0;
+      int kch, vch;
+      if (!C::CODES) {
+        kch = vch = ch ^ (r & 7);
+      } else if (C::DP == 64) {
+        kch = ch;
+        vch = ch ^ (r & 2);
+      } else {
+        kch = ch ^ (r & 4);
+        vch = ch ^ ((r & 3) << 1);
+      }
+      copy16(to + r * C::ROW + kch * 16, static_cast<const char *>(a.cache.d_k) + offset, real);
+      copy16(to + KEYS * C::ROW + r * C::ROW + vch * 16, static_cast<const char *>(a.cache.d_v) + offset, real);
+    }
+    if (C::CODES) {
+#pragma unroll
+      for (int u = 0; u < LOOK; ++u) {
+        const bool real = row[u] != 0xffffffffu;
+        if (KEYS == 16 && lane >= 16) break;
+        const uint32_t scales = to + 2 * KEYS * C::ROW + (lane + 32 * u) * 4;
+        copy4(scales, a.cache.d_k_scale + (real ? row[u] : 0), real);
+        copy4(scales + KEYS * 4, a.cache.d_v_scale + (real ? row[u] : 0), real);
+      }
+    }
+    if (++in.tile == in.tiles) next_unit(a, in, units, C::TILE);
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (s < steps) {
+      fetch(s);
+      look_up();
+    }
+    asm volatile("cp.async.commit_group;");
+  }
+
+  uint32_t q[NT][DT][2];
+  float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
+  float value_by = 0.0f;     // codes: the power of two that the values' scales are relative to
+  Sums<DT> sums[NT];
+  bool fresh = true;
+  int began = out.tile;
+  int stage = 0, stage_in = STAGES - 1;
+  bool first_piece = true;
+  for (int64_t step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2));
+    __syncwarp();
+    if (step + STAGES - 1 < steps) {
+      fetch(stage_in);
+      look_up();
+    }
+    asm volatile("cp.async.commit_group;");
+    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
+    if (fresh) {
+      fresh = false;
+      began = out.tile;
+      value_by = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        sums[n].clear();
+        const bool real = head0 + n * 8 + g < a.group;
+        const T *const from = static_cast<const T *>(a.q) + (int64_t)out.request * a.q_token_stride +
+                              (int64_t)(kv_head * a.group + (real ? head0 + n * 8 + g : 0)) * a.q_head_stride;
+        float x[DT][4], most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DT; ++k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = C::CODES ? (k / 4) * 64 + c * 16 + (k % 4) * 4 + e : k * 16 + c * 2 + (e & 1) + (e & 2) * 4;
+            x[k][e] = real && d < a.dim ? to_f32(from[d]) : 0.0f;
+            most = fmaxf(most, fabsf(x[k][e]));
+          }
+        }
+        float by = 1.0f;
+        if (C::CODES) {  // to [1, 2): 2^(127 - exponent)
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const int exponent = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
+          by = __uint_as_float((uint32_t)(254 - exponent) << 23);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int e = __shfl_sync(0xffffffffu, exponent, (2 * c + i) * 4);
+            score_by[n][i] = a.scale2 * __uint_as_float((uint32_t)e << 23);
+          }
+        } else {
+          score_by[n][0] = score_by[n][1] = a.scale2;
+        }
+#pragma unroll
+        for (int k = 0; k < DT; ++k) {
+          q[n][k][0] = pack2<C::HALF>(x[k][0] * by, x[k][1] * by);
+          q[n][k][1] = pack2<C::HALF>(x[k][2] * by, x[k][3] * by);
+        }
+      }
+    }
+
+    const uint32_t ks = ring + stage * C::STAGE, vs = ks + KEYS * C::ROW, scales = vs + KEYS * C::ROW;
+    float s[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.0f;
+      if (!C::CODES) {
+        const int r = mt * 16 + (lane & 8) + (lane & 7), half = lane >> 4;
+#pragma unroll
+        for (int k = 0; k < DT; ++k) {
+          uint32_t x[4];
+          ldmatrix4(x, ks + r * C::ROW + (((2 * k + half) ^ (r & 7)) * 16));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<C::HALF>(s[mt][n], x, q[n][k][0], q[n][k][1]);
+        }
+      } else {
+        const int r = mt * 16 + (g >> 1) + 4 * (g & 1), swizzle = C::DP == 64 ? 0 : r & 4;
+#pragma unroll
+        for (int k = 0; k < DT / 4; ++k) {
+          const uint4 top = load16(ks + r * C::ROW + (((k * 4 + c) ^ swizzle) * 16)), low = load16(ks + (r + 8) * C::ROW + (((k * 4 + c) ^ swizzle) * 16));
+          const uint32_t tw[4] = {top.x, top.y, top.z, top.w}, lw[4] = {low.x, low.y, low.z, low.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t flip = C::STORE == LAPIS_I8 ? 0x80808080u : 0, t = tw[j] ^ flip, l = lw[j] ^ flip;
+            const uint32_t x[4] = {codes2<C::STORE, false>(t), codes2<C::STORE, false>(l), codes2<C::STORE, true>(t), codes2<C::STORE, true>(l)};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma<C::HALF>(s[mt][n], x, q[n][k * 4 + j][0], q[n][k * 4 + j][1]);
+          }
+        }
+      }
+    }
+
+    // scores of keys (row g, row g + 8 of the tile) and heads (2c, 2c + 1)
+    const int key0 = out.lo + out.tile * C::TILE + warp * KEYS;
+    float value_scale[MT][2], most_value = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = mt * 16 + e * 8 + (C::CODES ? (g >> 1) + 4 * (g & 1) : g);
+        const bool seen = key0 + r < out.hi;
+        float by = 1.0f;
+        value_scale[mt][e] = 1.0f;
+        if (C::CODES) {
+          by = load4(scales + r * 4);
+          value_scale[mt][e] = load4(scales + (KEYS + r) * 4);
+          most_value = fmaxf(most_value, value_scale[mt][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          s[mt][n][2 * e] = seen ? s[mt][n][2 * e] * (score_by[n][0] * by) : -INFINITY;
+          s[mt][n][2 * e + 1] = seen ? s[mt][n][2 * e + 1] * (score_by[n][1] * by) : -INFINITY;
+        }
+      }
+    }
+    float most[NT][2], base[NT][2];
+    bool grows = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = sums[n].m[i];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) x = fmaxf(x, fmaxf(s[mt][n][i], s[mt][n][2 + i]));
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+        most[n][i] = x;
+        base[n][i] = x == -INFINITY ? 0.0f : x;
+        grows |= x > sums[n].m[i];
+      }
+    }
+    if (C::CODES) grows |= most_value > value_by;
+    if (__any_sync(0xffffffffu, grows)) {
+      float shrink = 1.0f;
+      if (C::CODES) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) most_value = fmaxf(most_value, __shfl_xor_sync(0xffffffffu, most_value, d));
+        if (most_value > value_by) {  // the next power of two
+          const uint32_t exponent = (__float_as_uint(most_value) >> 23) + 1;
+          const float now = exponent >= 255 ? most_value : __uint_as_float(exponent << 23);
+          shrink = value_by / now;
+          value_by = now;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float f[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f[i] = exp2f(sums[n].m[i] - base[n][i]);
+          sums[n].l[i] *= f[i];
+          sums[n].m[i] = most[n][i];
+          f[i] *= shrink;
+        }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          sums[n].o[t][0] *= f[0];
+          sums[n].o[t][1] *= f[1];
+          sums[n].o[t][2] *= f[0];
+          sums[n].o[t][3] *= f[1];
+        }
+      }
+    }
+    const float values_in = C::CODES ? 1.0f / value_by : 1.0f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float p0 = exp2f(s[mt][n][2 * e] - (base[n][0] - C::OFFSET)), p1 = exp2f(s[mt][n][2 * e + 1] - (base[n][1] - C::OFFSET));
+          sums[n].l[0] += p0;
+          sums[n].l[1] += p1;
+          if (C::CODES) {
+            const float by = value_scale[mt][e] == 0.0f ? 0.0f : value_scale[mt][e] * values_in;
+            p0 *= by;
+            p1 *= by;
+          }
+          const uint32_t h = pack2<C::HALF>(p0, p1);
+          high[n][e] = transposed(h);
+          if (C::TWO_PARTS) {
+            const float2 back = unpack2<C::HALF>(h);
+            low[n][e] = transposed(pack2<C::HALF>(p0 - back.x, p1 - back.y));
+          }
+        }
+      }
+      if (!C::CODES) {
+        const int r = mt * 16 + ((lane & 16) >> 1) + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          uint32_t x[4];
+          ldmatrix4_trans(x, vs + r * C::ROW + (((2 * t + half) ^ (r & 7)) * 16));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma<C::HALF>(sums[n].o[t], x, high[n][0], high[n][1]);
+            if (C::TWO_PARTS) mma<C::HALF>(sums[n].o[t], x, low[n][0], low[n][1]);
+          }
+        }
+      } else {
+        constexpr int WORDS = C::DP == 64 ? 2 : 4;
+#pragma unroll
+        for (int j = 0; j < (C::DP + 127) / 128; ++j) {
+          uint32_t w[4][WORDS];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = mt * 16 + 4 * i + c;
+            if (C::DP == 64) {
+              const uint2 x = load8(vs + r * C::ROW + (((g >> 1) ^ (r & 2)) * 16) + (g & 1) * 8);
+              w[i][0] = x.x;
+              w[i][1] = x.y;
+            } else {
+              const uint4 x = load16(vs + r * C::ROW + (((g + 8 * j) ^ ((r & 3) << 1)) * 16));
+              w[i][0] = x.x;
+              w[i][1] = x.y;
+              w[i][WORDS - 2] = x.z;
+              w[i][WORDS - 1] = x.w;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < WORDS; ++k) {
+            const uint32_t flip = C::STORE == LAPIS_I8 ? 0x80808080u : 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // dimensions 4k, 4k + 1 and 4k + 2, 4k + 3: rows g and g + 8 of a tile
+              const uint32_t ab = __byte_perm(w[0][k], w[1][k], h == 0 ? 0x5140 : 0x7362) ^ flip;
+              const uint32_t cd = __byte_perm(w[2][k], w[3][k], h == 0 ? 0x5140 : 0x7362) ^ flip;
+              const uint32_t x[4] = {codes2<C::STORE, false>(ab), codes2<C::STORE, true>(ab), codes2<C::STORE, false>(cd), codes2<C::STORE, true>(cd)};
+              const int t = j * 8 + 2 * k + h;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                mma<C::HALF>(sums[n].o[t], x, high[n][0], high[n][1]);
+                if (C::TWO_PARTS) mma<C::HALF>(sums[n].o[t], x, low[n][0], low[n][1]);
+              }
+            }
+          }
+        }
+      }
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    const bool unit_ends = ++out.tile == out.tiles;
+    if (unit_ends || step + 1 == steps) {
+      const bool whole = unit_ends && began == 0;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) sums[n].l[i] += __shfl_xor_sync(0xffffffffu, sums[n].l[i], d);
+        if (C::CODES) {
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= value_by;
+        }
+        float *const slot = a.partial + (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * NT + n) * C::REGS * 32;
+        give<C>(a, sums[n], exchange, out.request, kv_head * a.group + head0 + n * 8, a.group - head0 - n * 8, whole ? nullptr : slot);
+      }
+      first_piece = false;
+      fresh = true;
+      if (unit_ends) next_unit(a, out, units, C::TILE);
+    }
+  }
+  pdl_release();
+}
+
+// Adds up what the blocks left of a unit that was cut, in their order: a block for each unit, its warps the shares by turns.
+template <typename C>
+__global__ void __launch_bounds__(ATT_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
+  __shared__ __align__(16) float exchange[2 * C::REGS * 32];
+  const int request = blockIdx.y, unit = blockIdx.x, warp = threadIdx.x / 32;
+  const Cut cut = cut_of(a, request, unit, C::TILE);
+  if (cut.first == cut.last) return;
+  pdl_wait();
+  const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * 8 * C::NT;
+  for (int n = 0; n < C::NT; ++n) {
+    Sums<C::DT> sums;
+    sums.clear();
+    for (int64_t i = cut.first + warp; i <= cut.last; i += MMA_WARPS)
+      sums.add(a.partial + ((i * 2 + (i > cut.first ? 0 : cut.first_slot)) * C::NT + n) * C::REGS * 32);
+    give<C>(a, sums, exchange, request, kv_head * a.group + head0 + n * 8, a.group - head0 - n * 8, nullptr);
+  }
+}
+
+template <typename C>
+static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may use its shared memory
+  if ((allowed.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+    LAPIS_CUDA_TRY(cudaFuncSetAttribute(attend_mma_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  a.head_blocks = (a.group + 8 * C::NT - 1) / (8 * C::NT);
+  a.blocks = C::BLOCKS * sm_count();
+  a.min_tiles = 4;
+  PoolBuf partial;
+  LAPIS_TRY(partial.alloc((size_t)a.blocks * 2 * C::NT * C::REGS * 32 * sizeof(float), st));
+  a.partial = static_cast<float *>(partial.p);
+  attend_mma_kernel<C><<<a.blocks, ATT_THREADS, C::SMEM, st>>>(a);
+  LAPIS_CUDA_TRY(cudaGetLastError());
+  LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3((unsigned)(a.cache.heads * a.head_blocks), (unsigned)a.requests), ATT_THREADS, 0, st, a));
+  return LAPIS_OK;
+}
+
+template <typename T, int STORE>
+static int launch_mma_of(const AttendArgs &a, int dev, cudaStream_t st) {
+  if (a.dim <= 64) return a.group <= 8 ? launch_mma<MmaConfig<T, STORE, 64, 1>>(a, dev, st) : launch_mma<MmaConfig<T, STORE, 64, 2>>(a, dev, st);
+  if (a.dim <= 128) return a.group <= 8 ? launch_mma<MmaConfig<T, STORE, 128, 1>>(a, dev, st) : launch_mma<MmaConfig<T, STORE, 128, 2>>(a, dev, st);
+  return launch_mma<MmaConfig<T, STORE, 256, 1>>(a, dev, st);
+}
+
+// Whole 16 bytes from 16-byte addresses.
+static bool mma_fits(int type, const AttendArgs &a) {
+  if (type == LAPIS_F32) return false;
+  const int64_t row = a.dim * type_bytes(a.cache.type);
+  return row % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
+}
+
+template <typename T>
+static int launch_mma_type(const AttendArgs &a, int dev, cudaStream_t st) {
+  if (a.cache.type == LAPIS_I8) return launch_mma_of<T, LAPIS_I8>(a, dev, st);
+  if (a.cache.type == LAPIS_E4M3) return launch_mma_of<T, LAPIS_E4M3>(a, dev, st);
+  return launch_mma_of<T, LAPIS_F32>(a, dev, st);
 }
 
 }  // namespace lapis_b200
@@ -354,6 +987,8 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   a.out = d_out;
   a.lse = d_lse;
   cudaStream_t st = as_stream(stream);
+  a.page_shift = (cache->page_size & (cache->page_size - 1)) == 0 ? __builtin_ctzll(cache->page_size) : -1;
+  if (mma_fits(type, a)) return type == LAPIS_F16 ? launch_mma_type<__half>(a, dev, st) : launch_mma_type<__nv_bfloat16>(a, dev, st);
   if (type == LAPIS_F32) return launch_any<float>(a, dev, st);
   if (type == LAPIS_F16) return launch_any<__half>(a, dev, st);
   return launch_any<__nv_bfloat16>(a, dev, st);

@@ -10,6 +10,7 @@
 // Everything is computed in 32 bits and rounded once, when it is stored.
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "kv.h"
 
@@ -247,6 +248,468 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
   }
 }
 
+// ---- whole 16 bytes ---------------------------------------------------------------
+//
+// Bound by memory: every element is read and written once.  A row is held by LANES neighbouring lanes, CHUNKS pieces of 16
+// bytes each; the sums over a row and the partners of its rotation are shuffles among them.  A block takes up to ROWS rows a
+// lane group of one token, so that the weights and the token's line of the tables are read once for all of them, and has all
+// their loads in flight together.
+
+template <typename T>
+struct Piece {
+  static constexpr int V = 16 / sizeof(T);
+  float x[V];
+  __device__ __forceinline__ void set(uint4 raw) {
+    if constexpr (sizeof(T) == 4) {
+      x[0] = __uint_as_float(raw.x);
+      x[1] = __uint_as_float(raw.y);
+      x[2] = __uint_as_float(raw.z);
+      x[3] = __uint_as_float(raw.w);
+    } else {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+          x[2 * i] = f.x;
+          x[2 * i + 1] = f.y;
+        } else {
+          x[2 * i] = __uint_as_float(w[i] << 16);
+          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 get() const {
+    if constexpr (sizeof(T) == 4) {
+      return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) {
+          const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+};
+
+// V codes of a piece, as bytes one behind the other.
+template <int V>
+__device__ __forceinline__ void store_codes(void *to, const float *x, float by, int type) {
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    w[i] = 0;
+    if (type == LAPIS_I8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)(uint8_t)to_i8(x[4 * i + j] * by) << (8 * j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2)
+        w[i] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + j] * by, x[4 * i + j + 1] * by), __NV_SATFINITE, __NV_E4M3) << (8 * j);
+    }
+  }
+  if constexpr (V == 8) *static_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+  else *static_cast<uint32_t *>(to) = w[0];
+}
+template <int V>
+__device__ __forceinline__ void load_codes(float *x, const void *from, int type) {
+  uint32_t w[V / 4];
+  if constexpr (V == 8) {
+    const uint2 raw = *static_cast<const uint2 *>(from);
+    w[0] = raw.x;
+    w[1] = raw.y;
+  } else {
+    w[0] = *static_cast<const uint32_t *>(from);
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint8_t c = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    x[i] = type == LAPIS_I8 ? (float)(int8_t)c : from_e4m3(c);
+  }
+}
+
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float x) {
+#pragma unroll
+  for (int d = LANES / 2; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+
+// N floats from an address that is a multiple of their size, up to 16 bytes.
+template <int N>
+__device__ __forceinline__ void load_floats(float (&x)[N], const float *from) {
+  if constexpr (N == 2) {
+    const float2 f = *reinterpret_cast<const float2 *>(from);
+    x[0] = f.x;
+    x[1] = f.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const float4 f = *reinterpret_cast<const float4 *>(from + j);
+      x[j] = f.x;
+      x[j + 1] = f.y;
+      x[j + 2] = f.z;
+      x[j + 3] = f.w;
+    }
+  }
+}
+
+// The cosines and sines that a lane's pieces are turned by, and where the partners are: for pairs of halves the same place of
+// another piece, `apart` pieces away (negative: this is the second half, whose sine counts the other way).
+template <typename T, int LANES, int CHUNKS>
+struct Turn {
+  static constexpr int V = Piece<T>::V;
+  float c[CHUNKS][V], s[CHUNKS][V];
+  int from[CHUNKS];  // piece of the partner
+
+  // back: the other way round, for gradients.  Pieces that are not turned have cosine 1 and sine 0.
+  __device__ __forceinline__ void load(const RotateArgs &a, int64_t place, int lane, bool back) {
+    const int half = a.rot / 2;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+      const int piece = lane + k * LANES, i = piece * V;
+      from[k] = piece;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        c[k][j] = 1.0f;
+        s[k][j] = 0.0f;
+      }
+      if (i >= a.rot) continue;
+      const bool second = !a.interleaved && i >= half;
+      const float *const cs = a.cos + place * half + (a.interleaved ? i / 2 : second ? i - half : i);
+      const float *const sn = a.sin + (cs - a.cos);
+      if (!a.interleaved) from[k] = second ? piece - half / V : piece + half / V;
+      // first of a pair: a cos - b sin; second: b cos + a sin
+      if (a.interleaved) {
+        float ct[V / 2], st[V / 2];
+        load_floats(ct, cs);
+        load_floats(st, sn);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[k][j] = ct[j / 2];
+          s[k][j] = (j % 2 == 1) != back ? st[j / 2] : -st[j / 2];
+        }
+      } else {
+        load_floats(c[k], cs);
+        load_floats(s[k], sn);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[k][j] = second != back ? s[k][j] : -s[k][j];
+      }
+    }
+  }
+  // y = x turned.
+  __device__ __forceinline__ void apply(const RotateArgs &a, const float (&x)[CHUNKS][V], float (&y)[CHUNKS][V]) const {
+    if (a.interleaved) {
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[k][j] = fmaf(x[k][j], c[k][j], x[k][j ^ 1] * s[k][j]);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float other = __shfl_sync(0xffffffffu, x[0][j], from[k] % LANES, LANES);
+#pragma unroll
+        for (int q = 1; q < CHUNKS; ++q) {
+          const float there = __shfl_sync(0xffffffffu, x[q][j], from[k] % LANES, LANES);
+          other = from[k] / LANES == q ? there : other;
+        }
+        y[k][j] = fmaf(x[k][j], c[k][j], other * s[k][j]);
+      }
+    }
+  }
+};
+
+template <typename T, int LANES, int CHUNKS>
+__device__ __forceinline__ void load_weights(const RotateArgs &a, int which, int lane, float (&w)[CHUNKS][Piece<T>::V]) {
+  constexpr int V = Piece<T>::V;
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k) {
+    const int i = (lane + k * LANES) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[k][j] = 0.0f;
+    if (i >= a.dim) continue;
+    if (a.weight_f32) {
+      load_floats(w[k], static_cast<const float *>(a.weight[which]) + i);
+    } else {
+      Piece<T> p;
+      p.set(*reinterpret_cast<const uint4 *>(static_cast<const T *>(a.weight[which]) + i));
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[k][j] = p.x[j];
+    }
+  }
+}
+
+template <typename T, int LANES, int CHUNKS, int ROWS>
+__global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a) {
+  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int64_t token = blockIdx.x;
+  const int all = a.heads[0] + a.heads[1] + a.heads[2], first = blockIdx.y * GROUPS * ROWS + group;
+  uint4 raw[ROWS][CHUNKS];
+  int which[ROWS], head[ROWS];
+#pragma unroll
+  for (int u = 0; u < ROWS; ++u) {
+    const int row = first + u * GROUPS;
+    which[u] = row < a.heads[0] ? 0 : row < a.heads[0] + a.heads[1] ? 1 : row < all ? 2 : -1;
+    head[u] = row - (which[u] > 0 ? a.heads[0] : 0) - (which[u] > 1 ? a.heads[1] : 0);
+    const Rows &in = a.in[which[u] < 0 ? 0 : which[u]];
+    const T *const from = static_cast<const T *>(in.d) + token * in.token_stride + head[u] * in.head_stride;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+      const int i = (lane + k * LANES) * V;
+      raw[u][k] = which[u] >= 0 && i < a.dim ? *reinterpret_cast<const uint4 *>(from + i) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  const int64_t place = load_index(a.place, token, a.idx_bytes);
+  const bool real = !a.norm || (place >= 0 && place < a.places);
+  Turn<T, LANES, CHUNKS> turn;
+  float weight[2][CHUNKS][V];
+  if (a.norm && real) {
+    turn.load(a, place, lane, false);
+    load_weights<T, LANES, CHUNKS>(a, 0, lane, weight[0]);
+    load_weights<T, LANES, CHUNKS>(a, 1, lane, weight[1]);
+  }
+  int64_t first_row = -1;
+  if (a.to_cache && real && blockIdx.y * GROUPS * ROWS + GROUPS * ROWS > a.heads[0])
+    first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place);
+#pragma unroll
+  for (int u = 0; u < ROWS; ++u) {
+    if (first - group + u * GROUPS >= all) break;  // the whole block is through
+    const bool turned = which[u] >= 0 && which[u] < 2 && a.norm && real;
+    float x[CHUNKS][V], y[CHUNKS][V];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+      Piece<T> p;
+      p.set(raw[u][k]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        x[k][j] = real ? p.x[j] : 0.0f;
+        y[k][j] = x[k][j];
+        sum = fmaf(x[k][j], x[k][j], sum);
+      }
+    }
+    if (a.norm && real) {  // all lanes: a group's rows may be of two kinds, a warp's groups too
+      const float r = 1.0f / sqrtf(lanes_sum<LANES>(sum) / (float)a.dim + a.eps);
+      float n[CHUNKS][V], z[CHUNKS][V];
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) n[k][j] = x[k][j] * r * (which[u] == 1 ? weight[1][k][j] : weight[0][k][j]);
+      turn.apply(a, n, z);
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[k][j] = turned ? z[k][j] : y[k][j];
+    }
+    float most = 0.0f;
+    const bool codes = a.to_cache && is_quantised(a.cache.type);
+    if (codes) {
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(y[k][j]));
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+    }
+    if (which[u] < 0) continue;
+    if (which[u] == 0 || !a.to_cache) {
+      T *const out = static_cast<T *>(a.out[which[u]]) + (token * a.heads[which[u]] + head[u]) * a.dim;
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k) {
+        const int i = (lane + k * LANES) * V;
+        Piece<T> p;
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.x[j] = y[k][j];
+        if (i < a.dim) *reinterpret_cast<uint4 *>(out + i) = p.get();
+      }
+      continue;
+    }
+    if (first_row < 0) continue;
+    const int64_t row = first_row + head[u] * a.cache.page_size;
+    void *const store = which[u] == 1 ? a.cache.d_k : a.cache.d_v;
+    const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+    if (codes && lane == 0) (which[u] == 1 ? a.cache.d_k_scale : a.cache.d_v_scale)[row] = scale_of(most, big);
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+      const int i = (lane + k * LANES) * V;
+      if (i >= a.dim) continue;
+      if (codes) {
+        store_codes<V>(static_cast<char *>(store) + row * a.dim + i, y[k], by, a.cache.type);
+      } else {
+        Piece<T> p;
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.x[j] = y[k][j];
+        *reinterpret_cast<uint4 *>(static_cast<T *>(store) + row * a.dim + i) = p.get();
+      }
+    }
+  }
+}
+
+// Backward: blocks take tokens a grid apart, a lane group rows of a token, and a lane keeps its share of the weights' gradients.
+// The lane groups of a block are added in order, the blocks by rotate_weights_kernel.
+template <typename T, int LANES, int CHUNKS, int ROWS>
+__global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a) {
+  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
+  __shared__ float shares[GROUPS][LANES * CHUNKS * V];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  float weight[2][CHUNKS][V], dw[2][CHUNKS][V];
+  load_weights<T, LANES, CHUNKS>(a, 0, lane, weight[0]);
+  load_weights<T, LANES, CHUNKS>(a, 1, lane, weight[1]);
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[0][k][j] = dw[1][k][j] = 0.0f;
+  const int all = a.heads[0] + a.heads[1];
+  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+    const int64_t place = load_index(a.place, token, a.idx_bytes);
+    const bool real = place >= 0 && place < a.places;
+    Turn<T, LANES, CHUNKS> turn;
+    turn.load(a, real ? place : 0, lane, true);
+    for (int row0 = 0; row0 < all; row0 += GROUPS * ROWS) {
+      uint4 raw[ROWS][2][CHUNKS];
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        const int row = row0 + u * GROUPS + group, which = row >= a.heads[0], head = row - (which ? a.heads[0] : 0);
+        const T *const x = static_cast<const T *>(a.in[which].d) + token * a.in[which].token_stride + head * a.in[which].head_stride;
+        const T *const dy = static_cast<const T *>(a.grad[which].d) + token * a.grad[which].token_stride + head * a.grad[which].head_stride;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          const int i = (lane + k * LANES) * V;
+          const bool in = row < all && i < a.dim && real;
+          raw[u][0][k] = in ? *reinterpret_cast<const uint4 *>(x + i) : make_uint4(0, 0, 0, 0);
+          raw[u][1][k] = in ? *reinterpret_cast<const uint4 *>(dy + i) : make_uint4(0, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < ROWS; ++u) {
+        if (row0 + u * GROUPS >= all) break;
+        const int row = row0 + u * GROUPS + group, which = row >= a.heads[0], head = row - (which ? a.heads[0] : 0);
+        float x[CHUNKS][V], dy[CHUNKS][V], dn[CHUNKS][V];
+        float sum = 0.0f, inner = 0.0f;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          Piece<T> p, q;
+          p.set(raw[u][0][k]);
+          q.set(raw[u][1][k]);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            x[k][j] = p.x[j];
+            dy[k][j] = q.x[j];
+          }
+        }
+        turn.apply(a, dy, dn);
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            sum = fmaf(x[k][j], x[k][j], sum);
+            inner = fmaf(dn[k][j] * (which ? weight[1][k][j] : weight[0][k][j]), x[k][j], inner);
+          }
+#pragma unroll
+        for (int d = LANES / 2; d > 0; d /= 2) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          inner += __shfl_xor_sync(0xffffffffu, inner, d);
+        }
+        const float r = 1.0f / sqrtf(sum / (float)a.dim + a.eps), back = inner / (float)a.dim * r * r;
+        T *const out = static_cast<T *>(a.out[which]) + (token * a.heads[which] + head) * a.dim;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          const int i = (lane + k * LANES) * V;
+          Piece<T> p;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float t = dn[k][j] * x[k][j] * r;
+            if (which) dw[1][k][j] += t;
+            else dw[0][k][j] += t;
+            p.x[j] = r * (dn[k][j] * (which ? weight[1][k][j] : weight[0][k][j]) - x[k][j] * back);
+          }
+          if (row < all && i < a.dim) *reinterpret_cast<uint4 *>(out + i) = p.get();
+        }
+      }
+    }
+  }
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) shares[group][(lane + k * LANES) * V + j] = which ? dw[1][k][j] : dw[0][k][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.dim; i += ROW_THREADS) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) sum += shares[g][i];
+      a.partial[((int64_t)blockIdx.x * 2 + which) * a.dim + i] = sum;
+    }
+  }
+}
+
+// Keys and values of listed tokens, a lane group a head of TOKENS tokens; the cache's rows are codes or T.
+template <typename T, int LANES, int CHUNKS, int TOKENS>
+__global__ void __launch_bounds__(ROW_THREADS)
+kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row, const void *place, T *k, T *v) {
+  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
+  const int lane = threadIdx.x % LANES, head = blockIdx.y * GROUPS + threadIdx.x / LANES;
+  if (head >= cache.heads) return;
+  const bool codes = is_quantised(cache.type);
+  const int dim = (int)cache.dim;
+  int64_t at[TOKENS];
+#pragma unroll
+  for (int u = 0; u < TOKENS; ++u) {
+    const int64_t token = (int64_t)blockIdx.x * TOKENS + u;
+    at[u] = token < tokens ? cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes)) : -1;
+    if (at[u] >= 0) at[u] += head * cache.page_size;
+  }
+  Piece<T> got[TOKENS][2][CHUNKS];
+#pragma unroll
+  for (int u = 0; u < TOKENS; ++u)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const void *const store = w == 0 ? cache.d_k : cache.d_v;
+      float scale = 1.0f;
+      if (codes && at[u] >= 0) scale = (w == 0 ? cache.d_k_scale : cache.d_v_scale)[at[u]];
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (lane + c * LANES) * V;
+        Piece<T> &p = got[u][w][c];
+#pragma unroll
+        for (int j = 0; j < V; ++j) p.x[j] = 0.0f;
+        if (at[u] < 0 || i >= dim) continue;
+        if (codes) {
+          load_codes<V>(p.x, static_cast<const char *>(store) + at[u] * dim + i, cache.type);
+#pragma unroll
+          for (int j = 0; j < V; ++j) p.x[j] *= scale;
+        } else {
+          p.set(*reinterpret_cast<const uint4 *>(static_cast<const T *>(store) + at[u] * dim + i));
+        }
+      }
+    }
+#pragma unroll
+  for (int u = 0; u < TOKENS; ++u) {
+    const int64_t token = (int64_t)blockIdx.x * TOKENS + u;
+    if (token >= tokens) break;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (lane + c * LANES) * V;
+        if (i < dim) *reinterpret_cast<uint4 *>((w == 0 ? k : v) + (token * cache.heads + head) * dim + i) = got[u][w][c].get();
+      }
+  }
+}
+
 // ---- host -------------------------------------------------------------------
 
 int check_cache(const char *what, const lapis_b200_kv_cache *c) {
@@ -316,14 +779,82 @@ static int with_type(int type, F run) {
   return run(__nv_bfloat16());
 }
 
+static bool aligned(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+static bool aligned(const Rows &r, int size) {
+  return aligned(r.d, 16) && r.token_stride * size % 16 == 0 && r.head_stride * size % 16 == 0;
+}
+// Whether 16-byte pieces fit the rows of a type, the pairs of their rotation and all arrays.
+static bool pieces_fit(int type, const RotateArgs &a, bool backward) {
+  const int size = type_bytes(type), v = 16 / size;
+  if (a.dim % v != 0) return false;
+  if (a.norm && (a.interleaved ? a.rot % v != 0 : a.rot / 2 % v != 0)) return false;
+  if (a.norm && !(aligned(a.cos, 16) && aligned(a.sin, 16) && aligned(a.weight[0], 16) && aligned(a.weight[1], 16))) return false;
+  for (int w = 0; w < 3; ++w)
+    if (a.heads[w] > 0 && !aligned(a.in[w], size)) return false;
+  for (int w = 0; w < 2; ++w)
+    if (a.heads[w] > 0 && ((backward && !aligned(a.grad[w], size)) || !aligned(a.out[w], 16))) return false;
+  return !a.to_cache || (aligned(a.cache.d_k, 16) && aligned(a.cache.d_v, 16));
+}
+
+// Calls run(LANES, CHUNKS) as compile-time numbers for rows of `dim` values.
+template <typename T, typename F>
+static int with_lanes(int dim, F run) {
+  using std::integral_constant;
+  const int pieces = dim / Piece<T>::V;
+  if (pieces <= 4) return run(integral_constant<int, 4>(), integral_constant<int, 1>());
+  if (pieces <= 8) return run(integral_constant<int, 8>(), integral_constant<int, 1>());
+  if (pieces <= 16) return run(integral_constant<int, 16>(), integral_constant<int, 1>());
+  if constexpr (KV_MAX_DIM / Piece<T>::V > 32)
+    if (pieces > 32) return run(integral_constant<int, 32>(), integral_constant<int, 2>());
+  return run(integral_constant<int, 32>(), integral_constant<int, 1>());
+}
+
 static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
-  const int64_t rows = a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]);
+  const int64_t heads = a.heads[0] + a.heads[1] + a.heads[2], rows = a.tokens * heads;
   if (rows == 0) return LAPIS_OK;
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    rotate_any_kernel<T><<<(unsigned)((rows + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, st>>>(a);
-    LAPIS_CUDA_TRY(cudaGetLastError());
-    return (int)LAPIS_OK;
+    if (!pieces_fit(type, a, false)) {
+      rotate_any_kernel<T><<<(unsigned)((rows + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, st>>>(a);
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    }
+    return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = ROW_THREADS / LANES;
+      // few tokens: a block for each round of rows
+      if (a.tokens * heads <= (int64_t)GROUPS * 4 * sm_count()) {
+        rotate_kernel<T, LANES, CHUNKS, 1><<<dim3((unsigned)a.tokens, (unsigned)((heads + GROUPS - 1) / GROUPS)), ROW_THREADS, 0, st>>>(a);
+      } else {
+        constexpr int ROWS = CHUNKS == 1 ? 4 : 2;
+        rotate_kernel<T, LANES, CHUNKS, ROWS><<<dim3((unsigned)a.tokens, (unsigned)((heads + GROUPS * ROWS - 1) / (GROUPS * ROWS))), ROW_THREADS, 0, st>>>(a);
+      }
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    });
+  });
+}
+
+// Launches the backward kernel that fits and leaves in *blocks how many shares of the weights' gradients there are.
+static int launch_backward(int type, RotateArgs &a, PoolBuf &partial, int *blocks, cudaStream_t st) {
+  const bool pieces = pieces_fit(type, a, true);
+  const int most = 8 * sm_count();
+  *blocks = (int)std::min<int64_t>(pieces ? a.tokens : (a.tokens + ROW_WARPS - 1) / ROW_WARPS, most);
+  LAPIS_TRY(partial.alloc((size_t)*blocks * 2 * a.dim * sizeof(float), st));
+  a.partial = static_cast<float *>(partial.p);
+  if (*blocks == 0) return LAPIS_OK;
+  return with_type(type, [&](auto t) {
+    using T = decltype(t);
+    if (!pieces) {
+      rotate_any_backward_kernel<T><<<*blocks, ROW_THREADS, 0, st>>>(a);
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    }
+    return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value;
+      rotate_backward_kernel<T, LANES, CHUNKS, CHUNKS == 1 ? 2 : 1><<<*blocks, ROW_THREADS, 0, st>>>(a);
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    });
   });
 }
 
@@ -388,18 +919,9 @@ extern "C" int lapis_b200_qk_norm_rope_backward(int type, int64_t tokens, int64_
   a.idx_bytes = idx_bytes;
   a.place = d_place;
   cudaStream_t st = as_stream(stream);
-  const int blocks = (int)std::min<int64_t>((tokens + ROW_WARPS - 1) / ROW_WARPS, 8LL * sm_count());
+  int blocks = 0;
   PoolBuf partial;
-  LAPIS_TRY(partial.alloc((size_t)blocks * 2 * dim * sizeof(float), st));
-  a.partial = static_cast<float *>(partial.p);
-  if (blocks > 0) {
-    LAPIS_TRY(with_type(type, [&](auto t) {
-      using T = decltype(t);
-      rotate_any_backward_kernel<T><<<blocks, ROW_THREADS, 0, st>>>(a);
-      LAPIS_CUDA_TRY(cudaGetLastError());
-      return (int)LAPIS_OK;
-    }));
-  }
+  LAPIS_TRY(launch_backward(type, a, partial, &blocks, st));
   rotate_weights_kernel<<<dim3((unsigned)((dim + 31) / 32), 2), dim3(32, 32), 0, st>>>(a.partial, blocks, (int)dim, d_q_weight_grad, d_k_weight_grad);
   LAPIS_CUDA_TRY(cudaGetLastError());
   return LAPIS_OK;
@@ -451,11 +973,29 @@ extern "C" int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_
   LAPIS_TRY(check_sizes(what, type, tokens, cache->dim, cache->heads));
   if (tokens == 0) return LAPIS_OK;
   if (d_row == nullptr || d_place == nullptr || d_k == nullptr || d_v == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  const int size = type_bytes(type);
+  const bool pieces = cache->dim * size % 16 == 0 && (is_quantised(cache->type) || cache->type == type) && aligned(cache->d_k, 16) &&
+                      aligned(cache->d_v, 16) && aligned(d_k, 16) && aligned(d_v, 16);
+  cudaStream_t st = as_stream(stream);
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    kv_read_any_kernel<T><<<(unsigned)((tokens * cache->heads + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, as_stream(stream)>>>(
-        *cache, *lists, tokens, d_row, d_place, static_cast<T *>(d_k), static_cast<T *>(d_v));
-    LAPIS_CUDA_TRY(cudaGetLastError());
-    return (int)LAPIS_OK;
+    T *const k = static_cast<T *>(d_k), *const v = static_cast<T *>(d_v);
+    if (!pieces) {
+      kv_read_any_kernel<T><<<(unsigned)((tokens * cache->heads + ROW_WARPS - 1) / ROW_WARPS), ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, k, v);
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    }
+    return with_lanes<T>((int)cache->dim, [&](auto lanes, auto chunks) {
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = ROW_THREADS / LANES;
+      const unsigned rounds = (unsigned)((cache->heads + GROUPS - 1) / GROUPS);
+      if (tokens * rounds <= 8LL * sm_count()) {
+        kv_read_kernel<T, LANES, CHUNKS, 1><<<dim3((unsigned)tokens, rounds), ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, k, v);
+      } else {
+        constexpr int TOKENS = CHUNKS == 1 ? 4 : 2;
+        kv_read_kernel<T, LANES, CHUNKS, TOKENS><<<dim3((unsigned)((tokens + TOKENS - 1) / TOKENS), rounds), ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, k, v);
+      }
+      LAPIS_CUDA_TRY(cudaGetLastError());
+      return (int)LAPIS_OK;
+    });
   });
 }

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
       __syncthreads();
       for (int j = warp; j < ANY_TILE; j += ATT_THREADS / 32) {
         const bool in = key0 + j < span.hi;
-        const int64_t row0 = in ? cache_row(a.cache, a.lists, request, key0 + j) : -1, row = row0 + kv_head * a.cache.page_size;
+        const int64_t row0 = in ? cache_row(a.cache, a.lists, request, key0 + j, a.page_shift) : -1, row = row0 + kv_head * a.cache.page_size;
         float kscale = 1.0f, vscale = 1.0f;
         if (row0 >= 0 && is_quantised(a.cache.type)) {
           kscale = a.cache.d_k_scale[row];
@@ -987,7 +987,7 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   a.out = d_out;
   a.lse = d_lse;
   cudaStream_t st = as_stream(stream);
-  a.page_shift = (cache->page_size & (cache->page_size - 1)) == 0 ? __builtin_ctzll(cache->page_size) : -1;
+  a.page_shift = page_shift_of(cache->page_size);
   if (mma_fits(type, a)) return type == LAPIS_F16 ? launch_mma_type<__half>(a, dev, st) : launch_mma_type<__nv_bfloat16>(a, dev, st);
   if (type == LAPIS_F32) return launch_any<float>(a, dev, st);
   if (type == LAPIS_F16) return launch_any<__half>(a, dev, st);

@@ -20,6 +20,9 @@ __host__ __device__
 #endif
 inline bool is_quantised(int type) { return type == LAPIS_I8 || type == LAPIS_E4M3; }
 
+// log2 of the slots of a page, or -1: places are shifted instead of divided, where that is the same.
+inline int page_shift_of(int64_t page_size) { return (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1; }
+
 // Checks of the descriptions that the entry points take (rotate.cu); 0 or a recorded error.
 int check_cache(const char *what, const lapis_b200_kv_cache *cache);
 int check_lists(const char *what, const lapis_b200_page_lists *lists);
@@ -73,14 +76,15 @@ __device__ __forceinline__ int64_t load_index(const void *p, int64_t i, int byte
 }
 
 // Row of the cache (as [pages * heads * page_size, dim]) that holds head 0 of the token at `place` of request `row`, or -1
-// where the lists name none: what the lists say is checked, as nothing on the host has seen it.
-__device__ __forceinline__ int64_t cache_row(const lapis_b200_kv_cache &cache, const lapis_b200_page_lists &lists, int64_t row, int64_t place) {
+// where the lists name none (page_shift: page_shift_of, or -1): what the lists say is checked, as nothing on the host has seen it.
+__device__ __forceinline__ int64_t cache_row(const lapis_b200_kv_cache &cache, const lapis_b200_page_lists &lists, int64_t row, int64_t place, int page_shift) {
   if (row < 0 || row >= lists.rows || place < 0) return -1;
-  const int64_t entry = load_index(lists.d_pos, row, lists.idx_bytes) + place / cache.page_size;
+  const int64_t nth = page_shift >= 0 ? place >> page_shift : place <= 0x7fffffff ? (int64_t)((uint32_t)place / (uint32_t)cache.page_size) : place / cache.page_size;
+  const int64_t entry = load_index(lists.d_pos, row, lists.idx_bytes) + nth;
   if (entry < 0 || entry >= load_index(lists.d_pos, row + 1, lists.idx_bytes) || entry >= lists.entries) return -1;
   const int64_t page = load_index(lists.d_crd, entry, lists.idx_bytes);
   if (page < 0 || page >= cache.pages) return -1;
-  return page * cache.heads * cache.page_size + place % cache.page_size;
+  return page * cache.heads * cache.page_size + (place - nth * cache.page_size);
 }
 #endif
 

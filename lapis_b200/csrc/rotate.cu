@@ -42,6 +42,7 @@ struct RotateArgs {
   int to_cache;
   lapis_b200_kv_cache cache;
   lapis_b200_page_lists lists;
+  int page_shift;  // log2 of the slots of a page, or -1
   float *partial;  // backward: [blocks][2][dim]
 };
 
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_any_kernel(const __grid_co
     return;
   }
   if (!real) return;
-  const int64_t first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place);
+  const int64_t first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place, a.page_shift);
   if (first_row < 0) return;
   const int64_t row = first_row + head * a.cache.page_size;
   void *const store = which == 1 ? a.cache.d_k : a.cache.d_v;
@@ -215,14 +216,18 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_any_backward_kernel(const 
 // dw = sum of the blocks' shares, in the order of the blocks: 32 sums a block apart, then those.
 __global__ void __launch_bounds__(1024) rotate_weights_kernel(const float *partial, int blocks, int dim, float *dqw, float *dkw) {
   __shared__ float sums[32][33];
-  const int i = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
+  const int lane = threadIdx.x % 32, nth = threadIdx.x / 32, i = blockIdx.x * 32 + lane, which = blockIdx.y;
   float sum = 0.0f;
-  if (i < dim)
-    for (int b = threadIdx.y; b < blocks; b += 32) sum += partial[((int64_t)b * 2 + which) * dim + i];
-  sums[threadIdx.y][threadIdx.x] = sum;
+  pdl_wait();
+  if (i < dim) {
+#pragma unroll 8
+    for (int b = nth; b < blocks; b += 32) sum += partial[((int64_t)b * 2 + which) * dim + i];
+  }
+  sums[nth][lane] = sum;
   __syncthreads();
-  if (threadIdx.y == 0 && i < dim) {
-    for (int b = 1; b < 32; ++b) sum += sums[b][threadIdx.x];
+  if (nth == 0 && i < dim) {
+#pragma unroll
+    for (int b = 1; b < 32; ++b) sum += sums[b][lane];
     (which == 0 ? dqw : dkw)[i] = sum;
   }
 }
@@ -235,7 +240,7 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + warp;
   if (task >= tokens * cache.heads) return;
   const int64_t token = task / cache.heads, head = task % cache.heads;
-  const int64_t first = cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes));
+  const int64_t first = cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes), -1);
   const int64_t at = first + head * cache.page_size;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -250,97 +255,106 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
 
 // ---- whole 16 bytes ---------------------------------------------------------------
 //
-// Bound by memory: every element is read and written once.  A row is held by LANES neighbouring lanes, CHUNKS pieces of 16
-// bytes each; the sums over a row and the partners of its rotation are shuffles among them.  A block takes up to ROWS rows a
-// lane group of one token, so that the weights and the token's line of the tables are read once for all of them, and has all
-// their loads in flight together.
+// Bound by memory: every element is read and written once, so what a row costs in instructions has to stay small next to the
+// 0.7 pieces of 16 bytes that an SM can read and write in a cycle.  A row is held by LANES neighbouring lanes, CHUNKS pieces
+// each; a warp holds 32 / LANES rows at a time and walks the rows of a token, so that the token's line of the tables, the
+// weights and the place in the cache are looked up once for many rows.  Weight and rotation are one product each with a row's
+// own piece and its partner's: y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin, and the partner's piece comes by a shuffle of
+// the row as it was read, while the sum of squares is still under way.
 
 template <typename T>
 struct Piece {
   static constexpr int V = 16 / sizeof(T);
   float x[V];
-  __device__ __forceinline__ void set(uint4 raw) {
-    if constexpr (sizeof(T) == 4) {
-      x[0] = __uint_as_float(raw.x);
-      x[1] = __uint_as_float(raw.y);
-      x[2] = __uint_as_float(raw.z);
-      x[3] = __uint_as_float(raw.w);
-    } else {
-      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  __device__ __forceinline__ void set(const uint32_t (&w)[4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<T, __half>::value) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
-        } else {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
   }
   __device__ __forceinline__ uint4 get() const {
-    if constexpr (sizeof(T) == 4) {
-      return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
-    } else {
-      uint32_t w[4];
+    uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (std::is_same<T, __half>::value) {
-          const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(x[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
       }
-      return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
-// V codes of a piece, as bytes one behind the other.
+struct Raw {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const void *p, bool in) {
+    const uint4 x = in ? *static_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+    w[0] = x.x;
+    w[1] = x.y;
+    w[2] = x.z;
+    w[3] = x.w;
+  }
+};
+
+// V codes of a piece, one behind the other.  int8: adding 1.5 * 2^23 rounds to a whole number, ties to even, and leaves it in
+// the low byte; a product is at most 127 (1 + 2^-23).
 template <int V>
 __device__ __forceinline__ void store_codes(void *to, const float *x, float by, int type) {
   uint32_t w[V / 4];
 #pragma unroll
   for (int i = 0; i < V / 4; ++i) {
-    w[i] = 0;
+    const float *const y = x + 4 * i;
     if (type == LAPIS_I8) {
+      uint32_t b[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)(uint8_t)to_i8(x[4 * i + j] * by) << (8 * j);
+      for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(__fadd_rn(__fmul_rn(y[j], by), 12582912.0f));
+      w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; j += 2)
-        w[i] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + j] * by, x[4 * i + j + 1] * by), __NV_SATFINITE, __NV_E4M3) << (8 * j);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0] * by, y[1] * by), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2] * by, y[3] * by), __NV_SATFINITE, __NV_E4M3);
+      w[i] = lo | hi << 16;
     }
   }
   if constexpr (V == 8) *static_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
   else *static_cast<uint32_t *>(to) = w[0];
 }
+// The values of V codes.  int8: 2^23 + 128 + code is a float with the biased code in its low byte.
 template <int V>
-__device__ __forceinline__ void load_codes(float *x, const void *from, int type) {
-  uint32_t w[V / 4];
-  if constexpr (V == 8) {
-    const uint2 raw = *static_cast<const uint2 *>(from);
-    w[0] = raw.x;
-    w[1] = raw.y;
-  } else {
-    w[0] = *static_cast<const uint32_t *>(from);
-  }
+__device__ __forceinline__ void values_of(float *x, uint2 raw, float scale, int type) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint8_t c = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
-    x[i] = type == LAPIS_I8 ? (float)(int8_t)c : from_e4m3(c);
-  }
-}
-
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float x) {
+  for (int i = 0; i < V / 4; ++i) {
+    const uint32_t w = i == 0 ? raw.x : raw.y;
+    if (type == LAPIS_I8) {
+      const uint32_t u = w ^ 0x80808080u;
+      x[4 * i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f;
+      x[4 * i + 1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f;
+      x[4 * i + 2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f;
+      x[4 * i + 3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f;
+    } else {
 #pragma unroll
-  for (int d = LANES / 2; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
-  return x;
+      for (int j = 0; j < 4; j += 2) {
+        const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (8 * j)), __NV_E4M3)));
+        x[4 * i + j] = f.x;
+        x[4 * i + j + 1] = f.y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[4 * i + j] *= scale;
+  }
 }
 
 // N floats from an address that is a multiple of their size, up to 16 bytes.
@@ -362,16 +376,16 @@ __device__ __forceinline__ void load_floats(float (&x)[N], const float *from) {
   }
 }
 
-// The cosines and sines that a lane's pieces are turned by, and where the partners are: for pairs of halves the same place of
-// another piece, `apart` pieces away (negative: this is the second half, whose sine counts the other way).
+// What a lane knows of the rotation: y_j = x_j c_j + x'_j s_j with x' the partners, which for neighbouring pairs are in the same
+// piece and for pairs of halves in piece `from`.  Pieces that are not turned have cosine 1 and sine 0.
 template <typename T, int LANES, int CHUNKS>
 struct Turn {
   static constexpr int V = Piece<T>::V;
   float c[CHUNKS][V], s[CHUNKS][V];
-  int from[CHUNKS];  // piece of the partner
+  int from[CHUNKS];
 
-  // back: the other way round, for gradients.  Pieces that are not turned have cosine 1 and sine 0.
-  __device__ __forceinline__ void load(const RotateArgs &a, int64_t place, int lane, bool back) {
+  // back: the other way round, for gradients.
+  __device__ __forceinline__ void load(const RotateArgs &a, int64_t place, bool real, int lane, bool back) {
     const int half = a.rot / 2;
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
@@ -382,11 +396,10 @@ struct Turn {
         c[k][j] = 1.0f;
         s[k][j] = 0.0f;
       }
-      if (i >= a.rot) continue;
+      if (i >= a.rot || !real) continue;
       const bool second = !a.interleaved && i >= half;
       const float *const cs = a.cos + place * half + (a.interleaved ? i / 2 : second ? i - half : i);
       const float *const sn = a.sin + (cs - a.cos);
-      if (!a.interleaved) from[k] = second ? piece - half / V : piece + half / V;
       // first of a pair: a cos - b sin; second: b cos + a sin
       if (a.interleaved) {
         float ct[V / 2], st[V / 2];
@@ -398,6 +411,7 @@ struct Turn {
           s[k][j] = (j % 2 == 1) != back ? st[j / 2] : -st[j / 2];
         }
       } else {
+        from[k] = second ? piece - half / V : piece + half / V;
         load_floats(c[k], cs);
         load_floats(s[k], sn);
 #pragma unroll
@@ -405,237 +419,265 @@ struct Turn {
       }
     }
   }
-  // y = x turned.
-  __device__ __forceinline__ void apply(const RotateArgs &a, const float (&x)[CHUNKS][V], float (&y)[CHUNKS][V]) const {
+  // x' of a row's pieces; all lanes of the warp take part.
+  __device__ __forceinline__ void partners(const RotateArgs &a, const Raw (&raw)[CHUNKS], const Piece<T> (&x)[CHUNKS], Piece<T> (&other)[CHUNKS]) const {
     if (a.interleaved) {
 #pragma unroll
       for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[k][j] = fmaf(x[k][j], c[k][j], x[k][j ^ 1] * s[k][j]);
+        for (int j = 0; j < V; ++j) other[k].x[j] = x[k].x[j ^ 1];
       return;
     }
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float other = __shfl_sync(0xffffffffu, x[0][j], from[k] % LANES, LANES);
+      for (int i = 0; i < 4; ++i) {
+        w[i] = __shfl_sync(0xffffffffu, raw[0].w[i], from[k] % LANES, LANES);
 #pragma unroll
         for (int q = 1; q < CHUNKS; ++q) {
-          const float there = __shfl_sync(0xffffffffu, x[q][j], from[k] % LANES, LANES);
-          other = from[k] / LANES == q ? there : other;
+          const uint32_t there = __shfl_sync(0xffffffffu, raw[q].w[i], from[k] % LANES, LANES);
+          w[i] = from[k] / LANES == q ? there : w[i];
         }
-        y[k][j] = fmaf(x[k][j], c[k][j], other * s[k][j]);
       }
+      other[k].set(w);
     }
   }
 };
 
-template <typename T, int LANES, int CHUNKS>
-__device__ __forceinline__ void load_weights(const RotateArgs &a, int which, int lane, float (&w)[CHUNKS][Piece<T>::V]) {
+// The weights of a lane's pieces, or of the partners'.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ void load_weights(const RotateArgs &a, int which, const int (&piece)[CHUNKS], float (&w)[CHUNKS][Piece<T>::V]) {
   constexpr int V = Piece<T>::V;
 #pragma unroll
   for (int k = 0; k < CHUNKS; ++k) {
-    const int i = (lane + k * LANES) * V;
+    const int i = piece[k] * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) w[k][j] = 0.0f;
     if (i >= a.dim) continue;
     if (a.weight_f32) {
       load_floats(w[k], static_cast<const float *>(a.weight[which]) + i);
     } else {
+      Raw raw;
       Piece<T> p;
-      p.set(*reinterpret_cast<const uint4 *>(static_cast<const T *>(a.weight[which]) + i));
+      raw.load(static_cast<const T *>(a.weight[which]) + i, true);
+      p.set(raw.w);
 #pragma unroll
       for (int j = 0; j < V; ++j) w[k][j] = p.x[j];
     }
   }
 }
 
-template <typename T, int LANES, int CHUNKS, int ROWS>
-__global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a) {
-  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int64_t token = blockIdx.x;
-  const int all = a.heads[0] + a.heads[1] + a.heads[2], first = blockIdx.y * GROUPS * ROWS + group;
-  uint4 raw[ROWS][CHUNKS];
-  int which[ROWS], head[ROWS];
+// Rounds [from, to) of a warp's rows of one kind: `count` heads, GROUPS at a time, ROUNDS loads in flight.
+template <typename T, int LANES, int CHUNKS, bool NORM, bool CODES>
+__device__ __forceinline__ void rotate_rows(const RotateArgs &a, const Rows &in, int64_t token, int count, int from, int to,
+                                            const Turn<T, LANES, CHUNKS> &turn, const float (&wc)[CHUNKS][Piece<T>::V],
+                                            const float (&ws)[CHUNKS][Piece<T>::V], char *out, int64_t out_stride, float *scales,
+                                            int64_t scale_stride, bool real) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 4 : 2;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
+  const T *const rows = static_cast<const T *>(in.d) + token * in.token_stride + lane * V;
+  const float by_dim = 1.0f / (float)a.dim;
+  for (int round = from; round < to; round += ROUNDS) {
+    Raw raw[ROUNDS][CHUNKS];
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    const int row = first + u * GROUPS;
-    which[u] = row < a.heads[0] ? 0 : row < a.heads[0] + a.heads[1] ? 1 : row < all ? 2 : -1;
-    head[u] = row - (which[u] > 0 ? a.heads[0] : 0) - (which[u] > 1 ? a.heads[1] : 0);
-    const Rows &in = a.in[which[u] < 0 ? 0 : which[u]];
-    const T *const from = static_cast<const T *>(in.d) + token * in.token_stride + head[u] * in.head_stride;
+    for (int u = 0; u < ROUNDS; ++u) {
+      const int head = (round + u) * GROUPS + group;
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      const int i = (lane + k * LANES) * V;
-      raw[u][k] = which[u] >= 0 && i < a.dim ? *reinterpret_cast<const uint4 *>(from + i) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < CHUNKS; ++k)
+        raw[u][k].load(rows + head * in.head_stride + k * LANES * V, real && round + u < to && head < count && (lane + k * LANES) * V < a.dim);
     }
-  }
-  const int64_t place = load_index(a.place, token, a.idx_bytes);
-  const bool real = !a.norm || (place >= 0 && place < a.places);
-  Turn<T, LANES, CHUNKS> turn;
-  float weight[2][CHUNKS][V];
-  if (a.norm && real) {
-    turn.load(a, place, lane, false);
-    load_weights<T, LANES, CHUNKS>(a, 0, lane, weight[0]);
-    load_weights<T, LANES, CHUNKS>(a, 1, lane, weight[1]);
-  }
-  int64_t first_row = -1;
-  if (a.to_cache && real && blockIdx.y * GROUPS * ROWS + GROUPS * ROWS > a.heads[0])
-    first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place);
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    if (first - group + u * GROUPS >= all) break;  // the whole block is through
-    const bool turned = which[u] >= 0 && which[u] < 2 && a.norm && real;
-    float x[CHUNKS][V], y[CHUNKS][V];
-    float sum = 0.0f;
+    for (int u = 0; u < ROUNDS; ++u) {
+      if (round + u >= to) break;
+      const int head = (round + u) * GROUPS + group;
+      Piece<T> x[CHUNKS];
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      Piece<T> p;
-      p.set(raw[u][k]);
+      for (int k = 0; k < CHUNKS; ++k) x[k].set(raw[u][k].w);
+      if constexpr (NORM) {
+        Piece<T> other[CHUNKS];
+        turn.partners(a, raw[u], x, other);
+        float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        x[k][j] = real ? p.x[j] : 0.0f;
-        y[k][j] = x[k][j];
-        sum = fmaf(x[k][j], x[k][j], sum);
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) sum = fmaf(x[k].x[j], x[k].x[j], sum);
+#pragma unroll
+        for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        const float r = rsqrtf(fmaf(sum, by_dim, a.eps));
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) x[k].x[j] = real ? fmaf(x[k].x[j], wc[k][j], other[k].x[j] * ws[k][j]) * r : 0.0f;
       }
-    }
-    if (a.norm && real) {  // all lanes: a group's rows may be of two kinds, a warp's groups too
-      const float r = 1.0f / sqrtf(lanes_sum<LANES>(sum) / (float)a.dim + a.eps);
-      float n[CHUNKS][V], z[CHUNKS][V];
+      float most = 0.0f;
+      if constexpr (CODES) {
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
+        for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) n[k][j] = x[k][j] * r * (which[u] == 1 ? weight[1][k][j] : weight[0][k][j]);
-      turn.apply(a, n, z);
+          for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(x[k].x[j]));
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) y[k][j] = turned ? z[k][j] : y[k][j];
-    }
-    float most = 0.0f;
-    const bool codes = a.to_cache && is_quantised(a.cache.type);
-    if (codes) {
-#pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(y[k][j]));
-#pragma unroll
-      for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-    }
-    if (which[u] < 0) continue;
-    if (which[u] == 0 || !a.to_cache) {
-      T *const out = static_cast<T *>(a.out[which[u]]) + (token * a.heads[which[u]] + head[u]) * a.dim;
-#pragma unroll
-      for (int k = 0; k < CHUNKS; ++k) {
-        const int i = (lane + k * LANES) * V;
-        Piece<T> p;
-#pragma unroll
-        for (int j = 0; j < V; ++j) p.x[j] = y[k][j];
-        if (i < a.dim) *reinterpret_cast<uint4 *>(out + i) = p.get();
+        for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
       }
-      continue;
-    }
-    if (first_row < 0) continue;
-    const int64_t row = first_row + head[u] * a.cache.page_size;
-    void *const store = which[u] == 1 ? a.cache.d_k : a.cache.d_v;
-    const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
-    if (codes && lane == 0) (which[u] == 1 ? a.cache.d_k_scale : a.cache.d_v_scale)[row] = scale_of(most, big);
+      if (head >= count) continue;
+      char *const to_row = out + head * out_stride;
+      if constexpr (CODES) {
+        const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+        if (lane == 0) scales[head * scale_stride] = scale_of(most, big);
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      const int i = (lane + k * LANES) * V;
-      if (i >= a.dim) continue;
-      if (codes) {
-        store_codes<V>(static_cast<char *>(store) + row * a.dim + i, y[k], by, a.cache.type);
+        for (int k = 0; k < CHUNKS; ++k)
+          if ((lane + k * LANES) * V < a.dim) store_codes<V>(to_row + (lane + k * LANES) * V, x[k].x, by, a.cache.type);
       } else {
-        Piece<T> p;
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.x[j] = y[k][j];
-        *reinterpret_cast<uint4 *>(static_cast<T *>(store) + row * a.dim + i) = p.get();
+        for (int k = 0; k < CHUNKS; ++k)
+          if ((lane + k * LANES) * V < a.dim) reinterpret_cast<uint4 *>(to_row)[lane + k * LANES] = x[k].get();
       }
     }
   }
 }
 
-// Backward: blocks take tokens a grid apart, a lane group rows of a token, and a lane keeps its share of the weights' gradients.
-// The lane groups of a block are added in order, the blocks by rotate_weights_kernel.
-template <typename T, int LANES, int CHUNKS, int ROWS>
-__global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a) {
-  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
-  __shared__ float shares[GROUPS][LANES * CHUNKS * V];
-  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  float weight[2][CHUNKS][V], dw[2][CHUNKS][V];
-  load_weights<T, LANES, CHUNKS>(a, 0, lane, weight[0]);
-  load_weights<T, LANES, CHUNKS>(a, 1, lane, weight[1]);
+// A warp takes `each` of the rounds of one token: those of the queries come first, then the keys', then the values'.  CACHE: keys
+// and values go to the cache, CODES: as codes.
+template <typename T, int LANES, int CHUNKS, bool NORM, bool CACHE, bool CODES>
+__global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES;
+  const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
+  if (token >= a.tokens) return;
+  const int lane = threadIdx.x % LANES;
+  int from = (int)(task % parts) * each, to = from + each;
+  const int64_t place = load_index(a.place, token, a.idx_bytes);
+  const bool real = !NORM || (place >= 0 && place < a.places);
+  Turn<T, LANES, CHUNKS> turn;
+  int own[CHUNKS];
 #pragma unroll
-  for (int k = 0; k < CHUNKS; ++k)
+  for (int k = 0; k < CHUNKS; ++k) own[k] = lane + k * LANES;
+  if (NORM) turn.load(a, place, real, lane, false);
+  int64_t first_row = -1;
+  const int q_rounds = (a.heads[0] + GROUPS - 1) / GROUPS, k_rounds = (a.heads[1] + GROUPS - 1) / GROUPS;
+  if (CACHE && real && to > q_rounds) first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place, a.page_shift);
+  float wc[CHUNKS][V], ws[CHUNKS][V];
+#pragma unroll
+  for (int which = 0; which < (CACHE ? 3 : 2); ++which) {
+    const int rounds = which == 0 ? q_rounds : which == 1 ? k_rounds : (a.heads[2] + GROUPS - 1) / GROUPS;
+    if (from < rounds && to > 0 && (which == 0 || !CACHE || first_row >= 0)) {
+      if (NORM && which < 2) {
+        load_weights<T, CHUNKS>(a, which, own, wc);
+        load_weights<T, CHUNKS>(a, which, turn.from, ws);
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          float w[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            w[j] = a.interleaved ? wc[k][j ^ 1] : ws[k][j];
+            ws[k][j] = w[j] * turn.s[k][j];
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) wc[k][j] *= turn.c[k][j];
+        }
+      }
+      const int lo = max(from, 0), hi = min(to, rounds);
+      if (which == 0 || !CACHE) {
+        rotate_rows<T, LANES, CHUNKS, NORM, false>(a, a.in[which], token, a.heads[which], lo, hi, turn, wc, ws,
+                                                   static_cast<char *>(a.out[which]) + token * a.heads[which] * a.dim * sizeof(T),
+                                                   a.dim * sizeof(T), nullptr, 0, real);
+      } else {
+        const int size = CODES ? 1 : sizeof(T);
+        char *const store = static_cast<char *>(which == 1 ? a.cache.d_k : a.cache.d_v) + first_row * a.dim * size;
+        float *const scales = CODES ? (which == 1 ? a.cache.d_k_scale : a.cache.d_v_scale) + first_row : nullptr;
+        const int64_t stride = a.cache.page_size * a.dim * size;
+        if (which == 1) rotate_rows<T, LANES, CHUNKS, NORM, CODES>(a, a.in[1], token, a.heads[1], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true);
+        else rotate_rows<T, LANES, CHUNKS, false, CODES>(a, a.in[2], token, a.heads[2], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true);
+      }
+    }
+    from -= rounds;
+    to -= rounds;
+  }
+}
+
+// Backward: warps take tokens a grid apart and keep their share of the weights' gradients in registers.  The warps' lane groups
+// are added in order by the block, the blocks by rotate_weights_kernel.
+template <typename T, int LANES, int CHUNKS>
+__global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 2 : 1;
+  __shared__ float shares[ROW_THREADS / LANES][LANES * CHUNKS * V];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
+  int own[CHUNKS];
+  float dw[2][CHUNKS][V];
+#pragma unroll
+  for (int k = 0; k < CHUNKS; ++k) {
+    own[k] = lane + k * LANES;
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[0][k][j] = dw[1][k][j] = 0.0f;
-  const int all = a.heads[0] + a.heads[1];
-  for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) {
+  }
+  const float by_dim = 1.0f / (float)a.dim;
+  const int64_t tasks = a.tokens * parts;
+  for (int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32; task < tasks; task += (int64_t)gridDim.x * ROW_WARPS) {
+    const int64_t token = task / parts;
+    int from = (int)(task - token * parts) * each, to = from + each;
     const int64_t place = load_index(a.place, token, a.idx_bytes);
     const bool real = place >= 0 && place < a.places;
     Turn<T, LANES, CHUNKS> turn;
-    turn.load(a, real ? place : 0, lane, true);
-    for (int row0 = 0; row0 < all; row0 += GROUPS * ROWS) {
-      uint4 raw[ROWS][2][CHUNKS];
+    turn.load(a, place, real, lane, true);
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int row = row0 + u * GROUPS + group, which = row >= a.heads[0], head = row - (which ? a.heads[0] : 0);
-        const T *const x = static_cast<const T *>(a.in[which].d) + token * a.in[which].token_stride + head * a.in[which].head_stride;
-        const T *const dy = static_cast<const T *>(a.grad[which].d) + token * a.grad[which].token_stride + head * a.grad[which].head_stride;
+    for (int which = 0; which < 2; ++which) {
+      const int rounds = (a.heads[which] + GROUPS - 1) / GROUPS, lo = max(from, 0), hi = min(to, rounds);
+      from -= rounds;
+      to -= rounds;
+      if (lo >= hi) continue;
+      float weight[CHUNKS][V];
+      load_weights<T, CHUNKS>(a, which, own, weight);
+      const T *const xs = static_cast<const T *>(a.in[which].d) + token * a.in[which].token_stride + lane * V;
+      const T *const dys = static_cast<const T *>(a.grad[which].d) + token * a.grad[which].token_stride + lane * V;
+      T *const dxs = static_cast<T *>(a.out[which]) + token * a.heads[which] * a.dim;
+      for (int round = lo; round < hi; round += ROUNDS) {
+        Raw raw[ROUNDS][2][CHUNKS];
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          const int i = (lane + k * LANES) * V;
-          const bool in = row < all && i < a.dim && real;
-          raw[u][0][k] = in ? *reinterpret_cast<const uint4 *>(x + i) : make_uint4(0, 0, 0, 0);
-          raw[u][1][k] = in ? *reinterpret_cast<const uint4 *>(dy + i) : make_uint4(0, 0, 0, 0);
-        }
-      }
+        for (int u = 0; u < ROUNDS; ++u) {
+          const int head = (round + u) * GROUPS + group;
 #pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        if (row0 + u * GROUPS >= all) break;
-        const int row = row0 + u * GROUPS + group, which = row >= a.heads[0], head = row - (which ? a.heads[0] : 0);
-        float x[CHUNKS][V], dy[CHUNKS][V], dn[CHUNKS][V];
-        float sum = 0.0f, inner = 0.0f;
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          Piece<T> p, q;
-          p.set(raw[u][0][k]);
-          q.set(raw[u][1][k]);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            x[k][j] = p.x[j];
-            dy[k][j] = q.x[j];
+          for (int k = 0; k < CHUNKS; ++k) {
+            const bool in = real && round + u < hi && head < a.heads[which] && own[k] * V < a.dim;
+            raw[u][0][k].load(xs + head * a.in[which].head_stride + k * LANES * V, in);
+            raw[u][1][k].load(dys + head * a.grad[which].head_stride + k * LANES * V, in);
           }
         }
-        turn.apply(a, dy, dn);
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
+        for (int u = 0; u < ROUNDS; ++u) {
+          if (round + u >= hi) break;
+          const int head = (round + u) * GROUPS + group;
+          Piece<T> x[CHUNKS], dn[CHUNKS], other[CHUNKS];
+          float sum = 0.0f, inner = 0.0f;
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            sum = fmaf(x[k][j], x[k][j], sum);
-            inner = fmaf(dn[k][j] * (which ? weight[1][k][j] : weight[0][k][j]), x[k][j], inner);
+          for (int k = 0; k < CHUNKS; ++k) {
+            x[k].set(raw[u][0][k].w);
+            dn[k].set(raw[u][1][k].w);
           }
+          turn.partners(a, raw[u][1], dn, other);
 #pragma unroll
-        for (int d = LANES / 2; d > 0; d /= 2) {
-          sum += __shfl_xor_sync(0xffffffffu, sum, d);
-          inner += __shfl_xor_sync(0xffffffffu, inner, d);
-        }
-        const float r = 1.0f / sqrtf(sum / (float)a.dim + a.eps), back = inner / (float)a.dim * r * r;
-        T *const out = static_cast<T *>(a.out[which]) + (token * a.heads[which] + head) * a.dim;
+          for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          const int i = (lane + k * LANES) * V;
-          Piece<T> p;
+            for (int j = 0; j < V; ++j) {
+              dn[k].x[j] = fmaf(dn[k].x[j], turn.c[k][j], other[k].x[j] * turn.s[k][j]);
+              sum = fmaf(x[k].x[j], x[k].x[j], sum);
+              other[k].x[j] = dn[k].x[j] * weight[k][j];  // g
+              inner = fmaf(other[k].x[j], x[k].x[j], inner);
+            }
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float t = dn[k][j] * x[k][j] * r;
-            if (which) dw[1][k][j] += t;
-            else dw[0][k][j] += t;
-            p.x[j] = r * (dn[k][j] * (which ? weight[1][k][j] : weight[0][k][j]) - x[k][j] * back);
+          for (int d = LANES / 2; d > 0; d /= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            inner += __shfl_xor_sync(0xffffffffu, inner, d);
           }
-          if (row < all && i < a.dim) *reinterpret_cast<uint4 *>(out + i) = p.get();
+          const float r = rsqrtf(fmaf(sum, by_dim, a.eps)), back = -inner * by_dim * r * r;
+#pragma unroll
+          for (int k = 0; k < CHUNKS; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float unit = x[k].x[j] * r;
+              dw[which][k][j] = fmaf(dn[k].x[j], unit, dw[which][k][j]);
+              x[k].x[j] = fmaf(other[k].x[j], r, unit * back);
+            }
+            if (head < a.heads[which] && own[k] * V < a.dim) reinterpret_cast<uint4 *>(dxs + head * a.dim)[own[k]] = x[k].get();
+          }
         }
       }
     }
@@ -645,68 +687,76 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-      for (int j = 0; j < V; ++j) shares[group][(lane + k * LANES) * V + j] = which ? dw[1][k][j] : dw[0][k][j];
+      for (int j = 0; j < V; ++j) shares[threadIdx.x / LANES][own[k] * V + j] = which ? dw[1][k][j] : dw[0][k][j];
     __syncthreads();
     for (int i = threadIdx.x; i < a.dim; i += ROW_THREADS) {
       float sum = 0.0f;
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) sum += shares[g][i];
+      for (int g = 0; g < ROW_THREADS / LANES; ++g) sum += shares[g][i];
       a.partial[((int64_t)blockIdx.x * 2 + which) * a.dim + i] = sum;
     }
   }
 }
 
-// Keys and values of listed tokens, a lane group a head of TOKENS tokens; the cache's rows are codes or T.
-template <typename T, int LANES, int CHUNKS, int TOKENS>
+// Keys and values of listed tokens: a warp takes `each` rounds of a token's heads; the cache's rows are codes or T.
+template <typename T, int LANES, int CHUNKS, bool CODES>
 __global__ void __launch_bounds__(ROW_THREADS)
-kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row, const void *place, T *k, T *v) {
-  constexpr int V = Piece<T>::V, GROUPS = ROW_THREADS / LANES;
-  const int lane = threadIdx.x % LANES, head = blockIdx.y * GROUPS + threadIdx.x / LANES;
-  if (head >= cache.heads) return;
-  const bool codes = is_quantised(cache.type);
-  const int dim = (int)cache.dim;
-  int64_t at[TOKENS];
+kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row,
+               const void *place, int page_shift, int parts, int each, T *k, T *v) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 4 : 2;
+  const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
+  if (token >= tokens) return;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES, dim = (int)cache.dim, heads = (int)cache.heads;
+  const int from = (int)(task % parts) * each, to = min(from + each, (heads + GROUPS - 1) / GROUPS);
+  const int64_t first = cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes), page_shift);
 #pragma unroll
-  for (int u = 0; u < TOKENS; ++u) {
-    const int64_t token = (int64_t)blockIdx.x * TOKENS + u;
-    at[u] = token < tokens ? cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes)) : -1;
-    if (at[u] >= 0) at[u] += head * cache.page_size;
-  }
-  Piece<T> got[TOKENS][2][CHUNKS];
+  for (int w = 0; w < 2; ++w) {
+    const char *const store = static_cast<const char *>(w == 0 ? cache.d_k : cache.d_v) + max(first, (int64_t)0) * dim * (CODES ? 1 : sizeof(T));
+    const float *const scales = CODES ? (w == 0 ? cache.d_k_scale : cache.d_v_scale) + max(first, (int64_t)0) : nullptr;
+    T *const out = (w == 0 ? k : v) + token * heads * dim;
+    for (int round = from; round < to; round += ROUNDS) {
+      Raw raw[ROUNDS][CHUNKS];
+      float scale[ROUNDS];
 #pragma unroll
-  for (int u = 0; u < TOKENS; ++u)
+      for (int u = 0; u < ROUNDS; ++u) {
+        const int head = (round + u) * GROUPS + group;
+        const bool in = first >= 0 && round + u < to && head < heads;
+        const int64_t at = head * cache.page_size;
+        if (CODES) scale[u] = in ? scales[at] : 0.0f;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const void *const store = w == 0 ? cache.d_k : cache.d_v;
-      float scale = 1.0f;
-      if (codes && at[u] >= 0) scale = (w == 0 ? cache.d_k_scale : cache.d_v_scale)[at[u]];
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int i = (lane + c * LANES) * V;
+          if constexpr (!CODES) {
+            raw[u][c].load(store + (at * dim + i) * (int)sizeof(T), in && i < dim);
+          } else {
+            uint2 x = make_uint2(0, 0);
+            if (in && i < dim) {
+              if constexpr (V == 8) x = *reinterpret_cast<const uint2 *>(store + at * dim + i);
+              else x.x = *reinterpret_cast<const uint32_t *>(store + at * dim + i);
+            }
+            raw[u][c].w[0] = x.x;
+            raw[u][c].w[1] = x.y;
+          }
+        }
+      }
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const int i = (lane + c * LANES) * V;
-        Piece<T> &p = got[u][w][c];
+      for (int u = 0; u < ROUNDS; ++u) {
+        const int head = (round + u) * GROUPS + group;
+        if (round + u >= to || head >= heads) continue;
 #pragma unroll
-        for (int j = 0; j < V; ++j) p.x[j] = 0.0f;
-        if (at[u] < 0 || i >= dim) continue;
-        if (codes) {
-          load_codes<V>(p.x, static_cast<const char *>(store) + at[u] * dim + i, cache.type);
-#pragma unroll
-          for (int j = 0; j < V; ++j) p.x[j] *= scale;
-        } else {
-          p.set(*reinterpret_cast<const uint4 *>(static_cast<const T *>(store) + at[u] * dim + i));
+        for (int c = 0; c < CHUNKS; ++c) {
+          if ((lane + c * LANES) * V >= dim) continue;
+          uint4 *const to_piece = reinterpret_cast<uint4 *>(out + head * dim) + lane + c * LANES;
+          if constexpr (CODES) {
+            Piece<T> p;
+            values_of<V>(p.x, make_uint2(raw[u][c].w[0], raw[u][c].w[1]), scale[u], cache.type);
+            *to_piece = p.get();
+          } else {
+            *to_piece = make_uint4(raw[u][c].w[0], raw[u][c].w[1], raw[u][c].w[2], raw[u][c].w[3]);
+          }
         }
       }
     }
-#pragma unroll
-  for (int u = 0; u < TOKENS; ++u) {
-    const int64_t token = (int64_t)blockIdx.x * TOKENS + u;
-    if (token >= tokens) break;
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const int i = (lane + c * LANES) * V;
-        if (i < dim) *reinterpret_cast<uint4 *>((w == 0 ? k : v) + (token * cache.heads + head) * dim + i) = got[u][w][c].get();
-      }
   }
 }
 
@@ -809,8 +859,24 @@ static int with_lanes(int dim, F run) {
   return run(integral_constant<int, 32>(), integral_constant<int, 1>());
 }
 
+// How the rounds of a token are shared out: few tokens are cut into parts, down to a round, so that there are eight warps' work for
+// every SM's scheduler; many are walked by one warp each.
+struct Parts {
+  int parts, each;
+  unsigned blocks;
+};
+static Parts parts_of(int64_t tokens, int rounds) {
+  const int64_t wanted = 32LL * sm_count();
+  Parts p;
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, (wanted + tokens - 1) / tokens));
+  p.each = (rounds + p.parts - 1) / p.parts;
+  p.parts = (rounds + p.each - 1) / p.each;
+  p.blocks = (unsigned)((tokens * p.parts + ROW_WARPS - 1) / ROW_WARPS);
+  return p;
+}
+
 static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
-  const int64_t heads = a.heads[0] + a.heads[1] + a.heads[2], rows = a.tokens * heads;
+  const int64_t rows = a.tokens * (a.heads[0] + a.heads[1] + a.heads[2]);
   if (rows == 0) return LAPIS_OK;
   return with_type(type, [&](auto t) {
     using T = decltype(t);
@@ -820,14 +886,15 @@ static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
       return (int)LAPIS_OK;
     }
     return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = ROW_THREADS / LANES;
-      // few tokens: a block for each round of rows
-      if (a.tokens * heads <= (int64_t)GROUPS * 4 * sm_count()) {
-        rotate_kernel<T, LANES, CHUNKS, 1><<<dim3((unsigned)a.tokens, (unsigned)((heads + GROUPS - 1) / GROUPS)), ROW_THREADS, 0, st>>>(a);
-      } else {
-        constexpr int ROWS = CHUNKS == 1 ? 4 : 2;
-        rotate_kernel<T, LANES, CHUNKS, ROWS><<<dim3((unsigned)a.tokens, (unsigned)((heads + GROUPS * ROWS - 1) / (GROUPS * ROWS))), ROW_THREADS, 0, st>>>(a);
-      }
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+      int rounds = 0;
+      for (int heads : a.heads) rounds += (heads + GROUPS - 1) / GROUPS;
+      const Parts p = parts_of(a.tokens, rounds);
+      if (!a.to_cache) rotate_kernel<T, LANES, CHUNKS, true, false, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (a.norm && is_quantised(a.cache.type)) rotate_kernel<T, LANES, CHUNKS, true, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (a.norm) rotate_kernel<T, LANES, CHUNKS, true, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (is_quantised(a.cache.type)) rotate_kernel<T, LANES, CHUNKS, false, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else rotate_kernel<T, LANES, CHUNKS, false, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });
@@ -836,22 +903,27 @@ static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
 
 // Launches the backward kernel that fits and leaves in *blocks how many shares of the weights' gradients there are.
 static int launch_backward(int type, RotateArgs &a, PoolBuf &partial, int *blocks, cudaStream_t st) {
-  const bool pieces = pieces_fit(type, a, true);
-  const int most = 8 * sm_count();
-  *blocks = (int)std::min<int64_t>(pieces ? a.tokens : (a.tokens + ROW_WARPS - 1) / ROW_WARPS, most);
-  LAPIS_TRY(partial.alloc((size_t)*blocks * 2 * a.dim * sizeof(float), st));
-  a.partial = static_cast<float *>(partial.p);
-  if (*blocks == 0) return LAPIS_OK;
+  const int64_t most = 5LL * sm_count();  // what is resident at 96 registers a thread
   return with_type(type, [&](auto t) {
     using T = decltype(t);
-    if (!pieces) {
-      rotate_any_backward_kernel<T><<<*blocks, ROW_THREADS, 0, st>>>(a);
+    auto room = [&](int64_t wanted) {
+      *blocks = (int)std::min(wanted, most);
+      const int status = partial.alloc((size_t)*blocks * 2 * a.dim * sizeof(float), st);
+      a.partial = static_cast<float *>(partial.p);
+      return status;
+    };
+    if (!pieces_fit(type, a, true)) {
+      LAPIS_TRY(room((a.tokens + ROW_WARPS - 1) / ROW_WARPS));
+      if (*blocks > 0) rotate_any_backward_kernel<T><<<*blocks, ROW_THREADS, 0, st>>>(a);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     }
     return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value;
-      rotate_backward_kernel<T, LANES, CHUNKS, CHUNKS == 1 ? 2 : 1><<<*blocks, ROW_THREADS, 0, st>>>(a);
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+      const int rounds = (a.heads[0] + GROUPS - 1) / GROUPS + (a.heads[1] + GROUPS - 1) / GROUPS;
+      const Parts p = a.tokens > 0 && rounds > 0 ? parts_of(a.tokens, rounds) : Parts{1, 1, 0};
+      LAPIS_TRY(room(p.blocks));
+      if (*blocks > 0) rotate_backward_kernel<T, LANES, CHUNKS><<<*blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });
@@ -922,8 +994,7 @@ extern "C" int lapis_b200_qk_norm_rope_backward(int type, int64_t tokens, int64_
   int blocks = 0;
   PoolBuf partial;
   LAPIS_TRY(launch_backward(type, a, partial, &blocks, st));
-  rotate_weights_kernel<<<dim3((unsigned)((dim + 31) / 32), 2), dim3(32, 32), 0, st>>>(a.partial, blocks, (int)dim, d_q_weight_grad, d_k_weight_grad);
-  LAPIS_CUDA_TRY(cudaGetLastError());
+  LAPIS_CUDA_TRY(launch_pdl(rotate_weights_kernel, dim3((unsigned)((dim + 31) / 32), 2), 1024, 0, st, a.partial, blocks, (int)dim, d_q_weight_grad, d_k_weight_grad));
   return LAPIS_OK;
 }
 
@@ -960,6 +1031,7 @@ extern "C" int lapis_b200_kv_append(int type, int64_t tokens, const lapis_b200_h
   a.row = d_row;
   a.to_cache = 1;
   a.cache = *cache;
+  a.page_shift = page_shift_of(cache->page_size);
   a.lists = *lists;
   return launch_rotate(type, a, as_stream(stream));
 }
@@ -986,14 +1058,13 @@ extern "C" int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_
       return (int)LAPIS_OK;
     }
     return with_lanes<T>((int)cache->dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = ROW_THREADS / LANES;
-      const unsigned rounds = (unsigned)((cache->heads + GROUPS - 1) / GROUPS);
-      if (tokens * rounds <= 8LL * sm_count()) {
-        kv_read_kernel<T, LANES, CHUNKS, 1><<<dim3((unsigned)tokens, rounds), ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, k, v);
-      } else {
-        constexpr int TOKENS = CHUNKS == 1 ? 4 : 2;
-        kv_read_kernel<T, LANES, CHUNKS, TOKENS><<<dim3((unsigned)((tokens + TOKENS - 1) / TOKENS), rounds), ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, k, v);
-      }
+      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+      const Parts p = parts_of(tokens, (int)((cache->heads + GROUPS - 1) / GROUPS));
+      const int shift = page_shift_of(cache->page_size);
+      if (is_quantised(cache->type))
+        kv_read_kernel<T, LANES, CHUNKS, true><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
+      else
+        kv_read_kernel<T, LANES, CHUNKS, false><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });

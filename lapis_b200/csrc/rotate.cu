@@ -256,11 +256,68 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
 // ---- whole 16 bytes ---------------------------------------------------------------
 //
 // Bound by memory: every element is read and written once, so what a row costs in instructions has to stay small next to the
-// 0.7 pieces of 16 bytes that an SM can read and write in a cycle.  A row is held by LANES neighbouring lanes, CHUNKS pieces
-// each; a warp holds 32 / LANES rows at a time and walks the rows of a token, so that the token's line of the tables, the
-// weights and the place in the cache are looked up once for many rows.  Weight and rotation are one product each with a row's
-// own piece and its partner's: y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin, and the partner's piece comes by a shuffle of
-// the row as it was read, while the sum of squares is still under way.
+// 0.7 pieces of 16 bytes that an SM can read and write in a cycle, and enough has to be on its way.  A row is held by LANES
+// neighbouring lanes, CHUNKS pieces each; a warp holds 32 / LANES rows at a time (a round) and walks the rows of a token, so
+// that the token's line of the tables, the weights and the place in the cache are looked up once for many rows.  Rows come by
+// cp.async, DEPTH rounds ahead, into a ring that only this warp uses: what is on its way takes no registers, and the partner's
+// piece of the rotation is there too.  Weight and rotation are one product each with a row's own piece and its partner's:
+// y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin.
+
+__device__ __forceinline__ uint32_t shared_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes on their way to shared memory, zeros where there is nothing.
+__device__ __forceinline__ void bring(uint32_t to, const void *from, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void brought() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_for_all_but() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Two products and sums in 32 bits by one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// The same for all of a piece, or of any even number of floats.
+template <int N>
+__device__ __forceinline__ void fma_all(float (&d)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 r = fma2({a[j], a[j + 1]}, {b[j], b[j + 1]}, {c[j], c[j + 1]});
+    d[j] = r.x;
+    d[j + 1] = r.y;
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_all(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 r = mul2({a[j], a[j + 1]}, {b[j], b[j + 1]});
+    d[j] = r.x;
+    d[j + 1] = r.y;
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_all(float (&d)[N], const float (&a)[N], float b) {
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    const float2 r = mul2({a[j], a[j + 1]}, {b, b});
+    d[j] = r.x;
+    d[j + 1] = r.y;
+  }
+}
 
 template <typename T>
 struct Piece {
@@ -280,6 +337,11 @@ struct Piece {
         x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
+  }
+  __device__ __forceinline__ void take(uint32_t at) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    set(w);
   }
   __device__ __forceinline__ uint4 get() const {
     uint32_t w[4];
@@ -419,28 +481,16 @@ struct Turn {
       }
     }
   }
-  // x' of a row's pieces; all lanes of the warp take part.
-  __device__ __forceinline__ void partners(const RotateArgs &a, const Raw (&raw)[CHUNKS], const Piece<T> (&x)[CHUNKS], Piece<T> (&other)[CHUNKS]) const {
-    if (a.interleaved) {
-#pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-        for (int j = 0; j < V; ++j) other[k].x[j] = x[k].x[j ^ 1];
-      return;
-    }
+  // x' of a row's pieces, the row being in shared memory from `row` on.
+  __device__ __forceinline__ void partners(const RotateArgs &a, uint32_t row, const Piece<T> (&x)[CHUNKS], Piece<T> (&other)[CHUNKS]) const {
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k) {
-      uint32_t w[4];
+      if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = __shfl_sync(0xffffffffu, raw[0].w[i], from[k] % LANES, LANES);
-#pragma unroll
-        for (int q = 1; q < CHUNKS; ++q) {
-          const uint32_t there = __shfl_sync(0xffffffffu, raw[q].w[i], from[k] % LANES, LANES);
-          w[i] = from[k] / LANES == q ? there : w[i];
-        }
+        for (int j = 0; j < V; ++j) other[k].x[j] = x[k].x[j ^ 1];
+      } else {
+        other[k].take(row + from[k] * 16);
       }
-      other[k].set(w);
     }
   }
 };
@@ -468,129 +518,208 @@ __device__ __forceinline__ void load_weights(const RotateArgs &a, int which, con
   }
 }
 
-// Rounds [from, to) of a warp's rows of one kind: `count` heads, GROUPS at a time, ROUNDS loads in flight.
-template <typename T, int LANES, int CHUNKS, bool NORM, bool CODES>
-__device__ __forceinline__ void rotate_rows(const RotateArgs &a, const Rows &in, int64_t token, int count, int from, int to,
-                                            const Turn<T, LANES, CHUNKS> &turn, const float (&wc)[CHUNKS][Piece<T>::V],
-                                            const float (&ws)[CHUNKS][Piece<T>::V], char *out, int64_t out_stride, float *scales,
-                                            int64_t scale_stride, bool real) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 4 : 2;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
-  const T *const rows = static_cast<const T *>(in.d) + token * in.token_stride + lane * V;
-  const float by_dim = 1.0f / (float)a.dim;
-  for (int round = from; round < to; round += ROUNDS) {
-    Raw raw[ROUNDS][CHUNKS];
+// The rows of a token that a warp walks, kind by kind, as they are sent on their way: KINDS kinds of ARRAYS arrays each.
+template <typename T, int LANES, int CHUNKS, int KINDS, int ARRAYS>
+struct Supply {
+  static constexpr int GROUPS = 32 / LANES, BYTES = CHUNKS * 512;  // of an array's round
+  const char *at[ARRAYS];
+  int64_t step[ARRAYS];
+  int kind, round, rounds, head, heads, left;
+  uint32_t to;
+
+  __device__ __forceinline__ void enter(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token) {
+    const int lane = threadIdx.x % LANES;
+    heads = a.heads[kind];
+    rounds = (heads + GROUPS - 1) / GROUPS;
+    head = round * GROUPS + threadIdx.x % 32 / LANES;
 #pragma unroll
-    for (int u = 0; u < ROUNDS; ++u) {
-      const int head = (round + u) * GROUPS + group;
+    for (int i = 0; i < ARRAYS; ++i) {
+      const Rows &r = rows[i][kind];
+      at[i] = static_cast<const char *>(r.d) + (token * r.token_stride + head * r.head_stride) * (int)sizeof(T) + lane * 16;
+      step[i] = GROUPS * r.head_stride * (int)sizeof(T);
+    }
+  }
+  // Round `from` of all of them is the first one.
+  __device__ __forceinline__ void begin(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token, int from, int count, uint32_t ring) {
+    round = from;
+    left = count;
+    to = ring + threadIdx.x % 32 * 16;
+    for (kind = 0; kind < KINDS - 1; ++kind) {
+      const int n = (a.heads[kind] + GROUPS - 1) / GROUPS;
+      if (round < n) break;
+      round -= n;
+    }
+    enter(a, rows, token);
+  }
+  // Sends the next round to slot `slot` of the ring; commits in any case.
+  __device__ __forceinline__ void send(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token, int slot) {
+    if (left > 0) {
+      --left;
+#pragma unroll
+      for (int i = 0; i < ARRAYS; ++i) {
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          const bool in = head < heads && (threadIdx.x % LANES + k * LANES) * Piece<T>::V < a.dim;
+          // a row's chunks lie behind one another in shared memory too
+          const uint32_t place = CHUNKS == 1 ? to : to + k * LANES * 16 + threadIdx.x % 32 / LANES * (CHUNKS - 1) * LANES * 16;
+          bring(place + (slot * ARRAYS + i) * BYTES, in ? at[i] + k * LANES * 16 : rows[i][kind].d, in);
+        }
+        at[i] += step[i];
+      }
+      head += GROUPS;
+      if (++round == rounds && left > 0) {
+        do {
+          round = 0;
+          ++kind;
+          enter(a, rows, token);
+        } while (rounds == 0);
+      }
+    }
+    brought();
+  }
+};
+
+// Rounds [from, to) of one kind: the rows come out of the ring, results go to `out`.
+template <typename T, int LANES, int CHUNKS, int DEPTH, bool NORM, bool CODES, typename Next>
+__device__ __forceinline__ void rotate_rows(const RotateArgs &a, int count, int from, int to, const Turn<T, LANES, CHUNKS> &turn,
+                                            const float (&wc)[CHUNKS][Piece<T>::V], const float (&ws)[CHUNKS][Piece<T>::V], char *out,
+                                            int64_t out_stride, float *scales, int64_t scale_stride, bool real, uint32_t ring, int &slot, Next next) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, BYTES = CHUNKS * 512;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
+  const float by_dim = 1.0f / (float)a.dim;
+  int head = from * GROUPS + group;
+  out += head * out_stride + (CODES ? lane * V : lane * 16);
+  const uint32_t mine = ring + group * LANES * CHUNKS * 16;
+  for (int round = from; round < to; ++round) {
+    wait_for_all_but<DEPTH - 1>();
+    __syncwarp();
+    const uint32_t row = mine + slot * BYTES;
+    Piece<T> x[CHUNKS], other[CHUNKS];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) x[k].take(row + (lane + k * LANES) * 16);
+    if constexpr (NORM) turn.partners(a, row, x, other);
+    __syncwarp();
+    next(slot);
+    slot = slot + 1 == DEPTH ? 0 : slot + 1;
+    if constexpr (NORM) {
+      float pair[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int k = 0; k < CHUNKS; ++k)
-        raw[u][k].load(rows + head * in.head_stride + k * LANES * V, real && round + u < to && head < count && (lane + k * LANES) * V < a.dim);
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float2 r = fma2({x[k].x[j], x[k].x[j + 1]}, {x[k].x[j], x[k].x[j + 1]}, {pair[0], pair[1]});
+          pair[0] = r.x;
+          pair[1] = r.y;
+        }
+      float sum = pair[0] + pair[1];
+#pragma unroll
+      for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float r = rsqrtf(fmaf(sum, by_dim, a.eps));
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k) {
+        mul_all(other[k].x, other[k].x, ws[k]);
+        fma_all(x[k].x, x[k].x, wc[k], other[k].x);
+        mul_all(x[k].x, x[k].x, r);
+      }
+      if (!real) {
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+          for (int j = 0; j < V; ++j) x[k].x[j] = 0.0f;
+      }
     }
-#pragma unroll
-    for (int u = 0; u < ROUNDS; ++u) {
-      if (round + u >= to) break;
-      const int head = (round + u) * GROUPS + group;
-      Piece<T> x[CHUNKS];
-#pragma unroll
-      for (int k = 0; k < CHUNKS; ++k) x[k].set(raw[u][k].w);
-      if constexpr (NORM) {
-        Piece<T> other[CHUNKS];
-        turn.partners(a, raw[u], x, other);
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) sum = fmaf(x[k].x[j], x[k].x[j], sum);
-#pragma unroll
-        for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const float r = rsqrtf(fmaf(sum, by_dim, a.eps));
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) x[k].x[j] = real ? fmaf(x[k].x[j], wc[k][j], other[k].x[j] * ws[k][j]) * r : 0.0f;
-      }
+    if constexpr (CODES) {
       float most = 0.0f;
-      if constexpr (CODES) {
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
+      for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(x[k].x[j]));
+        for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(x[k].x[j]));
 #pragma unroll
-        for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-      }
-      if (head >= count) continue;
-      char *const to_row = out + head * out_stride;
-      if constexpr (CODES) {
-        const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+      for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+      const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+      if (head < count) {
         if (lane == 0) scales[head * scale_stride] = scale_of(most, big);
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k)
-          if ((lane + k * LANES) * V < a.dim) store_codes<V>(to_row + (lane + k * LANES) * V, x[k].x, by, a.cache.type);
-      } else {
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
-          if ((lane + k * LANES) * V < a.dim) reinterpret_cast<uint4 *>(to_row)[lane + k * LANES] = x[k].get();
+          if ((lane + k * LANES) * V < a.dim) store_codes<V>(out + k * LANES * V, x[k].x, by, a.cache.type);
       }
+    } else if (head < count) {
+#pragma unroll
+      for (int k = 0; k < CHUNKS; ++k)
+        if ((lane + k * LANES) * V < a.dim) reinterpret_cast<uint4 *>(out)[k * LANES] = x[k].get();
     }
+    head += GROUPS;
+    out += GROUPS * out_stride;
   }
 }
 
 // A warp takes `each` of the rounds of one token: those of the queries come first, then the keys', then the values'.  CACHE: keys
 // and values go to the cache, CODES: as codes.
 template <typename T, int LANES, int CHUNKS, bool NORM, bool CACHE, bool CODES>
-__global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES;
+__global__ void __launch_bounds__(ROW_THREADS, CHUNKS == 1 ? 8 : 5) rotate_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 8 / CHUNKS, BYTES = CHUNKS * 512, KINDS = CACHE ? 3 : 2;
+  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * BYTES];
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= a.tokens) return;
   const int lane = threadIdx.x % LANES;
-  int from = (int)(task % parts) * each, to = from + each;
+  const uint32_t ring = shared_at(rings[threadIdx.x / 32]);
+  int from = (int)(task - token * parts) * each, rounds[KINDS], all = 0;
+#pragma unroll
+  for (int which = 0; which < KINDS; ++which) all += rounds[which] = (a.heads[which] + GROUPS - 1) / GROUPS;
+  int to = min(from + each, all);
+  const Rows *const rows[1] = {a.in};
+  Supply<T, LANES, CHUNKS, KINDS, 1> supply;
+  supply.begin(a, rows, token, from, to - from, ring);
+#pragma unroll
+  for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, token, i);
   const int64_t place = load_index(a.place, token, a.idx_bytes);
   const bool real = !NORM || (place >= 0 && place < a.places);
-  Turn<T, LANES, CHUNKS> turn;
   int own[CHUNKS];
 #pragma unroll
   for (int k = 0; k < CHUNKS; ++k) own[k] = lane + k * LANES;
-  if (NORM) turn.load(a, place, real, lane, false);
   int64_t first_row = -1;
-  const int q_rounds = (a.heads[0] + GROUPS - 1) / GROUPS, k_rounds = (a.heads[1] + GROUPS - 1) / GROUPS;
-  if (CACHE && real && to > q_rounds) first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place, a.page_shift);
-  float wc[CHUNKS][V], ws[CHUNKS][V];
+  if (CACHE && real && to > rounds[0]) first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place, a.page_shift);
+  int slot = 0;
+  auto next = [&](int free) { supply.send(a, rows, token, free); };
 #pragma unroll
-  for (int which = 0; which < (CACHE ? 3 : 2); ++which) {
-    const int rounds = which == 0 ? q_rounds : which == 1 ? k_rounds : (a.heads[2] + GROUPS - 1) / GROUPS;
-    if (from < rounds && to > 0 && (which == 0 || !CACHE || first_row >= 0)) {
+  for (int which = 0; which < KINDS; ++which) {
+    if (from < rounds[which] && to > 0) {
+      if (CACHE && which > 0 && first_row < 0) {  // nowhere to write
+        wait_for_all_but<0>();
+        return;
+      }
+      float wc[CHUNKS][V], ws[CHUNKS][V];
+      Turn<T, LANES, CHUNKS> turn;
       if (NORM && which < 2) {
+        turn.load(a, place, real, lane, false);
         load_weights<T, CHUNKS>(a, which, own, wc);
         load_weights<T, CHUNKS>(a, which, turn.from, ws);
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
-          float w[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            w[j] = a.interleaved ? wc[k][j ^ 1] : ws[k][j];
-            ws[k][j] = w[j] * turn.s[k][j];
-          }
+          for (int j = 0; j < V; ++j) ws[k][j] = (a.interleaved ? wc[k][j ^ 1] : ws[k][j]) * turn.s[k][j];
 #pragma unroll
           for (int j = 0; j < V; ++j) wc[k][j] *= turn.c[k][j];
         }
       }
-      const int lo = max(from, 0), hi = min(to, rounds);
+      const int lo = max(from, 0), hi = min(to, rounds[which]);
       if (which == 0 || !CACHE) {
-        rotate_rows<T, LANES, CHUNKS, NORM, false>(a, a.in[which], token, a.heads[which], lo, hi, turn, wc, ws,
-                                                   static_cast<char *>(a.out[which]) + token * a.heads[which] * a.dim * sizeof(T),
-                                                   a.dim * sizeof(T), nullptr, 0, real);
+        rotate_rows<T, LANES, CHUNKS, DEPTH, NORM, false>(a, a.heads[which], lo, hi, turn, wc, ws,
+                                                          static_cast<char *>(a.out[which]) + token * a.heads[which] * a.dim * (int)sizeof(T),
+                                                          a.dim * (int)sizeof(T), nullptr, 0, real, ring, slot, next);
       } else {
         const int size = CODES ? 1 : sizeof(T);
         char *const store = static_cast<char *>(which == 1 ? a.cache.d_k : a.cache.d_v) + first_row * a.dim * size;
         float *const scales = CODES ? (which == 1 ? a.cache.d_k_scale : a.cache.d_v_scale) + first_row : nullptr;
         const int64_t stride = a.cache.page_size * a.dim * size;
-        if (which == 1) rotate_rows<T, LANES, CHUNKS, NORM, CODES>(a, a.in[1], token, a.heads[1], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true);
-        else rotate_rows<T, LANES, CHUNKS, false, CODES>(a, a.in[2], token, a.heads[2], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true);
+        if (which == 1)
+          rotate_rows<T, LANES, CHUNKS, DEPTH, NORM, CODES>(a, a.heads[1], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
+        else
+          rotate_rows<T, LANES, CHUNKS, DEPTH, false, CODES>(a, a.heads[2], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
       }
     }
-    from -= rounds;
-    to -= rounds;
+    from -= rounds[which];
+    to -= rounds[which];
   }
 }
 
@@ -598,9 +727,11 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_consta
 // are added in order by the block, the blocks by rotate_weights_kernel.
 template <typename T, int LANES, int CHUNKS>
 __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 2 : 1;
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 4 / CHUNKS, BYTES = CHUNKS * 512;
+  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 2 * BYTES];
   __shared__ float shares[ROW_THREADS / LANES][LANES * CHUNKS * V];
   const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
+  const uint32_t ring = shared_at(rings[threadIdx.x / 32]);
   int own[CHUNKS];
   float dw[2][CHUNKS][V];
 #pragma unroll
@@ -611,77 +742,87 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
   }
   const float by_dim = 1.0f / (float)a.dim;
   const int64_t tasks = a.tokens * parts;
+  const int rounds[2] = {(a.heads[0] + GROUPS - 1) / GROUPS, (a.heads[1] + GROUPS - 1) / GROUPS};
+  const Rows *const rows[2] = {a.in, a.grad};
   for (int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32; task < tasks; task += (int64_t)gridDim.x * ROW_WARPS) {
     const int64_t token = task / parts;
-    int from = (int)(task - token * parts) * each, to = from + each;
+    int from = (int)(task - token * parts) * each, to = min(from + each, rounds[0] + rounds[1]);
+    Supply<T, LANES, CHUNKS, 2, 2> supply;
+    supply.begin(a, rows, token, from, to - from, ring);
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, token, i);
     const int64_t place = load_index(a.place, token, a.idx_bytes);
     const bool real = place >= 0 && place < a.places;
     Turn<T, LANES, CHUNKS> turn;
     turn.load(a, place, real, lane, true);
+    int slot = 0;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const int rounds = (a.heads[which] + GROUPS - 1) / GROUPS, lo = max(from, 0), hi = min(to, rounds);
-      from -= rounds;
-      to -= rounds;
+      const int lo = max(from, 0), hi = min(to, rounds[which]);
+      from -= rounds[which];
+      to -= rounds[which];
       if (lo >= hi) continue;
       float weight[CHUNKS][V];
       load_weights<T, CHUNKS>(a, which, own, weight);
-      const T *const xs = static_cast<const T *>(a.in[which].d) + token * a.in[which].token_stride + lane * V;
-      const T *const dys = static_cast<const T *>(a.grad[which].d) + token * a.grad[which].token_stride + lane * V;
-      T *const dxs = static_cast<T *>(a.out[which]) + token * a.heads[which] * a.dim;
-      for (int round = lo; round < hi; round += ROUNDS) {
-        Raw raw[ROUNDS][2][CHUNKS];
+      int head = lo * GROUPS + group;
+      char *out = static_cast<char *>(a.out[which]) + (token * a.heads[which] + head) * a.dim * (int)sizeof(T) + lane * 16;
+      for (int round = lo; round < hi; ++round) {
+        wait_for_all_but<DEPTH - 1>();
+        __syncwarp();
+        const uint32_t row = ring + slot * 2 * BYTES + group * LANES * CHUNKS * 16;
+        Piece<T> x[CHUNKS], dn[CHUNKS], other[CHUNKS];
 #pragma unroll
-        for (int u = 0; u < ROUNDS; ++u) {
-          const int head = (round + u) * GROUPS + group;
+        for (int k = 0; k < CHUNKS; ++k) {
+          x[k].take(row + own[k] * 16);
+          dn[k].take(row + BYTES + own[k] * 16);
+        }
+        turn.partners(a, row + BYTES, dn, other);
+        __syncwarp();
+        supply.send(a, rows, token, slot);
+        slot = slot + 1 == DEPTH ? 0 : slot + 1;
+        float sum = 0.0f, inner = 0.0f;
 #pragma unroll
-          for (int k = 0; k < CHUNKS; ++k) {
-            const bool in = real && round + u < hi && head < a.heads[which] && own[k] * V < a.dim;
-            raw[u][0][k].load(xs + head * a.in[which].head_stride + k * LANES * V, in);
-            raw[u][1][k].load(dys + head * a.grad[which].head_stride + k * LANES * V, in);
+        for (int k = 0; k < CHUNKS; ++k) {
+          if (!real) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[k].x[j] = dn[k].x[j] = other[k].x[j] = 0.0f;
+          }
+          float square[V], product[V];
+          mul_all(other[k].x, other[k].x, turn.s[k]);
+          fma_all(dn[k].x, dn[k].x, turn.c[k], other[k].x);
+          mul_all(other[k].x, dn[k].x, weight[k]);  // g
+          mul_all(square, x[k].x, x[k].x);
+          mul_all(product, other[k].x, x[k].x);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            sum += square[j];
+            inner += product[j];
           }
         }
 #pragma unroll
-        for (int u = 0; u < ROUNDS; ++u) {
-          if (round + u >= hi) break;
-          const int head = (round + u) * GROUPS + group;
-          Piece<T> x[CHUNKS], dn[CHUNKS], other[CHUNKS];
-          float sum = 0.0f, inner = 0.0f;
-#pragma unroll
-          for (int k = 0; k < CHUNKS; ++k) {
-            x[k].set(raw[u][0][k].w);
-            dn[k].set(raw[u][1][k].w);
-          }
-          turn.partners(a, raw[u][1], dn, other);
-#pragma unroll
-          for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              dn[k].x[j] = fmaf(dn[k].x[j], turn.c[k][j], other[k].x[j] * turn.s[k][j]);
-              sum = fmaf(x[k].x[j], x[k].x[j], sum);
-              other[k].x[j] = dn[k].x[j] * weight[k][j];  // g
-              inner = fmaf(other[k].x[j], x[k].x[j], inner);
-            }
-#pragma unroll
-          for (int d = LANES / 2; d > 0; d /= 2) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            inner += __shfl_xor_sync(0xffffffffu, inner, d);
-          }
-          const float r = rsqrtf(fmaf(sum, by_dim, a.eps)), back = -inner * by_dim * r * r;
-#pragma unroll
-          for (int k = 0; k < CHUNKS; ++k) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const float unit = x[k].x[j] * r;
-              dw[which][k][j] = fmaf(dn[k].x[j], unit, dw[which][k][j]);
-              x[k].x[j] = fmaf(other[k].x[j], r, unit * back);
-            }
-            if (head < a.heads[which] && own[k] * V < a.dim) reinterpret_cast<uint4 *>(dxs + head * a.dim)[own[k]] = x[k].get();
-          }
+        for (int d = LANES / 2; d > 0; d /= 2) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          inner += __shfl_xor_sync(0xffffffffu, inner, d);
         }
+        const float r = rsqrtf(fmaf(sum, by_dim, a.eps)), back = -inner * by_dim * r * r;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+          mul_all(x[k].x, x[k].x, r);
+          fma_all(dw[which][k], dn[k].x, x[k].x, dw[which][k]);
+          mul_all(other[k].x, other[k].x, r);
+          mul_all(x[k].x, x[k].x, back);
+#pragma unroll
+          for (int j = 0; j < V; ++j) x[k].x[j] += other[k].x[j];
+          if (head < a.heads[which] && own[k] * V < a.dim) reinterpret_cast<uint4 *>(out)[k * LANES] = x[k].get();
+        }
+        head += GROUPS;
+        out += GROUPS * a.dim * (int)sizeof(T);
       }
     }
+    wait_for_all_but<0>();
+    __syncwarp();
   }
+  pdl_release();
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
 #pragma unroll

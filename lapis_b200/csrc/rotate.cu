@@ -257,11 +257,11 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
 //
 // Bound by memory: every element is read and written once, so what a row costs in instructions has to stay small next to the
 // 0.7 pieces of 16 bytes that an SM can read and write in a cycle, and enough has to be on its way.  A row is held by LANES
-// neighbouring lanes, CHUNKS pieces each; a warp holds 32 / LANES rows at a time (a round) and walks the rows of a token, so
-// that the token's line of the tables, the weights and the place in the cache are looked up once for many rows.  Rows come by
-// cp.async, DEPTH rounds ahead, into a ring that only this warp uses: what is on its way takes no registers, and the partner's
-// piece of the rotation is there too.  Weight and rotation are one product each with a row's own piece and its partner's:
-// y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin.
+// neighbouring lanes, two pieces each, so chosen that a value and its partner in the rotation are in one lane; a warp holds
+// 32 / LANES rows at a time (a round) and walks the rows of a token, so that the token's line of the tables, the weights and
+// the place in the cache are looked up once for many rows.  Rows come by cp.async, DEPTH rounds ahead, into a ring that every
+// lane uses for itself: what is on its way takes no registers.  Weight and rotation are one product each with a value and
+// its partner, y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin, two values an instruction.
 
 __device__ __forceinline__ uint32_t shared_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes on their way to shared memory, zeros where there is nothing.
@@ -323,7 +323,8 @@ template <typename T>
 struct Piece {
   static constexpr int V = 16 / sizeof(T);
   float x[V];
-  __device__ __forceinline__ void set(const uint32_t (&w)[4]) {
+  __device__ __forceinline__ void set(uint4 raw) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 4) {
@@ -339,8 +340,8 @@ struct Piece {
     }
   }
   __device__ __forceinline__ void take(uint32_t at) {
-    uint32_t w[4];
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+    uint4 w;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
     set(w);
   }
   __device__ __forceinline__ uint4 get() const {
@@ -358,17 +359,6 @@ struct Piece {
       }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-
-struct Raw {
-  uint32_t w[4];
-  __device__ __forceinline__ void load(const void *p, bool in) {
-    const uint4 x = in ? *static_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
-    w[0] = x.x;
-    w[1] = x.y;
-    w[2] = x.z;
-    w[3] = x.w;
   }
 };
 
@@ -402,10 +392,8 @@ __device__ __forceinline__ void values_of(float *x, uint2 raw, float scale, int 
     const uint32_t w = i == 0 ? raw.x : raw.y;
     if (type == LAPIS_I8) {
       const uint32_t u = w ^ 0x80808080u;
-      x[4 * i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)) - 8388736.0f;
-      x[4 * i + 1] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)) - 8388736.0f;
-      x[4 * i + 2] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7442)) - 8388736.0f;
-      x[4 * i + 3] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7443)) - 8388736.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + j)) - 8388736.0f;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; j += 2) {
@@ -415,7 +403,11 @@ __device__ __forceinline__ void values_of(float *x, uint2 raw, float scale, int 
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[4 * i + j] *= scale;
+    for (int j = 0; j < 4; j += 2) {
+      const float2 f = mul2({x[4 * i + j], x[4 * i + j + 1]}, {scale, scale});
+      x[4 * i + j] = f.x;
+      x[4 * i + j + 1] = f.y;
+    }
   }
 }
 
@@ -438,112 +430,100 @@ __device__ __forceinline__ void load_floats(float (&x)[N], const float *from) {
   }
 }
 
-// What a lane knows of the rotation: y_j = x_j c_j + x'_j s_j with x' the partners, which for neighbouring pairs are in the same
-// piece and for pairs of halves in piece `from`.  Pieces that are not turned have cosine 1 and sine 0.
-template <typename T, int LANES, int CHUNKS>
+// The two pieces of a row that a lane holds: the halves of pairs, and what is not turned two by two.
+template <typename T, int LANES>
+struct Pieces {
+  static constexpr int V = Piece<T>::V;
+  int at[2];
+  bool in[2], turned;
+  __device__ __forceinline__ Pieces(int dim, int half) {
+    const int lane = threadIdx.x % LANES, apart = half / V;
+    turned = lane < apart;
+    at[0] = turned ? lane : 2 * lane;
+    at[1] = turned ? lane + apart : 2 * lane + 1;
+    in[0] = at[0] * V < dim;
+    in[1] = at[1] * V < dim;
+  }
+};
+
+// Cosines and sines of a lane's V pairs: (piece 0, piece 1) value by value, or, interleaved, neighbours in piece 0, then in piece 1.
+template <typename T, int LANES>
 struct Turn {
   static constexpr int V = Piece<T>::V;
-  float c[CHUNKS][V], s[CHUNKS][V];
-  int from[CHUNKS];
-
-  // back: the other way round, for gradients.
-  __device__ __forceinline__ void load(const RotateArgs &a, int64_t place, bool real, int lane, bool back) {
+  float c[V], s[V];
+  __device__ __forceinline__ void load(const RotateArgs &a, const Pieces<T, LANES> &p, int64_t place, bool real) {
     const int half = a.rot / 2;
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      const int piece = lane + k * LANES, i = piece * V;
-      from[k] = piece;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        c[k][j] = 1.0f;
-        s[k][j] = 0.0f;
-      }
-      if (i >= a.rot || !real) continue;
-      const bool second = !a.interleaved && i >= half;
-      const float *const cs = a.cos + place * half + (a.interleaved ? i / 2 : second ? i - half : i);
-      const float *const sn = a.sin + (cs - a.cos);
-      // first of a pair: a cos - b sin; second: b cos + a sin
-      if (a.interleaved) {
-        float ct[V / 2], st[V / 2];
-        load_floats(ct, cs);
-        load_floats(st, sn);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          c[k][j] = ct[j / 2];
-          s[k][j] = (j % 2 == 1) != back ? st[j / 2] : -st[j / 2];
-        }
-      } else {
-        from[k] = second ? piece - half / V : piece + half / V;
-        load_floats(c[k], cs);
-        load_floats(s[k], sn);
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[k][j] = second != back ? s[k][j] : -s[k][j];
-      }
+    for (int j = 0; j < V; ++j) {
+      c[j] = 1.0f;
+      s[j] = 0.0f;
     }
-  }
-  // x' of a row's pieces, the row being in shared memory from `row` on.
-  __device__ __forceinline__ void partners(const RotateArgs &a, uint32_t row, const Piece<T> (&x)[CHUNKS], Piece<T> (&other)[CHUNKS]) const {
+    if (!real) return;
+    const int64_t line = place * half;
+    if (!a.interleaved) {
+      if (!p.turned) return;
+      load_floats(c, a.cos + line + p.at[0] * V);
+      load_floats(s, a.sin + line + p.at[0] * V);
+      return;
+    }
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-      if (a.interleaved) {
+    for (int k = 0; k < 2; ++k) {
+      if (p.at[k] * V >= a.rot) continue;
+      float ct[V / 2], st[V / 2];
+      load_floats(ct, a.cos + line + p.at[k] * (V / 2));
+      load_floats(st, a.sin + line + p.at[k] * (V / 2));
 #pragma unroll
-        for (int j = 0; j < V; ++j) other[k].x[j] = x[k].x[j ^ 1];
-      } else {
-        other[k].take(row + from[k] * 16);
+      for (int j = 0; j < V / 2; ++j) {
+        c[k * (V / 2) + j] = ct[j];
+        s[k * (V / 2) + j] = st[j];
       }
     }
   }
 };
 
-// The weights of a lane's pieces, or of the partners'.
-template <typename T, int CHUNKS>
-__device__ __forceinline__ void load_weights(const RotateArgs &a, int which, const int (&piece)[CHUNKS], float (&w)[CHUNKS][Piece<T>::V]) {
+template <typename T, int LANES>
+__device__ __forceinline__ void load_weights(const RotateArgs &a, int which, const Pieces<T, LANES> &p, float (&w)[2][Piece<T>::V]) {
   constexpr int V = Piece<T>::V;
 #pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) {
-    const int i = piece[k] * V;
+  for (int k = 0; k < 2; ++k) {
 #pragma unroll
     for (int j = 0; j < V; ++j) w[k][j] = 0.0f;
-    if (i >= a.dim) continue;
+    if (!p.in[k]) continue;
     if (a.weight_f32) {
-      load_floats(w[k], static_cast<const float *>(a.weight[which]) + i);
+      load_floats(w[k], static_cast<const float *>(a.weight[which]) + p.at[k] * V);
     } else {
-      Raw raw;
-      Piece<T> p;
-      raw.load(static_cast<const T *>(a.weight[which]) + i, true);
-      p.set(raw.w);
+      Piece<T> x;
+      x.set(*reinterpret_cast<const uint4 *>(static_cast<const T *>(a.weight[which]) + p.at[k] * V));
 #pragma unroll
-      for (int j = 0; j < V; ++j) w[k][j] = p.x[j];
+      for (int j = 0; j < V; ++j) w[k][j] = x.x[j];
     }
   }
 }
 
-// The rows of a token that a warp walks, kind by kind, as they are sent on their way: KINDS kinds of ARRAYS arrays each.
-template <typename T, int LANES, int CHUNKS, int KINDS, int ARRAYS>
+// The rows of a token that a warp walks, kind by kind, as they are sent on their way: KINDS kinds of ARRAYS arrays each.  A
+// lane's pieces lie at slot * 1024 * ARRAYS + i * 1024 + k * 512 of its place in the ring.
+template <typename T, int LANES, int KINDS, int ARRAYS>
 struct Supply {
-  static constexpr int GROUPS = 32 / LANES, BYTES = CHUNKS * 512;  // of an array's round
+  static constexpr int GROUPS = 32 / LANES;
   const char *at[ARRAYS];
   int64_t step[ARRAYS];
   int kind, round, rounds, head, heads, left;
-  uint32_t to;
 
   __device__ __forceinline__ void enter(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token) {
-    const int lane = threadIdx.x % LANES;
     heads = a.heads[kind];
     rounds = (heads + GROUPS - 1) / GROUPS;
     head = round * GROUPS + threadIdx.x % 32 / LANES;
 #pragma unroll
     for (int i = 0; i < ARRAYS; ++i) {
       const Rows &r = rows[i][kind];
-      at[i] = static_cast<const char *>(r.d) + (token * r.token_stride + head * r.head_stride) * (int)sizeof(T) + lane * 16;
+      at[i] = static_cast<const char *>(r.d) + (token * r.token_stride + head * r.head_stride) * (int)sizeof(T);
       step[i] = GROUPS * r.head_stride * (int)sizeof(T);
     }
   }
   // Round `from` of all of them is the first one.
-  __device__ __forceinline__ void begin(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token, int from, int count, uint32_t ring) {
+  __device__ __forceinline__ void begin(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token, int from, int count) {
     round = from;
     left = count;
-    to = ring + threadIdx.x % 32 * 16;
     for (kind = 0; kind < KINDS - 1; ++kind) {
       const int n = (a.heads[kind] + GROUPS - 1) / GROUPS;
       if (round < n) break;
@@ -551,19 +531,14 @@ struct Supply {
     }
     enter(a, rows, token);
   }
-  // Sends the next round to slot `slot` of the ring; commits in any case.
-  __device__ __forceinline__ void send(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], int64_t token, int slot) {
+  // Sends the next round to `to`, this lane's place in a slot of the ring; commits in any case.
+  __device__ __forceinline__ void send(const RotateArgs &a, const Rows *const (&rows)[ARRAYS], const Pieces<T, LANES> &p, int64_t token, uint32_t to) {
     if (left > 0) {
       --left;
 #pragma unroll
       for (int i = 0; i < ARRAYS; ++i) {
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          const bool in = head < heads && (threadIdx.x % LANES + k * LANES) * Piece<T>::V < a.dim;
-          // a row's chunks lie behind one another in shared memory too
-          const uint32_t place = CHUNKS == 1 ? to : to + k * LANES * 16 + threadIdx.x % 32 / LANES * (CHUNKS - 1) * LANES * 16;
-          bring(place + (slot * ARRAYS + i) * BYTES, in ? at[i] + k * LANES * 16 : rows[i][kind].d, in);
-        }
+        for (int k = 0; k < 2; ++k) bring(to + i * 1024 + k * 512, at[i] + (head < heads && p.in[k] ? p.at[k] * 16 : 0), head < heads && p.in[k]);
         at[i] += step[i];
       }
       head += GROUPS;
@@ -580,73 +555,78 @@ struct Supply {
 };
 
 // Rounds [from, to) of one kind: the rows come out of the ring, results go to `out`.
-template <typename T, int LANES, int CHUNKS, int DEPTH, bool NORM, bool CODES, typename Next>
-__device__ __forceinline__ void rotate_rows(const RotateArgs &a, int count, int from, int to, const Turn<T, LANES, CHUNKS> &turn,
-                                            const float (&wc)[CHUNKS][Piece<T>::V], const float (&ws)[CHUNKS][Piece<T>::V], char *out,
-                                            int64_t out_stride, float *scales, int64_t scale_stride, bool real, uint32_t ring, int &slot, Next next) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, BYTES = CHUNKS * 512;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
+template <typename T, int LANES, int DEPTH, bool NORM, bool CODES, typename Next>
+__device__ __forceinline__ void rotate_rows(const RotateArgs &a, const Pieces<T, LANES> &p, int count, int from, int to,
+                                            const float (&wc)[2][Piece<T>::V], const float (&ws)[2][Piece<T>::V], char *out, int64_t out_stride,
+                                            float *scales, int64_t scale_stride, bool real, uint32_t ring, int &slot, Next next) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, PIECE = CODES ? V : 16;
+  const int group = threadIdx.x % 32 / LANES;
   const float by_dim = 1.0f / (float)a.dim;
   int head = from * GROUPS + group;
-  out += head * out_stride + (CODES ? lane * V : lane * 16);
-  const uint32_t mine = ring + group * LANES * CHUNKS * 16;
+  out += head * out_stride;
+  if (CODES) scales += head * scale_stride;
   for (int round = from; round < to; ++round) {
     wait_for_all_but<DEPTH - 1>();
-    __syncwarp();
-    const uint32_t row = mine + slot * BYTES;
-    Piece<T> x[CHUNKS], other[CHUNKS];
-#pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) x[k].take(row + (lane + k * LANES) * 16);
-    if constexpr (NORM) turn.partners(a, row, x, other);
-    __syncwarp();
-    next(slot);
+    const uint32_t row = ring + slot * 1024;
+    Piece<T> x[2];
+    x[0].take(row);
+    x[1].take(row + 512);
+    next(row);
     slot = slot + 1 == DEPTH ? 0 : slot + 1;
     if constexpr (NORM) {
-      float pair[2] = {0.0f, 0.0f};
+      float2 pair = {0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const float2 r = fma2({x[k].x[j], x[k].x[j + 1]}, {x[k].x[j], x[k].x[j + 1]}, {pair[0], pair[1]});
-          pair[0] = r.x;
-          pair[1] = r.y;
-        }
-      float sum = pair[0] + pair[1];
+        for (int j = 0; j < V; j += 2) pair = fma2({x[k].x[j], x[k].x[j + 1]}, {x[k].x[j], x[k].x[j + 1]}, pair);
+      float sum = pair.x + pair.y;
 #pragma unroll
       for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       const float r = rsqrtf(fmaf(sum, by_dim, a.eps));
+      float y[2][V];
+      if (a.interleaved) {
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k) {
-        mul_all(other[k].x, other[k].x, ws[k]);
-        fma_all(x[k].x, x[k].x, wc[k], other[k].x);
-        mul_all(x[k].x, x[k].x, r);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < V; j += 2) {
+            const float2 t = mul2({x[k].x[j + 1], x[k].x[j]}, {ws[k][j], ws[k][j + 1]});
+            const float2 u = fma2({x[k].x[j], x[k].x[j + 1]}, {wc[k][j], wc[k][j + 1]}, t);
+            y[k][j] = u.x;
+            y[k][j + 1] = u.y;
+          }
+      } else {
+        mul_all(y[0], x[1].x, ws[0]);
+        fma_all(y[0], x[0].x, wc[0], y[0]);
+        mul_all(y[1], x[0].x, ws[1]);
+        fma_all(y[1], x[1].x, wc[1], y[1]);
       }
+      mul_all(x[0].x, y[0], r);
+      mul_all(x[1].x, y[1], r);
       if (!real) {
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-          for (int j = 0; j < V; ++j) x[k].x[j] = 0.0f;
+        for (int j = 0; j < V; ++j) x[0].x[j] = x[1].x[j] = 0.0f;
       }
     }
     if constexpr (CODES) {
       float most = 0.0f;
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
+      for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(x[k].x[j]));
 #pragma unroll
       for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
       const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
       if (head < count) {
-        if (lane == 0) scales[head * scale_stride] = scale_of(most, big);
+        if (threadIdx.x % LANES == 0) *scales = scale_of(most, big);
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k)
-          if ((lane + k * LANES) * V < a.dim) store_codes<V>(out + k * LANES * V, x[k].x, by, a.cache.type);
+        for (int k = 0; k < 2; ++k)
+          if (p.in[k]) store_codes<V>(out + p.at[k] * PIECE, x[k].x, by, a.cache.type);
       }
-    } else if (head < count) {
+      scales += GROUPS * scale_stride;
+    } else {
 #pragma unroll
-      for (int k = 0; k < CHUNKS; ++k)
-        if ((lane + k * LANES) * V < a.dim) reinterpret_cast<uint4 *>(out)[k * LANES] = x[k].get();
+      for (int k = 0; k < 2; ++k)
+        if (head < count && p.in[k]) *reinterpret_cast<uint4 *>(out + p.at[k] * PIECE) = x[k].get();
     }
     head += GROUPS;
     out += GROUPS * out_stride;
@@ -655,32 +635,29 @@ __device__ __forceinline__ void rotate_rows(const RotateArgs &a, int count, int 
 
 // A warp takes `each` of the rounds of one token: those of the queries come first, then the keys', then the values'.  CACHE: keys
 // and values go to the cache, CODES: as codes.
-template <typename T, int LANES, int CHUNKS, bool NORM, bool CACHE, bool CODES>
-__global__ void __launch_bounds__(ROW_THREADS, CHUNKS == 1 ? 8 : 5) rotate_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 8 / CHUNKS, BYTES = CHUNKS * 512, KINDS = CACHE ? 3 : 2;
-  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * BYTES];
+template <typename T, int LANES, bool NORM, bool CACHE, bool CODES>
+__global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 4, KINDS = CACHE ? 3 : 2;
+  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 1024];
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= a.tokens) return;
-  const int lane = threadIdx.x % LANES;
-  const uint32_t ring = shared_at(rings[threadIdx.x / 32]);
+  const uint32_t ring = shared_at(rings[threadIdx.x / 32]) + threadIdx.x % 32 * 16;
+  const Pieces<T, LANES> p(a.dim, NORM && !a.interleaved ? a.rot / 2 : 0);
   int from = (int)(task - token * parts) * each, rounds[KINDS], all = 0;
 #pragma unroll
   for (int which = 0; which < KINDS; ++which) all += rounds[which] = (a.heads[which] + GROUPS - 1) / GROUPS;
   int to = min(from + each, all);
   const Rows *const rows[1] = {a.in};
-  Supply<T, LANES, CHUNKS, KINDS, 1> supply;
-  supply.begin(a, rows, token, from, to - from, ring);
+  Supply<T, LANES, KINDS, 1> supply;
+  supply.begin(a, rows, token, from, to - from);
 #pragma unroll
-  for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, token, i);
+  for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, p, token, ring + i * 1024);
   const int64_t place = load_index(a.place, token, a.idx_bytes);
   const bool real = !NORM || (place >= 0 && place < a.places);
-  int own[CHUNKS];
-#pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) own[k] = lane + k * LANES;
   int64_t first_row = -1;
   if (CACHE && real && to > rounds[0]) first_row = cache_row(a.cache, a.lists, load_index(a.row, token, a.idx_bytes), place, a.page_shift);
   int slot = 0;
-  auto next = [&](int free) { supply.send(a, rows, token, free); };
+  auto next = [&](uint32_t free) { supply.send(a, rows, p, token, free); };
 #pragma unroll
   for (int which = 0; which < KINDS; ++which) {
     if (from < rounds[which] && to > 0) {
@@ -688,34 +665,44 @@ __global__ void __launch_bounds__(ROW_THREADS, CHUNKS == 1 ? 8 : 5) rotate_kerne
         wait_for_all_but<0>();
         return;
       }
-      float wc[CHUNKS][V], ws[CHUNKS][V];
-      Turn<T, LANES, CHUNKS> turn;
+      float wc[2][V], ws[2][V];
       if (NORM && which < 2) {
-        turn.load(a, place, real, lane, false);
-        load_weights<T, CHUNKS>(a, which, own, wc);
-        load_weights<T, CHUNKS>(a, which, turn.from, ws);
+        Turn<T, LANES> turn;
+        turn.load(a, p, place, real);
+        load_weights(a, which, p, wc);
+        if (a.interleaved) {
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) ws[k][j] = (a.interleaved ? wc[k][j ^ 1] : ws[k][j]) * turn.s[k][j];
+            for (int j = 0; j < V; ++j) ws[k][j] = wc[k][j ^ 1] * (j % 2 == 0 ? -turn.s[k * (V / 2) + j / 2] : turn.s[k * (V / 2) + j / 2]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) wc[k][j] *= turn.c[k][j];
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) wc[k][j] *= turn.c[k * (V / 2) + j / 2];
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            ws[0][j] = wc[1][j] * -turn.s[j];
+            ws[1][j] = wc[0][j] * turn.s[j];
+            wc[0][j] *= turn.c[j];
+            wc[1][j] *= turn.c[j];
+          }
         }
       }
       const int lo = max(from, 0), hi = min(to, rounds[which]);
       if (which == 0 || !CACHE) {
-        rotate_rows<T, LANES, CHUNKS, DEPTH, NORM, false>(a, a.heads[which], lo, hi, turn, wc, ws,
-                                                          static_cast<char *>(a.out[which]) + token * a.heads[which] * a.dim * (int)sizeof(T),
-                                                          a.dim * (int)sizeof(T), nullptr, 0, real, ring, slot, next);
+        rotate_rows<T, LANES, DEPTH, NORM, false>(a, p, a.heads[which], lo, hi, wc, ws,
+                                                  static_cast<char *>(a.out[which]) + token * a.heads[which] * a.dim * (int)sizeof(T),
+                                                  a.dim * (int)sizeof(T), nullptr, 0, real, ring, slot, next);
       } else {
         const int size = CODES ? 1 : sizeof(T);
         char *const store = static_cast<char *>(which == 1 ? a.cache.d_k : a.cache.d_v) + first_row * a.dim * size;
         float *const scales = CODES ? (which == 1 ? a.cache.d_k_scale : a.cache.d_v_scale) + first_row : nullptr;
         const int64_t stride = a.cache.page_size * a.dim * size;
         if (which == 1)
-          rotate_rows<T, LANES, CHUNKS, DEPTH, NORM, CODES>(a, a.heads[1], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
+          rotate_rows<T, LANES, DEPTH, NORM, CODES>(a, p, a.heads[1], lo, hi, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
         else
-          rotate_rows<T, LANES, CHUNKS, DEPTH, false, CODES>(a, a.heads[2], lo, hi, turn, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
+          rotate_rows<T, LANES, DEPTH, false, CODES>(a, p, a.heads[2], lo, hi, wc, ws, store, stride, scales, a.cache.page_size, true, ring, slot, next);
       }
     }
     from -= rounds[which];
@@ -725,21 +712,18 @@ __global__ void __launch_bounds__(ROW_THREADS, CHUNKS == 1 ? 8 : 5) rotate_kerne
 
 // Backward: warps take tokens a grid apart and keep their share of the weights' gradients in registers.  The warps' lane groups
 // are added in order by the block, the blocks by rotate_weights_kernel.
-template <typename T, int LANES, int CHUNKS>
+template <typename T, int LANES>
 __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 4 / CHUNKS, BYTES = CHUNKS * 512;
-  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 2 * BYTES];
-  __shared__ float shares[ROW_THREADS / LANES][LANES * CHUNKS * V];
-  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES;
-  const uint32_t ring = shared_at(rings[threadIdx.x / 32]);
-  int own[CHUNKS];
-  float dw[2][CHUNKS][V];
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 3;
+  __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 2048];
+  __shared__ float shares[ROW_THREADS / LANES][LANES * 2 * V];
+  const uint32_t ring = shared_at(rings[threadIdx.x / 32]) + threadIdx.x % 32 * 16;
+  const Pieces<T, LANES> p(a.dim, a.interleaved ? 0 : a.rot / 2);
+  float dw[2][2][V];
 #pragma unroll
-  for (int k = 0; k < CHUNKS; ++k) {
-    own[k] = lane + k * LANES;
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[0][k][j] = dw[1][k][j] = 0.0f;
-  }
   const float by_dim = 1.0f / (float)a.dim;
   const int64_t tasks = a.tokens * parts;
   const int rounds[2] = {(a.heads[0] + GROUPS - 1) / GROUPS, (a.heads[1] + GROUPS - 1) / GROUPS};
@@ -747,14 +731,14 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
   for (int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32; task < tasks; task += (int64_t)gridDim.x * ROW_WARPS) {
     const int64_t token = task / parts;
     int from = (int)(task - token * parts) * each, to = min(from + each, rounds[0] + rounds[1]);
-    Supply<T, LANES, CHUNKS, 2, 2> supply;
-    supply.begin(a, rows, token, from, to - from, ring);
+    Supply<T, LANES, 2, 2> supply;
+    supply.begin(a, rows, token, from, to - from);
 #pragma unroll
-    for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, token, i);
+    for (int i = 0; i < DEPTH; ++i) supply.send(a, rows, p, token, ring + i * 2048);
     const int64_t place = load_index(a.place, token, a.idx_bytes);
     const bool real = place >= 0 && place < a.places;
-    Turn<T, LANES, CHUNKS> turn;
-    turn.load(a, place, real, lane, true);
+    Turn<T, LANES> turn;
+    turn.load(a, p, place, real);
     int slot = 0;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -762,43 +746,53 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
       from -= rounds[which];
       to -= rounds[which];
       if (lo >= hi) continue;
-      float weight[CHUNKS][V];
-      load_weights<T, CHUNKS>(a, which, own, weight);
-      int head = lo * GROUPS + group;
-      char *out = static_cast<char *>(a.out[which]) + (token * a.heads[which] + head) * a.dim * (int)sizeof(T) + lane * 16;
+      float weight[2][V];
+      load_weights(a, which, p, weight);
+      int head = lo * GROUPS + threadIdx.x % 32 / LANES;
+      char *out = static_cast<char *>(a.out[which]) + (token * a.heads[which] + head) * a.dim * (int)sizeof(T);
       for (int round = lo; round < hi; ++round) {
         wait_for_all_but<DEPTH - 1>();
-        __syncwarp();
-        const uint32_t row = ring + slot * 2 * BYTES + group * LANES * CHUNKS * 16;
-        Piece<T> x[CHUNKS], dn[CHUNKS], other[CHUNKS];
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          x[k].take(row + own[k] * 16);
-          dn[k].take(row + BYTES + own[k] * 16);
-        }
-        turn.partners(a, row + BYTES, dn, other);
-        __syncwarp();
-        supply.send(a, rows, token, slot);
+        const uint32_t row = ring + slot * 2048;
+        Piece<T> x[2], dy[2];
+        x[0].take(row);
+        x[1].take(row + 512);
+        dy[0].take(row + 1024);
+        dy[1].take(row + 1536);
+        supply.send(a, rows, p, token, row);
         slot = slot + 1 == DEPTH ? 0 : slot + 1;
-        float sum = 0.0f, inner = 0.0f;
+        if (!real) {
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-          if (!real) {
+          for (int j = 0; j < V; ++j) x[0].x[j] = x[1].x[j] = dy[0].x[j] = dy[1].x[j] = 0.0f;
+        }
+        float dn[2][V], g[2][V], part[V];
+        if (a.interleaved) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[k].x[j] = dn[k].x[j] = other[k].x[j] = 0.0f;
-          }
-          float square[V], product[V];
-          mul_all(other[k].x, other[k].x, turn.s[k]);
-          fma_all(dn[k].x, dn[k].x, turn.c[k], other[k].x);
-          mul_all(other[k].x, dn[k].x, weight[k]);  // g
-          mul_all(square, x[k].x, x[k].x);
-          mul_all(product, other[k].x, x[k].x);
+          for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            sum += square[j];
-            inner += product[j];
+            for (int j = 0; j < V; j += 2) {
+              const float c = turn.c[k * (V / 2) + j / 2], s = turn.s[k * (V / 2) + j / 2];
+              dn[k][j] = fmaf(dy[k].x[j], c, dy[k].x[j + 1] * s);
+              dn[k][j + 1] = fmaf(dy[k].x[j + 1], c, -(dy[k].x[j] * s));
+            }
+        } else {
+          mul_all(dn[0], dy[1].x, turn.s);
+          fma_all(dn[0], dy[0].x, turn.c, dn[0]);
+          mul_all(part, dy[0].x, turn.s);
+          mul_all(dn[1], dy[1].x, turn.c);
+#pragma unroll
+          for (int j = 0; j < V; ++j) dn[1][j] -= part[j];
+        }
+        float2 squares = {0.0f, 0.0f}, products = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          mul_all(g[k], dn[k], weight[k]);
+#pragma unroll
+          for (int j = 0; j < V; j += 2) {
+            squares = fma2({x[k].x[j], x[k].x[j + 1]}, {x[k].x[j], x[k].x[j + 1]}, squares);
+            products = fma2({g[k][j], g[k][j + 1]}, {x[k].x[j], x[k].x[j + 1]}, products);
           }
         }
+        float sum = squares.x + squares.y, inner = products.x + products.y;
 #pragma unroll
         for (int d = LANES / 2; d > 0; d /= 2) {
           sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -806,29 +800,32 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
         }
         const float r = rsqrtf(fmaf(sum, by_dim, a.eps)), back = -inner * by_dim * r * r;
 #pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
+        for (int k = 0; k < 2; ++k) {
           mul_all(x[k].x, x[k].x, r);
-          fma_all(dw[which][k], dn[k].x, x[k].x, dw[which][k]);
-          mul_all(other[k].x, other[k].x, r);
-          mul_all(x[k].x, x[k].x, back);
+          fma_all(dw[which][k], dn[k], x[k].x, dw[which][k]);
+          mul_all(g[k], g[k], r);
 #pragma unroll
-          for (int j = 0; j < V; ++j) x[k].x[j] += other[k].x[j];
-          if (head < a.heads[which] && own[k] * V < a.dim) reinterpret_cast<uint4 *>(out)[k * LANES] = x[k].get();
+          for (int j = 0; j < V; j += 2) {
+            const float2 t = fma2({x[k].x[j], x[k].x[j + 1]}, {back, back}, {g[k][j], g[k][j + 1]});
+            x[k].x[j] = t.x;
+            x[k].x[j + 1] = t.y;
+          }
+          if (head < a.heads[which] && p.in[k]) *reinterpret_cast<uint4 *>(out + p.at[k] * 16) = x[k].get();
         }
         head += GROUPS;
         out += GROUPS * a.dim * (int)sizeof(T);
       }
     }
-    wait_for_all_but<0>();
-    __syncwarp();
   }
   pdl_release();
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < CHUNKS; ++k)
+    for (int k = 0; k < 2; ++k)
+      if (p.in[k]) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) shares[threadIdx.x / LANES][own[k] * V + j] = which ? dw[1][k][j] : dw[0][k][j];
+        for (int j = 0; j < V; ++j) shares[threadIdx.x / LANES][p.at[k] * V + j] = which ? dw[1][k][j] : dw[0][k][j];
+      }
     __syncthreads();
     for (int i = threadIdx.x; i < a.dim; i += ROW_THREADS) {
       float sum = 0.0f;
@@ -839,64 +836,88 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
   }
 }
 
-// Keys and values of listed tokens: a warp takes `each` rounds of a token's heads; the cache's rows are codes or T.
-template <typename T, int LANES, int CHUNKS, bool CODES>
+// Keys and values of listed tokens: a warp takes `each` rounds of a token's heads, two neighbouring pieces a lane; the cache's
+// rows are codes or T.
+template <typename T, int LANES, bool CODES>
 __global__ void __launch_bounds__(ROW_THREADS)
 kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row,
                const void *place, int page_shift, int parts, int each, T *k, T *v) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = CHUNKS == 1 ? 4 : 2;
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = 2, SIZE = CODES ? 1 : sizeof(T);
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= tokens) return;
-  const int lane = threadIdx.x % LANES, group = threadIdx.x % 32 / LANES, dim = (int)cache.dim, heads = (int)cache.heads;
-  const int from = (int)(task % parts) * each, to = min(from + each, (heads + GROUPS - 1) / GROUPS);
+  const int lane = threadIdx.x % LANES, dim = (int)cache.dim, heads = (int)cache.heads;
+  const int from = (int)(task - token * parts) * each, to = min(from + each, (heads + GROUPS - 1) / GROUPS);
   const int64_t first = cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes), page_shift);
+  const bool in[2] = {2 * lane * V < dim, (2 * lane + 1) * V < dim}, wide = dim % (2 * V) == 0;
+  int head = from * GROUPS + threadIdx.x % 32 / LANES;
+  const int64_t at = (max(first, (int64_t)0) + head * cache.page_size), step = GROUPS * cache.page_size;
+  const int64_t bytes = (at * dim + 2 * lane * V) * SIZE, byte_step = step * dim * SIZE, out = (token * heads + head) * dim + 2 * lane * V;
+  const char *rows[2] = {static_cast<const char *>(cache.d_k) + bytes, static_cast<const char *>(cache.d_v) + bytes};
+  const float *scales[2] = {cache.d_k_scale + at, cache.d_v_scale + at};
+  T *to_rows[2] = {k + out, v + out};
+  for (int round = from; round < to; round += ROUNDS) {
+    uint4 raw[ROUNDS][2][2];
+    float scale[ROUNDS][2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const char *const store = static_cast<const char *>(w == 0 ? cache.d_k : cache.d_v) + max(first, (int64_t)0) * dim * (CODES ? 1 : sizeof(T));
-    const float *const scales = CODES ? (w == 0 ? cache.d_k_scale : cache.d_v_scale) + max(first, (int64_t)0) : nullptr;
-    T *const out = (w == 0 ? k : v) + token * heads * dim;
-    for (int round = from; round < to; round += ROUNDS) {
-      Raw raw[ROUNDS][CHUNKS];
-      float scale[ROUNDS];
+    for (int u = 0; u < ROUNDS; ++u) {
+      const bool real = first >= 0 && round + u < to && head + u * GROUPS < heads;
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
-        const int head = (round + u) * GROUPS + group;
-        const bool in = first >= 0 && round + u < to && head < heads;
-        const int64_t at = head * cache.page_size;
-        if (CODES) scale[u] = in ? scales[at] : 0.0f;
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          const int i = (lane + c * LANES) * V;
-          if constexpr (!CODES) {
-            raw[u][c].load(store + (at * dim + i) * (int)sizeof(T), in && i < dim);
-          } else {
-            uint2 x = make_uint2(0, 0);
-            if (in && i < dim) {
-              if constexpr (V == 8) x = *reinterpret_cast<const uint2 *>(store + at * dim + i);
-              else x.x = *reinterpret_cast<const uint32_t *>(store + at * dim + i);
+      for (int w = 0; w < 2; ++w) {
+        raw[u][w][0] = raw[u][w][1] = make_uint4(0, 0, 0, 0);
+        if (CODES) {
+          scale[u][w] = real ? *scales[w] : 0.0f;
+          scales[w] += step;
+          uint32_t c[4] = {0, 0, 0, 0};
+          if (real && wide && in[0]) {  // both pieces in one
+            if constexpr (V == 8) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(rows[w]);
+              c[0] = x.x;
+              c[1] = x.y;
+              c[2] = x.z;
+              c[3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2 *>(rows[w]);
+              c[0] = x.x;
+              c[1] = x.y;
             }
-            raw[u][c].w[0] = x.x;
-            raw[u][c].w[1] = x.y;
+          } else if (real) {  // a row that begins at a multiple of one piece only
+#pragma unroll
+            for (int i = 0; i < 2 * V / 4; ++i)
+              if (in[i / (V / 4)]) c[i] = reinterpret_cast<const uint32_t *>(rows[w])[i];
           }
+          raw[u][w][0] = make_uint4(c[0], c[1], c[2], c[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (real && in[i]) raw[u][w][i] = reinterpret_cast<const uint4 *>(rows[w])[i];
         }
+        rows[w] += byte_step;
       }
+    }
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
-        const int head = (round + u) * GROUPS + group;
-        if (round + u >= to || head >= heads) continue;
+    for (int u = 0; u < ROUNDS; ++u) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          if ((lane + c * LANES) * V >= dim) continue;
-          uint4 *const to_piece = reinterpret_cast<uint4 *>(out + head * dim) + lane + c * LANES;
-          if constexpr (CODES) {
-            Piece<T> p;
-            values_of<V>(p.x, make_uint2(raw[u][c].w[0], raw[u][c].w[1]), scale[u], cache.type);
-            *to_piece = p.get();
+      for (int w = 0; w < 2; ++w) {
+        const bool real = round + u < to && head < heads;
+        if constexpr (CODES) {
+          const uint4 r = raw[u][w][0];
+          Piece<T> p[2];
+          if constexpr (V == 8) {
+            values_of<V>(p[0].x, make_uint2(r.x, r.y), scale[u][w], cache.type);
+            values_of<V>(p[1].x, make_uint2(r.z, r.w), scale[u][w], cache.type);
           } else {
-            *to_piece = make_uint4(raw[u][c].w[0], raw[u][c].w[1], raw[u][c].w[2], raw[u][c].w[3]);
+            values_of<V>(p[0].x, make_uint2(r.x, 0), scale[u][w], cache.type);
+            values_of<V>(p[1].x, make_uint2(r.y, 0), scale[u][w], cache.type);
           }
+          raw[u][w][0] = p[0].get();
+          raw[u][w][1] = p[1].get();
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (real && in[i]) reinterpret_cast<uint4 *>(to_rows[w])[i] = raw[u][w][i];
+        to_rows[w] += GROUPS * dim;
       }
+      head += GROUPS;
     }
   }
 }
@@ -987,17 +1008,16 @@ static bool pieces_fit(int type, const RotateArgs &a, bool backward) {
   return !a.to_cache || (aligned(a.cache.d_k, 16) && aligned(a.cache.d_v, 16));
 }
 
-// Calls run(LANES, CHUNKS) as compile-time numbers for rows of `dim` values.
+// Calls run(LANES) as a compile-time number: two pieces a lane of rows of `dim` values.
 template <typename T, typename F>
 static int with_lanes(int dim, F run) {
   using std::integral_constant;
-  const int pieces = dim / Piece<T>::V;
-  if (pieces <= 4) return run(integral_constant<int, 4>(), integral_constant<int, 1>());
-  if (pieces <= 8) return run(integral_constant<int, 8>(), integral_constant<int, 1>());
-  if (pieces <= 16) return run(integral_constant<int, 16>(), integral_constant<int, 1>());
-  if constexpr (KV_MAX_DIM / Piece<T>::V > 32)
-    if (pieces > 32) return run(integral_constant<int, 32>(), integral_constant<int, 2>());
-  return run(integral_constant<int, 32>(), integral_constant<int, 1>());
+  const int pairs = (dim / Piece<T>::V + 1) / 2;
+  if constexpr (KV_MAX_DIM / Piece<T>::V / 2 > 16)
+    if (pairs > 16) return run(integral_constant<int, 32>());
+  if (pairs <= 4) return run(integral_constant<int, 4>());
+  if (pairs <= 8) return run(integral_constant<int, 8>());
+  return run(integral_constant<int, 16>());
 }
 
 // How the rounds of a token are shared out: few tokens are cut into parts, down to a round, so that there are eight warps' work for
@@ -1026,16 +1046,16 @@ static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     }
-    return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+    return with_lanes<T>(a.dim, [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value, GROUPS = 32 / LANES;
       int rounds = 0;
       for (int heads : a.heads) rounds += (heads + GROUPS - 1) / GROUPS;
       const Parts p = parts_of(a.tokens, rounds);
-      if (!a.to_cache) rotate_kernel<T, LANES, CHUNKS, true, false, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (a.norm && is_quantised(a.cache.type)) rotate_kernel<T, LANES, CHUNKS, true, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (a.norm) rotate_kernel<T, LANES, CHUNKS, true, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (is_quantised(a.cache.type)) rotate_kernel<T, LANES, CHUNKS, false, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else rotate_kernel<T, LANES, CHUNKS, false, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      if (!a.to_cache) rotate_kernel<T, LANES, true, false, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (a.norm && is_quantised(a.cache.type)) rotate_kernel<T, LANES, true, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (a.norm) rotate_kernel<T, LANES, true, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else if (is_quantised(a.cache.type)) rotate_kernel<T, LANES, false, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      else rotate_kernel<T, LANES, false, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });
@@ -1059,12 +1079,12 @@ static int launch_backward(int type, RotateArgs &a, PoolBuf &partial, int *block
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     }
-    return with_lanes<T>(a.dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+    return with_lanes<T>(a.dim, [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value, GROUPS = 32 / LANES;
       const int rounds = (a.heads[0] + GROUPS - 1) / GROUPS + (a.heads[1] + GROUPS - 1) / GROUPS;
       const Parts p = a.tokens > 0 && rounds > 0 ? parts_of(a.tokens, rounds) : Parts{1, 1, 0};
       LAPIS_TRY(room(p.blocks));
-      if (*blocks > 0) rotate_backward_kernel<T, LANES, CHUNKS><<<*blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
+      if (*blocks > 0) rotate_backward_kernel<T, LANES><<<*blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });
@@ -1198,14 +1218,14 @@ extern "C" int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     }
-    return with_lanes<T>((int)cache->dim, [&](auto lanes, auto chunks) {
-      constexpr int LANES = decltype(lanes)::value, CHUNKS = decltype(chunks)::value, GROUPS = 32 / LANES;
+    return with_lanes<T>((int)cache->dim, [&](auto lanes) {
+      constexpr int LANES = decltype(lanes)::value, GROUPS = 32 / LANES;
       const Parts p = parts_of(tokens, (int)((cache->heads + GROUPS - 1) / GROUPS));
       const int shift = page_shift_of(cache->page_size);
       if (is_quantised(cache->type))
-        kv_read_kernel<T, LANES, CHUNKS, true><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
+        kv_read_kernel<T, LANES, true><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
       else
-        kv_read_kernel<T, LANES, CHUNKS, false><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
+        kv_read_kernel<T, LANES, false><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
       LAPIS_CUDA_TRY(cudaGetLastError());
       return (int)LAPIS_OK;
     });

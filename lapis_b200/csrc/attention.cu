@@ -22,7 +22,9 @@
 namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int MIN_TILES = 4;      // of a share, if there is more than one
+constexpr int MOST_BLOCKS = 320;  // shares that a join has room for: two blocks an SM
+constexpr float LN2 = 0.6931471805599453f;
 
 struct AttendArgs {
   const void *q;
@@ -36,118 +38,139 @@ struct AttendArgs {
   const void *length;
   void *out;
   float *lse;
-  float *partial;  // [blocks][2][HEADS][dim + 2]
-  int blocks, min_tiles;
+  float *partial;     // what blocks leave of units that are cut: two pieces each
+  struct Cut *cuts;   // one for each block
+  int blocks;
   int page_shift;  // log2 of the slots of a page, or -1
 };
 
 // A request's tokens beyond these are not looked at: places are 32-bit numbers in the kernels.
 constexpr int MOST_TOKENS = 0x7fff0000;
 
-// Keys [lo, hi) of request b that are attended.
+// Keys [lo, hi) of a request that are attended; its pages are crd[entry] onward.  Tiles begin at `origin`, lo rounded down to a
+// multiple of 16, so that 16 keys of a tile lie in one page where that has a multiple of 16 slots.
 struct Span {
-  int64_t lo, hi;
+  int lo, hi, origin;
+  int64_t entry;
 };
-__device__ __forceinline__ Span span_of(const AttendArgs &a, int64_t b) {
-  const int64_t first = load_index(a.lists.d_pos, b, a.lists.idx_bytes), last = load_index(a.lists.d_pos, b + 1, a.lists.idx_bytes);
-  const int64_t room = (last - first) * a.cache.page_size, n = load_index(a.length, b, a.lists.idx_bytes);
+__device__ __forceinline__ Span span_of(const AttendArgs &a, int request) {
+  const int64_t first = load_index(a.lists.d_pos, request, a.lists.idx_bytes), last = load_index(a.lists.d_pos, request + 1, a.lists.idx_bytes);
+  const int64_t room = (last - first) * a.cache.page_size, n = load_index(a.length, request, a.lists.idx_bytes);
   Span s;
-  s.hi = max((int64_t)0, min(min(n, room), (int64_t)MOST_TOKENS));
-  s.lo = a.window > 0 ? max((int64_t)0, s.hi - a.window) : 0;
+  s.hi = (int)max((int64_t)0, min(min(n, room), (int64_t)MOST_TOKENS));
+  s.lo = a.window > 0 && a.window < s.hi ? s.hi - (int)a.window : 0;
+  s.origin = s.lo & ~15;
+  s.entry = first;
   return s;
 }
 // Tiles of a unit of a request; a request without tokens has one, which writes its zeros.
-__device__ __forceinline__ int64_t tiles_of(const Span &s, int tile) { return max((int64_t)1, (s.hi - s.lo + tile - 1) / tile); }
+__device__ __forceinline__ int tiles_of(const Span &s, int tile) { return max(1, (s.hi - s.origin + tile - 1) / tile); }
 
-// Where a share of the tiles begins: all threads of the block return the same.
+// n * all / shares: where share n of the tiles begins.
+__device__ __forceinline__ int64_t share_start(int n, int64_t all, int shares) {
+  if (all < (1 << 22) && shares < (1 << 10)) return (uint32_t)n * (uint32_t)all / (uint32_t)shares;
+  return n * all / shares;
+}
+
+// A block's share of the tiles.  Where units are few and none is much longer than a share would be, a share is one unit, and
+// nothing has to be joined; otherwise the shares are equal and cut units anywhere.
 struct Share {
-  int64_t all;         // tiles of all units
-  int64_t shares;      // blocks that get some
-  int64_t from, to;    // this block's tiles
-  int64_t request, in_request;  // the request of the first one, and its number among the request's
+  int64_t all, from, steps;  // tiles of all units; this share's
+  int shares;
+  bool whole;
+  int request, unit, tile;  // of its first one
+  Span span;
 };
-__device__ __forceinline__ int64_t shares_of(const AttendArgs &a, int64_t all) { return max((int64_t)1, min((int64_t)a.blocks, all / a.min_tiles)); }
-__device__ __forceinline__ int64_t share_start(int64_t i, int64_t all, int64_t shares) { return i * all / shares; }
 
-// Sums the tiles of all requests (a thread takes a run of them), and finds the request of tile `at(all, shares)`.
-template <typename At>
-__device__ __forceinline__ Share find_share(const AttendArgs &a, int tile, At at) {
-  __shared__ int64_t warp_sums[ATT_THREADS / 32], found[2];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, units = (int)a.cache.heads * a.head_blocks;
+// Sums the tiles of all requests (a thread takes a run of them) and finds the unit of this block's first one.  All threads return
+// the same; steps is 0 for a block that gets none.
+__device__ __forceinline__ Share find_share(const AttendArgs &a, int tile) {
+  __shared__ int64_t warp_sums[ATT_THREADS / 32];
+  __shared__ int warp_longest[ATT_THREADS / 32], found_request, found_unit, found_tile;
+  __shared__ Span found_span;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, units = (int)a.cache.heads * a.head_blocks, me = blockIdx.x;
   const int run = (a.requests + ATT_THREADS - 1) / ATT_THREADS, first = threadIdx.x * run;
+  Share s;
+  s.request = me / units;  // if units are shares
+  s.unit = me - s.request * units;
+  s.tile = 0;
+  if (s.request < a.requests) s.span = span_of(a, s.request);
   int64_t sum = 0;
-  for (int b = first; b < min(first + run, a.requests); ++b) sum += tiles_of(span_of(a, b), tile) * units;
+  int longest = 0;
+  Span last;
+  for (int b = first; b < min(first + run, a.requests); ++b) {
+    last = span_of(a, b);
+    const int n = tiles_of(last, tile);
+    sum += (int64_t)n * units;
+    longest = max(longest, n);
+  }
   int64_t upto = sum;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
     const int64_t below = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += below;
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
   }
-  if (lane == 31) warp_sums[warp] = upto;
+  if (lane == 31) {
+    warp_sums[warp] = upto;
+    warp_longest[warp] = longest;
+  }
   __syncthreads();
-  Share s;
   s.all = 0;
   for (int w = 0; w < ATT_THREADS / 32; ++w) {
     if (w < warp) upto += warp_sums[w];
     s.all += warp_sums[w];
+    longest = max(longest, warp_longest[w]);
   }
-  s.shares = shares_of(a, s.all);
-  s.from = at(s);
-  s.to = s.from;
+  s.shares = (int)max((int64_t)1, min((int64_t)a.blocks, s.all / MIN_TILES));
+  const int64_t all_units = (int64_t)a.requests * units;
+  s.whole = all_units <= a.blocks && (longest - 4) * (int64_t)s.shares <= s.all;
+  if (s.whole) {
+    s.from = 0;
+    s.steps = me < all_units ? tiles_of(s.span, tile) : 0;
+    return s;
+  }
+  if (me >= s.shares) {
+    s.steps = 0;
+    return s;
+  }
+  s.from = share_start(me, s.all, s.shares);
+  s.steps = share_start(me + 1, s.all, s.shares) - s.from;
   if (s.from >= upto - sum && s.from < upto) {
     int64_t left = s.from - (upto - sum);
-    for (int b = first; b < min(first + run, a.requests); ++b) {
-      const int64_t n = tiles_of(span_of(a, b), tile) * units;
-      if (left < n) {
-        found[0] = b;
-        found[1] = left;
-        break;
-      }
+    int b = first;
+    while (run > 1) {
+      last = span_of(a, b);
+      const int64_t n = (int64_t)tiles_of(last, tile) * units;
+      if (left < n) break;
       left -= n;
+      ++b;
     }
+    const int n = tiles_of(last, tile);
+    found_request = b;
+    found_unit = (int)(left / n);
+    found_tile = (int)(left % n);
+    found_span = last;
   }
   __syncthreads();
-  s.request = found[0];
-  s.in_request = found[1];
-  __syncthreads();
+  s.request = found_request;
+  s.unit = found_unit;
+  s.tile = found_tile;
+  s.span = found_span;
   return s;
 }
 
-// Which shares hold the tiles of a unit, and where the first of them left its part (0: its first piece, 1: its last).
+// What a block leaves for the join: the unit that begins in its share and goes on in the next ones, up to share `last`; `slot` is
+// where its own part is (0: its first piece, 1: its last).  last = 0: there is none.
 struct Cut {
-  int64_t first, last;
-  int first_slot;
+  int last, slot, request, unit;
 };
-__device__ __forceinline__ Cut cut_of(const AttendArgs &a, int64_t request, int unit, int tile) {
-  __shared__ int64_t sums[2][ATT_THREADS / 32];
-  const int units = (int)a.cache.heads * a.head_blocks;
-  int64_t front = 0, all = 0;
-  for (int b = threadIdx.x; b < a.requests; b += ATT_THREADS) {
-    const int64_t n = tiles_of(span_of(a, b), tile) * units;
-    all += n;
-    if (b < request) front += n;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    all += __shfl_xor_sync(0xffffffffu, all, d);
-    front += __shfl_xor_sync(0xffffffffu, front, d);
-  }
-  if (threadIdx.x % 32 == 0) {
-    sums[0][threadIdx.x / 32] = front;
-    sums[1][threadIdx.x / 32] = all;
-  }
-  __syncthreads();
-  front = all = 0;
-  for (int w = 0; w < ATT_THREADS / 32; ++w) {
-    front += sums[0][w];
-    all += sums[1][w];
-  }
-  const int64_t tiles = tiles_of(span_of(a, request), tile), shares = shares_of(a, all), from = front + unit * tiles, to = from + tiles;
-  Cut c;  // the share of tile t is the largest i with i * all / shares < t + 1
-  c.first = ((from + 1) * shares + all - 1) / all - 1;
-  c.last = (to * shares + all - 1) / all - 1;
-  c.first_slot = share_start(c.first, all, shares) == from ? 0 : 1;
-  return c;
+// Of a unit that began at tile `from` of all and has `tiles`.
+__device__ __forceinline__ int last_share(const Share &s, int64_t from, int tiles) {
+  // the share of tile t is the largest n with n * all / shares < t + 1
+  const int64_t to = from + tiles;
+  if (s.all < (1 << 22) && s.shares < (1 << 10)) return (int)(((uint32_t)to * (uint32_t)s.shares + (uint32_t)s.all - 1) / (uint32_t)s.all) - 1;
+  return (int)((to * s.shares + s.all - 1) / s.all) - 1;
 }
 
 // ---- any type, width, stride and alignment --------------------------------------
@@ -165,27 +188,26 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
   float *const qs = smem, *const ks = qs + ANY_HEADS * dim, *const vs = ks + ANY_TILE * pitch, *const ps = vs + ANY_TILE * pitch;
   float *const factor = ps + ANY_HEADS * ANY_TILE, *const total = factor + ANY_HEADS;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  Share s = find_share(a, ANY_TILE, [&](const Share &x) { return share_start(min((int64_t)blockIdx.x, x.shares - 1), x.all, x.shares); });
-  if (blockIdx.x >= s.shares) return;
-  s.to = share_start(blockIdx.x + 1, s.all, s.shares);
-  int64_t request = s.request;
-  Span span = span_of(a, request);
-  int64_t tiles = tiles_of(span, ANY_TILE);
-  int unit = (int)(s.in_request / tiles);
-  int64_t tile = s.in_request % tiles;
+  pdl_wait();
+  const Share s = find_share(a, ANY_TILE);
+  pdl_release();
+  if (threadIdx.x == 0) a.cuts[blockIdx.x].last = 0;
+  int request = s.request, unit = s.unit, tile = s.tile;
+  Span span = s.span;
   const int units = (int)a.cache.heads * a.head_blocks;
-  for (int64_t at = s.from; at < s.to;) {
+  bool first_piece = true;
+  for (int64_t at = 0; at < s.steps;) {
     const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
-    const int64_t end = min(tiles, tile + (s.to - at));
+    const int tiles = tiles_of(span, ANY_TILE), end = (int)min((int64_t)tiles, tile + (s.steps - at));
     __syncthreads();
     for (int i = threadIdx.x; i < heads * dim; i += ATT_THREADS)
       qs[i] = to_f32(static_cast<const T *>(a.q)[request * a.q_token_stride + (int64_t)(kv_head * a.group + head0 + i / dim) * a.q_head_stride + i % dim]);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, acc[2][ANY_HEADS] = {};
-    for (int64_t t = tile; t < end; ++t) {
-      const int64_t key0 = span.lo + t * ANY_TILE;
+    for (int t = tile; t < end; ++t) {
+      const int key0 = span.origin + t * ANY_TILE;
       __syncthreads();
       for (int j = warp; j < ANY_TILE; j += ATT_THREADS / 32) {
-        const bool in = key0 + j < span.hi;
+        const bool in = key0 + j >= span.lo && key0 + j < span.hi;
         const int64_t row0 = in ? cache_row(a.cache, a.lists, request, key0 + j, a.page_shift) : -1, row = row0 + kv_head * a.cache.page_size;
         float kscale = 1.0f, vscale = 1.0f;
         if (row0 >= 0 && is_quantised(a.cache.type)) {
@@ -204,7 +226,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
         if (h >= heads) continue;
         float score = 0.0f;
         for (int i = 0; i < dim; ++i) score = fmaf(qs[h * dim + i], ks[lane * pitch + i], score);
-        score = key0 + lane < span.hi ? score * a.scale2 : -INFINITY;
+        score = key0 + lane >= span.lo && key0 + lane < span.hi ? score * a.scale2 : -INFINITY;
         float most = score;
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
@@ -230,7 +252,9 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
       }
     }
     const bool whole = tile == 0 && end == tiles;
-    float *const slot = a.partial + ((int64_t)blockIdx.x * 2 + (at == s.from ? 0 : 1)) * ANY_HEADS * (dim + 2);
+    float *const slot = a.partial + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * ANY_HEADS * (dim + 2);
+    if (!whole && tile == 0 && threadIdx.x == 0)
+      a.cuts[blockIdx.x] = {last_share(s, s.from + at, tiles), first_piece ? 0 : 1, request, unit};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int h = warp + 4 * u;
@@ -241,7 +265,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
       if (lane != 0) continue;
       total[h] = sum;
       if (whole && a.lse != nullptr)
-        a.lse[request * a.q_heads + kv_head * a.group + head0 + h] = sum == 0.0f ? -INFINITY : m[u] * LN2 + logf(sum);
+        a.lse[(int64_t)request * a.q_heads + kv_head * a.group + head0 + h] = sum == 0.0f ? -INFINITY : m[u] * LN2 + logf(sum);
       if (!whole) {
         slot[h * (dim + 2)] = m[u];
         slot[h * (dim + 2) + 1] = sum;
@@ -256,52 +280,62 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
       for (int h = 0; h < ANY_HEADS; ++h) {
         if (h >= heads) continue;
         if (whole)
-          static_cast<T *>(a.out)[(request * a.q_heads + kv_head * a.group + head0 + h) * dim + i] = from_f32<T>(total[h] == 0.0f ? 0.0f : acc[e][h] / total[h]);
+          static_cast<T *>(a.out)[((int64_t)request * a.q_heads + kv_head * a.group + head0 + h) * dim + i] = from_f32<T>(total[h] == 0.0f ? 0.0f : acc[e][h] / total[h]);
         else
           slot[h * (dim + 2) + 2 + i] = acc[e][h];
       }
     }
+    first_piece = false;
     at += end - tile;
     tile = 0;
-    if (++unit == units && at < s.to) {
+    if (++unit == units && at < s.steps) {
       unit = 0;
       span = span_of(a, ++request);
-      tiles = tiles_of(span, ANY_TILE);
     }
   }
 }
 
-// Adds up what the blocks left of the units that were cut: block (unit, request), a thread a dimension or two of each head.
+// Adds up what the blocks left of the units that were cut, in their order: block (share where the unit begins, head), a thread a
+// dimension or two.
 template <typename T>
 __global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_constant__ AttendArgs a) {
-  const int64_t request = blockIdx.y;
-  const int unit = blockIdx.x, dim = a.dim;
-  const Cut cut = cut_of(a, request, unit, ANY_TILE);
-  if (cut.first == cut.last) return;
-  const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
-  for (int h = 0; h < heads; ++h) {
-    auto slot = [&](int64_t i) { return a.partial + ((i * 2 + (i > cut.first ? 0 : cut.first_slot)) * ANY_HEADS + h) * (dim + 2); };
-    float most = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int64_t i = cut.first; i <= cut.last; ++i) most = fmaxf(most, slot(i)[0]);
-    const float base = most == -INFINITY ? 0.0f : most;
-    for (int64_t i = cut.first; i <= cut.last; ++i) {
-      const float *p = slot(i);
-      const float f = exp2f(p[0] - base);
-      sum = fmaf(p[1], f, sum);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = threadIdx.x + e * ATT_THREADS;
-        if (d < dim) acc[e] = fmaf(p[2 + d], f, acc[e]);
-      }
-    }
-    const int64_t head = request * a.q_heads + kv_head * a.group + head0 + h;
+  pdl_wait();
+  const Cut cut = a.cuts[blockIdx.x];
+  const int first = blockIdx.x, h = blockIdx.y, dim = a.dim;
+  const int head0 = (cut.unit % a.head_blocks) * ANY_HEADS;
+  if (cut.last == 0 || head0 + h >= a.group) return;
+  auto slot = [&](int i) { return a.partial + ((int64_t)(i * 2 + (i > first ? 0 : cut.slot)) * ANY_HEADS + h) * (dim + 2); };
+  float most = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
+  for (int i = first; i <= cut.last; ++i) most = fmaxf(most, slot(i)[0]);
+  const float base = most == -INFINITY ? 0.0f : most;
+#pragma unroll 4
+  for (int i = first; i <= cut.last; ++i) {
+    const float *p = slot(i);
+    const float f = exp2f(p[0] - base);
+    sum = fmaf(p[1], f, sum);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int d = threadIdx.x + e * ATT_THREADS;
-      if (d < dim) static_cast<T *>(a.out)[head * dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+      if (d < dim) acc[e] = fmaf(p[2 + d], f, acc[e]);
     }
-    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : most * LN2 + logf(sum);
   }
+  const int64_t head = (int64_t)cut.request * a.q_heads + cut.unit / a.head_blocks * a.group + head0 + h;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int d = threadIdx.x + e * ATT_THREADS;
+    if (d < dim) static_cast<T *>(a.out)[head * dim + d] = from_f32<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+  }
+  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : most * LN2 + logf(sum);
+}
+
+// The workspace of a call: `floats` for the pieces of each block, and the cuts behind them.
+static int make_workspace(AttendArgs &a, PoolBuf &work, int blocks, size_t floats, cudaStream_t st) {
+  a.blocks = std::min(blocks, MOST_BLOCKS);
+  const size_t pieces = ((size_t)a.blocks * floats * sizeof(float) + 15) / 16 * 16;
+  LAPIS_TRY(work.alloc(pieces + a.blocks * sizeof(Cut), st));
+  a.partial = static_cast<float *>(work.p);
+  a.cuts = reinterpret_cast<Cut *>(static_cast<char *>(work.p) + pieces);
+  return LAPIS_OK;
 }
 
 template <typename T>
@@ -312,15 +346,10 @@ static int launch_any(AttendArgs a, int dev, cudaStream_t st) {
     allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   a.head_blocks = (a.group + ANY_HEADS - 1) / ANY_HEADS;
-  a.blocks = 2 * sm_count();
-  a.min_tiles = 4;
-  PoolBuf partial;
-  LAPIS_TRY(partial.alloc((size_t)a.blocks * 2 * ANY_HEADS * (a.dim + 2) * sizeof(float), st));
-  a.partial = static_cast<float *>(partial.p);
-  attend_any_kernel<T><<<a.blocks, ATT_THREADS, any_smem(a.dim), st>>>(a);
-  LAPIS_CUDA_TRY(cudaGetLastError());
-  join_any_kernel<T><<<dim3((unsigned)(a.cache.heads * a.head_blocks), (unsigned)a.requests), ATT_THREADS, 0, st>>>(a);
-  LAPIS_CUDA_TRY(cudaGetLastError());
+  PoolBuf work;
+  LAPIS_TRY(make_workspace(a, work, 2 * sm_count(), 2 * ANY_HEADS * (a.dim + 2), st));
+  LAPIS_CUDA_TRY(launch_pdl(attend_any_kernel<T>, dim3(a.blocks), ATT_THREADS, any_smem(a.dim), st, a));
+  LAPIS_CUDA_TRY(launch_pdl(join_any_kernel<T>, dim3(a.blocks, ANY_HEADS), ATT_THREADS, 0, st, a));
   return LAPIS_OK;
 }
 
@@ -432,20 +461,24 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
 
 // Position in a block's share of the tiles.
 struct Cursor {
-  int request, unit, tile, tiles, lo, hi;
+  int request, unit, tile, tiles;
+  Span span;
 };
-__device__ __forceinline__ void enter(const AttendArgs &a, Cursor &c, int request, int tile_keys) {
-  const Span s = span_of(a, request);
-  c.request = request;
-  c.lo = (int)s.lo;
-  c.hi = (int)s.hi;
-  c.tiles = (int)tiles_of(s, tile_keys);
-}
 __device__ __forceinline__ void next_unit(const AttendArgs &a, Cursor &c, int units, int tile_keys) {
   c.tile = 0;
   if (++c.unit < units) return;
   c.unit = 0;
-  if (c.request + 1 < a.requests) enter(a, c, c.request + 1, tile_keys);
+  if (c.request + 1 < a.requests) {
+    c.span = span_of(a, ++c.request);
+    c.tiles = tiles_of(c.span, tile_keys);
+  }
+}
+
+// 2^x to 2 units in the last place; what is below 2^-126 is zero.
+__device__ __forceinline__ float power2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // What a warp has summed of eight heads: lane (g, c), g = lane / 4, c = lane % 4, holds dimensions by g of heads 2c and 2c + 1.
@@ -539,75 +572,122 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   unsigned char *const mine = stages + warp * STAGES * C::STAGE;
   const uint32_t ring = shared_address(mine);
   const int units = (int)a.cache.heads * a.head_blocks;
-  Share share = find_share(a, C::TILE, [&](const Share &x) { return share_start(min((int64_t)blockIdx.x, x.shares - 1), x.all, x.shares); });
-  if (blockIdx.x >= share.shares) return;
-  const int64_t steps = share_start(blockIdx.x + 1, share.all, share.shares) - share.from;
+  pdl_wait();
+  const Share share = find_share(a, C::TILE);
+  pdl_release();
+  if (threadIdx.x == 0) a.cuts[blockIdx.x].last = 0;
+  const int64_t steps = share.steps;
+  if (steps == 0) return;
   if (a.dim != C::DP)  // what is beyond the head is never copied
     for (int i = lane; i < STAGES * C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
   __syncwarp();
 
   Cursor in, out;  // of the copies and of the products
-  enter(a, in, (int)share.request, C::TILE);
-  in.unit = (int)(share.in_request / in.tiles);
-  in.tile = (int)(share.in_request % in.tiles);
+  in.request = share.request;
+  in.unit = share.unit;
+  in.tile = share.tile;
+  in.span = share.span;
+  in.tiles = tiles_of(in.span, C::TILE);
   out = in;
 
-  // Pages of the next step to copy: a lane looks up key `lane` (and lane + 32) of it one step ahead.
-  constexpr int LOOK = KEYS == 64 ? 2 : 1;
+  // Pages of the next step to copy, looked up one step ahead.  `grouped`: pages have a multiple of 16 slots, and a lane looks up
+  // 16 keys; otherwise a lane looks up key `lane` (and lane + 32).
+  constexpr int LOOK = KEYS == 64 ? 2 : 1, NONE = -1;
+  const bool grouped = a.cache.page_size % 16 == 0;
+  const int page_size = (int)a.cache.page_size, row_bytes = a.dim * (C::CODES ? 1 : 2);
   int64_t page[LOOK];
   int slot_in_page[LOOK];
   auto look_up = [&]() {
 #pragma unroll
     for (int u = 0; u < LOOK; ++u) {
-      const int key = in.lo + in.tile * C::TILE + warp * KEYS + (KEYS == 16 ? lane % 16 : lane) + 32 * u;
-      page[u] = -1;
+      const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + (grouped ? lane % MT * 16 : (KEYS == 16 ? lane % 16 : lane) + 32 * u);
+      page[u] = NONE;
       slot_in_page[u] = 0;
-      if (key < in.hi) {
-        const int nth = a.page_shift >= 0 ? key >> a.page_shift : key / (int)a.cache.page_size;
-        slot_in_page[u] = key - nth * (int)a.cache.page_size;
-        const int64_t entry = load_index(a.lists.d_pos, in.request, a.lists.idx_bytes) + nth;
+      if (key < in.span.hi && key >= (grouped ? in.span.origin : in.span.lo)) {
+        const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
+        slot_in_page[u] = key - nth * page_size;
+        const int64_t entry = in.span.entry + nth;
         if (entry >= 0 && entry < a.lists.entries) page[u] = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
       }
+      if (grouped) break;
     }
   };
-  const int row_bytes = a.dim * (C::CODES ? 1 : 2);
+  // Where this lane's piece of 16 bytes of row r goes, r = i * ROWS + lane / CHUNKS: the rows are swizzled so that neither the
+  // reads of K nor those of V meet in a bank.
+  constexpr int ROWS = 32 / C::CHUNKS;  // of a copy
+  const int ch = lane % C::CHUNKS, low = lane / C::CHUNKS;
+  const bool in_row = ch * 16 < row_bytes;
+  auto k_at = [&](int r) { return r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch : ch ^ (r & 4)) * 16; };
+  auto v_at = [&](int r) { return KEYS * C::ROW + r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch ^ (r & 2) : ch ^ ((r & 3) << 1)) * 16; };
+  const char *const k_store = static_cast<const char *>(a.cache.d_k) + ch * 16, *const v_store = static_cast<const char *>(a.cache.d_v) + ch * 16;
+  const uint32_t head_rows = (uint32_t)page_size, page_rows = (uint32_t)(a.cache.heads * a.cache.page_size);
   auto fetch = [&](int stage) {
-    const uint32_t to = ring + stage * C::STAGE;
+    const uint32_t to = ring + stage * C::STAGE, head_row = (uint32_t)(in.unit / a.head_blocks) * head_rows;
     uint32_t row[LOOK];
-    const int kv_head = in.unit / a.head_blocks;
 #pragma unroll
-    for (int u = 0; u < LOOK; ++u)
-      row[u] = page[u] < 0 || page[u] >= a.cache.pages
-                   ? 0xffffffffu
-                   : (uint32_t)((page[u] * a.cache.heads + kv_head) * a.cache.page_size + slot_in_page[u]);
-#pragma unroll
-    for (int i = 0; i < KEYS * C::CHUNKS / 32; ++i) {
-      const int at = i * 32 + lane, r = at / C::CHUNKS, ch = at % C::CHUNKS;
-      const uint32_t from_row = __shfl_sync(0xffffffffu, row[LOOK == 2 && i >= KEYS * C::CHUNKS / 64 ? 1 : 0], r % 32);
-      if (ch * 16 >= row_bytes) continue;
-      const bool real = from_row != 0xffffffffu;
-      const int64_t offset = real ? (int64_t)from_row * row_bytes + ch * 16 : 0;
-      int kch, vch;
-      if (!C::CODES) {
-        kch = vch = ch ^ (r & 7);
-      } else if (C::DP == 64) {
-        kch = ch;
-        vch = ch ^ (r & 2);
-      } else {
-        kch = ch ^ (r & 4);
-        vch = ch ^ ((r & 3) << 1);
-      }
-      copy16(to + r * C::ROW + kch * 16, static_cast<const char *>(a.cache.d_k) + offset, real);
-      copy16(to + KEYS * C::ROW + r * C::ROW + vch * 16, static_cast<const char *>(a.cache.d_v) + offset, real);
+    for (int u = 0; u < LOOK; ++u) {
+      const bool real = page[u] >= 0 && page[u] < a.cache.pages;
+      row[u] = real ? (uint32_t)page[u] * page_rows + head_row + slot_in_page[u] : 0xffffffffu;
+      if (grouped) break;
     }
-    if (C::CODES) {
+    if (grouped) {
 #pragma unroll
-      for (int u = 0; u < LOOK; ++u) {
-        const bool real = row[u] != 0xffffffffu;
-        if (KEYS == 16 && lane >= 16) break;
-        const uint32_t scales = to + 2 * KEYS * C::ROW + (lane + 32 * u) * 4;
-        copy4(scales, a.cache.d_k_scale + (real ? row[u] : 0), real);
-        copy4(scales + KEYS * 4, a.cache.d_v_scale + (real ? row[u] : 0), real);
+      for (int mt = 0; mt < MT; ++mt) {
+        const uint32_t first = __shfl_sync(0xffffffffu, row[0], mt);
+        const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + mt * 16;
+        const bool real = first != 0xffffffffu, all = real && key >= in.span.lo && key + 16 <= in.span.hi;
+        const int64_t offset = real ? (int64_t)first * row_bytes + low * row_bytes : 0;
+        const char *kp = k_store + offset, *vp = v_store + offset;
+        if (!in_row) continue;
+        if (all) {
+#pragma unroll
+          for (int i = 0; i < 16 / ROWS; ++i) {
+            const int r = mt * 16 + i * ROWS + low;
+            copy16(to + k_at(r), kp + i * ROWS * row_bytes, true);
+            copy16(to + v_at(r), vp + i * ROWS * row_bytes, true);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 / ROWS; ++i) {
+            const int r = mt * 16 + i * ROWS + low, at = key + i * ROWS + low;
+            const bool there = real && at >= in.span.lo && at < in.span.hi;
+            copy16(to + k_at(r), kp + (there ? i * ROWS * row_bytes : 0), there);
+            copy16(to + v_at(r), vp + (there ? i * ROWS * row_bytes : 0), there);
+          }
+        }
+      }
+      if (C::CODES) {
+#pragma unroll
+        for (int u = 0; u < LOOK; ++u) {
+          const int r = lane + 32 * u, at = in.span.origin + in.tile * C::TILE + warp * KEYS + r;
+          const uint32_t first = __shfl_sync(0xffffffffu, row[0], r / 16 % MT);
+          const bool there = first != 0xffffffffu && at >= in.span.lo && at < in.span.hi;
+          if (KEYS == 16 && lane >= 16) break;
+          const uint32_t scales = to + 2 * KEYS * C::ROW + r * 4, from = there ? first + r % 16 : 0;
+          copy4(scales, a.cache.d_k_scale + from, there);
+          copy4(scales + KEYS * 4, a.cache.d_v_scale + from, there);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < KEYS / ROWS; ++i) {
+        const int r = i * ROWS + low;
+        const uint32_t from = __shfl_sync(0xffffffffu, row[LOOK == 2 && i >= KEYS / ROWS / 2 ? 1 : 0], r % 32);
+        if (!in_row) continue;
+        const bool there = from != 0xffffffffu;
+        const int64_t offset = there ? (int64_t)from * row_bytes : 0;
+        copy16(to + k_at(r), k_store + offset, there);
+        copy16(to + v_at(r), v_store + offset, there);
+      }
+      if (C::CODES) {
+#pragma unroll
+        for (int u = 0; u < LOOK; ++u) {
+          const bool there = row[u] != 0xffffffffu;
+          if (KEYS == 16 && lane >= 16) break;
+          const uint32_t scales = to + 2 * KEYS * C::ROW + (lane + 32 * u) * 4;
+          copy4(scales, a.cache.d_k_scale + (there ? row[u] : 0), there);
+          copy4(scales + KEYS * 4, a.cache.d_v_scale + (there ? row[u] : 0), there);
+        }
       }
     }
     if (++in.tile == in.tiles) next_unit(a, in, units, C::TILE);
@@ -624,26 +704,20 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 
   uint32_t q[NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
-  float value_by = 0.0f;     // codes: the power of two that the values' scales are relative to
+  float value_by = 0.0f, values_in = 0.0f;  // codes: the power of two that the values' scales are relative to, and 1 / it
   Sums<DT> sums[NT];
   bool fresh = true;
   int began = out.tile;
+  int64_t began_step = 0;
   int stage = 0, stage_in = STAGES - 1;
   bool first_piece = true;
   for (int64_t step = 0; step < steps; ++step) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2));
-    __syncwarp();
-    if (step + STAGES - 1 < steps) {
-      fetch(stage_in);
-      look_up();
-    }
-    asm volatile("cp.async.commit_group;");
-    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
     const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
     if (fresh) {
       fresh = false;
       began = out.tile;
-      value_by = 0.0f;
+      began_step = step;
+      value_by = values_in = 0.0f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         sums[n].clear();
@@ -682,6 +756,15 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       }
     }
 
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();
+    if (step + STAGES - 1 < steps) {
+      fetch(stage_in);
+      look_up();
+    }
+    asm volatile("cp.async.commit_group;");
+    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+
     const uint32_t ks = ring + stage * C::STAGE, vs = ks + KEYS * C::ROW, scales = vs + KEYS * C::ROW;
     float s[MT][NT][4];
 #pragma unroll
@@ -715,14 +798,15 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     }
 
     // scores of keys (row g, row g + 8 of the tile) and heads (2c, 2c + 1)
-    const int key0 = out.lo + out.tile * C::TILE + warp * KEYS;
+    const int key0 = out.span.origin + out.tile * C::TILE + warp * KEYS;
+    const bool all_seen = key0 >= out.span.lo && key0 + KEYS <= out.span.hi;
     float value_scale[MT][2], most_value = 0.0f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = mt * 16 + e * 8 + (C::CODES ? (g >> 1) + 4 * (g & 1) : g);
-        const bool seen = key0 + r < out.hi;
+        const bool seen = all_seen || (key0 + r >= out.span.lo && key0 + r < out.span.hi);
         float by = 1.0f;
         value_scale[mt][e] = 1.0f;
         if (C::CODES) {
@@ -764,6 +848,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
           const float now = exponent >= 255 ? most_value : __uint_as_float(exponent << 23);
           shrink = value_by / now;
           value_by = now;
+          values_in = 1.0f / now;
         }
       }
 #pragma unroll
@@ -771,7 +856,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          f[i] = exp2f(sums[n].m[i] - base[n][i]);
+          f[i] = power2(sums[n].m[i] - base[n][i]);
           sums[n].l[i] *= f[i];
           sums[n].m[i] = most[n][i];
           f[i] *= shrink;
@@ -785,7 +870,6 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         }
       }
     }
-    const float values_in = C::CODES ? 1.0f / value_by : 1.0f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint32_t high[NT][2], low[NT][2];
@@ -793,11 +877,11 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float p0 = exp2f(s[mt][n][2 * e] - (base[n][0] - C::OFFSET)), p1 = exp2f(s[mt][n][2 * e + 1] - (base[n][1] - C::OFFSET));
+          float p0 = power2(s[mt][n][2 * e] - (base[n][0] - C::OFFSET)), p1 = power2(s[mt][n][2 * e + 1] - (base[n][1] - C::OFFSET));
           sums[n].l[0] += p0;
           sums[n].l[1] += p1;
           if (C::CODES) {
-            const float by = value_scale[mt][e] == 0.0f ? 0.0f : value_scale[mt][e] * values_in;
+            const float by = value_scale[mt][e] * values_in;
             p0 *= by;
             p1 *= by;
           }
@@ -865,6 +949,8 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     const bool unit_ends = ++out.tile == out.tiles;
     if (unit_ends || step + 1 == steps) {
       const bool whole = unit_ends && began == 0;
+      if (!unit_ends && began == 0 && threadIdx.x == 0)
+        a.cuts[blockIdx.x] = {last_share(share, share.from + began_step, out.tiles), first_piece ? 0 : 1, out.request, out.unit};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -885,24 +971,81 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       if (unit_ends) next_unit(a, out, units, C::TILE);
     }
   }
-  pdl_release();
 }
 
-// Adds up what the blocks left of a unit that was cut, in their order: a block for each unit, its warps the shares by turns.
+// Adds up what the blocks left of the units that were cut, in their order: block (share where the unit begins, eight heads, two of
+// the sixteens of dimensions), a thread four sums of every fourth share.
+constexpr int JOIN_THREADS = 256;
 template <typename C>
-__global__ void __launch_bounds__(ATT_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
-  __shared__ __align__(16) float exchange[2 * C::REGS * 32];
-  const int request = blockIdx.y, unit = blockIdx.x, warp = threadIdx.x / 32;
-  const Cut cut = cut_of(a, request, unit, C::TILE);
-  if (cut.first == cut.last) return;
+__global__ void __launch_bounds__(JOIN_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
+  using T = typename C::T;
+  constexpr int PART = C::REGS * 32, PARTS = JOIN_THREADS / 64;
+  __shared__ float weight[MOST_BLOCKS][8], most[8], total[8];
+  __shared__ float4 others[PARTS - 1][64];
   pdl_wait();
-  const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * 8 * C::NT;
-  for (int n = 0; n < C::NT; ++n) {
-    Sums<C::DT> sums;
-    sums.clear();
-    for (int64_t i = cut.first + warp; i <= cut.last; i += MMA_WARPS)
-      sums.add(a.partial + ((i * 2 + (i > cut.first ? 0 : cut.first_slot)) * C::NT + n) * C::REGS * 32);
-    give<C>(a, sums, exchange, request, kv_head * a.group + head0 + n * 8, a.group - head0 - n * 8, nullptr);
+  const Cut cut = a.cuts[blockIdx.x];
+  if (cut.last == 0) return;
+  const int first = blockIdx.x, n = blockIdx.y, shares = cut.last - first + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int first_head = cut.unit / a.head_blocks * a.group, head0 = (cut.unit % a.head_blocks) * 8 * C::NT + n * 8, heads = a.group - head0;
+  auto slot = [&](int i) { return reinterpret_cast<const float4 *>(a.partial + ((int64_t)((first + i) * 2 + (i > 0 ? 0 : cut.slot)) * C::NT + n) * PART); };
+  for (int x = threadIdx.x; x < shares * 4; x += JOIN_THREADS) {  // lane c of a part has m and l of heads 2c and 2c + 1
+    const float4 ml = slot(x / 4)[C::DT * 32 + x % 4];
+    weight[x / 4][2 * (x % 4)] = ml.x;
+    weight[x / 4][2 * (x % 4) + 1] = ml.y;
+  }
+  __syncthreads();
+  {  // warp h: head h
+    float m = -INFINITY, l = 0.0f;
+    for (int i = lane; i < shares; i += 32) m = fmaxf(m, weight[i][warp]);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int i = lane; i < shares; i += 32) {
+      const float f = exp2f(weight[i][warp] - base);
+      const float4 ml = slot(i)[C::DT * 32 + warp / 2];
+      l = fmaf(warp % 2 ? ml.w : ml.z, f, l);
+      weight[i][warp] = f;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (lane == 0) {
+      most[warp] = m;
+      total[warp] = l;
+    }
+  }
+  __syncthreads();
+  const int of = threadIdx.x % 64, part = threadIdx.x / 64, t = blockIdx.z * 2 + of / 32, g = lane / 4, c = lane % 4;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = part; i < shares; i += PARTS) {
+    const float4 x = slot(i)[t * 32 + lane];
+    const float f0 = weight[i][2 * c], f1 = weight[i][2 * c + 1];
+    acc.x = fmaf(x.x, f0, acc.x);
+    acc.y = fmaf(x.y, f1, acc.y);
+    acc.z = fmaf(x.z, f0, acc.z);
+    acc.w = fmaf(x.w, f1, acc.w);
+  }
+  if (part > 0) others[part - 1][of] = acc;
+  __syncthreads();
+  if (part > 0) return;
+#pragma unroll
+  for (int i = 0; i < PARTS - 1; ++i) {
+    const float4 x = others[i][of];
+    acc.x += x.x;
+    acc.y += x.y;
+    acc.z += x.z;
+    acc.w += x.w;
+  }
+  const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (2 * c + i >= heads) continue;
+    const int64_t head = (int64_t)cut.request * a.q_heads + first_head + head0 + 2 * c + i;
+    const float l = total[2 * c + i], by = l == 0.0f ? 0.0f : 1.0f / l;
+    if (t == 0 && g == 0 && a.lse != nullptr) a.lse[head] = l == 0.0f ? -INFINITY : (most[2 * c + i] - C::OFFSET) * LN2 + logf(l);
+    T *const out = static_cast<T *>(a.out) + head * a.dim;
+    if (d0 < a.dim) out[d0] = from_f32<T>((i == 0 ? acc.x : acc.y) * by);
+    if (d1 < a.dim) out[d1] = from_f32<T>((i == 0 ? acc.z : acc.w) * by);
   }
 }
 
@@ -914,14 +1057,10 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
     allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   a.head_blocks = (a.group + 8 * C::NT - 1) / (8 * C::NT);
-  a.blocks = C::BLOCKS * sm_count();
-  a.min_tiles = 4;
-  PoolBuf partial;
-  LAPIS_TRY(partial.alloc((size_t)a.blocks * 2 * C::NT * C::REGS * 32 * sizeof(float), st));
-  a.partial = static_cast<float *>(partial.p);
-  attend_mma_kernel<C><<<a.blocks, ATT_THREADS, C::SMEM, st>>>(a);
-  LAPIS_CUDA_TRY(cudaGetLastError());
-  LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3((unsigned)(a.cache.heads * a.head_blocks), (unsigned)a.requests), ATT_THREADS, 0, st, a));
+  PoolBuf work;
+  LAPIS_TRY(make_workspace(a, work, C::BLOCKS * sm_count(), 2 * C::NT * C::REGS * 32, st));
+  LAPIS_CUDA_TRY(launch_pdl(attend_mma_kernel<C>, dim3(a.blocks), ATT_THREADS, C::SMEM, st, a));
+  LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3(a.blocks, C::NT, C::DT / 2), JOIN_THREADS, 0, st, a));
   return LAPIS_OK;
 }
 

@@ -23,7 +23,7 @@ namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
 constexpr int MIN_TILES = 4;      // of a share, if there is more than one
-constexpr int MOST_BLOCKS = 320;  // shares that a join has room for: two blocks an SM
+constexpr int MOST_BLOCKS = 480;  // shares that a join has room for: three blocks an SM
 constexpr float LN2 = 0.6931471805599453f;
 
 struct AttendArgs {
@@ -379,14 +379,15 @@ struct MmaConfig {
   static constexpr bool TWO_PARTS = !(CODES && std::is_same<T, __nv_bfloat16>::value);
   static constexpr int DP = DP_, NT = NT_;                  // padded head, and eights of query heads
   static constexpr int ROW = DP * (CODES ? 1 : 2);          // bytes of a key in shared memory
-  static constexpr int KEYS = ROW == 64 ? 64 : ROW == 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
+  static constexpr int KEYS = ROW <= 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
-  static constexpr int STAGES = DP <= 128 ? 3 : CODES ? 5 : 3;
-  static constexpr int BLOCKS = DP <= 128 ? 2 : 1;          // an SM
   static constexpr int DT = DP / 16, REGS = DT * 4 + 4;     // values a lane leaves of eight heads: O, m and l
-  static constexpr int EXCHANGE = 2 * REGS * 32 * 4;
+  static constexpr int EXCHANGE = REGS * 32 * 4;
+  static constexpr int BLOCKS = DP == 256 ? 1 : DP == 128 && NT == 2 ? 2 : 3;  // an SM, by registers
+  static constexpr int STAGES = (227 * 1024 / BLOCKS - 1024 - EXCHANGE) / (MMA_WARPS * STAGE);
   static constexpr int SMEM = MMA_WARPS * STAGES * STAGE + EXCHANGE;
+  static_assert(STAGES >= 2, "one is copied while another is read");
   static constexpr float OFFSET = HALF ? 14.0f : 0.0f;
 };
 
@@ -532,16 +533,14 @@ template <typename C>
 __device__ __forceinline__ void give(const AttendArgs &a, Sums<C::DT> &s, float *exchange, int request, int first_head, int heads, float *slot) {
   using T = typename C::T;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
-  constexpr int PART = C::REGS * 32;
-  __syncthreads();
-  if (warp >= 2) s.store(exchange + (warp - 2) * PART);
-  __syncthreads();
-  if (warp < 2) s.add(exchange + warp * PART);
-  __syncthreads();
-  if (warp == 1) s.store(exchange);
-  __syncthreads();
+#pragma unroll 1
+  for (int w = 1; w < MMA_WARPS; ++w) {  // one after the other: shared memory is for what is on its way
+    __syncthreads();
+    if (warp == w) s.store(exchange);
+    __syncthreads();
+    if (warp == 0) s.add(exchange);
+  }
   if (warp != 0) return;
-  s.add(exchange);
   if (slot != nullptr) {
     s.store(slot);
     return;
@@ -591,25 +590,20 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   out = in;
 
   // Pages of the next step to copy, looked up one step ahead.  `grouped`: pages have a multiple of 16 slots, and a lane looks up
-  // 16 keys; otherwise a lane looks up key `lane` (and lane + 32).
-  constexpr int LOOK = KEYS == 64 ? 2 : 1, NONE = -1;
+  // 16 keys; otherwise a lane looks up key `lane`.
   const bool grouped = a.cache.page_size % 16 == 0;
   const int page_size = (int)a.cache.page_size, row_bytes = a.dim * (C::CODES ? 1 : 2);
-  int64_t page[LOOK];
-  int slot_in_page[LOOK];
+  const int of_lane = lane % KEYS;  // the key of a step that is this lane's
+  int64_t page = -1;
+  int slot_in_page = 0;
   auto look_up = [&]() {
-#pragma unroll
-    for (int u = 0; u < LOOK; ++u) {
-      const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + (grouped ? lane % MT * 16 : (KEYS == 16 ? lane % 16 : lane) + 32 * u);
-      page[u] = NONE;
-      slot_in_page[u] = 0;
-      if (key < in.span.hi && key >= (grouped ? in.span.origin : in.span.lo)) {
-        const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
-        slot_in_page[u] = key - nth * page_size;
-        const int64_t entry = in.span.entry + nth;
-        if (entry >= 0 && entry < a.lists.entries) page[u] = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
-      }
-      if (grouped) break;
+    const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + (grouped ? lane % MT * 16 : of_lane);
+    page = -1;
+    if (key < in.span.hi) {
+      const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
+      slot_in_page = key - nth * page_size;
+      const int64_t entry = in.span.entry + nth;
+      if (entry >= 0 && entry < a.lists.entries) page = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
     }
   };
   // Where this lane's piece of 16 bytes of row r goes, r = i * ROWS + lane / CHUNKS: the rows are swizzled so that neither the
@@ -620,87 +614,53 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   auto k_at = [&](int r) { return r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch : ch ^ (r & 4)) * 16; };
   auto v_at = [&](int r) { return KEYS * C::ROW + r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch ^ (r & 2) : ch ^ ((r & 3) << 1)) * 16; };
   const char *const k_store = static_cast<const char *>(a.cache.d_k) + ch * 16, *const v_store = static_cast<const char *>(a.cache.d_v) + ch * 16;
-  const uint32_t head_rows = (uint32_t)page_size, page_rows = (uint32_t)(a.cache.heads * a.cache.page_size);
+  const uint32_t page_rows = (uint32_t)(a.cache.heads * a.cache.page_size);
   auto fetch = [&](int stage) {
-    const uint32_t to = ring + stage * C::STAGE, head_row = (uint32_t)(in.unit / a.head_blocks) * head_rows;
-    uint32_t row[LOOK];
-#pragma unroll
-    for (int u = 0; u < LOOK; ++u) {
-      const bool real = page[u] >= 0 && page[u] < a.cache.pages;
-      row[u] = real ? (uint32_t)page[u] * page_rows + head_row + slot_in_page[u] : 0xffffffffu;
-      if (grouped) break;
-    }
-    if (grouped) {
+    const uint32_t to = ring + stage * C::STAGE;
+    const int key0 = in.span.origin + in.tile * C::TILE + warp * KEYS, key = key0 + of_lane;
+    const bool listed = page >= 0 && page < a.cache.pages;
+    uint32_t row = (uint32_t)page * page_rows + (uint32_t)(in.unit / a.head_blocks * page_size + slot_in_page);
+    const bool plain = key0 >= in.span.lo && key0 + KEYS <= in.span.hi && grouped && __all_sync(0xffffffffu, listed);
+    // the row of this lane's key
+    const uint32_t first = __shfl_sync(0xffffffffu, row, of_lane / 16);
+    const bool first_listed = __shfl_sync(0xffffffffu, listed, of_lane / 16);
+    const bool there = key >= in.span.lo && key < in.span.hi && (grouped ? first_listed : listed);
+    if (grouped) row = first + of_lane % 16;
+    if (!there) row = 0;
+    if (plain) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t first = __shfl_sync(0xffffffffu, row[0], mt);
-        const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + mt * 16;
-        const bool real = first != 0xffffffffu, all = real && key >= in.span.lo && key + 16 <= in.span.hi;
-        const int64_t offset = real ? (int64_t)first * row_bytes + low * row_bytes : 0;
-        const char *kp = k_store + offset, *vp = v_store + offset;
-        if (!in_row) continue;
-        if (all) {
+        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, mt * 16) * row_bytes + low * row_bytes;
+        const char *const kp = k_store + offset, *const vp = v_store + offset;
+        if (in_row) {
 #pragma unroll
           for (int i = 0; i < 16 / ROWS; ++i) {
             const int r = mt * 16 + i * ROWS + low;
             copy16(to + k_at(r), kp + i * ROWS * row_bytes, true);
             copy16(to + v_at(r), vp + i * ROWS * row_bytes, true);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16 / ROWS; ++i) {
-            const int r = mt * 16 + i * ROWS + low, at = key + i * ROWS + low;
-            const bool there = real && at >= in.span.lo && at < in.span.hi;
-            copy16(to + k_at(r), kp + (there ? i * ROWS * row_bytes : 0), there);
-            copy16(to + v_at(r), vp + (there ? i * ROWS * row_bytes : 0), there);
-          }
-        }
-      }
-      if (C::CODES) {
-#pragma unroll
-        for (int u = 0; u < LOOK; ++u) {
-          const int r = lane + 32 * u, at = in.span.origin + in.tile * C::TILE + warp * KEYS + r;
-          const uint32_t first = __shfl_sync(0xffffffffu, row[0], r / 16 % MT);
-          const bool there = first != 0xffffffffu && at >= in.span.lo && at < in.span.hi;
-          if (KEYS == 16 && lane >= 16) break;
-          const uint32_t scales = to + 2 * KEYS * C::ROW + r * 4, from = there ? first + r % 16 : 0;
-          copy4(scales, a.cache.d_k_scale + from, there);
-          copy4(scales + KEYS * 4, a.cache.d_v_scale + from, there);
         }
       }
     } else {
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < KEYS / ROWS; ++i) {
         const int r = i * ROWS + low;
-        const uint32_t from = __shfl_sync(0xffffffffu, row[LOOK == 2 && i >= KEYS / ROWS / 2 ? 1 : 0], r % 32);
-        if (!in_row) continue;
-        const bool there = from != 0xffffffffu;
-        const int64_t offset = there ? (int64_t)from * row_bytes : 0;
-        copy16(to + k_at(r), k_store + offset, there);
-        copy16(to + v_at(r), v_store + offset, there);
-      }
-      if (C::CODES) {
-#pragma unroll
-        for (int u = 0; u < LOOK; ++u) {
-          const bool there = row[u] != 0xffffffffu;
-          if (KEYS == 16 && lane >= 16) break;
-          const uint32_t scales = to + 2 * KEYS * C::ROW + (lane + 32 * u) * 4;
-          copy4(scales, a.cache.d_k_scale + (there ? row[u] : 0), there);
-          copy4(scales + KEYS * 4, a.cache.d_v_scale + (there ? row[u] : 0), there);
+        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, r) * row_bytes;
+        const bool real = __shfl_sync(0xffffffffu, there, r);
+        if (in_row) {
+          copy16(to + k_at(r), k_store + offset, real);
+          copy16(to + v_at(r), v_store + offset, real);
         }
       }
+    }
+    if (C::CODES && lane < KEYS) {
+      const uint32_t scales = to + 2 * KEYS * C::ROW + lane * 4;
+      copy4(scales, a.cache.d_k_scale + row, there);
+      copy4(scales + KEYS * 4, a.cache.d_v_scale + row, there);
     }
     if (++in.tile == in.tiles) next_unit(a, in, units, C::TILE);
   };
   look_up();
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (s < steps) {
-      fetch(s);
-      look_up();
-    }
-    asm volatile("cp.async.commit_group;");
-  }
 
   uint32_t q[NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
@@ -709,61 +669,64 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   bool fresh = true;
   int began = out.tile;
   int64_t began_step = 0;
-  int stage = 0, stage_in = STAGES - 1;
+  int stage = 0, stage_in = 0;
   bool first_piece = true;
-  for (int64_t step = 0; step < steps; ++step) {
+  auto load_q = [&](int64_t step) {
     const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
-    if (fresh) {
-      fresh = false;
-      began = out.tile;
-      began_step = step;
-      value_by = values_in = 0.0f;
+    fresh = false;
+    began = out.tile;
+    began_step = step;
+    value_by = values_in = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        sums[n].clear();
-        const bool real = head0 + n * 8 + g < a.group;
-        const T *const from = static_cast<const T *>(a.q) + (int64_t)out.request * a.q_token_stride +
-                              (int64_t)(kv_head * a.group + (real ? head0 + n * 8 + g : 0)) * a.q_head_stride;
-        float x[DT][4], most = 0.0f;
+    for (int n = 0; n < NT; ++n) {
+      sums[n].clear();
+      const bool real = head0 + n * 8 + g < a.group;
+      const T *const from = static_cast<const T *>(a.q) + (int64_t)out.request * a.q_token_stride +
+                            (int64_t)(kv_head * a.group + (real ? head0 + n * 8 + g : 0)) * a.q_head_stride;
+      float x[DT][4], most = 0.0f;
 #pragma unroll
-        for (int k = 0; k < DT; ++k) {
+      for (int k = 0; k < DT; ++k) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = C::CODES ? (k / 4) * 64 + c * 16 + (k % 4) * 4 + e : k * 16 + c * 2 + (e & 1) + (e & 2) * 4;
-            x[k][e] = real && d < a.dim ? to_f32(from[d]) : 0.0f;
-            most = fmaxf(most, fabsf(x[k][e]));
-          }
-        }
-        float by = 1.0f;
-        if (C::CODES) {  // to [1, 2): 2^(127 - exponent)
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const int exponent = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
-          by = __uint_as_float((uint32_t)(254 - exponent) << 23);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int e = __shfl_sync(0xffffffffu, exponent, (2 * c + i) * 4);
-            score_by[n][i] = a.scale2 * __uint_as_float((uint32_t)e << 23);
-          }
-        } else {
-          score_by[n][0] = score_by[n][1] = a.scale2;
-        }
-#pragma unroll
-        for (int k = 0; k < DT; ++k) {
-          q[n][k][0] = pack2<C::HALF>(x[k][0] * by, x[k][1] * by);
-          q[n][k][1] = pack2<C::HALF>(x[k][2] * by, x[k][3] * by);
+        for (int e = 0; e < 4; ++e) {
+          const int d = C::CODES ? (k / 4) * 64 + c * 16 + (k % 4) * 4 + e : k * 16 + c * 2 + (e & 1) + (e & 2) * 4;
+          x[k][e] = real && d < a.dim ? to_f32(from[d]) : 0.0f;
+          most = fmaxf(most, fabsf(x[k][e]));
         }
       }
+      float by = 1.0f;
+      if (C::CODES) {  // to [1, 2): 2^(127 - exponent)
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int exponent = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
+        by = __uint_as_float((uint32_t)(254 - exponent) << 23);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int e = __shfl_sync(0xffffffffu, exponent, (2 * c + i) * 4);
+          score_by[n][i] = a.scale2 * __uint_as_float((uint32_t)e << 23);
+        }
+      } else {
+        score_by[n][0] = score_by[n][1] = a.scale2;
+      }
+#pragma unroll
+      for (int k = 0; k < DT; ++k) {
+        q[n][k][0] = pack2<C::HALF>(x[k][0] * by, x[k][1] * by);
+        q[n][k][1] = pack2<C::HALF>(x[k][2] * by, x[k][3] * by);
+      }
     }
-
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+  };
+#pragma unroll 1
+  for (int64_t step = 1 - STAGES; step < steps; ++step) {
+    if (step >= 0 && fresh) load_q(step);
+    if (step >= 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
     if (step + STAGES - 1 < steps) {
       fetch(stage_in);
       look_up();
     }
-    asm volatile("cp.async.commit_group;");
+    asm volatile("cp.async.commit_group;" ::: "memory");
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    if (step < 0) continue;
+    const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
 
     const uint32_t ks = ring + stage * C::STAGE, vs = ks + KEYS * C::ROW, scales = vs + KEYS * C::ROW;
     float s[MT][NT][4];

@@ -78,29 +78,24 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, place, eps: float = 1e-6, i
 
     ``cos``/``sin`` [places, rot / 2]: the first ``rot`` values of a head are turned in pairs (i, i + rot/2), or (2i, 2i+1)
     with ``interleaved``.  Computed in 32 bits.  A token whose place is outside the tables is padding and gives zeros."""
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    status = _calls.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_out, k_out)
-    if status:
-        if status < 0:
+    got = _calls.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place)
+    if type(got) is int:
+        if got < 0:
             _check_rows("q", q, q.dtype, q.shape[0], q.shape[-1])
             _check_rows("k", k, q.dtype, q.shape[0], q.shape[2])
             _check_how(q.dtype, q.shape[2], q_weight, k_weight, cos, sin)
             _check_indices(getattr(place, "dtype", None), place=(place, q.shape[0]))
             _raise("qk_norm_rope")
-        check(status)
-    return q_out, k_out
+        check(got)
+    return got
 
 
 def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, place, eps: float = 1e-6, interleaved: bool = False):
     """Gradients of :func:`qk_norm_rope` for those of its outputs, ``dq`` and ``dk``, and its inputs: (of q, of k, of
     q_weight, of k_weight).  Those of the weights are float32, sums over all tokens and heads in a fixed order."""
-    q_grad = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_grad = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    weights = torch.empty((2, q.shape[-1]), dtype=torch.float32, device=q.device)
-    status = _calls.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_grad, k_grad, weights)
-    if status:
-        if status < 0:
+    got = _calls.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place)
+    if type(got) is int:
+        if got < 0:
             _check_rows("q", q, q.dtype, q.shape[0], q.shape[-1])
             _check_rows("k", k, q.dtype, q.shape[0], q.shape[2])
             _check_rows("dq", dq, q.dtype, q.shape[0], q.shape[2], q.shape[1])
@@ -108,8 +103,9 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, place, eps
             _check_how(q.dtype, q.shape[2], q_weight, k_weight, cos, sin)
             _check_indices(getattr(place, "dtype", None), place=(place, q.shape[0]))
             _raise("qk_norm_rope_backward")
-        check(status)
-    return q_grad, k_grad, weights[0], weights[1]
+        check(got)
+    q_grad, k_grad, weights = got
+    return q_grad, k_grad, *weights.unbind()
 
 
 class PagedCache:
@@ -180,33 +176,30 @@ class PagedCache:
         """:func:`qk_norm_rope` and :meth:`append` in one launch: returns the queries; the keys are quantised, where the cache
         is, from 32 bits, without a rounding to their own type in between.  Padding (see there) is not written."""
         self._here("append_norm_rope")
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        status = _calls.kv_append_norm_rope(self._addr, q, k, v, q_weight, k_weight, cos, sin, eps, interleaved, pos, crd, row, place, q_out)
-        if status:
-            if status < 0:
+        got = _calls.kv_append_norm_rope(self._addr, q, k, v, q_weight, k_weight, cos, sin, eps, interleaved, pos, crd, row, place)
+        if type(got) is int:
+            if got < 0:
                 self._check_new(k, v, pos, crd, row, place)
                 _check_rows("q", q, k.dtype, k.shape[0], self.dim)
                 _check_how(k.dtype, self.dim, q_weight, k_weight, cos, sin)
                 _raise("append_norm_rope")
-            check(status)
-        return q_out
+            check(got)
+        return got
 
     def read(self, pos, crd, row, place, dtype: torch.dtype = torch.bfloat16):
         """(k, v) [tokens, heads, dim] of the tokens at ``place[t]`` of requests ``row[t]``, in ``dtype``; zeros where the lists
         name no page."""
         self._here("read")
-        shape = (row.numel(), self.heads, self.dim)
-        k, v = torch.empty(shape, dtype=dtype, device=self.k.device), torch.empty(shape, dtype=dtype, device=self.k.device)
-        status = _calls.kv_read(self._addr, pos, crd, row, place, k, v)
-        if status:
-            if status < 0:
-                if dtype not in _ROW_TYPES:
-                    raise TypeError("read: dtype must be float32, float16 or bfloat16")
+        if dtype not in _ROW_TYPES:
+            raise TypeError("read: dtype must be float32, float16 or bfloat16")
+        got = _calls.kv_read(self._addr, pos, crd, row, place, _CACHE_TYPES[dtype])
+        if type(got) is int:
+            if got < 0:
                 _check_lists(pos, crd)
                 _check_indices(pos.dtype, crd=(crd, None), row=(row, row.numel()), place=(place, row.numel()))
                 _raise("read")
-            check(status)
-        return k, v
+            check(got)
+        return got
 
 
 def paged_attention(q, cache: PagedCache, pos, crd, length, scale: float | None = None, window: int = 0, return_lse: bool = False):
@@ -217,14 +210,12 @@ def paged_attention(q, cache: PagedCache, pos, crd, length, scale: float | None 
     the natural logarithm of each head's sum of exponentials, float32 [requests, heads], with which results over parts of a
     context are joined.  A request of length 0 gets zeros and -inf."""
     cache._here("paged_attention")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    status = _calls.paged_attention(cache._addr, q, pos, crd, length, cache.dim ** -0.5 if scale is None else scale, window or 0, out, lse)
-    if status:
-        if status < 0:
+    got = _calls.paged_attention(cache._addr, q, pos, crd, length, cache.dim ** -0.5 if scale is None else scale, window or 0, return_lse)
+    if type(got) is int:
+        if got < 0:
             _check_rows("q", q, getattr(q, "dtype", None), q.shape[0], cache.dim)
             _check_lists(pos, crd)
             _check_indices(pos.dtype, crd=(crd, None), length=(length, q.shape[0]))
             _raise("paged_attention")
-        check(status)
-    return (out, lse) if return_lse else out
+        check(got)
+    return got

@@ -23,6 +23,7 @@ namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
 constexpr int MIN_TILES = 4;      // of a share, if there is more than one
+constexpr int WHOLE_TILES = 4;    // by which a unit may be longer than a share and is not cut
 constexpr int MOST_BLOCKS = 480;  // shares that a join has room for: three blocks an SM
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -124,7 +125,7 @@ __device__ __forceinline__ Share find_share(const AttendArgs &a, int tile) {
   }
   s.shares = (int)max((int64_t)1, min((int64_t)a.blocks, s.all / MIN_TILES));
   const int64_t all_units = (int64_t)a.requests * units;
-  s.whole = all_units <= a.blocks && (longest - 4) * (int64_t)s.shares <= s.all;
+  s.whole = all_units <= a.blocks && (longest - WHOLE_TILES) * (int64_t)s.shares <= s.all;
   if (s.whole) {
     s.from = 0;
     s.steps = me < all_units ? tiles_of(s.span, tile) : 0;
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
   pdl_wait();
   const Share s = find_share(a, ANY_TILE);
   pdl_release();
-  if (threadIdx.x == 0) a.cuts[blockIdx.x].last = 0;
+  if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
   int request = s.request, unit = s.unit, tile = s.tile;
   Span span = s.span;
   const int units = (int)a.cache.heads * a.head_blocks;
@@ -328,9 +329,15 @@ __global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_cons
   if (threadIdx.x == 0 && a.lse != nullptr) a.lse[head] = sum == 0.0f ? -INFINITY : most * LN2 + logf(sum);
 }
 
+// Whether the lists cannot hold more than what find_share leaves whole: then nothing is cut, and there is nothing to join (a short
+// request of one user: 1 x 129 tokens %%).
+static bool always_whole(const AttendArgs &a, int tile) {
+  const int64_t most_tokens = a.lists.entries > MOST_TOKENS / a.cache.page_size ? MOST_TOKENS : a.lists.entries * a.cache.page_size;
+  return (int64_t)a.requests * a.cache.heads * a.head_blocks <= a.blocks && most_tokens <= WHOLE_TILES * tile - 16;
+}
+
 // The workspace of a call: `floats` for the pieces of each block, and the cuts behind them.
-static int make_workspace(AttendArgs &a, PoolBuf &work, int blocks, size_t floats, cudaStream_t st) {
-  a.blocks = std::min(blocks, MOST_BLOCKS);
+static int make_workspace(AttendArgs &a, PoolBuf &work, size_t floats, cudaStream_t st) {
   const size_t pieces = ((size_t)a.blocks * floats * sizeof(float) + 15) / 16 * 16;
   LAPIS_TRY(work.alloc(pieces + a.blocks * sizeof(Cut), st));
   a.partial = static_cast<float *>(work.p);
@@ -346,9 +353,12 @@ static int launch_any(AttendArgs a, int dev, cudaStream_t st) {
     allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   a.head_blocks = (a.group + ANY_HEADS - 1) / ANY_HEADS;
+  a.blocks = std::min(2 * sm_count(), MOST_BLOCKS);
   PoolBuf work;
-  LAPIS_TRY(make_workspace(a, work, 2 * sm_count(), 2 * ANY_HEADS * (a.dim + 2), st));
+  const bool whole = always_whole(a, ANY_TILE);
+  if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * ANY_HEADS * (a.dim + 2), st));
   LAPIS_CUDA_TRY(launch_pdl(attend_any_kernel<T>, dim3(a.blocks), ATT_THREADS, any_smem(a.dim), st, a));
+  if (whole) return LAPIS_OK;
   LAPIS_CUDA_TRY(launch_pdl(join_any_kernel<T>, dim3(a.blocks, ANY_HEADS), ATT_THREADS, 0, st, a));
   return LAPIS_OK;
 }
@@ -574,7 +584,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   pdl_wait();
   const Share share = find_share(a, C::TILE);
   pdl_release();
-  if (threadIdx.x == 0) a.cuts[blockIdx.x].last = 0;
+  if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
   const int64_t steps = share.steps;
   if (steps == 0) return;
   if (a.dim != C::DP)  // what is beyond the head is never copied
@@ -1020,9 +1030,12 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
     allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
   }
   a.head_blocks = (a.group + 8 * C::NT - 1) / (8 * C::NT);
+  a.blocks = std::min(C::BLOCKS * sm_count(), MOST_BLOCKS);
   PoolBuf work;
-  LAPIS_TRY(make_workspace(a, work, C::BLOCKS * sm_count(), 2 * C::NT * C::REGS * 32, st));
-  LAPIS_CUDA_TRY(launch_pdl(attend_mma_kernel<C>, dim3(a.blocks), ATT_THREADS, C::SMEM, st, a));
+  const bool whole = always_whole(a, C::TILE);
+  if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * C::NT * C::REGS * 32, st));
+  LAPIS_CUDA_TRY(launch_pdl(attend_mma_kernel<C>, dim3(whole ? a.requests * (int)a.cache.heads * a.head_blocks : a.blocks), ATT_THREADS, C::SMEM, st, a));
+  if (whole) return LAPIS_OK;
   LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3(a.blocks, C::NT, C::DT / 2), JOIN_THREADS, 0, st, a));
   return LAPIS_OK;
 }

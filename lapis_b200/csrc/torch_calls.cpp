@@ -4,11 +4,13 @@
 // A small call is bound by the host: at 10,000 rows the SpMV kernel takes 2-3 us and the launch 2 us, while the same
 // checks written in Python with a ctypes call took 11 us (3.5 us of it torch.cuda.current_stream()).
 // Every function returns the library's status, or -1 when an operand is not the kind of tensor it takes; the caller
-// (lapis_b200/device.py) then names the operand in the exception it raises.
+// (lapis_b200/device.py) then names the operand in the exception it raises.  Those of lapis_b200/attention.py make their results
+// here (torch.empty took 3.3 us where it was measured, at::empty 0.8) and return them where all went well.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
@@ -149,13 +151,15 @@ bool heads_of(PyObject *o, int type, int64_t tokens, int64_t dim, lapis_b200_hea
   *h = {addr(t), t->size(1), t->stride(0), t->stride(1)};
   return true;
 }
-// A contiguous result [tokens, heads, dim].
-bool result_of(PyObject *o, int type, int64_t tokens, int64_t heads, int64_t dim, void **p) {
-  const at::Tensor *t = tensor(o);
-  if (t == nullptr || t->dim() != 3 || !on_device(t) || type_of(t) != type || !t->is_contiguous()) return false;
-  if (t->size(0) != tokens || t->size(1) != heads || t->size(2) != dim) return false;
-  *p = addr(t);
-  return true;
+at::Tensor result(const at::Tensor *like, at::IntArrayRef sizes) { return at::empty(sizes, like->options()); }
+at::Tensor result(const at::Tensor *like, at::ScalarType type, at::IntArrayRef sizes) { return at::empty(sizes, like->options().dtype(type)); }
+// The status of a call where it is not 0; otherwise the results, one as itself, several as a tuple.
+template <typename... R>
+PyObject *results(PyObject *code, const R &...r) {
+  if (code == nullptr || PyLong_AsLong(code) != 0) return code;
+  Py_DECREF(code);
+  if constexpr (sizeof...(R) == 1) return THPVariable_Wrap(r...);
+  return Py_BuildValue(sizeof...(R) == 2 ? "(NN)" : "(NNN)", THPVariable_Wrap(r)...);
 }
 bool indices_of(PyObject *o, int64_t count, int *idx_bytes, const void **p) {
   const at::Tensor *t = tensor(o);
@@ -190,9 +194,9 @@ bool norm_rope_of(PyObject *const *a, int type, int64_t dim, lapis_b200_norm_rop
 }
 const lapis_b200_kv_cache *cache_of(PyObject *o) { return static_cast<const lapis_b200_kv_cache *>(PyLong_AsVoidPtr(o)); }
 
-// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_out, k_out)
+// qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place) -> q, k
 PyObject *py_qk_norm_rope(PyObject *const *a) {
-  const at::Tensor *q = tensor(a[0]);
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]);
   if (q == nullptr || q->dim() != 3) return status(-1);
   const int64_t tokens = q->size(0), dim = q->size(2);
   const int type = type_of(q);
@@ -200,18 +204,17 @@ PyObject *py_qk_norm_rope(PyObject *const *a) {
   lapis_b200_norm_rope how;
   int idx_bytes = 0;
   const void *place;
-  void *q_out, *k_out;
   if (type < 0 || !heads_of(a[0], type, tokens, dim, &hq) || !heads_of(a[1], type, tokens, dim, &hk) || !norm_rope_of(a + 2, type, dim, &how) ||
-      !indices_of(a[8], tokens, &idx_bytes, &place) || !result_of(a[9], type, tokens, hq.heads, dim, &q_out) ||
-      !result_of(a[10], type, tokens, hk.heads, dim, &k_out))
+      !indices_of(a[8], tokens, &idx_bytes, &place))
     return status(-1);
   if (PyErr_Occurred()) return nullptr;
-  return call(lapis_b200_qk_norm_rope, type, tokens, dim, &hq, &hk, &how, idx_bytes, place, q_out, k_out, stream());
+  const at::Tensor q_out = result(q, q->sizes()), k_out = result(k, k->sizes());
+  return results(call(lapis_b200_qk_norm_rope, type, tokens, dim, &hq, &hk, &how, idx_bytes, place, addr(&q_out), addr(&k_out), stream()), q_out, k_out);
 }
 
-// qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place, q_grad, k_grad, weight_grads [2, dim])
+// qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place) -> of q, of k, of the weights [2, dim]
 PyObject *py_qk_norm_rope_backward(PyObject *const *a) {
-  const at::Tensor *q = tensor(a[2]), *dw = tensor(a[13]);
+  const at::Tensor *q = tensor(a[2]), *k = tensor(a[3]);
   if (q == nullptr || q->dim() != 3) return status(-1);
   const int64_t tokens = q->size(0), dim = q->size(2);
   const int type = type_of(q);
@@ -219,16 +222,16 @@ PyObject *py_qk_norm_rope_backward(PyObject *const *a) {
   lapis_b200_norm_rope how;
   int idx_bytes = 0;
   const void *place;
-  void *q_grad, *k_grad;
   if (type < 0 || !heads_of(a[0], type, tokens, dim, &hdq) || !heads_of(a[1], type, tokens, dim, &hdk) ||
       !heads_of(a[2], type, tokens, dim, &hq) || !heads_of(a[3], type, tokens, dim, &hk) || !norm_rope_of(a + 4, type, dim, &how) ||
-      !indices_of(a[10], tokens, &idx_bytes, &place) || !result_of(a[11], type, tokens, hq.heads, dim, &q_grad) ||
-      !result_of(a[12], type, tokens, hk.heads, dim, &k_grad) || !is(dw, at::kFloat) || !on_device(dw) || dw->numel() != 2 * dim)
+      !indices_of(a[10], tokens, &idx_bytes, &place) || hdq.heads != hq.heads || hdk.heads != hk.heads)
     return status(-1);
   if (PyErr_Occurred()) return nullptr;
-  float *const dqw = addr_of<float>(dw);
-  return call(lapis_b200_qk_norm_rope_backward, type, tokens, dim, &hdq, &hdk, &hq, &hk, &how, idx_bytes, place, q_grad, k_grad, dqw,
-              dqw == nullptr ? nullptr : dqw + dim, stream());
+  const at::Tensor q_grad = result(q, q->sizes()), k_grad = result(k, k->sizes()), weights = result(q, at::kFloat, {2, dim});
+  float *const dqw = addr_of<float>(&weights);
+  return results(call(lapis_b200_qk_norm_rope_backward, type, tokens, dim, &hdq, &hdk, &hq, &hk, &how, idx_bytes, place, addr(&q_grad), addr(&k_grad), dqw,
+                      dqw == nullptr ? nullptr : dqw + dim, stream()),
+                 q_grad, k_grad, weights);
 }
 
 // kv_append(cache, k, v, pos, crd, row, place)
@@ -247,10 +250,10 @@ PyObject *py_kv_append(PyObject *const *a) {
   return call(lapis_b200_kv_append, type, tokens, nullptr, &hk, &hv, nullptr, cache, &lists, row, place, nullptr, stream());
 }
 
-// kv_append_norm_rope(cache, q, k, v, q_weight, k_weight, cos, sin, eps, interleaved, pos, crd, row, place, q_out)
+// kv_append_norm_rope(cache, q, k, v, q_weight, k_weight, cos, sin, eps, interleaved, pos, crd, row, place) -> q
 PyObject *py_kv_append_norm_rope(PyObject *const *a) {
   const lapis_b200_kv_cache *cache = cache_of(a[0]);
-  const at::Tensor *k = tensor(a[2]);
+  const at::Tensor *q = tensor(a[1]), *k = tensor(a[2]);
   if (cache == nullptr || k == nullptr || k->dim() != 3) return status(-1);
   const int64_t tokens = k->size(0);
   const int type = type_of(k);
@@ -258,53 +261,54 @@ PyObject *py_kv_append_norm_rope(PyObject *const *a) {
   lapis_b200_norm_rope how;
   lapis_b200_page_lists lists;
   const void *row, *place;
-  void *q_out;
   if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hq) || !heads_of(a[2], type, tokens, cache->dim, &hk) ||
       !heads_of(a[3], type, tokens, cache->dim, &hv) || !norm_rope_of(a + 4, type, cache->dim, &how) || !lists_of(a[10], a[11], &lists) ||
-      !indices_of(a[12], tokens, &lists.idx_bytes, &row) || !indices_of(a[13], tokens, &lists.idx_bytes, &place) ||
-      !result_of(a[14], type, tokens, hq.heads, cache->dim, &q_out))
+      !indices_of(a[12], tokens, &lists.idx_bytes, &row) || !indices_of(a[13], tokens, &lists.idx_bytes, &place))
     return status(-1);
   if (PyErr_Occurred()) return nullptr;
-  return call(lapis_b200_kv_append, type, tokens, &hq, &hk, &hv, &how, cache, &lists, row, place, q_out, stream());
+  const at::Tensor q_out = result(q, q->sizes());
+  return results(call(lapis_b200_kv_append, type, tokens, &hq, &hk, &hv, &how, cache, &lists, row, place, addr(&q_out), stream()), q_out);
 }
 
-// kv_read(cache, pos, crd, row, place, k_out, v_out)
+// kv_read(cache, pos, crd, row, place, type: LAPIS_F32, LAPIS_F16 or LAPIS_BF16) -> k, v
 PyObject *py_kv_read(PyObject *const *a) {
   const lapis_b200_kv_cache *cache = cache_of(a[0]);
-  const at::Tensor *k = tensor(a[5]), *row_of = tensor(a[3]);
-  if (cache == nullptr || k == nullptr || row_of == nullptr) return status(-1);
+  const at::Tensor *row_of = tensor(a[3]);
+  const long type = PyLong_AsLong(a[5]);
+  if (cache == nullptr || row_of == nullptr || type < LAPIS_F32 || type > LAPIS_BF16) return status(-1);
   const int64_t tokens = row_of->numel();
-  const int type = type_of(k);
   lapis_b200_page_lists lists;
   const void *row, *place;
-  void *k_out, *v_out;
-  if (type < 0 || !lists_of(a[1], a[2], &lists) || !indices_of(a[3], tokens, &lists.idx_bytes, &row) ||
-      !indices_of(a[4], tokens, &lists.idx_bytes, &place) || !result_of(a[5], type, tokens, cache->heads, cache->dim, &k_out) ||
-      !result_of(a[6], type, tokens, cache->heads, cache->dim, &v_out))
+  if (!lists_of(a[1], a[2], &lists) || !indices_of(a[3], tokens, &lists.idx_bytes, &row) || !indices_of(a[4], tokens, &lists.idx_bytes, &place))
     return status(-1);
-  return call(lapis_b200_kv_read, cache, &lists, tokens, row, place, type, k_out, v_out, stream());
+  const at::ScalarType scalar = type == LAPIS_F32 ? at::kFloat : type == LAPIS_F16 ? at::kHalf : at::kBFloat16;
+  const at::Tensor k = result(row_of, scalar, {tokens, cache->heads, cache->dim}), v = result(row_of, scalar, {tokens, cache->heads, cache->dim});
+  return results(call(lapis_b200_kv_read, cache, &lists, tokens, row, place, type, addr(&k), addr(&v), stream()), k, v);
 }
 
-// paged_attention(cache, q, pos, crd, length, scale, window, out, lse or None)
+// paged_attention(cache, q, pos, crd, length, scale, window, return_lse) -> out, or out and lse
 PyObject *py_paged_attention(PyObject *const *a) {
   const lapis_b200_kv_cache *cache = cache_of(a[0]);
-  const at::Tensor *q = tensor(a[1]), *lse = tensor(a[8]);
+  const at::Tensor *q = tensor(a[1]);
   if (cache == nullptr || q == nullptr || q->dim() != 3) return status(-1);
   const int64_t requests = q->size(0);
   const int type = type_of(q);
   lapis_b200_heads hq;
   lapis_b200_page_lists lists;
   const void *length;
-  void *out;
   const double scale = PyFloat_AsDouble(a[5]);
   const long long window = PyLong_AsLongLong(a[6]);
-  if (type < 0 || !heads_of(a[1], type, requests, cache->dim, &hq) || !lists_of(a[2], a[3], &lists) ||
-      !indices_of(a[4], requests, &lists.idx_bytes, &length) || !result_of(a[7], type, requests, hq.heads, cache->dim, &out))
-    return status(-1);
-  if (a[8] != Py_None && (!is(lse, at::kFloat) || !on_device(lse) || lse->numel() != requests * hq.heads)) return status(-1);
+  const int with_lse = PyObject_IsTrue(a[7]);
   if (PyErr_Occurred()) return nullptr;
-  return call(lapis_b200_paged_attention, type, requests, &hq, cache, &lists, length, scale, window, out,
-              lse == nullptr ? nullptr : addr_of<float>(lse), stream());
+  if (type < 0 || !heads_of(a[1], type, requests, cache->dim, &hq) || !lists_of(a[2], a[3], &lists) ||
+      !indices_of(a[4], requests, &lists.idx_bytes, &length))
+    return status(-1);
+  const at::Tensor out = result(q, q->sizes());
+  if (!with_lse)
+    return results(call(lapis_b200_paged_attention, type, requests, &hq, cache, &lists, length, scale, window, addr(&out), nullptr, stream()), out);
+  const at::Tensor lse = result(q, at::kFloat, {requests, hq.heads});
+  return results(call(lapis_b200_paged_attention, type, requests, &hq, cache, &lists, length, scale, window, addr(&out), addr_of<float>(&lse), stream()),
+                 out, lse);
 }
 
 template <PyObject *(*CALL)(PyObject *const *), Py_ssize_t ARGS>
@@ -313,9 +317,9 @@ PyMethodDef method(const char *name) {
 }
 PyMethodDef methods[] = {method<py_spmv, 6>("spmv"),   method<py_spmm, 6>("spmm"),   method<py_spmm_dcsr, 7>("spmm_dcsr"),
                          method<py_bspmm, 7>("bspmm"), method<py_bgemm, 3>("bgemm"),
-                         method<py_qk_norm_rope, 11>("qk_norm_rope"), method<py_qk_norm_rope_backward, 14>("qk_norm_rope_backward"),
-                         method<py_kv_append, 7>("kv_append"), method<py_kv_append_norm_rope, 15>("kv_append_norm_rope"),
-                         method<py_kv_read, 7>("kv_read"), method<py_paged_attention, 9>("paged_attention"), {nullptr, nullptr, 0, nullptr}};
+                         method<py_qk_norm_rope, 9>("qk_norm_rope"), method<py_qk_norm_rope_backward, 11>("qk_norm_rope_backward"),
+                         method<py_kv_append, 7>("kv_append"), method<py_kv_append_norm_rope, 14>("kv_append_norm_rope"),
+                         method<py_kv_read, 6>("kv_read"), method<py_paged_attention, 8>("paged_attention"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -22,7 +22,8 @@
 namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
-constexpr int MIN_TILES = 4;      // of a share, if there is more than one
+constexpr int UNIT_COST = 1;      // what a unit costs beside its tiles, in tiles
+constexpr int MIN_WORK = 4;       // of a share, if there is more than one
 constexpr int WHOLE_TILES = 4;    // by which a unit may be longer than a share and is not cut
 constexpr int MOST_BLOCKS = 480;  // shares that a join has room for: three blocks an SM
 constexpr float LN2 = 0.6931471805599453f;
@@ -43,6 +44,7 @@ struct AttendArgs {
   struct Cut *cuts;   // one for each block
   int blocks;
   int page_shift;  // log2 of the slots of a page, or -1
+  int q_pairs;     // two 16-bit values of q lie at a multiple of 4 bytes
 };
 
 // A request's tokens beyond these are not looked at: places are 32-bit numbers in the kernels.
@@ -67,97 +69,135 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int request) {
 // Tiles of a unit of a request; a request without tokens has one, which writes its zeros.
 __device__ __forceinline__ int tiles_of(const Span &s, int tile) { return max(1, (s.hi - s.origin + tile - 1) / tile); }
 
-// n * all / shares: where share n of the tiles begins.
+// n * all / shares: where share n of the work begins.
 __device__ __forceinline__ int64_t share_start(int n, int64_t all, int shares) {
   if (all < (1 << 22) && shares < (1 << 10)) return (uint32_t)n * (uint32_t)all / (uint32_t)shares;
   return n * all / shares;
 }
 
-// A block's share of the tiles.  Where units are few and none is much longer than a share would be, a share is one unit, and
-// nothing has to be joined; otherwise the shares are equal and cut units anywhere.
-struct Share {
-  int64_t all, from, steps;  // tiles of all units; this share's
-  int shares;
-  bool whole;
-  int request, unit, tile;  // of its first one
+// A block's way through its share.  The work of a unit is UNIT_COST, for its queries and its result, and one for each tile, in
+// this order; all units lie one behind the other, and a share is a stretch of that line.  A unit's tile belongs to the share
+// that it lies in.
+struct Walk {
+  int request, unit, tile, end, tiles;  // of this unit: the next tile, the first one that is not this share's, and how many it has
+  int64_t left;                         // from the unit's beginning to the share's end
   Span span;
+  bool done;
+
+  __device__ __forceinline__ void enter(int tile_keys) {
+    tiles = tiles_of(span, tile_keys);
+    end = (int)min((int64_t)tiles, left - UNIT_COST);
+    done = end <= tile;
+  }
+  __device__ __forceinline__ void next_unit(const AttendArgs &a, int units, int tile_keys) {
+    left -= UNIT_COST + tiles;
+    tile = 0;
+    done = left <= UNIT_COST;
+    if (done) return;
+    if (++unit == units) {
+      unit = 0;
+      if (++request == a.requests) {
+        done = true;
+        return;
+      }
+      span = span_of(a, request);
+    }
+    enter(tile_keys);
+  }
+  __device__ __forceinline__ void next_tile(const AttendArgs &a, int units, int tile_keys) {
+    if (++tile == end) next_unit(a, units, tile_keys);
+  }
 };
 
-// Sums the tiles of all requests (a thread takes a run of them) and finds the unit of this block's first one.  All threads return
-// the same; steps is 0 for a block that gets none.
-__device__ __forceinline__ Share find_share(const AttendArgs &a, int tile) {
-  __shared__ int64_t warp_sums[ATT_THREADS / 32];
-  __shared__ int warp_longest[ATT_THREADS / 32], found_request, found_unit, found_tile;
+struct Share {
+  int64_t all, to;  // all work, and where this share ends
+  int shares;
+  // The last share that has a tile of the unit that begins where `left` is left of this one.
+  __device__ __forceinline__ int last_of(int64_t left, int tiles) const {
+    // the share of position x is the largest n with n * all / shares < x + 1
+    const int64_t x = to - left + UNIT_COST + tiles;
+    if (all < (1 << 22) && shares < (1 << 10)) return (int)(((uint32_t)x * (uint32_t)shares + (uint32_t)all - 1) / (uint32_t)all) - 1;
+    return (int)((x * shares + all - 1) / all) - 1;
+  }
+};
+
+// Sums the work of all requests (a thread takes a run of them) and finds where this block's share begins; all threads return the
+// same.  Where units are few and none is much longer than a share would be, every unit is a share, and nothing has to be
+// joined; otherwise the shares are equal and cut units anywhere.
+__device__ __forceinline__ Share find_share(const AttendArgs &a, int tile_keys, Walk &w) {
+  __shared__ int64_t warp_sums[ATT_THREADS / 32], found_left;
+  __shared__ int warp_longest[ATT_THREADS / 32], found_request, found_unit;
   __shared__ Span found_span;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, units = (int)a.cache.heads * a.head_blocks, me = blockIdx.x;
-  const int run = (a.requests + ATT_THREADS - 1) / ATT_THREADS, first = threadIdx.x * run;
-  Share s;
-  s.request = me / units;  // if units are shares
-  s.unit = me - s.request * units;
-  s.tile = 0;
-  if (s.request < a.requests) s.span = span_of(a, s.request);
-  int64_t sum = 0;
-  int longest = 0;
-  Span last;
-  for (int b = first; b < min(first + run, a.requests); ++b) {
-    last = span_of(a, b);
-    const int n = tiles_of(last, tile);
-    sum += (int64_t)n * units;
-    longest = max(longest, n);
-  }
-  int64_t upto = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int64_t below = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += below;
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
-  }
-  if (lane == 31) {
-    warp_sums[warp] = upto;
-    warp_longest[warp] = longest;
-  }
-  __syncthreads();
-  s.all = 0;
-  for (int w = 0; w < ATT_THREADS / 32; ++w) {
-    if (w < warp) upto += warp_sums[w];
-    s.all += warp_sums[w];
-    longest = max(longest, warp_longest[w]);
-  }
-  s.shares = (int)max((int64_t)1, min((int64_t)a.blocks, s.all / MIN_TILES));
   const int64_t all_units = (int64_t)a.requests * units;
-  s.whole = all_units <= a.blocks && (longest - WHOLE_TILES) * (int64_t)s.shares <= s.all;
-  if (s.whole) {
-    s.from = 0;
-    s.steps = me < all_units ? tiles_of(s.span, tile) : 0;
-    return s;
-  }
-  if (me >= s.shares) {
-    s.steps = 0;
-    return s;
-  }
-  s.from = share_start(me, s.all, s.shares);
-  s.steps = share_start(me + 1, s.all, s.shares) - s.from;
-  if (s.from >= upto - sum && s.from < upto) {
-    int64_t left = s.from - (upto - sum);
-    int b = first;
-    while (run > 1) {
+  Share s = {};
+  w.tile = 0;
+  w.request = me / units;  // if units are shares
+  w.unit = me - w.request * units;
+  w.left = UNIT_COST + MOST_TOKENS;
+  if (w.request < a.requests) w.span = span_of(a, w.request);
+  bool whole = a.cuts == nullptr;
+  if (!whole) {
+    const int run = (a.requests + ATT_THREADS - 1) / ATT_THREADS, first = threadIdx.x * run;
+    int64_t sum = 0;
+    int longest = 0;
+    Span last;
+    for (int b = first; b < min(first + run, a.requests); ++b) {
       last = span_of(a, b);
-      const int64_t n = (int64_t)tiles_of(last, tile) * units;
-      if (left < n) break;
-      left -= n;
-      ++b;
+      const int n = UNIT_COST + tiles_of(last, tile_keys);
+      sum += (int64_t)n * units;
+      longest = max(longest, n);
     }
-    const int n = tiles_of(last, tile);
-    found_request = b;
-    found_unit = (int)(left / n);
-    found_tile = (int)(left % n);
-    found_span = last;
+    int64_t upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int64_t below = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += below;
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+    }
+    if (lane == 31) {
+      warp_sums[warp] = upto;
+      warp_longest[warp] = longest;
+    }
+    __syncthreads();
+    for (int v = 0; v < ATT_THREADS / 32; ++v) {
+      if (v < warp) upto += warp_sums[v];
+      s.all += warp_sums[v];
+      longest = max(longest, warp_longest[v]);
+    }
+    s.shares = (int)max((int64_t)1, min((int64_t)a.blocks, s.all / MIN_WORK));
+    whole = all_units <= a.blocks && (longest - UNIT_COST - WHOLE_TILES) * (int64_t)s.shares <= s.all;
+    const int64_t from = share_start(min(me, s.shares - 1), s.all, s.shares);
+    s.to = share_start(min(me, s.shares - 1) + 1, s.all, s.shares);
+    if (!whole && from >= upto - sum && from < upto) {
+      int64_t into = from - (upto - sum);
+      int b = first;
+      while (run > 1) {
+        last = span_of(a, b);
+        const int64_t n = (int64_t)(UNIT_COST + tiles_of(last, tile_keys)) * units;
+        if (into < n) break;
+        into -= n;
+        ++b;
+      }
+      const int n = UNIT_COST + tiles_of(last, tile_keys);
+      found_request = b;
+      found_unit = (int)(into / n);
+      found_left = into % n;
+      found_span = last;
+    }
+    __syncthreads();
+    if (!whole) {
+      w.request = found_request;
+      w.unit = found_unit;
+      w.tile = (int)max((int64_t)0, found_left - UNIT_COST);
+      w.left = s.to - from + found_left;
+      w.span = found_span;
+    }
   }
-  __syncthreads();
-  s.request = found_request;
-  s.unit = found_unit;
-  s.tile = found_tile;
-  s.span = found_span;
+  w.done = whole ? me >= all_units : me >= s.shares;
+  if (w.done) return s;
+  if (whole) w.left = UNIT_COST + tiles_of(w.span, tile_keys);
+  w.enter(tile_keys);
   return s;
 }
 
@@ -166,13 +206,6 @@ __device__ __forceinline__ Share find_share(const AttendArgs &a, int tile) {
 struct Cut {
   int last, slot, request, unit;
 };
-// Of a unit that began at tile `from` of all and has `tiles`.
-__device__ __forceinline__ int last_share(const Share &s, int64_t from, int tiles) {
-  // the share of tile t is the largest n with n * all / shares < t + 1
-  const int64_t to = from + tiles;
-  if (s.all < (1 << 22) && s.shares < (1 << 10)) return (int)(((uint32_t)to * (uint32_t)s.shares + (uint32_t)s.all - 1) / (uint32_t)s.all) - 1;
-  return (int)((to * s.shares + s.all - 1) / s.all) - 1;
-}
 
 // ---- any type, width, stride and alignment --------------------------------------
 
@@ -190,21 +223,20 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
   float *const factor = ps + ANY_HEADS * ANY_TILE, *const total = factor + ANY_HEADS;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   pdl_wait();
-  const Share s = find_share(a, ANY_TILE);
+  Walk w;
+  const Share share = find_share(a, ANY_TILE, w);
   pdl_release();
   if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
-  int request = s.request, unit = s.unit, tile = s.tile;
-  Span span = s.span;
   const int units = (int)a.cache.heads * a.head_blocks;
-  bool first_piece = true;
-  for (int64_t at = 0; at < s.steps;) {
-    const int kv_head = unit / a.head_blocks, head0 = (unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
-    const int tiles = tiles_of(span, ANY_TILE), end = (int)min((int64_t)tiles, tile + (s.steps - at));
+  for (bool first_piece = true; !w.done; first_piece = false) {
+    const int kv_head = w.unit / a.head_blocks, head0 = (w.unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
+    const int request = w.request;
+    const Span span = w.span;
     __syncthreads();
     for (int i = threadIdx.x; i < heads * dim; i += ATT_THREADS)
       qs[i] = to_f32(static_cast<const T *>(a.q)[request * a.q_token_stride + (int64_t)(kv_head * a.group + head0 + i / dim) * a.q_head_stride + i % dim]);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, acc[2][ANY_HEADS] = {};
-    for (int t = tile; t < end; ++t) {
+    for (int t = w.tile; t < w.end; ++t) {
       const int key0 = span.origin + t * ANY_TILE;
       __syncthreads();
       for (int j = warp; j < ANY_TILE; j += ATT_THREADS / 32) {
@@ -252,10 +284,9 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
         }
       }
     }
-    const bool whole = tile == 0 && end == tiles;
+    const bool whole = w.tile == 0 && w.end == w.tiles;
     float *const slot = a.partial + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * ANY_HEADS * (dim + 2);
-    if (!whole && tile == 0 && threadIdx.x == 0)
-      a.cuts[blockIdx.x] = {last_share(s, s.from + at, tiles), first_piece ? 0 : 1, request, unit};
+    if (!whole && w.tile == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = {share.last_of(w.left, w.tiles), first_piece ? 0 : 1, request, w.unit};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int h = warp + 4 * u;
@@ -286,13 +317,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
           slot[h * (dim + 2) + 2 + i] = acc[e][h];
       }
     }
-    first_piece = false;
-    at += end - tile;
-    tile = 0;
-    if (++unit == units && at < s.steps) {
-      unit = 0;
-      span = span_of(a, ++request);
-    }
+    w.next_unit(a, units, ANY_TILE);
   }
 }
 
@@ -386,24 +411,28 @@ struct MmaConfig {
   static constexpr int STORE = STORE_;                      // LAPIS_I8, LAPIS_E4M3, or anything else: T
   static constexpr bool CODES = STORE == LAPIS_I8 || STORE == LAPIS_E4M3;
   static constexpr bool HALF = CODES || std::is_same<T, __half>::value;  // fp16 products, or bf16
-  static constexpr bool TWO_PARTS = !(CODES && std::is_same<T, __nv_bfloat16>::value);
+  static constexpr bool TWO_PARTS = !(CODES && std::is_same<T, __nv_bfloat16>::value);  // of the weights
+  static constexpr int QP = std::is_same<T, float>::value ? 2 : 1;                      // parts of the queries
   static constexpr int DP = DP_, NT = NT_;                  // padded head, and eights of query heads
   static constexpr int ROW = DP * (CODES ? 1 : 2);          // bytes of a key in shared memory
   static constexpr int KEYS = ROW <= 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
-  static constexpr int DT = DP / 16, REGS = DT * 4 + 4;     // values a lane leaves of eight heads: O, m and l
-  static constexpr int EXCHANGE = REGS * 32 * 4;
-  static constexpr int BLOCKS = DP == 256 ? 1 : DP == 128 && NT == 2 ? 2 : 3;  // an SM, by registers
-  static constexpr int STAGES = (227 * 1024 / BLOCKS - 1024 - EXCHANGE) / (MMA_WARPS * STAGE);
-  static constexpr int SMEM = MMA_WARPS * STAGES * STAGE + EXCHANGE;
+  static constexpr int DT = DP / 16, PART = DT * 128 + 16;  // floats of eight heads' sums: O, then m and l
+  static constexpr int BLOCKS = DP == 256 ? 1 : DP * NT * QP >= 256 ? 2 : 3;  // an SM, by registers
+  static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048) / (MMA_WARPS * STAGE);
+  static constexpr int SMEM = MMA_WARPS * STAGES * STAGE;
   static_assert(STAGES >= 2, "one is copied while another is read");
+  static_assert(PART * 4 <= STAGE, "a warp's sums fit where its last keys were");
   static constexpr float OFFSET = HALF ? 14.0f : 0.0f;
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool real) {  // zeros where it is not
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0));
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void *from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(real ? 8 : 0));
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool real) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0));
@@ -470,21 +499,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
   return r;
 }
 
-// Position in a block's share of the tiles.
-struct Cursor {
-  int request, unit, tile, tiles;
-  Span span;
-};
-__device__ __forceinline__ void next_unit(const AttendArgs &a, Cursor &c, int units, int tile_keys) {
-  c.tile = 0;
-  if (++c.unit < units) return;
-  c.unit = 0;
-  if (c.request + 1 < a.requests) {
-    c.span = span_of(a, ++c.request);
-    c.tiles = tiles_of(c.span, tile_keys);
-  }
-}
-
 // 2^x to 2 units in the last place; what is below 2^-126 is zero.
 __device__ __forceinline__ float power2(float x) {
   float r;
@@ -502,33 +516,6 @@ struct Sums {
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.0f;
   }
-  __device__ __forceinline__ void store(float *p) const {
-    const int lane = threadIdx.x % 32;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) reinterpret_cast<float4 *>(p)[t * 32 + lane] = make_float4(o[t][0], o[t][1], o[t][2], o[t][3]);
-    reinterpret_cast<float4 *>(p)[DT * 32 + lane] = make_float4(m[0], m[1], l[0], l[1]);
-  }
-  __device__ __forceinline__ void add(const float *p) {
-    const int lane = threadIdx.x % 32;
-    const float4 x = reinterpret_cast<const float4 *>(p)[DT * 32 + lane];
-    float f[2], e[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float om = i == 0 ? x.x : x.y, ol = i == 0 ? x.z : x.w, most = fmaxf(m[i], om), base = most == -INFINITY ? 0.0f : most;
-      f[i] = exp2f(m[i] - base);
-      e[i] = exp2f(om - base);
-      m[i] = most;
-      l[i] = l[i] * f[i] + ol * e[i];
-    }
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      const float4 y = reinterpret_cast<const float4 *>(p)[t * 32 + lane];
-      o[t][0] = o[t][0] * f[0] + y.x * e[0];
-      o[t][1] = o[t][1] * f[1] + y.y * e[1];
-      o[t][2] = o[t][2] * f[0] + y.z * e[0];
-      o[t][3] = o[t][3] * f[1] + y.w * e[1];
-    }
-  }
 };
 
 // Dimension of o[t][0] of group g; that of o[t][2] is the one 8 further (16-bit caches) or the next (codes).
@@ -538,37 +525,69 @@ __device__ __forceinline__ int dimension(int t, int g) {
   return C::DP == 64 ? g * 8 + 2 * t : (g + 8 * (t / 8)) * 16 + 2 * (t % 8);
 }
 
-// Adds up the warps of the block and gives eight heads out: as results, or to `slot` where the unit was cut.
+// Adds up the warps of the block and gives eight heads out: as results, or to `part` where the unit was cut.  The warps' sums meet
+// where their last keys were (`mine`, and warp w's `apart` bytes times w behind the first one's); each adds up a quarter.
 template <typename C>
-__device__ __forceinline__ void give(const AttendArgs &a, Sums<C::DT> &s, float *exchange, int request, int first_head, int heads, float *slot) {
+__device__ __forceinline__ void give(const AttendArgs &a, const Sums<C::DT> &s, unsigned char *mine, int apart, int request, int first_head, int heads, float *part) {
   using T = typename C::T;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+  float4 *const to = reinterpret_cast<float4 *>(mine);
+  const unsigned char *const all = mine - warp * apart;
+#pragma unroll
+  for (int t = 0; t < C::DT; ++t) to[t * 32 + lane] = make_float4(s.o[t][0], s.o[t][1], s.o[t][2], s.o[t][3]);
+  if (g == 0) to[C::DT * 32 + c] = make_float4(s.m[0], s.m[1], s.l[0], s.l[1]);
+  __syncthreads();
+  float4 ml[MMA_WARPS];
+  float2 f[MMA_WARPS];
+#pragma unroll
+  for (int w = 0; w < MMA_WARPS; ++w) ml[w] = reinterpret_cast<const float4 *>(all + w * apart)[C::DT * 32 + c];
+  float m[2] = {ml[0].x, ml[0].y}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int w = 1; w < MMA_WARPS; ++w) {
+    m[0] = fmaxf(m[0], ml[w].x);
+    m[1] = fmaxf(m[1], ml[w].y);
+  }
+#pragma unroll
+  for (int w = 0; w < MMA_WARPS; ++w) {
+    f[w] = make_float2(power2(ml[w].x - (m[0] == -INFINITY ? 0.0f : m[0])), power2(ml[w].y - (m[1] == -INFINITY ? 0.0f : m[1])));
+    l[0] = fmaf(ml[w].z, f[w].x, l[0]);
+    l[1] = fmaf(ml[w].w, f[w].y, l[1]);
+  }
+  if (warp == 0 && g == 0) {
+    if (part != nullptr) reinterpret_cast<float4 *>(part)[C::DT * 32 + c] = make_float4(m[0], m[1], l[0], l[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (part == nullptr && a.lse != nullptr && 2 * c + i < heads)
+        a.lse[(int64_t)request * a.q_heads + first_head + 2 * c + i] = l[i] == 0.0f ? -INFINITY : (m[i] - C::OFFSET) * LN2 + logf(l[i]);
+  }
+  const float by[2] = {l[0] == 0.0f ? 0.0f : 1.0f / l[0], l[1] == 0.0f ? 0.0f : 1.0f / l[1]};
+  T *const out = static_cast<T *>(a.out) + ((int64_t)request * a.q_heads + first_head + 2 * c) * a.dim;
 #pragma unroll 1
-  for (int w = 1; w < MMA_WARPS; ++w) {  // one after the other: shared memory is for what is on its way
-    __syncthreads();
-    if (warp == w) s.store(exchange);
-    __syncthreads();
-    if (warp == 0) s.add(exchange);
-  }
-  if (warp != 0) return;
-  if (slot != nullptr) {
-    s.store(slot);
-    return;
-  }
+  for (int t = warp; t < C::DT; t += MMA_WARPS) {
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (2 * c + i >= heads) continue;
-    const int64_t head = (int64_t)request * a.q_heads + first_head + 2 * c + i;
-    const float by = s.l[i] == 0.0f ? 0.0f : 1.0f / s.l[i];
-    if (g == 0 && a.lse != nullptr) a.lse[head] = s.l[i] == 0.0f ? -INFINITY : (s.m[i] - C::OFFSET) * LN2 + logf(s.l[i]);
-    T *const out = static_cast<T *>(a.out) + head * a.dim;
-#pragma unroll
-    for (int t = 0; t < C::DT; ++t) {
-      const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
-      if (d0 < a.dim) out[d0] = from_f32<T>(s.o[t][i] * by);
-      if (d1 < a.dim) out[d1] = from_f32<T>(s.o[t][2 + i] * by);
+    for (int w = 0; w < MMA_WARPS; ++w) {
+      const float4 y = reinterpret_cast<const float4 *>(all + w * apart)[t * 32 + lane];
+      x.x = fmaf(y.x, f[w].x, x.x);
+      x.y = fmaf(y.y, f[w].y, x.y);
+      x.z = fmaf(y.z, f[w].x, x.z);
+      x.w = fmaf(y.w, f[w].y, x.w);
+    }
+    if (part != nullptr) {
+      reinterpret_cast<float4 *>(part)[t * 32 + lane] = x;
+      continue;
+    }
+    const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
+    if (2 * c < heads) {
+      if (d0 < a.dim) out[d0] = from_f32<T>(x.x * by[0]);
+      if (d1 < a.dim) out[d1] = from_f32<T>(x.z * by[0]);
+    }
+    if (2 * c + 1 < heads) {
+      if (d0 < a.dim) out[a.dim + d0] = from_f32<T>(x.y * by[1]);
+      if (d1 < a.dim) out[a.dim + d1] = from_f32<T>(x.w * by[1]);
     }
   }
+  __syncthreads();
 }
 
 template <typename C>
@@ -577,27 +596,22 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   constexpr int KEYS = C::KEYS, MT = C::MT, NT = C::NT, DT = C::DT, STAGES = C::STAGES;
   extern __shared__ __align__(128) unsigned char stages[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
-  float *const exchange = reinterpret_cast<float *>(stages + MMA_WARPS * STAGES * C::STAGE);
   unsigned char *const mine = stages + warp * STAGES * C::STAGE;
   const uint32_t ring = shared_address(mine);
   const int units = (int)a.cache.heads * a.head_blocks;
   pdl_wait();
-  const Share share = find_share(a, C::TILE);
+  Walk in, out;  // of the copies and of the products
+  const Share share = find_share(a, C::TILE, in);
   pdl_release();
   if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
-  const int64_t steps = share.steps;
-  if (steps == 0) return;
-  if (a.dim != C::DP)  // what is beyond the head is never copied
-    for (int i = lane; i < STAGES * C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);
-  __syncwarp();
-
-  Cursor in, out;  // of the copies and of the products
-  in.request = share.request;
-  in.unit = share.unit;
-  in.tile = share.tile;
-  in.span = share.span;
-  in.tiles = tiles_of(in.span, C::TILE);
+  if (in.done) return;
   out = in;
+  auto clear_stage = [&](int stage) {  // what is beyond the head is never copied
+    for (int i = lane; i < C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine + stage * C::STAGE)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  };
+  if (a.dim != C::DP)
+    for (int i = 0; i < STAGES; ++i) clear_stage(i);
 
   // Pages of the next step to copy, looked up one step ahead.  `grouped`: pages have a multiple of 16 slots, and a lane looks up
   // 16 keys; otherwise a lane looks up key `lane`.
@@ -630,7 +644,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     const int key0 = in.span.origin + in.tile * C::TILE + warp * KEYS, key = key0 + of_lane;
     const bool listed = page >= 0 && page < a.cache.pages;
     uint32_t row = (uint32_t)page * page_rows + (uint32_t)(in.unit / a.head_blocks * page_size + slot_in_page);
-    const bool plain = key0 >= in.span.lo && key0 + KEYS <= in.span.hi && grouped && __all_sync(0xffffffffu, listed);
+    const bool plain = key0 >= in.span.lo && key0 + KEYS <= in.span.hi && grouped && row_bytes % 16 == 0 && __all_sync(0xffffffffu, listed);
     // the row of this lane's key
     const uint32_t first = __shfl_sync(0xffffffffu, row, of_lane / 16);
     const bool first_listed = __shfl_sync(0xffffffffu, listed, of_lane / 16);
@@ -657,9 +671,16 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         const int r = i * ROWS + low;
         const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, r) * row_bytes;
         const bool real = __shfl_sync(0xffffffffu, there, r);
-        if (in_row) {
+        if (in_row && row_bytes % 16 == 0) {
           copy16(to + k_at(r), k_store + offset, real);
           copy16(to + v_at(r), v_store + offset, real);
+        } else if (in_row) {  // rows begin at multiples of 8 bytes
+          copy8(to + k_at(r), k_store + offset, real);
+          copy8(to + v_at(r), v_store + offset, real);
+          if (ch * 16 + 8 < row_bytes) {
+            copy8(to + k_at(r) + 8, k_store + offset + 8, real);
+            copy8(to + v_at(r) + 8, v_store + offset + 8, real);
+          }
         }
       }
     }
@@ -668,75 +689,116 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       copy4(scales, a.cache.d_k_scale + row, there);
       copy4(scales + KEYS * 4, a.cache.d_v_scale + row, there);
     }
-    if (++in.tile == in.tiles) next_unit(a, in, units, C::TILE);
+    in.next_tile(a, units, C::TILE);
   };
   look_up();
 
-  uint32_t q[NT][DT][2];
+  uint32_t q[C::QP][NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
   float value_by = 0.0f, values_in = 0.0f;  // codes: the power of two that the values' scales are relative to, and 1 / it
   Sums<DT> sums[NT];
-  bool fresh = true;
-  int began = out.tile;
-  int64_t began_step = 0;
-  int stage = 0, stage_in = 0;
-  bool first_piece = true;
-  auto load_q = [&](int64_t step) {
+  // The queries of unit `out` as they are; q takes them once the unit in front has been given out.  Four values of a lane: for
+  // codes they are neighbours.
+  uint2 raw[C::QP][NT][DT];
+  auto load_q = [&]() {
     const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
-    fresh = false;
-    began = out.tile;
-    began_step = step;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool real = head0 + n * 8 + g < a.group;
+      const T *const from = static_cast<const T *>(a.q) + (int64_t)out.request * a.q_token_stride +
+                            (int64_t)(kv_head * a.group + (real ? head0 + n * 8 + g : 0)) * a.q_head_stride;
+#pragma unroll
+      for (int k = 0; k < DT; ++k) {
+        const int d = C::CODES ? (k / 4) * 64 + c * 16 + (k % 4) * 4 : k * 16 + c * 2, e = C::CODES ? d + 2 : d + 8;
+        if constexpr (C::QP == 2) {
+          raw[0][n][k] = raw[1][n][k] = make_uint2(0, 0);
+          if (real && d < a.dim) {
+            raw[0][n][k] = make_uint2(__float_as_uint(from[d]), __float_as_uint(from[d + 1]));
+            raw[1][n][k] = make_uint2(__float_as_uint(from[e]), __float_as_uint(from[e + 1]));
+          }
+        } else {
+          const uint16_t *const at = reinterpret_cast<const uint16_t *>(from);
+          uint2 x = make_uint2(0, 0);
+          if (a.q_pairs) {
+            if (real && d < a.dim) x.x = *reinterpret_cast<const uint32_t *>(at + d);
+            if (real && e < a.dim) x.y = *reinterpret_cast<const uint32_t *>(at + e);
+          } else {
+            if (real && d < a.dim) x.x = at[d] | (uint32_t)at[d + 1] << 16;
+            if (real && e < a.dim) x.y = at[e] | (uint32_t)at[e + 1] << 16;
+          }
+          raw[0][n][k] = x;
+        }
+      }
+    }
+  };
+  auto take_q = [&]() {
     value_by = values_in = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       sums[n].clear();
-      const bool real = head0 + n * 8 + g < a.group;
-      const T *const from = static_cast<const T *>(a.q) + (int64_t)out.request * a.q_token_stride +
-                            (int64_t)(kv_head * a.group + (real ? head0 + n * 8 + g : 0)) * a.q_head_stride;
-      float x[DT][4], most = 0.0f;
+      if constexpr (!C::CODES) {
+        score_by[n][0] = score_by[n][1] = a.scale2;
 #pragma unroll
-      for (int k = 0; k < DT; ++k) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = C::CODES ? (k / 4) * 64 + c * 16 + (k % 4) * 4 + e : k * 16 + c * 2 + (e & 1) + (e & 2) * 4;
-          x[k][e] = real && d < a.dim ? to_f32(from[d]) : 0.0f;
-          most = fmaxf(most, fabsf(x[k][e]));
+        for (int k = 0; k < DT; ++k) {
+          q[0][n][k][0] = raw[0][n][k].x;
+          q[0][n][k][1] = raw[0][n][k].y;
         }
-      }
-      float by = 1.0f;
-      if (C::CODES) {  // to [1, 2): 2^(127 - exponent)
+      } else {  // to [2^13, 2^14), by a power of two for each head
+        constexpr bool IS_HALF = std::is_same<T, __half>::value;
+        float most = 0.0f;
+        auto value = [&](int k) {
+          if constexpr (C::QP == 2) {
+            return make_float4(__uint_as_float(raw[0][n][k].x), __uint_as_float(raw[0][n][k].y), __uint_as_float(raw[1][n][k].x), __uint_as_float(raw[1][n][k].y));
+          } else {
+            const float2 x = unpack2<IS_HALF>(raw[0][n][k].x), y = unpack2<IS_HALF>(raw[0][n][k].y);
+            return make_float4(x.x, x.y, y.x, y.y);
+          }
+        };
+#pragma unroll
+        for (int k = 0; k < DT; ++k) {
+          const float4 x = value(k);
+          most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        }
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int exponent = min(max((int)(__float_as_uint(most) >> 23), 1), 253);
-        by = __uint_as_float((uint32_t)(254 - exponent) << 23);
+        const int exponent = min(max((int)(__float_as_uint(most) >> 23), 14), 254);
+        const float by = __uint_as_float((uint32_t)(267 - exponent) << 23);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int e = __shfl_sync(0xffffffffu, exponent, (2 * c + i) * 4);
-          score_by[n][i] = a.scale2 * __uint_as_float((uint32_t)e << 23);
+          score_by[n][i] = a.scale2 * __uint_as_float((uint32_t)(e - 13) << 23);
         }
-      } else {
-        score_by[n][0] = score_by[n][1] = a.scale2;
-      }
 #pragma unroll
-      for (int k = 0; k < DT; ++k) {
-        q[n][k][0] = pack2<C::HALF>(x[k][0] * by, x[k][1] * by);
-        q[n][k][1] = pack2<C::HALF>(x[k][2] * by, x[k][3] * by);
+        for (int k = 0; k < DT; ++k) {
+          const float4 x = value(k);
+          q[0][n][k][0] = pack2<true>(x.x * by, x.y * by);
+          q[0][n][k][1] = pack2<true>(x.z * by, x.w * by);
+          if constexpr (C::QP == 2) {
+            const float2 h0 = unpack2<true>(q[0][n][k][0]), h1 = unpack2<true>(q[0][n][k][1]);
+            q[1][n][k][0] = pack2<true>(x.x * by - h0.x, x.y * by - h0.y);
+            q[1][n][k][1] = pack2<true>(x.z * by - h1.x, x.w * by - h1.y);
+          }
+        }
       }
     }
   };
+  load_q();
+  int began = out.tile, stage = 0, stage_in = 0;
+  bool first_piece = true;
 #pragma unroll 1
-  for (int64_t step = 1 - STAGES; step < steps; ++step) {
-    if (step >= 0 && fresh) load_q(step);
-    if (step >= 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+  for (int ahead = 1 - STAGES;; ahead = min(ahead + 1, 0)) {  // below 0: there are not enough copies on their way
+    if (ahead == 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
-    if (step + STAGES - 1 < steps) {
+    if (!in.done) {
       fetch(stage_in);
-      look_up();
+      if (!in.done) look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
-    if (step < 0) continue;
-    const int kv_head = out.unit / a.head_blocks, head0 = (out.unit % a.head_blocks) * 8 * NT;
+    if (ahead < 0) {
+      if (ahead == -1) take_q();
+      continue;
+    }
 
     const uint32_t ks = ring + stage * C::STAGE, vs = ks + KEYS * C::ROW, scales = vs + KEYS * C::ROW;
     float s[MT][NT][4];
@@ -751,7 +813,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
           uint32_t x[4];
           ldmatrix4(x, ks + r * C::ROW + (((2 * k + half) ^ (r & 7)) * 16));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<C::HALF>(s[mt][n], x, q[n][k][0], q[n][k][1]);
+          for (int n = 0; n < NT; ++n) mma<C::HALF>(s[mt][n], x, q[0][n][k][0], q[0][n][k][1]);
         }
       } else {
         const int r = mt * 16 + (g >> 1) + 4 * (g & 1), swizzle = C::DP == 64 ? 0 : r & 4;
@@ -764,7 +826,9 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
             const uint32_t flip = C::STORE == LAPIS_I8 ? 0x80808080u : 0, t = tw[j] ^ flip, l = lw[j] ^ flip;
             const uint32_t x[4] = {codes2<C::STORE, false>(t), codes2<C::STORE, false>(l), codes2<C::STORE, true>(t), codes2<C::STORE, true>(l)};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma<C::HALF>(s[mt][n], x, q[n][k * 4 + j][0], q[n][k * 4 + j][1]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int p = 0; p < C::QP; ++p) mma<C::HALF>(s[mt][n], x, q[p][n][k * 4 + j][0], q[p][n][k * 4 + j][1]);
           }
         }
       }
@@ -917,32 +981,38 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         }
       }
     }
+    const int used = stage;
     stage = stage + 1 == STAGES ? 0 : stage + 1;
-
-    const bool unit_ends = ++out.tile == out.tiles;
-    if (unit_ends || step + 1 == steps) {
-      const bool whole = unit_ends && began == 0;
-      if (!unit_ends && began == 0 && threadIdx.x == 0)
-        a.cuts[blockIdx.x] = {last_share(share, share.from + began_step, out.tiles), first_piece ? 0 : 1, out.request, out.unit};
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2) sums[n].l[i] += __shfl_xor_sync(0xffffffffu, sums[n].l[i], d);
-        if (C::CODES) {
-#pragma unroll
-          for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= value_by;
-        }
-        float *const slot = a.partial + (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * NT + n) * C::REGS * 32;
-        give<C>(a, sums[n], exchange, out.request, kv_head * a.group + head0 + n * 8, a.group - head0 - n * 8, whole ? nullptr : slot);
-      }
-      first_piece = false;
-      fresh = true;
-      if (unit_ends) next_unit(a, out, units, C::TILE);
+    if (out.tile + 1 < out.end) {
+      ++out.tile;
+      continue;
     }
+    const int request = out.request, head0 = (out.unit % a.head_blocks) * 8 * NT, first_head = out.unit / a.head_blocks * a.group + head0;
+    const bool whole = began == 0 && out.end == out.tiles;
+    if (!whole && began == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = {share.last_of(out.left, out.tiles), first_piece ? 0 : 1, request, out.unit};
+    out.next_unit(a, units, C::TILE);
+    if (!out.done) load_q();  // on its way while the sums are given out
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) sums[n].l[i] += __shfl_xor_sync(0xffffffffu, sums[n].l[i], d);
+      if (C::CODES) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= value_by;
+      }
+      float *const part = a.partial + (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * NT + n) * C::PART;
+      __syncwarp();
+      give<C>(a, sums[n], mine + used * C::STAGE, STAGES * C::STAGE, request, first_head + n * 8, a.group - head0 - n * 8, whole ? nullptr : part);
+    }
+    if (out.done) return;
+    if (a.dim != C::DP) clear_stage(used);
+    first_piece = false;
+    began = 0;
+    take_q();
   }
 }
 
@@ -952,7 +1022,7 @@ constexpr int JOIN_THREADS = 256;
 template <typename C>
 __global__ void __launch_bounds__(JOIN_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
   using T = typename C::T;
-  constexpr int PART = C::REGS * 32, PARTS = JOIN_THREADS / 64;
+  constexpr int PART = C::PART, PARTS = JOIN_THREADS / 64;
   __shared__ float weight[MOST_BLOCKS][8], most[8], total[8];
   __shared__ float4 others[PARTS - 1][64];
   pdl_wait();
@@ -1033,7 +1103,7 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
   a.blocks = std::min(C::BLOCKS * sm_count(), MOST_BLOCKS);
   PoolBuf work;
   const bool whole = always_whole(a, C::TILE);
-  if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * C::NT * C::REGS * 32, st));
+  if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * C::NT * C::PART, st));
   LAPIS_CUDA_TRY(launch_pdl(attend_mma_kernel<C>, dim3(whole ? a.requests * (int)a.cache.heads * a.head_blocks : a.blocks), ATT_THREADS, C::SMEM, st, a));
   if (whole) return LAPIS_OK;
   LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3(a.blocks, C::NT, C::DT / 2), JOIN_THREADS, 0, st, a));
@@ -1043,22 +1113,25 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
 template <typename T, int STORE>
 static int launch_mma_of(const AttendArgs &a, int dev, cudaStream_t st) {
   if (a.dim <= 64) return a.group <= 8 ? launch_mma<MmaConfig<T, STORE, 64, 1>>(a, dev, st) : launch_mma<MmaConfig<T, STORE, 64, 2>>(a, dev, st);
-  if (a.dim <= 128) return a.group <= 8 ? launch_mma<MmaConfig<T, STORE, 128, 1>>(a, dev, st) : launch_mma<MmaConfig<T, STORE, 128, 2>>(a, dev, st);
-  return launch_mma<MmaConfig<T, STORE, 256, 1>>(a, dev, st);
+  if (a.dim > 128) return launch_mma<MmaConfig<T, STORE, 256, 1>>(a, dev, st);
+  if constexpr (!std::is_same<T, float>::value)
+    if (a.group > 8) return launch_mma<MmaConfig<T, STORE, 128, 2>>(a, dev, st);
+  return launch_mma<MmaConfig<T, STORE, 128, 1>>(a, dev, st);
 }
 
-// Whole 16 bytes from 16-byte addresses.
+// Rows of whole 8 bytes from 16-byte addresses, of 16-bit numbers or of codes.
 static bool mma_fits(int type, const AttendArgs &a) {
-  if (type == LAPIS_F32) return false;
-  const int64_t row = a.dim * type_bytes(a.cache.type);
-  return row % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
+  if (type == LAPIS_F32 && !is_quantised(a.cache.type)) return false;
+  return a.dim * type_bytes(a.cache.type) % 8 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
 }
 
 template <typename T>
-static int launch_mma_type(const AttendArgs &a, int dev, cudaStream_t st) {
+static int launch_type(const AttendArgs &a, bool fits, int dev, cudaStream_t st) {
+  if (!fits) return launch_any<T>(a, dev, st);
   if (a.cache.type == LAPIS_I8) return launch_mma_of<T, LAPIS_I8>(a, dev, st);
   if (a.cache.type == LAPIS_E4M3) return launch_mma_of<T, LAPIS_E4M3>(a, dev, st);
-  return launch_mma_of<T, LAPIS_F32>(a, dev, st);
+  if constexpr (std::is_same<T, float>::value) return launch_any<T>(a, dev, st);
+  else return launch_mma_of<T, LAPIS_F32>(a, dev, st);
 }
 
 }  // namespace lapis_b200
@@ -1103,8 +1176,9 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   a.lse = d_lse;
   cudaStream_t st = as_stream(stream);
   a.page_shift = page_shift_of(cache->page_size);
-  if (mma_fits(type, a)) return type == LAPIS_F16 ? launch_mma_type<__half>(a, dev, st) : launch_mma_type<__nv_bfloat16>(a, dev, st);
-  if (type == LAPIS_F32) return launch_any<float>(a, dev, st);
-  if (type == LAPIS_F16) return launch_any<__half>(a, dev, st);
-  return launch_any<__nv_bfloat16>(a, dev, st);
+  a.q_pairs = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && a.q_token_stride % 2 == 0 && a.q_head_stride % 2 == 0;
+  const bool fits = mma_fits(type, a);
+  if (type == LAPIS_F32) return launch_type<float>(a, fits, dev, st);
+  if (type == LAPIS_F16) return launch_type<__half>(a, fits, dev, st);
+  return launch_type<__nv_bfloat16>(a, fits, dev, st);
 }

@@ -22,7 +22,7 @@
 namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
-constexpr int UNIT_COST = 1;      // what a unit costs beside its tiles, in tiles
+constexpr int UNIT_COST = 2;      // what a unit costs beside its tiles, in tiles: 128 x 8192 int8 214 us with 1, 204 with 2 or 3
 constexpr int MIN_WORK = 4;       // of a share, if there is more than one
 constexpr int WHOLE_TILES = 4;    // by which a unit may be longer than a share and is not cut
 constexpr int MOST_BLOCKS = 480;  // shares that a join has room for: three blocks an SM
@@ -613,15 +613,16 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   if (a.dim != C::DP)
     for (int i = 0; i < STAGES; ++i) clear_stage(i);
 
-  // Pages of the next step to copy, looked up one step ahead.  `grouped`: pages have a multiple of 16 slots, and a lane looks up
-  // 16 keys; otherwise a lane looks up key `lane`.
+  // Pages of the next steps to copy.  `grouped`: pages have a multiple of 16 slots; lane n then has the page of the n-th 16 keys of
+  // this warp from tile `looked` on, 32 / MT steps of a unit by one look.  Otherwise lane n has that of key n of the next step.
   const bool grouped = a.cache.page_size % 16 == 0;
   const int page_size = (int)a.cache.page_size, row_bytes = a.dim * (C::CODES ? 1 : 2);
   const int of_lane = lane % KEYS;  // the key of a step that is this lane's
   int64_t page = -1;
-  int slot_in_page = 0;
+  int slot_in_page = 0, looked = 0;
   auto look_up = [&]() {
-    const int key = in.span.origin + in.tile * C::TILE + warp * KEYS + (grouped ? lane % MT * 16 : of_lane);
+    looked = in.tile;
+    const int key = in.span.origin + warp * KEYS + (grouped ? (looked + lane / MT) * C::TILE + lane % MT * 16 : looked * C::TILE + of_lane);
     page = -1;
     if (key < in.span.hi) {
       const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
@@ -643,14 +644,13 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     const uint32_t to = ring + stage * C::STAGE;
     const int key0 = in.span.origin + in.tile * C::TILE + warp * KEYS, key = key0 + of_lane;
     const bool listed = page >= 0 && page < a.cache.pages;
-    uint32_t row = (uint32_t)page * page_rows + (uint32_t)(in.unit / a.head_blocks * page_size + slot_in_page);
-    const bool plain = key0 >= in.span.lo && key0 + KEYS <= in.span.hi && grouped && row_bytes % 16 == 0 && __all_sync(0xffffffffu, listed);
-    // the row of this lane's key
-    const uint32_t first = __shfl_sync(0xffffffffu, row, of_lane / 16);
-    const bool first_listed = __shfl_sync(0xffffffffu, listed, of_lane / 16);
-    const bool there = key >= in.span.lo && key < in.span.hi && (grouped ? first_listed : listed);
-    if (grouped) row = first + of_lane % 16;
+    const uint32_t looked_row = (uint32_t)page * page_rows + (uint32_t)(in.unit / a.head_blocks * page_size + slot_in_page);
+    const int at = grouped ? (in.tile - looked) * MT + of_lane / 16 : of_lane;  // the lane that looked this one's key up
+    const bool found = __shfl_sync(0xffffffffu, listed, at);
+    uint32_t row = __shfl_sync(0xffffffffu, looked_row, at) + (grouped ? of_lane % 16 : 0);  // of this lane's key
+    const bool there = found && key >= in.span.lo && key < in.span.hi;
     if (!there) row = 0;
+    const bool plain = grouped && row_bytes % 16 == 0 && __all_sync(0xffffffffu, there);
     if (plain) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -689,7 +689,9 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       copy4(scales, a.cache.d_k_scale + row, there);
       copy4(scales + KEYS * 4, a.cache.d_v_scale + row, there);
     }
+    const int unit = in.unit, request = in.request;
     in.next_tile(a, units, C::TILE);
+    if (!in.done && (!grouped || in.unit != unit || in.request != request || in.tile - looked == 32 / MT)) look_up();
   };
   look_up();
 
@@ -789,10 +791,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   for (int ahead = 1 - STAGES;; ahead = min(ahead + 1, 0)) {  // below 0: there are not enough copies on their way
     if (ahead == 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
-    if (!in.done) {
-      fetch(stage_in);
-      if (!in.done) look_up();
-    }
+    if (!in.done) fetch(stage_in);
     asm volatile("cp.async.commit_group;" ::: "memory");
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
     if (ahead < 0) {

@@ -641,6 +641,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_consta
   __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 1024];
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= a.tokens) return;
+  pdl_wait();
   const uint32_t ring = shared_at(rings[threadIdx.x / 32]) + threadIdx.x % 32 * 16;
   const Pieces<T, LANES> p(a.dim, NORM && !a.interleaved ? a.rot / 2 : 0);
   int from = (int)(task - token * parts) * each, rounds[KINDS], all = 0;
@@ -708,6 +709,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_consta
     from -= rounds[which];
     to -= rounds[which];
   }
+  pdl_release();
 }
 
 // Backward: warps take tokens a grid apart and keep their share of the weights' gradients in registers.  The warps' lane groups
@@ -728,6 +730,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __gr
   const int64_t tasks = a.tokens * parts;
   const int rounds[2] = {(a.heads[0] + GROUPS - 1) / GROUPS, (a.heads[1] + GROUPS - 1) / GROUPS};
   const Rows *const rows[2] = {a.in, a.grad};
+  pdl_wait();
   for (int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32; task < tasks; task += (int64_t)gridDim.x * ROW_WARPS) {
     const int64_t token = task / parts;
     int from = (int)(task - token * parts) * each, to = min(from + each, rounds[0] + rounds[1]);
@@ -847,6 +850,7 @@ kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_c
   if (token >= tokens) return;
   const int lane = threadIdx.x % LANES, dim = (int)cache.dim, heads = (int)cache.heads;
   const int from = (int)(task - token * parts) * each, to = min(from + each, (heads + GROUPS - 1) / GROUPS);
+  pdl_wait();
   const int64_t first = cache_row(cache, lists, load_index(row, token, lists.idx_bytes), load_index(place, token, lists.idx_bytes), page_shift);
   const bool in[2] = {2 * lane * V < dim, (2 * lane + 1) * V < dim}, wide = dim % (2 * V) == 0;
   int head = from * GROUPS + threadIdx.x % 32 / LANES;
@@ -920,6 +924,7 @@ kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_c
       head += GROUPS;
     }
   }
+  pdl_release();
 }
 
 // ---- host -------------------------------------------------------------------
@@ -1051,12 +1056,13 @@ static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
       int rounds = 0;
       for (int heads : a.heads) rounds += (heads + GROUPS - 1) / GROUPS;
       const Parts p = parts_of(a.tokens, rounds);
-      if (!a.to_cache) rotate_kernel<T, LANES, true, false, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (a.norm && is_quantised(a.cache.type)) rotate_kernel<T, LANES, true, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (a.norm) rotate_kernel<T, LANES, true, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else if (is_quantised(a.cache.type)) rotate_kernel<T, LANES, false, true, true><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      else rotate_kernel<T, LANES, false, true, false><<<p.blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      LAPIS_CUDA_TRY(cudaGetLastError());
+      cudaError_t launched;
+      if (!a.to_cache) launched = launch_pdl(rotate_kernel<T, LANES, true, false, false>, dim3(p.blocks), ROW_THREADS, 0, st, a, p.parts, p.each);
+      else if (a.norm && is_quantised(a.cache.type)) launched = launch_pdl(rotate_kernel<T, LANES, true, true, true>, dim3(p.blocks), ROW_THREADS, 0, st, a, p.parts, p.each);
+      else if (a.norm) launched = launch_pdl(rotate_kernel<T, LANES, true, true, false>, dim3(p.blocks), ROW_THREADS, 0, st, a, p.parts, p.each);
+      else if (is_quantised(a.cache.type)) launched = launch_pdl(rotate_kernel<T, LANES, false, true, true>, dim3(p.blocks), ROW_THREADS, 0, st, a, p.parts, p.each);
+      else launched = launch_pdl(rotate_kernel<T, LANES, false, true, false>, dim3(p.blocks), ROW_THREADS, 0, st, a, p.parts, p.each);
+      LAPIS_CUDA_TRY(launched);
       return (int)LAPIS_OK;
     });
   });
@@ -1084,8 +1090,7 @@ static int launch_backward(int type, RotateArgs &a, PoolBuf &partial, int *block
       const int rounds = (a.heads[0] + GROUPS - 1) / GROUPS + (a.heads[1] + GROUPS - 1) / GROUPS;
       const Parts p = a.tokens > 0 && rounds > 0 ? parts_of(a.tokens, rounds) : Parts{1, 1, 0};
       LAPIS_TRY(room(p.blocks));
-      if (*blocks > 0) rotate_backward_kernel<T, LANES><<<*blocks, ROW_THREADS, 0, st>>>(a, p.parts, p.each);
-      LAPIS_CUDA_TRY(cudaGetLastError());
+      if (*blocks > 0) LAPIS_CUDA_TRY(launch_pdl(rotate_backward_kernel<T, LANES>, dim3(*blocks), ROW_THREADS, 0, st, a, p.parts, p.each));
       return (int)LAPIS_OK;
     });
   });
@@ -1223,10 +1228,9 @@ extern "C" int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_
       const Parts p = parts_of(tokens, (int)((cache->heads + GROUPS - 1) / GROUPS));
       const int shift = page_shift_of(cache->page_size);
       if (is_quantised(cache->type))
-        kv_read_kernel<T, LANES, true><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
+        LAPIS_CUDA_TRY(launch_pdl(kv_read_kernel<T, LANES, true>, dim3(p.blocks), ROW_THREADS, 0, st, *cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v));
       else
-        kv_read_kernel<T, LANES, false><<<p.blocks, ROW_THREADS, 0, st>>>(*cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v);
-      LAPIS_CUDA_TRY(cudaGetLastError());
+        LAPIS_CUDA_TRY(launch_pdl(kv_read_kernel<T, LANES, false>, dim3(p.blocks), ROW_THREADS, 0, st, *cache, *lists, tokens, d_row, d_place, shift, p.parts, p.each, k, v));
       return (int)LAPIS_OK;
     });
   });

@@ -25,7 +25,7 @@ constexpr int ATT_THREADS = 128;
 constexpr int UNIT_COST = 2;      // what a unit costs beside its tiles, in tiles: 128 x 8192 int8 214 us with 1, 204 with 2 or 3
 constexpr int MIN_WORK = 4;       // of a share, if there is more than one
 constexpr int WHOLE_TILES = 4;    // by which a unit may be longer than a share and is not cut
-constexpr int MOST_BLOCKS = 480;  // shares that a join has room for: three blocks an SM
+constexpr int MOST_BLOCKS = 1 << 10;  // shares
 constexpr float LN2 = 0.6931471805599453f;
 
 struct AttendArgs {
@@ -109,17 +109,41 @@ struct Walk {
   }
 };
 
+// A unit that is cut: its shares, where the first of them leaves its part (0: its first piece, 1: its last; the others' parts are
+// their first), and which it is.  last = 0: there is none.
+struct CutUnit {
+  int first, last, slot, request, unit;
+};
+// What a block leaves for the join: the unit that begins in its share and goes on, and the one that its share goes on with.
+struct Cut {
+  CutUnit begins, goes_on;
+};
+
 struct Share {
   int64_t all, to;  // all work, and where this share ends
   int shares;
-  // The last share that has a tile of the unit that begins where `left` is left of this one.
-  __device__ __forceinline__ int last_of(int64_t left, int tiles) const {
-    // the share of position x is the largest n with n * all / shares < x + 1
-    const int64_t x = to - left + UNIT_COST + tiles;
-    if (all < (1 << 22) && shares < (1 << 10)) return (int)(((uint32_t)x * (uint32_t)shares + (uint32_t)all - 1) / (uint32_t)all) - 1;
-    return (int)((x * shares + all - 1) / all) - 1;
+  // The share of position x: the largest n with n * all / shares < x + 1.
+  __device__ __forceinline__ int of(int64_t x) const {
+    if (all < (1 << 22) && shares < (1 << 10)) return (int)(((uint32_t)(x + 1) * (uint32_t)shares + (uint32_t)all - 1) / (uint32_t)all) - 1;
+    return (int)(((x + 1) * shares + all - 1) / all) - 1;
+  }
+  // The unit of a walk.
+  __device__ __forceinline__ CutUnit cut(const Walk &w) const {
+    const int64_t at = to - w.left;  // where it begins
+    const int first = of(at + UNIT_COST);
+    return {first, of(at + UNIT_COST + w.tiles - 1), share_start(first, all, shares) < at ? 1 : 0, w.request, w.unit};
   }
 };
+// Notes what is cut of the piece [began, w.end) of a unit.
+__device__ __forceinline__ void note_cut(const AttendArgs &a, const Share &share, const Walk &w, int began) {
+  if (threadIdx.x != 0 || (began == 0 && w.end == w.tiles)) return;
+  const CutUnit c = share.cut(w);
+  if (began == 0) a.cuts[blockIdx.x].begins = c;
+  else a.cuts[blockIdx.x].goes_on = c;
+}
+__device__ __forceinline__ void note_none(const AttendArgs &a) {
+  if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].begins.last = a.cuts[blockIdx.x].goes_on.last = 0;
+}
 
 // Sums the work of all requests (a thread takes a run of them) and finds where this block's share begins; all threads return the
 // same.  Where units are few and none is much longer than a share would be, every unit is a share, and nothing has to be
@@ -201,12 +225,6 @@ __device__ __forceinline__ Share find_share(const AttendArgs &a, int tile_keys, 
   return s;
 }
 
-// What a block leaves for the join: the unit that begins in its share and goes on in the next ones, up to share `last`; `slot` is
-// where its own part is (0: its first piece, 1: its last).  last = 0: there is none.
-struct Cut {
-  int last, slot, request, unit;
-};
-
 // ---- any type, width, stride and alignment --------------------------------------
 
 constexpr int ANY_HEADS = 8, ANY_TILE = 32;
@@ -226,7 +244,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
   Walk w;
   const Share share = find_share(a, ANY_TILE, w);
   pdl_release();
-  if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
+  note_none(a);
   const int units = (int)a.cache.heads * a.head_blocks;
   for (bool first_piece = true; !w.done; first_piece = false) {
     const int kv_head = w.unit / a.head_blocks, head0 = (w.unit % a.head_blocks) * ANY_HEADS, heads = min(ANY_HEADS, a.group - head0);
@@ -286,7 +304,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
     }
     const bool whole = w.tile == 0 && w.end == w.tiles;
     float *const slot = a.partial + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * ANY_HEADS * (dim + 2);
-    if (!whole && w.tile == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = {share.last_of(w.left, w.tiles), first_piece ? 0 : 1, request, w.unit};
+    note_cut(a, share, w, w.tile);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int h = warp + 4 * u;
@@ -326,7 +344,7 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
 template <typename T>
 __global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_constant__ AttendArgs a) {
   pdl_wait();
-  const Cut cut = a.cuts[blockIdx.x];
+  const CutUnit cut = a.cuts[blockIdx.x].begins;
   const int first = blockIdx.x, h = blockIdx.y, dim = a.dim;
   const int head0 = (cut.unit % a.head_blocks) * ANY_HEADS;
   if (cut.last == 0 || head0 + h >= a.group) return;
@@ -388,6 +406,149 @@ static int launch_any(AttendArgs a, int dev, cudaStream_t st) {
   return LAPIS_OK;
 }
 
+// ---- a warp's pipeline --------------------------------------------------------------
+//
+// Keys and values come by cp.async into a ring that one warp uses for itself, STAGES deep: KEYS keys of a tile at a time, the
+// part of it that is this warp's.  C: the configuration of a kernel.
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool real) {  // zeros where it is not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0));
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void *from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(real ? 8 : 0));
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0));
+}
+__device__ __forceinline__ uint4 load16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 load8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ float load4(uint32_t at) {
+  float r;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
+  return r;
+}
+// 2^x to 2 units in the last place; what is below 2^-126 is zero.
+__device__ __forceinline__ float power2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <typename C>
+struct Feed {
+  static constexpr int KEYS = C::KEYS, GROUP = KEYS < 16 ? KEYS : 16, GROUPS = KEYS / GROUP, ROWS = 32 / C::CHUNKS > 0 ? 32 / C::CHUNKS : 1;
+  static constexpr int PASSES = C::CHUNKS > 32 ? C::CHUNKS / 32 : 1;  // copies of a row
+  Walk in;
+  uint32_t ring;
+  // Pages of the next steps to copy.  `grouped`: pages have a multiple of GROUP slots; lane n then has the page of the n-th GROUP
+  // keys of this warp from tile `looked` on, 32 / GROUPS steps of a unit by one look.  Otherwise lane n has that of key n of the
+  // next step.
+  int64_t page;
+  int slot_in_page, looked;
+  uint32_t page_rows, head_row;
+  bool grouped;
+
+  __device__ __forceinline__ int of_lane() const { return threadIdx.x % KEYS; }  // the key of a step that is this lane's
+  __device__ __forceinline__ int first_key() const { return in.span.origin + in.tile * C::TILE + threadIdx.x / 32 * KEYS; }
+  __device__ __forceinline__ void look_up(const AttendArgs &a) {
+    const int lane = threadIdx.x % 32, page_size = (int)a.cache.page_size;
+    looked = in.tile;
+    head_row = (uint32_t)(in.unit / a.head_blocks * page_size);
+    const int key = first_key() + (grouped ? lane / GROUPS * C::TILE + lane % GROUPS * GROUP : of_lane());
+    page = -1;
+    if (key < in.span.hi) {
+      const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
+      slot_in_page = key - nth * page_size;
+      const int64_t entry = in.span.entry + nth;
+      if (entry >= 0 && entry < a.lists.entries) page = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
+    }
+  }
+  __device__ __forceinline__ void begin(const AttendArgs &a, uint32_t ring_) {
+    ring = ring_;
+    grouped = a.cache.page_size % GROUP == 0;
+    page_rows = (uint32_t)(a.cache.heads * a.cache.page_size);
+    slot_in_page = 0;
+    look_up(a);
+  }
+  // Where piece ch of 16 bytes of row r goes: the rows are swizzled so that neither the reads of K nor those of V meet in a bank.
+  static __device__ __forceinline__ int k_at(int r, int ch) { return r * C::ROW + (ch ^ C::k_swizzle(r)) * 16; }
+  static __device__ __forceinline__ int v_at(int r, int ch) { return KEYS * C::ROW + r * C::ROW + (ch ^ C::v_swizzle(r)) * 16; }
+  static constexpr int SCALES = 2 * KEYS * C::ROW;
+
+  // Sends the next step to a stage of the ring.  A key that is not attended is zeros there, whatever its slot holds.
+  __device__ __forceinline__ void fetch(const AttendArgs &a, int stage, int units) {
+    const int lane = threadIdx.x % 32, ch0 = lane % C::CHUNKS, low = C::CHUNKS > 32 ? 0 : lane / C::CHUNKS, row_bytes = a.dim * C::ELEMENT;
+    const uint32_t to = ring + stage * C::STAGE;
+    const int key = first_key() + of_lane();
+    const bool listed = page >= 0 && page < a.cache.pages;
+    const uint32_t looked_row = (uint32_t)page * page_rows + head_row + (uint32_t)slot_in_page;
+    const int at = grouped ? (in.tile - looked) * GROUPS + of_lane() / GROUP : of_lane();  // the lane that looked this one's key up
+    const bool found = __shfl_sync(0xffffffffu, listed, at);
+    uint32_t row = __shfl_sync(0xffffffffu, looked_row, at) + (grouped ? of_lane() % GROUP : 0);  // of this lane's key
+    const bool there = found && key >= in.span.lo && key < in.span.hi;
+    if (!there) row = 0;
+    if (grouped && row_bytes % 16 == 0 && __all_sync(0xffffffffu, there)) {
+#pragma unroll
+      for (int n = 0; n < GROUPS; ++n) {
+        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, n * GROUP) * row_bytes + low * row_bytes;
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+          const int ch = ch0 + p * 32;
+          const char *const kp = static_cast<const char *>(a.cache.d_k) + ch * 16 + offset, *const vp = static_cast<const char *>(a.cache.d_v) + ch * 16 + offset;
+          if (ch * 16 < row_bytes) {
+#pragma unroll
+            for (int i = 0; i < GROUP / ROWS; ++i) {
+              const int r = n * GROUP + i * ROWS + low;
+              copy16(to + k_at(r, ch), kp + i * ROWS * row_bytes, true);
+              copy16(to + v_at(r, ch), vp + i * ROWS * row_bytes, true);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < KEYS / ROWS; ++i) {
+        const int r = i * ROWS + low;
+        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, r) * row_bytes;
+        const bool real = __shfl_sync(0xffffffffu, there, r);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+          const int ch = ch0 + p * 32;
+          const char *const kp = static_cast<const char *>(a.cache.d_k) + ch * 16 + offset, *const vp = static_cast<const char *>(a.cache.d_v) + ch * 16 + offset;
+          if (ch * 16 >= row_bytes) continue;
+          if (row_bytes % 16 == 0) {
+            copy16(to + k_at(r, ch), kp, real);
+            copy16(to + v_at(r, ch), vp, real);
+          } else {  // rows begin at multiples of 8 bytes
+            copy8(to + k_at(r, ch), kp, real);
+            copy8(to + v_at(r, ch), vp, real);
+            if (ch * 16 + 8 < row_bytes) {
+              copy8(to + k_at(r, ch) + 8, kp + 8, real);
+              copy8(to + v_at(r, ch) + 8, vp + 8, real);
+            }
+          }
+        }
+      }
+    }
+    if (C::CODES && lane < KEYS) {
+      copy4(to + SCALES + lane * 4, a.cache.d_k_scale + row, there);
+      copy4(to + SCALES + KEYS * 4 + lane * 4, a.cache.d_v_scale + row, there);
+    }
+    const int unit = in.unit, request = in.request;
+    in.next_tile(a, units, C::TILE);
+    if (!in.done && (!grouped || in.unit != unit || in.request != request || in.tile - looked == 32 / GROUPS)) look_up(a);
+  }
+};
+
 // ---- 16-bit queries: products on the tensor cores ----------------------------------
 //
 // Bound by the cache coming from memory, so the products only have to keep out of its way: mma.sync of 16 keys by 8 heads by
@@ -414,7 +575,7 @@ struct MmaConfig {
   static constexpr bool TWO_PARTS = !(CODES && std::is_same<T, __nv_bfloat16>::value);  // of the weights
   static constexpr int QP = std::is_same<T, float>::value ? 2 : 1;                      // parts of the queries
   static constexpr int DP = DP_, NT = NT_;                  // padded head, and eights of query heads
-  static constexpr int ROW = DP * (CODES ? 1 : 2);          // bytes of a key in shared memory
+  static constexpr int ELEMENT = CODES ? 1 : 2, ROW = DP * ELEMENT;  // bytes of a key in shared memory
   static constexpr int KEYS = ROW <= 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
@@ -425,38 +586,15 @@ struct MmaConfig {
   static_assert(STAGES >= 2, "one is copied while another is read");
   static_assert(PART * 4 <= STAGE, "a warp's sums fit where its last keys were");
   static constexpr float OFFSET = HALF ? 14.0f : 0.0f;
+  static __device__ __forceinline__ int k_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? 0 : r & 4; }
+  static __device__ __forceinline__ int v_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? r & 2 : (r & 3) << 1; }
 };
 
-__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool real) {  // zeros where it is not
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0));
-}
-__device__ __forceinline__ void copy8(uint32_t to, const void *from, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(real ? 8 : 0));
-}
-__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0));
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
-__device__ __forceinline__ uint4 load16(uint32_t at) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
-  return r;
-}
-__device__ __forceinline__ uint2 load8(uint32_t at) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
-  return r;
-}
-__device__ __forceinline__ float load4(uint32_t at) {
-  float r;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(at));
-  return r;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   uint32_t r;
@@ -496,13 +634,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
   uint32_t r;
   const uint16_t two = (uint16_t)(HIGH ? x >> 16 : x);
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
-  return r;
-}
-
-// 2^x to 2 units in the last place; what is below 2^-126 is zero.
-__device__ __forceinline__ float power2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
@@ -600,100 +731,19 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   const uint32_t ring = shared_address(mine);
   const int units = (int)a.cache.heads * a.head_blocks;
   pdl_wait();
-  Walk in, out;  // of the copies and of the products
-  const Share share = find_share(a, C::TILE, in);
+  Feed<C> feed;
+  const Share share = find_share(a, C::TILE, feed.in);
   pdl_release();
-  if (threadIdx.x == 0 && a.cuts != nullptr) a.cuts[blockIdx.x].last = 0;
-  if (in.done) return;
-  out = in;
+  note_none(a);
+  if (feed.in.done) return;
+  Walk out = feed.in;  // of the products; that of the copies is ahead
   auto clear_stage = [&](int stage) {  // what is beyond the head is never copied
     for (int i = lane; i < C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine + stage * C::STAGE)[i] = make_uint4(0, 0, 0, 0);
     __syncwarp();
   };
   if (a.dim != C::DP)
     for (int i = 0; i < STAGES; ++i) clear_stage(i);
-
-  // Pages of the next steps to copy.  `grouped`: pages have a multiple of 16 slots; lane n then has the page of the n-th 16 keys of
-  // this warp from tile `looked` on, 32 / MT steps of a unit by one look.  Otherwise lane n has that of key n of the next step.
-  const bool grouped = a.cache.page_size % 16 == 0;
-  const int page_size = (int)a.cache.page_size, row_bytes = a.dim * (C::CODES ? 1 : 2);
-  const int of_lane = lane % KEYS;  // the key of a step that is this lane's
-  int64_t page = -1;
-  int slot_in_page = 0, looked = 0;
-  auto look_up = [&]() {
-    looked = in.tile;
-    const int key = in.span.origin + warp * KEYS + (grouped ? (looked + lane / MT) * C::TILE + lane % MT * 16 : looked * C::TILE + of_lane);
-    page = -1;
-    if (key < in.span.hi) {
-      const int nth = a.page_shift >= 0 ? key >> a.page_shift : (int)((uint32_t)key / (uint32_t)page_size);
-      slot_in_page = key - nth * page_size;
-      const int64_t entry = in.span.entry + nth;
-      if (entry >= 0 && entry < a.lists.entries) page = load_index(a.lists.d_crd, entry, a.lists.idx_bytes);
-    }
-  };
-  // Where this lane's piece of 16 bytes of row r goes, r = i * ROWS + lane / CHUNKS: the rows are swizzled so that neither the
-  // reads of K nor those of V meet in a bank.
-  constexpr int ROWS = 32 / C::CHUNKS;  // of a copy
-  const int ch = lane % C::CHUNKS, low = lane / C::CHUNKS;
-  const bool in_row = ch * 16 < row_bytes;
-  auto k_at = [&](int r) { return r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch : ch ^ (r & 4)) * 16; };
-  auto v_at = [&](int r) { return KEYS * C::ROW + r * C::ROW + (!C::CODES ? ch ^ (r & 7) : C::DP == 64 ? ch ^ (r & 2) : ch ^ ((r & 3) << 1)) * 16; };
-  const char *const k_store = static_cast<const char *>(a.cache.d_k) + ch * 16, *const v_store = static_cast<const char *>(a.cache.d_v) + ch * 16;
-  const uint32_t page_rows = (uint32_t)(a.cache.heads * a.cache.page_size);
-  auto fetch = [&](int stage) {
-    const uint32_t to = ring + stage * C::STAGE;
-    const int key0 = in.span.origin + in.tile * C::TILE + warp * KEYS, key = key0 + of_lane;
-    const bool listed = page >= 0 && page < a.cache.pages;
-    const uint32_t looked_row = (uint32_t)page * page_rows + (uint32_t)(in.unit / a.head_blocks * page_size + slot_in_page);
-    const int at = grouped ? (in.tile - looked) * MT + of_lane / 16 : of_lane;  // the lane that looked this one's key up
-    const bool found = __shfl_sync(0xffffffffu, listed, at);
-    uint32_t row = __shfl_sync(0xffffffffu, looked_row, at) + (grouped ? of_lane % 16 : 0);  // of this lane's key
-    const bool there = found && key >= in.span.lo && key < in.span.hi;
-    if (!there) row = 0;
-    const bool plain = grouped && row_bytes % 16 == 0 && __all_sync(0xffffffffu, there);
-    if (plain) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, mt * 16) * row_bytes + low * row_bytes;
-        const char *const kp = k_store + offset, *const vp = v_store + offset;
-        if (in_row) {
-#pragma unroll
-          for (int i = 0; i < 16 / ROWS; ++i) {
-            const int r = mt * 16 + i * ROWS + low;
-            copy16(to + k_at(r), kp + i * ROWS * row_bytes, true);
-            copy16(to + v_at(r), vp + i * ROWS * row_bytes, true);
-          }
-        }
-      }
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < KEYS / ROWS; ++i) {
-        const int r = i * ROWS + low;
-        const int64_t offset = (int64_t)__shfl_sync(0xffffffffu, row, r) * row_bytes;
-        const bool real = __shfl_sync(0xffffffffu, there, r);
-        if (in_row && row_bytes % 16 == 0) {
-          copy16(to + k_at(r), k_store + offset, real);
-          copy16(to + v_at(r), v_store + offset, real);
-        } else if (in_row) {  // rows begin at multiples of 8 bytes
-          copy8(to + k_at(r), k_store + offset, real);
-          copy8(to + v_at(r), v_store + offset, real);
-          if (ch * 16 + 8 < row_bytes) {
-            copy8(to + k_at(r) + 8, k_store + offset + 8, real);
-            copy8(to + v_at(r) + 8, v_store + offset + 8, real);
-          }
-        }
-      }
-    }
-    if (C::CODES && lane < KEYS) {
-      const uint32_t scales = to + 2 * KEYS * C::ROW + lane * 4;
-      copy4(scales, a.cache.d_k_scale + row, there);
-      copy4(scales + KEYS * 4, a.cache.d_v_scale + row, there);
-    }
-    const int unit = in.unit, request = in.request;
-    in.next_tile(a, units, C::TILE);
-    if (!in.done && (!grouped || in.unit != unit || in.request != request || in.tile - looked == 32 / MT)) look_up();
-  };
-  look_up();
+  feed.begin(a, ring);
 
   uint32_t q[C::QP][NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
@@ -791,7 +841,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   for (int ahead = 1 - STAGES;; ahead = min(ahead + 1, 0)) {  // below 0: there are not enough copies on their way
     if (ahead == 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();
-    if (!in.done) fetch(stage_in);
+    if (!feed.in.done) feed.fetch(a, stage_in, units);
     asm volatile("cp.async.commit_group;" ::: "memory");
     stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
     if (ahead < 0) {
@@ -988,7 +1038,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     }
     const int request = out.request, head0 = (out.unit % a.head_blocks) * 8 * NT, first_head = out.unit / a.head_blocks * a.group + head0;
     const bool whole = began == 0 && out.end == out.tiles;
-    if (!whole && began == 0 && threadIdx.x == 0) a.cuts[blockIdx.x] = {share.last_of(out.left, out.tiles), first_piece ? 0 : 1, request, out.unit};
+    note_cut(a, share, out, began);
     out.next_unit(a, units, C::TILE);
     if (!out.done) load_q();  // on its way while the sums are given out
 #pragma unroll
@@ -1015,80 +1065,71 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
   }
 }
 
-// Adds up what the blocks left of the units that were cut, in their order: block (share where the unit begins, eight heads, two of
-// the sixteens of dimensions), a thread four sums of every fourth share.
+// Adds up what the blocks left of the units that were cut: the blocks of a unit's first shares take some of its sixteens of
+// dimensions each, a thread four sums of every parts-th share.  Bound by the time of its loads: the record of the cut, then the
+// shares' sums, BATCH at a time.
 constexpr int JOIN_THREADS = 256;
 template <typename C>
-__global__ void __launch_bounds__(JOIN_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
+__device__ __forceinline__ void join_unit(const AttendArgs &a, const CutUnit &cut, int n, float4 (&others)[2][JOIN_THREADS]) {
   using T = typename C::T;
-  constexpr int PART = C::PART, PARTS = JOIN_THREADS / 64;
-  __shared__ float weight[MOST_BLOCKS][8], most[8], total[8];
-  __shared__ float4 others[PARTS - 1][64];
+  constexpr int BATCH = 4;
+  const int shares = cut.last - cut.first + 1, members = shares <= 8 ? 1 : min(shares, C::DT), member = (int)blockIdx.x - cut.first;
+  if (cut.last == 0 || member >= members) return;
+  const int each = (C::DT + members - 1) / members, parts = max(1, JOIN_THREADS / 32 / each), rounds = (each * 32 + JOIN_THREADS - 1) / JOIN_THREADS;
+  const int first_head = cut.unit / a.head_blocks * a.group, head0 = (cut.unit % a.head_blocks) * 8 * C::NT + n * 8, heads = a.group - head0;
+  const float4 nothing = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f);
+  for (int round = 0; round < rounds; ++round) {
+    const int in = round * JOIN_THREADS + (int)threadIdx.x, part = in / 32 / each % parts, t = member * each + in / 32 % each;
+    const int lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+    const bool real = t < C::DT && in / 32 < each * parts;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f), ml = nothing;
+    auto add = [&](const float4 &x, const float4 &xml) {
+      const float m0 = fmaxf(ml.x, xml.x), m1 = fmaxf(ml.y, xml.y), b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+      const float f0 = power2(ml.x - b0), f1 = power2(ml.y - b1), e0 = power2(xml.x - b0), e1 = power2(xml.y - b1);
+      acc = make_float4(acc.x * f0 + x.x * e0, acc.y * f1 + x.y * e1, acc.z * f0 + x.z * e0, acc.w * f1 + x.w * e1);
+      ml = make_float4(m0, m1, ml.z * f0 + xml.z * e0, ml.w * f1 + xml.w * e1);
+    };
+    for (int from = part; real && from < shares; from += BATCH * parts) {
+      float4 x[BATCH], xml[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int share = from + i * parts;
+        const float4 *const slot = reinterpret_cast<const float4 *>(a.partial + ((int64_t)((cut.first + share) * 2 + (share > 0 ? 0 : cut.slot)) * C::NT + n) * C::PART);
+        x[i] = share < shares ? slot[t * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        xml[i] = share < shares ? slot[C::DT * 32 + c] : nothing;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) add(x[i], xml[i]);
+    }
+    if (parts > 1) {
+      __syncthreads();
+      others[0][threadIdx.x] = acc;
+      others[1][threadIdx.x] = ml;
+      __syncthreads();
+      if (part == 0 && real)
+        for (int i = 1; i < parts; ++i) add(others[0][threadIdx.x + i * each * 32], others[1][threadIdx.x + i * each * 32]);
+    }
+    if (part > 0 || !real) continue;
+    const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (2 * c + i >= heads) continue;
+      const int64_t head = (int64_t)cut.request * a.q_heads + first_head + head0 + 2 * c + i;
+      const float m = i == 0 ? ml.x : ml.y, l = i == 0 ? ml.z : ml.w, by = l == 0.0f ? 0.0f : 1.0f / l;
+      if (t == 0 && g == 0 && a.lse != nullptr) a.lse[head] = l == 0.0f ? -INFINITY : (m - C::OFFSET) * LN2 + logf(l);
+      T *const out = static_cast<T *>(a.out) + head * a.dim;
+      if (d0 < a.dim) out[d0] = from_f32<T>((i == 0 ? acc.x : acc.y) * by);
+      if (d1 < a.dim) out[d1] = from_f32<T>((i == 0 ? acc.z : acc.w) * by);
+    }
+  }
+}
+template <typename C>
+__global__ void __launch_bounds__(JOIN_THREADS) join_mma_kernel(const __grid_constant__ AttendArgs a) {
+  __shared__ float4 others[2][JOIN_THREADS];
   pdl_wait();
   const Cut cut = a.cuts[blockIdx.x];
-  if (cut.last == 0) return;
-  const int first = blockIdx.x, n = blockIdx.y, shares = cut.last - first + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int first_head = cut.unit / a.head_blocks * a.group, head0 = (cut.unit % a.head_blocks) * 8 * C::NT + n * 8, heads = a.group - head0;
-  auto slot = [&](int i) { return reinterpret_cast<const float4 *>(a.partial + ((int64_t)((first + i) * 2 + (i > 0 ? 0 : cut.slot)) * C::NT + n) * PART); };
-  for (int x = threadIdx.x; x < shares * 4; x += JOIN_THREADS) {  // lane c of a part has m and l of heads 2c and 2c + 1
-    const float4 ml = slot(x / 4)[C::DT * 32 + x % 4];
-    weight[x / 4][2 * (x % 4)] = ml.x;
-    weight[x / 4][2 * (x % 4) + 1] = ml.y;
-  }
-  __syncthreads();
-  {  // warp h: head h
-    float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < shares; i += 32) m = fmaxf(m, weight[i][warp]);
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const float base = m == -INFINITY ? 0.0f : m;
-    for (int i = lane; i < shares; i += 32) {
-      const float f = exp2f(weight[i][warp] - base);
-      const float4 ml = slot(i)[C::DT * 32 + warp / 2];
-      l = fmaf(warp % 2 ? ml.w : ml.z, f, l);
-      weight[i][warp] = f;
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
-    if (lane == 0) {
-      most[warp] = m;
-      total[warp] = l;
-    }
-  }
-  __syncthreads();
-  const int of = threadIdx.x % 64, part = threadIdx.x / 64, t = blockIdx.z * 2 + of / 32, g = lane / 4, c = lane % 4;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-  for (int i = part; i < shares; i += PARTS) {
-    const float4 x = slot(i)[t * 32 + lane];
-    const float f0 = weight[i][2 * c], f1 = weight[i][2 * c + 1];
-    acc.x = fmaf(x.x, f0, acc.x);
-    acc.y = fmaf(x.y, f1, acc.y);
-    acc.z = fmaf(x.z, f0, acc.z);
-    acc.w = fmaf(x.w, f1, acc.w);
-  }
-  if (part > 0) others[part - 1][of] = acc;
-  __syncthreads();
-  if (part > 0) return;
-#pragma unroll
-  for (int i = 0; i < PARTS - 1; ++i) {
-    const float4 x = others[i][of];
-    acc.x += x.x;
-    acc.y += x.y;
-    acc.z += x.z;
-    acc.w += x.w;
-  }
-  const int d0 = dimension<C>(t, g), d1 = C::CODES ? d0 + 1 : d0 + 8;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (2 * c + i >= heads) continue;
-    const int64_t head = (int64_t)cut.request * a.q_heads + first_head + head0 + 2 * c + i;
-    const float l = total[2 * c + i], by = l == 0.0f ? 0.0f : 1.0f / l;
-    if (t == 0 && g == 0 && a.lse != nullptr) a.lse[head] = l == 0.0f ? -INFINITY : (most[2 * c + i] - C::OFFSET) * LN2 + logf(l);
-    T *const out = static_cast<T *>(a.out) + head * a.dim;
-    if (d0 < a.dim) out[d0] = from_f32<T>((i == 0 ? acc.x : acc.y) * by);
-    if (d1 < a.dim) out[d1] = from_f32<T>((i == 0 ? acc.z : acc.w) * by);
-  }
+  join_unit<C>(a, cut.begins, blockIdx.y, others);
+  join_unit<C>(a, cut.goes_on, blockIdx.y, others);
 }
 
 template <typename C>
@@ -1105,7 +1146,7 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
   if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * C::NT * C::PART, st));
   LAPIS_CUDA_TRY(launch_pdl(attend_mma_kernel<C>, dim3(whole ? a.requests * (int)a.cache.heads * a.head_blocks : a.blocks), ATT_THREADS, C::SMEM, st, a));
   if (whole) return LAPIS_OK;
-  LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3(a.blocks, C::NT, C::DT / 2), JOIN_THREADS, 0, st, a));
+  LAPIS_CUDA_TRY(launch_pdl(join_mma_kernel<C>, dim3(a.blocks, C::NT), JOIN_THREADS, 0, st, a));
   return LAPIS_OK;
 }
 

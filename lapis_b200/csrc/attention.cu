@@ -342,11 +342,11 @@ __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_co
 // Adds up what the blocks left of the units that were cut, in their order: block (share where the unit begins, head), a thread a
 // dimension or two.
 template <typename T>
-__global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_constant__ AttendArgs a, int heads_of_unit) {
   pdl_wait();
   const CutUnit cut = a.cuts[blockIdx.x].begins;
   const int first = blockIdx.x, h = blockIdx.y, dim = a.dim;
-  const int head0 = (cut.unit % a.head_blocks) * ANY_HEADS;
+  const int head0 = (cut.unit % a.head_blocks) * heads_of_unit;
   if (cut.last == 0 || head0 + h >= a.group) return;
   auto slot = [&](int i) { return a.partial + ((int64_t)(i * 2 + (i > first ? 0 : cut.slot)) * ANY_HEADS + h) * (dim + 2); };
   float most = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
@@ -402,7 +402,7 @@ static int launch_any(AttendArgs a, int dev, cudaStream_t st) {
   if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * ANY_HEADS * (a.dim + 2), st));
   LAPIS_CUDA_TRY(launch_pdl(attend_any_kernel<T>, dim3(a.blocks), ATT_THREADS, any_smem(a.dim), st, a));
   if (whole) return LAPIS_OK;
-  LAPIS_CUDA_TRY(launch_pdl(join_any_kernel<T>, dim3(a.blocks, ANY_HEADS), ATT_THREADS, 0, st, a));
+  LAPIS_CUDA_TRY(launch_pdl(join_any_kernel<T>, dim3(a.blocks, ANY_HEADS), ATT_THREADS, 0, st, a, ANY_HEADS));
   return LAPIS_OK;
 }
 
@@ -548,6 +548,320 @@ struct Feed {
     if (!in.done && (!grouped || in.unit != unit || in.request != request || in.tile - looked == 32 / GROUPS)) look_up(a);
   }
 };
+
+// ---- 32-bit queries and caches ----------------------------------------------------
+//
+// Products and sums in 32 bits on the CUDA cores: bound by the cache for a query head or two a key head, and with eight by
+// shared memory and the products, about even with it.  A warp's KEYS keys of a step: four lanes share a key, a quarter of its
+// pieces each, and add up their parts of HEADS scores so that lane c of the four ends with heads c * HEADS / 4 onward; the
+// weights go through shared memory, and then a lane owns four dimensions (of every SPLIT-th key, where heads are narrow).
+
+template <int DP_, int HEADS_>
+struct F32Config {
+  static constexpr int DP = DP_, HEADS = HEADS_;            // padded head; query heads of a unit
+  static constexpr bool CODES = false;
+  static constexpr int ELEMENT = 4, ROW = DP * 4, CHUNKS = DP / 4;
+  static constexpr int KEYS = DP == 64 ? 16 : 8, TILE = KEYS * (ATT_THREADS / 32);
+  static constexpr int STAGE = 2 * KEYS * ROW;
+  static constexpr int OWN = HEADS >= 4 ? HEADS / 4 : 1;    // heads of a lane while there are scores
+  static constexpr int SPLIT = DP == 64 ? 2 : 1, OWNED = DP == 256 ? 2 : 1;  // keys side by side; fours of dimensions of a lane
+  static constexpr int PART = HEADS * DP + 2 * HEADS;       // floats of a warp's sums: O, then m and l
+  static constexpr int WEIGHTS = KEYS * HEADS + HEADS;      // floats of a warp's weights, and of the factors for older sums
+  static constexpr int EXTRA = (HEADS * DP + ATT_THREADS / 32 * WEIGHTS) * 4;
+  static constexpr int BLOCKS = DP == 256 ? 1 : 3;
+  static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048 - EXTRA) / (ATT_THREADS / 32 * STAGE);
+  static constexpr int SMEM = ATT_THREADS / 32 * STAGES * STAGE + EXTRA;
+  static_assert(STAGES >= 2, "one is copied while another is read");
+  static_assert(PART * 4 <= STAGE, "a warp's sums fit where its last keys were");
+  static __device__ __forceinline__ int k_swizzle(int r) { return (r & 1) << 2; }
+  static __device__ __forceinline__ int v_swizzle(int) { return 0; }
+};
+
+__device__ __forceinline__ float4 load_float4(uint32_t at) {
+  const uint4 x = load16(at);
+  return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+}
+
+template <typename C>
+__global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_f32_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int WARPS = ATT_THREADS / 32, KEYS = C::KEYS, HEADS = C::HEADS, OWN = C::OWN, STAGES = C::STAGES, ROUNDS = KEYS / 8;
+  extern __shared__ __align__(128) unsigned char stages[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
+  unsigned char *const mine = stages + warp * STAGES * C::STAGE;
+  float *const qs = reinterpret_cast<float *>(stages + WARPS * STAGES * C::STAGE), *const weights = qs + HEADS * C::DP + warp * C::WEIGHTS;
+  float *const factors = weights + KEYS * HEADS;
+  const int units = (int)a.cache.heads * a.head_blocks;
+  pdl_wait();
+  Feed<C> feed;
+  const Share share = find_share(a, C::TILE, feed.in);
+  pdl_release();
+  note_none(a);
+  if (feed.in.done) return;
+  Walk out = feed.in;
+  for (int i = lane; i < STAGES * C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(mine)[i] = make_uint4(0, 0, 0, 0);  // beyond the head
+  __syncwarp();
+  feed.begin(a, shared_address(mine));
+
+  // The queries of a unit are fetched while the one in front is given out.
+  constexpr int MINE = HEADS * C::DP / ATT_THREADS > 0 ? HEADS * C::DP / ATT_THREADS : 1;
+  float raw[MINE];
+  auto load_q = [&]() {
+    const int head0 = (out.unit % a.head_blocks) * HEADS;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+      const int at = i * ATT_THREADS + threadIdx.x, h = at / C::DP, d = at % C::DP;
+      raw[i] = at < HEADS * C::DP && d < a.dim && head0 + h < a.group
+                   ? static_cast<const float *>(a.q)[out.request * a.q_token_stride + (int64_t)(out.unit / a.head_blocks * a.group + head0 + h) * a.q_head_stride + d]
+                   : 0.0f;
+    }
+  };
+  auto take_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i)
+      if (i * ATT_THREADS + threadIdx.x < HEADS * C::DP) qs[i * ATT_THREADS + threadIdx.x] = raw[i];
+    __syncthreads();
+  };
+  float4 acc[HEADS][C::OWNED];
+  float m[OWN], l[OWN];
+  auto clear = [&]() {
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+      for (int o = 0; o < C::OWNED; ++o) acc[h][o] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+    }
+  };
+  load_q();
+  int began = out.tile, stage = 0, stage_in = 0;
+  bool first_piece = true;
+  const int rounds = (a.dim + 15) / 16;  // pieces of a key that a lane multiplies
+#pragma unroll 1
+  for (int ahead = 1 - STAGES;; ahead = min(ahead + 1, 0)) {  // below 0: there are not enough copies on their way
+    if (ahead == 0) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();
+    if (!feed.in.done) feed.fetch(a, stage_in, units);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    if (ahead < 0) {
+      if (ahead == -1) {
+        take_q();
+        clear();
+      }
+      continue;
+    }
+
+    const uint32_t ks = feed.ring + stage * C::STAGE, vs = ks + KEYS * C::ROW, q_at = shared_address(qs);
+    const int key0 = out.span.origin + out.tile * C::TILE + warp * KEYS;
+    float score[ROUNDS][OWN];
+#pragma unroll
+    for (int u = 0; u < ROUNDS; ++u) {
+      const int r = u * 8 + g;
+      float2 part[HEADS];
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) part[h] = make_float2(0.0f, 0.0f);
+#pragma unroll 2
+      for (int i = 0; i < rounds; ++i) {
+        const float4 k = load_float4(ks + r * C::ROW + (((c + 4 * i) ^ C::k_swizzle(r)) * 16));
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+          const float4 x = load_float4(q_at + (h * C::DP + (c + 4 * i) * 4) * 4);
+          part[h] = fma2({k.x, k.y}, {x.x, x.y}, part[h]);
+          part[h] = fma2({k.z, k.w}, {x.z, x.w}, part[h]);
+        }
+      }
+      float sum[HEADS];
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) sum[h] = part[h].x + part[h].y;
+      if constexpr (HEADS == 1) {
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
+        score[u][0] = sum[0];
+      } else {
+        float half[HEADS / 2];
+#pragma unroll
+        for (int h = 0; h < HEADS / 2; ++h) {
+          const float keep = c & 2 ? sum[HEADS / 2 + h] : sum[h], send = c & 2 ? sum[h] : sum[HEADS / 2 + h];
+          half[h] = keep + __shfl_xor_sync(0xffffffffu, send, 2);
+        }
+#pragma unroll
+        for (int h = 0; h < OWN; ++h) {
+          const float keep = c & 1 ? half[OWN + h] : half[h], send = c & 1 ? half[h] : half[OWN + h];
+          score[u][h] = keep + __shfl_xor_sync(0xffffffffu, send, 1);
+        }
+      }
+      const bool seen = key0 + r >= out.span.lo && key0 + r < out.span.hi;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) score[u][i] = seen ? score[u][i] * a.scale2 : -INFINITY;
+    }
+    bool grows = false;
+    float base[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      float x = m[i];
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) x = fmaxf(x, score[u][i]);
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+      base[i] = x == -INFINITY ? 0.0f : x;
+      grows |= x > m[i];
+      const float f = exp2f(m[i] - base[i]);
+      l[i] *= f;
+      m[i] = x;
+      if (g == 0) factors[(HEADS == 1 ? 0 : c * OWN) + i] = f;
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        const float p = exp2f(score[u][i] - base[i]);
+        l[i] += p;
+        weights[(u * 8 + g) * HEADS + (HEADS == 1 ? 0 : c * OWN) + i] = p;
+      }
+    }
+    grows = __any_sync(0xffffffffu, grows);
+    __syncwarp();
+    if (grows) {
+#pragma unroll
+      for (int h = 0; h < HEADS; ++h) {
+        const float f = factors[h];
+#pragma unroll
+        for (int o = 0; o < C::OWNED; ++o) {
+          acc[h][o].x *= f;
+          acc[h][o].y *= f;
+          acc[h][o].z *= f;
+          acc[h][o].w *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < KEYS; j += C::SPLIT) {
+      const int r = j + (C::SPLIT == 2 ? lane / 16 : 0), ch = C::SPLIT == 2 ? lane % 16 : lane;
+      float p[HEADS];
+      if constexpr (HEADS >= 4) {
+#pragma unroll
+        for (int h = 0; h < HEADS; h += 4) {
+          const float4 x = *reinterpret_cast<const float4 *>(weights + r * HEADS + h);
+          p[h] = x.x;
+          p[h + 1] = x.y;
+          p[h + 2] = x.z;
+          p[h + 3] = x.w;
+        }
+      } else {
+        p[0] = weights[r];
+      }
+#pragma unroll
+      for (int o = 0; o < C::OWNED; ++o) {
+        const float4 v = load_float4(vs + r * C::ROW + (ch + 32 * o) * 16);
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+          const float2 lo = fma2({v.x, v.y}, {p[h], p[h]}, {acc[h][o].x, acc[h][o].y}), hi = fma2({v.z, v.w}, {p[h], p[h]}, {acc[h][o].z, acc[h][o].w});
+          acc[h][o] = make_float4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+    }
+    __syncwarp();  // the weights have been read
+
+    const int used = stage;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    if (out.tile + 1 < out.end) {
+      ++out.tile;
+      continue;
+    }
+    const int request = out.request, head0 = (out.unit % a.head_blocks) * HEADS, heads = min(HEADS, a.group - head0);
+    const int64_t first_head = (int64_t)request * a.q_heads + out.unit / a.head_blocks * a.group + head0;
+    const bool whole = began == 0 && out.end == out.tiles;
+    note_cut(a, share, out, began);
+    out.next_unit(a, units, C::TILE);
+    if (!out.done) load_q();
+    // the warps' sums meet where their last keys were
+    float *const sums = reinterpret_cast<float *>(mine + used * C::STAGE);
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+      if (g == 0) {
+        const int h = (HEADS == 1 ? 0 : c * OWN) + i;
+        sums[HEADS * C::DP + 2 * h] = m[i];
+        sums[HEADS * C::DP + 2 * h + 1] = l[i];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h)
+#pragma unroll
+      for (int o = 0; o < C::OWNED; ++o) {
+        float4 x = acc[h][o];
+        if constexpr (C::SPLIT == 2) {
+          x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
+          x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
+          x.z += __shfl_xor_sync(0xffffffffu, x.z, 16);
+          x.w += __shfl_xor_sync(0xffffffffu, x.w, 16);
+        }
+        if (C::SPLIT == 1 || lane < 16) *reinterpret_cast<float4 *>(sums + h * C::DP + (lane % C::CHUNKS + 32 * o) * 4) = x;
+      }
+    __syncthreads();
+    auto of_warp = [&](int w) { return reinterpret_cast<const float *>(stages + (w * STAGES + used) * C::STAGE); };
+    float *const slot = a.partial + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * ANY_HEADS * (a.dim + 2);
+    for (int at = threadIdx.x; at < heads * C::DP; at += ATT_THREADS) {
+      const int h = at / C::DP, d = at % C::DP;
+      float most = -INFINITY, total = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) most = fmaxf(most, of_warp(w)[HEADS * C::DP + 2 * h]);
+      const float shift = most == -INFINITY ? 0.0f : most;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(of_warp(w)[HEADS * C::DP + 2 * h] - shift);
+        total = fmaf(of_warp(w)[HEADS * C::DP + 2 * h + 1], f, total);
+        x = fmaf(of_warp(w)[at], f, x);
+      }
+      if (d >= a.dim) continue;
+      if (whole) {
+        static_cast<float *>(a.out)[(first_head + h) * a.dim + d] = total == 0.0f ? 0.0f : x / total;
+        if (d == 0 && a.lse != nullptr) a.lse[first_head + h] = total == 0.0f ? -INFINITY : most * LN2 + logf(total);
+      } else {
+        slot[h * (a.dim + 2) + 2 + d] = x;
+        if (d == 0) {
+          slot[h * (a.dim + 2)] = most;
+          slot[h * (a.dim + 2) + 1] = total;
+        }
+      }
+    }
+    __syncthreads();
+    if (out.done) return;
+    if (a.dim != C::DP) {
+      for (int i = lane; i < C::STAGE / 16; i += 32) reinterpret_cast<uint4 *>(sums)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+    first_piece = false;
+    began = 0;
+    take_q();
+    clear();
+  }
+}
+
+template <typename C>
+static int launch_f32(AttendArgs a, int dev, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may use its shared memory
+  if ((allowed.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+    LAPIS_CUDA_TRY(cudaFuncSetAttribute(attend_f32_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    allowed.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
+  a.head_blocks = (a.group + C::HEADS - 1) / C::HEADS;
+  a.blocks = std::min(C::BLOCKS * sm_count(), MOST_BLOCKS);
+  PoolBuf work;
+  const bool whole = always_whole(a, C::TILE);
+  if (!whole) LAPIS_TRY(make_workspace(a, work, 2 * ANY_HEADS * (a.dim + 2), st));
+  LAPIS_CUDA_TRY(launch_pdl(attend_f32_kernel<C>, dim3(whole ? a.requests * (int)a.cache.heads * a.head_blocks : a.blocks), ATT_THREADS, C::SMEM, st, a));
+  if (whole) return LAPIS_OK;
+  LAPIS_CUDA_TRY(launch_pdl(join_any_kernel<float>, dim3(a.blocks, C::HEADS), ATT_THREADS, 0, st, a, C::HEADS));
+  return LAPIS_OK;
+}
+
+template <int HEADS>
+static int launch_f32_of(const AttendArgs &a, int dev, cudaStream_t st) {
+  if (a.dim <= 64) return launch_f32<F32Config<64, HEADS>>(a, dev, st);
+  if (a.dim <= 128) return launch_f32<F32Config<128, HEADS>>(a, dev, st);
+  return launch_f32<F32Config<256, HEADS>>(a, dev, st);
+}
 
 // ---- 16-bit queries: products on the tensor cores ----------------------------------
 //
@@ -1159,19 +1473,19 @@ static int launch_mma_of(const AttendArgs &a, int dev, cudaStream_t st) {
   return launch_mma<MmaConfig<T, STORE, 128, 1>>(a, dev, st);
 }
 
-// Rows of whole 8 bytes from 16-byte addresses, of 16-bit numbers or of codes.
-static bool mma_fits(int type, const AttendArgs &a) {
-  if (type == LAPIS_F32 && !is_quantised(a.cache.type)) return false;
-  return a.dim * type_bytes(a.cache.type) % 8 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
+// Rows of whole 8 bytes (of 32-bit numbers: of 16) from 16-byte addresses.
+static bool pieces_fit(const AttendArgs &a) {
+  const int64_t row = a.dim * type_bytes(a.cache.type);
+  return row % (a.cache.type == LAPIS_F32 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
 }
 
 template <typename T>
-static int launch_type(const AttendArgs &a, bool fits, int dev, cudaStream_t st) {
-  if (!fits) return launch_any<T>(a, dev, st);
+static int launch_type(const AttendArgs &a, int dev, cudaStream_t st) {
+  if (!pieces_fit(a)) return launch_any<T>(a, dev, st);
   if (a.cache.type == LAPIS_I8) return launch_mma_of<T, LAPIS_I8>(a, dev, st);
   if (a.cache.type == LAPIS_E4M3) return launch_mma_of<T, LAPIS_E4M3>(a, dev, st);
-  if constexpr (std::is_same<T, float>::value) return launch_any<T>(a, dev, st);
-  else return launch_mma_of<T, LAPIS_F32>(a, dev, st);
+  if constexpr (!std::is_same<T, float>::value) return launch_mma_of<T, LAPIS_F32>(a, dev, st);
+  else return a.group == 1 ? launch_f32_of<1>(a, dev, st) : a.group <= 4 ? launch_f32_of<4>(a, dev, st) : launch_f32_of<8>(a, dev, st);
 }
 
 }  // namespace lapis_b200
@@ -1217,8 +1531,7 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   cudaStream_t st = as_stream(stream);
   a.page_shift = page_shift_of(cache->page_size);
   a.q_pairs = reinterpret_cast<uintptr_t>(a.q) % 4 == 0 && a.q_token_stride % 2 == 0 && a.q_head_stride % 2 == 0;
-  const bool fits = mma_fits(type, a);
-  if (type == LAPIS_F32) return launch_type<float>(a, fits, dev, st);
-  if (type == LAPIS_F16) return launch_type<__half>(a, fits, dev, st);
-  return launch_type<__nv_bfloat16>(a, fits, dev, st);
+  if (type == LAPIS_F32) return launch_type<float>(a, dev, st);
+  if (type == LAPIS_F16) return launch_type<__half>(a, dev, st);
+  return launch_type<__nv_bfloat16>(a, dev, st);
 }

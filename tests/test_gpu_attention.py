@@ -382,6 +382,34 @@ ATTEND = [
     ([9000, 1], 4, 1, 40, 16, F32, F32, 0),
     (list(range(0, 400, 3)), 4, 2, 128, 16, BF16, BF16, 0),   # 134 ragged requests
     ([40] * 700, 2, 1, 64, 16, BF16, E4M3, 0),
+    # 32 bits: eight, four and one query heads a unit, wide and narrow heads, pages that split a group of keys
+    ([300, 0, 41], 8, 1, 64, 16, F32, F32, 0),
+    ([300, 0, 41], 5, 1, 128, 12, F32, F32, 0),
+    ([300, 0, 41], 11, 1, 256, 16, F32, F32, 0),
+    ([300, 0, 41], 9, 3, 256, 8, F32, F32, 50),
+    ([300, 0, 41], 2, 2, 256, 1, F32, F32, 0),
+    ([300, 0, 41], 2, 2, 32, 24, F32, F32, 33),
+    ([2500], 20, 2, 100, 64, F32, F32, 0),
+    ([70001, 5], 2, 2, 128, 16, F32, F32, 0),
+    ([300, 0, 41], 20, 1, 128, 16, F32, E4M3, 0),
+    ([300, 0, 41], 20, 2, 64, 12, F32, I8, 100),
+    ([300, 700], 3, 1, 256, 16, F32, I8, 0),
+    ([5000], 4, 4, 72, 16, F32, I8, 0),
+    # rows of whole 8 bytes, and of less
+    ([300, 0, 41], 4, 2, 36, 16, F16, F16, 0),
+    ([300, 0, 41], 4, 2, 100, 12, BF16, BF16, 40),
+    ([300, 0, 41], 20, 2, 132, 16, BF16, BF16, 0),
+    ([300, 0, 41], 4, 2, 40, 5, F16, E4M3, 0),
+    ([300, 0, 41], 4, 2, 200, 16, BF16, I8, 0),
+    ([300, 0, 41], 4, 2, 34, 16, F16, F16, 0),
+    ([300, 0, 41], 4, 2, 66, 16, F32, F32, 0),
+    # windows whose first key is no multiple of 16, of whole and of cut units
+    ([6000, 17, 100], 8, 2, 128, 16, BF16, BF16, 1001),
+    ([6000, 17, 100], 32, 2, 128, 48, F16, I8, 1001),
+    ([60000, 59999], 2, 1, 64, 128, F16, E4M3, 50007),
+    # many requests: more than a thread each, and many that are short
+    ([3] * 300 + [900, 0, 5] + [1] * 40, 8, 2, 128, 16, BF16, I8, 0),
+    ([17] * 500, 4, 4, 64, 16, F32, F32, 0),
 ]
 
 

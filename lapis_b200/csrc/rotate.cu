@@ -698,8 +698,9 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_kernel(const __grid_consta
 
 // Backward: warps take tokens a grid apart and keep their share of the weights' gradients in registers.  The warps' lane groups
 // are added in order by the block, the blocks by rotate_weights_kernel.
+constexpr int backward_blocks(int size) { return size == 4 ? 4 : 3; }  // an SM, by registers
 template <typename T, int LANES>
-__global__ void __launch_bounds__(ROW_THREADS) rotate_backward_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
+__global__ void __launch_bounds__(ROW_THREADS, backward_blocks(sizeof(T))) rotate_backward_kernel(const __grid_constant__ RotateArgs a, int parts, int each) {
   constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, DEPTH = 3;
   __shared__ __align__(16) unsigned char rings[ROW_WARPS][DEPTH * 2048];
   __shared__ float shares[ROW_THREADS / LANES][LANES * 2 * V];
@@ -1054,11 +1055,10 @@ static int launch_rotate(int type, const RotateArgs &a, cudaStream_t st) {
 
 // Launches the backward kernel that fits and leaves in *blocks how many shares of the weights' gradients there are.
 static int launch_backward(int type, RotateArgs &a, PoolBuf &partial, int *blocks, cudaStream_t st) {
-  const int64_t most = 5LL * sm_count();  // what is resident at 96 registers a thread
   return with_type(type, [&](auto t) {
     using T = decltype(t);
     auto room = [&](int64_t wanted) {
-      *blocks = (int)std::min(wanted, most);
+      *blocks = (int)std::min<int64_t>(wanted, backward_blocks(sizeof(T)) * sm_count());  // what is resident
       const int status = partial.alloc((size_t)*blocks * 2 * a.dim * sizeof(float), st);
       a.partial = static_cast<float *>(partial.p);
       return status;

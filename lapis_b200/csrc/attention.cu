@@ -1525,6 +1525,10 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   a.window = window;
   a.cache = *cache;
   a.lists = *lists;
+  if (cache->pages == 0) {  // nothing is read, but zeros are copied from somewhere
+    a.cache.d_k = a.cache.d_v = const_cast<void *>(q->d);
+    a.cache.d_k_scale = a.cache.d_v_scale = static_cast<float *>(a.cache.d_k);
+  }
   a.length = d_length;
   a.out = d_out;
   a.lse = d_lse;

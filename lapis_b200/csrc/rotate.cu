@@ -830,7 +830,7 @@ template <typename T, int LANES, bool CODES>
 __global__ void __launch_bounds__(ROW_THREADS)
 kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row,
                const void *place, int page_shift, int parts, int each, T *k, T *v) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = 2, SIZE = CODES ? 1 : sizeof(T);
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = 1, SIZE = CODES ? 1 : sizeof(T);
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= tokens) return;
   const int lane = threadIdx.x % LANES, dim = (int)cache.dim, heads = (int)cache.heads;

@@ -23,8 +23,8 @@ namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
 constexpr int UNIT_COST = 2;      // what a unit costs beside its tiles, in tiles: 128 x 8192 int8 214 us with 1, 204 with 2 or 3
-constexpr int MIN_WORK = 4;       // of a share, if there is more than one
-constexpr int WHOLE_TILES = 4;    // by which a unit may be longer than a share and is not cut
+constexpr int MIN_WORK = 2;       // of a share, if there is more than one
+constexpr int WHOLE_TILES = 6;    // by which a unit may be longer than a share and is not cut
 constexpr int MOST_BLOCKS = 1 << 10;  // shares
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -1382,7 +1382,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 // Adds up what the blocks left of the units that were cut: the blocks of a unit's first shares take some of its sixteens of
 // dimensions each, a thread four sums of every parts-th share.  Bound by the time of its loads: the record of the cut, then the
 // shares' sums, BATCH at a time.
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 512;
 template <typename C>
 __device__ __forceinline__ void join_unit(const AttendArgs &a, const CutUnit &cut, int n, float4 (&others)[2][JOIN_THREADS]) {
   using T = typename C::T;

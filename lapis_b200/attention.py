@@ -2,7 +2,8 @@
 and attention of one new token over it.
 
 Part of the device-resident layer (see ``device``): every operation is one call into ``liblapis_b200.so`` on torch's
-current stream, operands are tensors of the current device, results are new tensors.  A serving step is
+current stream, operands are tensors of the current device, results are new tensors.  Nothing is recorded for autograd.  A serving
+step is
 
     q = cache.append_norm_rope(q, k, v, q_weight, k_weight, cos, sin, pos, crd, row, place)
     out = paged_attention(q, cache, pos, crd, length)
@@ -23,6 +24,15 @@ from .device import _calls
 
 _CACHE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
 _ROW_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _tensors(**named):
+    """Operands that are looked at first: tensors, of three extents where the name says so."""
+    for name, t in named.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if name in ("q", "k", "v", "dq", "dk") and t.dim() != 3:
+            raise ValueError(f"{name} must be [tokens, heads, dim]")
 
 
 def _check_rows(name, t, dtype, tokens, dim, heads=None):
@@ -53,6 +63,7 @@ def _check_lists(pos, crd):
 
 
 def _check_how(dtype, dim, q_weight, k_weight, cos, sin):
+    _tensors(q_weight=q_weight, cos=cos)
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if not isinstance(w, torch.Tensor) or not w.is_cuda or not w.is_contiguous() or w.dtype not in (torch.float32, dtype) or w.dtype != q_weight.dtype:
             raise TypeError(f"{name} must be a contiguous CUDA tensor of float32 or of the rows' type, the same for both")
@@ -81,7 +92,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, place, eps: float = 1e-6, i
     got = _calls.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps, interleaved, place)
     if type(got) is int:
         if got < 0:
-            _check_rows("q", q, q.dtype, q.shape[0], q.shape[-1])
+            _tensors(q=q, k=k)
+            _check_rows("q", q, q.dtype, q.shape[0], q.shape[2])
             _check_rows("k", k, q.dtype, q.shape[0], q.shape[2])
             _check_how(q.dtype, q.shape[2], q_weight, k_weight, cos, sin)
             _check_indices(getattr(place, "dtype", None), place=(place, q.shape[0]))
@@ -96,7 +108,8 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, place, eps
     got = _calls.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, eps, interleaved, place)
     if type(got) is int:
         if got < 0:
-            _check_rows("q", q, q.dtype, q.shape[0], q.shape[-1])
+            _tensors(dq=dq, dk=dk, q=q, k=k)
+            _check_rows("q", q, q.dtype, q.shape[0], q.shape[2])
             _check_rows("k", k, q.dtype, q.shape[0], q.shape[2])
             _check_rows("dq", dq, q.dtype, q.shape[0], q.shape[2], q.shape[1])
             _check_rows("dk", dk, q.dtype, q.shape[0], q.shape[2], k.shape[1])
@@ -156,7 +169,8 @@ class PagedCache:
             raise TypeError(f"{what}: the cache must be on the current device")
 
     def _check_new(self, k, v, pos, crd, row, place):
-        _check_rows("k", k, getattr(k, "dtype", None), k.shape[0], self.dim, self.heads)
+        _tensors(k=k, v=v)
+        _check_rows("k", k, k.dtype, k.shape[0], self.dim, self.heads)
         _check_rows("v", v, k.dtype, k.shape[0], self.dim, self.heads)
         _check_lists(pos, crd)
         _check_indices(pos.dtype, crd=(crd, None), row=(row, k.shape[0]), place=(place, k.shape[0]))
@@ -180,6 +194,7 @@ class PagedCache:
         if type(got) is int:
             if got < 0:
                 self._check_new(k, v, pos, crd, row, place)
+                _tensors(q=q)
                 _check_rows("q", q, k.dtype, k.shape[0], self.dim)
                 _check_how(k.dtype, self.dim, q_weight, k_weight, cos, sin)
                 _raise("append_norm_rope")
@@ -196,6 +211,7 @@ class PagedCache:
         if type(got) is int:
             if got < 0:
                 _check_lists(pos, crd)
+                _tensors(row=row)
                 _check_indices(pos.dtype, crd=(crd, None), row=(row, row.numel()), place=(place, row.numel()))
                 _raise("read")
             check(got)
@@ -213,7 +229,8 @@ def paged_attention(q, cache: PagedCache, pos, crd, length, scale: float | None 
     got = _calls.paged_attention(cache._addr, q, pos, crd, length, cache.dim ** -0.5 if scale is None else scale, window or 0, return_lse)
     if type(got) is int:
         if got < 0:
-            _check_rows("q", q, getattr(q, "dtype", None), q.shape[0], cache.dim)
+            _tensors(q=q)
+            _check_rows("q", q, q.dtype, q.shape[0], cache.dim)
             _check_lists(pos, crd)
             _check_indices(pos.dtype, crd=(crd, None), length=(length, q.shape[0]))
             _raise("paged_attention")

@@ -244,7 +244,8 @@ PyObject *py_kv_append(PyObject *const *a) {
   lapis_b200_heads hk, hv;
   lapis_b200_page_lists lists;
   const void *row, *place;
-  if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hk) || !heads_of(a[2], type, tokens, cache->dim, &hv) || !lists_of(a[3], a[4], &lists) ||
+  if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hk) || !heads_of(a[2], type, tokens, cache->dim, &hv) ||
+      hk.heads != cache->heads || hv.heads != cache->heads || !lists_of(a[3], a[4], &lists) ||
       !indices_of(a[5], tokens, &lists.idx_bytes, &row) || !indices_of(a[6], tokens, &lists.idx_bytes, &place))
     return status(-1);
   return call(lapis_b200_kv_append, type, tokens, nullptr, &hk, &hv, nullptr, cache, &lists, row, place, nullptr, stream());
@@ -262,7 +263,7 @@ PyObject *py_kv_append_norm_rope(PyObject *const *a) {
   lapis_b200_page_lists lists;
   const void *row, *place;
   if (type < 0 || !heads_of(a[1], type, tokens, cache->dim, &hq) || !heads_of(a[2], type, tokens, cache->dim, &hk) ||
-      !heads_of(a[3], type, tokens, cache->dim, &hv) || !norm_rope_of(a + 4, type, cache->dim, &how) || !lists_of(a[10], a[11], &lists) ||
+      !heads_of(a[3], type, tokens, cache->dim, &hv) || hk.heads != cache->heads || hv.heads != cache->heads || !norm_rope_of(a + 4, type, cache->dim, &how) || !lists_of(a[10], a[11], &lists) ||
       !indices_of(a[12], tokens, &lists.idx_bytes, &row) || !indices_of(a[13], tokens, &lists.idx_bytes, &place))
     return status(-1);
   if (PyErr_Occurred()) return nullptr;

@@ -617,3 +617,81 @@ def test_attend_rows_beyond_32_bits(A):
     assert torch.equal(got[0].double(), torch.cat([h[0] for h in held])) and torch.equal(got[1].double(), torch.cat([h[1] for h in held]))
     q = normal(5, 2, 8, dim).bfloat16()
     holds(q, A.paged_attention(q, cache, pos, crd, torch.tensor(lens, device=DEV, dtype=torch.int32), return_lse=True), attend64(q, held, dim ** -0.5, 0))
+
+
+# ---- what the calls refuse ----------------------------------------------------
+
+
+@pytest.mark.parametrize("error,change", [
+    (TypeError, {"q": None}), (ValueError, {"q": lambda t: t[0]}), (TypeError, {"q": lambda t: t.double()}), (TypeError, {"q": lambda t: t.cpu()}),
+    (TypeError, {"q": lambda t: t.half()}), (TypeError, {"q": lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)}),
+    (TypeError, {"k": lambda t: t.half()}), (ValueError, {"k": lambda t: t[:2]}), (ValueError, {"v": lambda t: t[:, :1]}), (ValueError, {"k": lambda t: t[..., :32]}),
+    (ValueError, {"q_weight": lambda t: t[:32]}), (TypeError, {"k_weight": lambda t: t.double()}), (TypeError, {"q_weight": None}),
+    (ValueError, {"sin": lambda t: t[:5]}), (TypeError, {"cos": lambda t: t.half()}), (ValueError, {"cos": lambda t: t.repeat(1, 2), "sin": lambda t: t.repeat(1, 2)}),
+    (TypeError, {"place": lambda t: t.float()}), (ValueError, {"place": lambda t: t[:2]}), (TypeError, {"row": lambda t: t.float()}), (ValueError, {"row": lambda t: t[:2]}),
+    (TypeError, {"crd": lambda t: t.long()}), (TypeError, {"pos": None}), (ValueError, {"pos": lambda t: t[:0]}), (TypeError, {"place": lambda t: t[::2].repeat_interleave(2)[::2]}),
+])
+def test_append_norm_rope_raises(A, error, change):
+    cache, pos, crd = make_cache(A, ([8, 8], 2, 64, 4, BF16, I8, torch.int32))
+    cos, sin = tables(8, 64)
+    x = normal(1, 4, 8, 64).bfloat16()
+    i32 = dict(device=DEV, dtype=torch.int32)
+    a = dict(q=x[:, :4], k=x[:, 4:6], v=x[:, 6:], q_weight=torch.ones(64, device=DEV), k_weight=torch.ones(64, device=DEV), cos=cos, sin=sin, pos=pos, crd=crd,
+             row=torch.tensor([0, 0, 1, 1], **i32), place=torch.tensor([0, 1, 0, 1], **i32))
+    cache.append_norm_rope(**a)
+    before = cache.k.clone()
+    for name, f in change.items():
+        a[name] = f(a[name]) if f else None
+    with pytest.raises(error):
+        cache.append_norm_rope(**a)
+    if not {"pos", "crd", "row", "v"} & set(change):
+        b = {n: a[n] for n in ("q", "k", "q_weight", "k_weight", "cos", "sin", "place")}
+        with pytest.raises(error):
+            A.qk_norm_rope(**b)
+        with pytest.raises(error):
+            A.qk_norm_rope_backward(a["q"], a["k"], **b)
+    if {"k", "v", "row", "place", "pos", "crd"} & set(change):
+        with pytest.raises(error):
+            cache.append(a["k"], a["v"], pos=a["pos"], crd=a["crd"], row=a["row"], place=a["place"])
+    if {"row", "place", "pos", "crd"} & set(change):
+        with pytest.raises(error):
+            cache.read(a["pos"], a["crd"], a["row"], a["place"])
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, before)
+
+
+@pytest.mark.parametrize("error,change", [
+    (TypeError, {"q": None}), (ValueError, {"q": lambda t: t[0]}), (TypeError, {"q": lambda t: t.double()}), (TypeError, {"q": lambda t: t.cpu()}),
+    (ValueError, {"q": lambda t: t[..., :32]}), (ValueError, {"length": lambda t: t[:1]}), (TypeError, {"length": lambda t: t.long()}),
+    (TypeError, {"crd": lambda t: t.float()}), (ValueError, {"pos": lambda t: t[:0]}),
+])
+def test_attention_raises(A, error, change):
+    from lapis_b200._lib import LapisError
+    cache, pos, crd = make_cache(A, ([8, 8], 2, 64, 4, BF16, I8, torch.int32))
+    a = dict(q=normal(1, 2, 4, 64).bfloat16(), pos=pos, crd=crd, length=torch.tensor([3, 5], device=DEV, dtype=torch.int32))
+    for name, f in change.items():
+        a[name] = f(a[name]) if f else None
+    with pytest.raises(error):
+        A.paged_attention(cache=cache, **a)
+    with pytest.raises(TypeError):
+        cache.read(pos, crd, pos[:2], pos[:2], dtype=torch.float64)
+    with pytest.raises(LapisError):  # three query heads over two
+        A.paged_attention(normal(1, 2, 3, 64).bfloat16(), cache, pos, crd, torch.tensor([3, 5], device=DEV, dtype=torch.int32))
+    with pytest.raises(LapisError):  # a list too few
+        A.paged_attention(normal(1, 2, 4, 64).bfloat16(), cache, pos[:2], crd, torch.tensor([3, 5], device=DEV, dtype=torch.int32))
+    with pytest.raises(LapisError):
+        A.paged_attention(normal(1, 2, 4, 64).bfloat16(), cache, pos, crd, torch.tensor([3, 5], device=DEV, dtype=torch.int32), scale=math.inf)
+
+
+@pytest.mark.parametrize("store", [BF16, I8, F32])
+def test_cache_without_pages(A, store):
+    """No page at all: zeros, whatever the lists say."""
+    dtype = F32 if store == F32 else BF16
+    cache = A.PagedCache.empty(0, 2, 16, 64, store)
+    pos, crd = torch.tensor([0, 2, 2], device=DEV, dtype=torch.int32), torch.tensor([0, 5], device=DEV, dtype=torch.int32)
+    row, place = torch.tensor([0, 1], device=DEV, dtype=torch.int32), torch.tensor([3, 0], device=DEV, dtype=torch.int32)
+    x = normal(1, 2, 2, 64).to(dtype)
+    cache.append(x, x, pos, crd, row, place)
+    assert float(cache.read(pos, crd, row, place, dtype=F32)[0].abs().max()) == 0
+    out, lse = A.paged_attention(normal(1, 2, 4, 64).to(dtype), cache, pos, crd, torch.tensor([20, 0], device=DEV, dtype=torch.int32), return_lse=True)
+    assert float(out.abs().max()) == 0 and torch.allclose(lse[0], torch.full((4,), math.log(20), device=DEV), rtol=1e-6) and bool((lse[1] == -math.inf).all())

@@ -445,7 +445,7 @@ __device__ __forceinline__ float power2(float x) {
 
 template <typename C>
 struct Feed {
-  static constexpr int KEYS = C::KEYS, GROUP = KEYS < 16 ? KEYS : 16, GROUPS = KEYS / GROUP, ROWS = 32 / C::CHUNKS > 0 ? 32 / C::CHUNKS : 1;
+  static constexpr int KEYS = C::KEYS, GROUP = C::GROUP, GROUPS = KEYS / GROUP, ROWS = 32 / C::CHUNKS > 0 ? 32 / C::CHUNKS : 1;
   static constexpr int PASSES = C::CHUNKS > 32 ? C::CHUNKS / 32 : 1;  // copies of a row
   Walk in;
   uint32_t ring;
@@ -561,7 +561,7 @@ struct F32Config {
   static constexpr int DP = DP_, HEADS = HEADS_;            // padded head; query heads of a unit
   static constexpr bool CODES = false;
   static constexpr int ELEMENT = 4, ROW = DP * 4, CHUNKS = DP / 4;
-  static constexpr int KEYS = DP == 64 ? 16 : 8, TILE = KEYS * (ATT_THREADS / 32);
+  static constexpr int KEYS = DP == 64 ? 16 : 8, GROUP = 8, TILE = KEYS * (ATT_THREADS / 32);
   static constexpr int STAGE = 2 * KEYS * ROW;
   static constexpr int OWN = HEADS >= 4 ? HEADS / 4 : 1;    // heads of a lane while there are scores
   static constexpr int SPLIT = DP == 64 ? 2 : 1, OWNED = DP == 256 ? 2 : 1;  // keys side by side; fours of dimensions of a lane
@@ -891,10 +891,13 @@ struct MmaConfig {
   static constexpr int DP = DP_, NT = NT_;                  // padded head, and eights of query heads
   static constexpr int ELEMENT = CODES ? 1 : 2, ROW = DP * ELEMENT;  // bytes of a key in shared memory
   static constexpr int KEYS = ROW <= 128 ? 32 : 16, TILE = KEYS * MMA_WARPS, MT = KEYS / 16;
+  // Keys that are looked up together.  32 requests of up to 8192 tokens in int8: with 8, pages of 24 or 8 slots take 60 us (72 to 75
+  // with 16), those of 16 or 64 also 60 (59); with 16 query heads, or 16-bit caches, where copies count for less, 16.
+  static constexpr int GROUP = CODES && NT == 1 ? 8 : 16;
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
   static constexpr int DT = DP / 16, PART = DT * 128 + 16;  // floats of eight heads' sums: O, then m and l
-  static constexpr int BLOCKS = DP == 256 ? 1 : DP * NT * QP >= 256 ? 2 : 3;  // an SM, by registers
+  static constexpr int BLOCKS = DP == 256 ? (CODES ? 2 : 1) : DP * NT * QP >= 256 ? 2 : 3;  // an SM, by registers and shared memory
   static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048) / (MMA_WARPS * STAGE);
   static constexpr int SMEM = MMA_WARPS * STAGES * STAGE;
   static_assert(STAGES >= 2, "one is copied while another is read");

@@ -7,10 +7,13 @@
 // older m is scaled by exp(m_old - m_new).  A request without tokens gets zeros and lse = -inf.
 //
 // The work is the cache, which is read once.  It is cut along its length, whatever the lengths are: a unit is a request, a
-// key head and up to HEADS of the query heads that share it, its keys are cut into tiles, and the tiles of all units, one
+// key head and up to 8 or 16 of the query heads that share it, its keys are cut into tiles, and the tiles of all units, one
 // after the other, are dealt to the blocks in equal, contiguous shares.  A unit that lies in one share is finished there; the
-// others leave (m, l, sum) in a workspace and join_kernel adds them up in the order of the blocks, so that results are the
-// same from run to run.
+// others leave (m, l, sum) in a workspace, and a second kernel adds them up in a fixed order, so that results are the same from
+// run to run.
+//
+// Three kernels share this, one for each way to multiply: attend_mma_kernel (16-bit queries, and 32-bit ones over codes),
+// attend_f32_kernel (32 bits throughout), attend_any_kernel (rows that no copy of 8 bytes fits).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -23,8 +26,10 @@ namespace lapis_b200 {
 
 constexpr int ATT_THREADS = 128;
 constexpr int UNIT_COST = 2;      // what a unit costs beside its tiles, in tiles: 128 x 8192 int8 214 us with 1, 204 with 2 or 3
-constexpr int MIN_WORK = 2;       // of a share, if there is more than one
-constexpr int WHOLE_TILES = 6;    // by which a unit may be longer than a share and is not cut
+// Of a share, if there is more than one: 2 x 3000 tokens of 256 take 12.5 us with 2, 17.7 with 3; 1 x 4000 of int8 12.9 and 13.3.
+constexpr int MIN_WORK = 2;
+// By which a unit may be longer than a share and is not cut: 1 x 300 tokens take 7.8 us with 6, 10.3 with 4 (and a join).
+constexpr int WHOLE_TILES = 6;
 constexpr int MOST_BLOCKS = 1 << 10;  // shares
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -231,7 +236,9 @@ constexpr int ANY_HEADS = 8, ANY_TILE = 32;
 
 __host__ __device__ constexpr int any_smem(int dim) { return (ANY_HEADS * dim + 2 * ANY_TILE * (dim + 1) + ANY_HEADS * ANY_TILE + 2 * ANY_HEADS) * 4; }
 
-// A block walks its tiles of 32 keys: keys and values to shared memory in 32 bits, a thread a key and two heads for the
+// Right for everything, and for heads of odd widths the only one: 32 requests of up to 8192 tokens, 8 key heads of 30 bf16 values,
+// 64 query heads take 1146 us (114 GB/s), heads of 64 by attend_mma_kernel 53.  Bound by its loads of single values and by
+// shared memory.  A block walks its tiles of 32 keys: keys and values to shared memory in 32 bits, a thread a key and two heads for the
 // scores, a thread a dimension or two for the sums.
 template <typename T>
 __global__ void __launch_bounds__(ATT_THREADS) attend_any_kernel(const __grid_constant__ AttendArgs a) {
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(ATT_THREADS) join_any_kernel(const __grid_cons
 }
 
 // Whether the lists cannot hold more than what find_share leaves whole: then nothing is cut, and there is nothing to join (a short
-// request of one user: 1 x 129 tokens %%).
+// request of one user: 1 x 129 tokens take 10.3 us without, 14.4 with the join's launch).
 static bool always_whole(const AttendArgs &a, int tile) {
   const int64_t most_tokens = a.lists.entries > MOST_TOKENS / a.cache.page_size ? MOST_TOKENS : a.lists.entries * a.cache.page_size;
   return (int64_t)a.requests * a.cache.heads * a.head_blocks <= a.blocks && most_tokens <= WHOLE_TILES * tile - 16;
@@ -555,6 +562,8 @@ struct Feed {
 // shared memory and the products, about even with it.  A warp's KEYS keys of a step: four lanes share a key, a quarter of its
 // pieces each, and add up their parts of HEADS scores so that lane c of the four ends with heads c * HEADS / 4 onward; the
 // weights go through shared memory, and then a lane owns four dimensions (of every SPLIT-th key, where heads are narrow).
+// 16 requests of up to 2047 tokens, 8 heads of 72: 17 us alone (5.2 TB/s; a block's first data comes after 5 us) and 25 in all,
+// 182 by attend_any_kernel.  32 of up to 8192, 8 key heads of 128: 6.3 TB/s with 2 query heads each, 5.2 with 8.
 
 template <int DP_, int HEADS_>
 struct F32Config {
@@ -568,6 +577,7 @@ struct F32Config {
   static constexpr int PART = HEADS * DP + 2 * HEADS;       // floats of a warp's sums: O, then m and l
   static constexpr int WEIGHTS = KEYS * HEADS + HEADS;      // floats of a warp's weights, and of the factors for older sums
   static constexpr int EXTRA = (HEADS * DP + ATT_THREADS / 32 * WEIGHTS) * 4;
+  // Wide heads of codes: one block an SM takes 168 us of 32 requests of up to 8192, two 119.
   static constexpr int BLOCKS = DP == 256 ? 1 : 3;
   static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048 - EXTRA) / (ATT_THREADS / 32 * STAGE);
   static constexpr int SMEM = ATT_THREADS / 32 * STAGES * STAGE + EXTRA;
@@ -877,6 +887,12 @@ static int launch_f32_of(const AttendArgs &a, int dev, cudaStream_t st) {
 // at least 16 bits.  Quantised caches: codes are exact in fp16, so are queries after a power of two is taken out of each; a
 // key's scale is multiplied to its score in 32 bits, a value's scale to its weight, relative to the largest power of two so
 // far.  Weights in fp16 are times 2^14, so that they are subnormal only below 2^-28.
+// Measured, kernel alone: 1 x 131,072 tokens, 8 key heads of 128 in bf16, 32 query heads: 82 to 87 us, 6.2 to 6.5 TB/s, the rate of a copy; 128
+// requests of up to 8192, 64 query heads, int8: 194 us, 6.1 TB/s of DRAM, 870 instructions a step at 2.6 a cycle; called again and
+// again it falls to 215 to 235 us, as the power cap takes the clock.  Scores of int8 by whole-number products of three digits of the
+// queries (no conversion of the keys, 14 % fewer instructions) took 229 us where this took 231, and 62 where this took 59 on 32
+// requests.  Four warps of 168 registers, three blocks an SM: two blocks of 250 registers took 274 us of the second where three took
+// 244.
 
 constexpr int MMA_WARPS = ATT_THREADS / 32;
 
@@ -1384,7 +1400,9 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 
 // Adds up what the blocks left of the units that were cut: the blocks of a unit's first shares take some of its sixteens of
 // dimensions each, a thread four sums of every parts-th share.  Bound by the time of its loads: the record of the cut, then the
-// shares' sums, BATCH at a time.
+// shares' sums, BATCH at a time.  5.5 us for units of two shares, 7 for eight units of 55; one block a unit took 15 for the latter,
+// eight blocks for every unit 7.7 for the former.  512 threads join 157 shares in two trips where 256 take four (1 x 30,000: 14.7 us
+// of attention and 20.5).
 constexpr int JOIN_THREADS = 512;
 template <typename C>
 __device__ __forceinline__ void join_unit(const AttendArgs &a, const CutUnit &cut, int n, float4 (&others)[2][JOIN_THREADS]) {
@@ -1467,6 +1485,8 @@ static int launch_mma(AttendArgs a, int dev, cudaStream_t st) {
   return LAPIS_OK;
 }
 
+// Units of 8 query heads, or of 16 where more than 8 share a key head: 32 requests of up to 4096, 16 heads a key head, bf16 66 us
+// (by eights, the cache read twice, 89), int8 56 (67), e4m3 of 64 41 (45).
 template <typename T, int STORE>
 static int launch_mma_of(const AttendArgs &a, int dev, cudaStream_t st) {
   if (a.dim <= 64) return a.group <= 8 ? launch_mma<MmaConfig<T, STORE, 64, 1>>(a, dev, st) : launch_mma<MmaConfig<T, STORE, 64, 2>>(a, dev, st);
@@ -1482,6 +1502,8 @@ static bool pieces_fit(const AttendArgs &a) {
   return row % (a.cache.type == LAPIS_F32 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(a.cache.d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(a.cache.d_v) % 16 == 0;
 }
 
+// 32 bits: units of 1, 4 or 8 query heads.  32 requests of up to 4096, 8 key heads of 128, 1, 4 and 8 query heads each: 99, 101 and
+// 128 us; all by eights 125, 126 and 128.
 template <typename T>
 static int launch_type(const AttendArgs &a, int dev, cudaStream_t st) {
   if (!pieces_fit(a)) return launch_any<T>(a, dev, st);

@@ -263,9 +263,8 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
 // lane uses for itself: what is on its way takes no registers.  Weight and rotation are one product each with a value and
 // its partner, y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin, two values an instruction.
 // Measured, bf16 heads of 128: 8192 tokens of 32 + 8 heads 31 us (5.5 TB/s; 40 us with the partner in another lane, 180
-// instructions for two rows), backward of 16,384 83 us (6.2 TB/s) and 4 to add up the weights' gradients, 32,768 tokens of 32 + 8 + 8 normalised and written as int8 139 us
-// (5.3 TB/s), read back 40 (5.0 TB/s).  More registers would be needed for more on its way: eight blocks an SM, or six, spill and
-// take 33 us of the first.
+// instructions for two rows; 33 with six blocks an SM, which spill), backward of 16,384 83 us (6.2 TB/s) and 4 to add up the
+// weights' gradients, 32,768 tokens of 32 + 8 + 8 normalised and written as int8 139 us (5.3 TB/s), read back 40 (5.0 TB/s).
 
 __device__ __forceinline__ uint32_t shared_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes on their way to shared memory, zeros where there is nothing.

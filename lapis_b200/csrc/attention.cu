@@ -943,6 +943,15 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d += a (low + high), for results in 32 bits: the tensor cores cut what lies below the last place of the largest term, and over
+// long sums that adds up to 1 to 4e-6 of a result; two products at a time, added by rounding, are as near as a sum in 32 bits.
+__device__ __forceinline__ void mma_apart(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&low)[2], const uint32_t (&high)[2]) {
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  mma<true>(part, a, low[0], low[1]);
+  mma<true>(part, a, high[0], high[1]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] += part[i];
+}
 // Two numbers of 32 bits as two of 16, the first in the low half; `back`: the 16-bit numbers in 32 bits.
 template <bool HALF>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -1208,9 +1217,13 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
             const uint32_t flip = C::STORE == LAPIS_I8 ? 0x80808080u : 0, t = tw[j] ^ flip, l = lw[j] ^ flip;
             const uint32_t x[4] = {codes2<C::STORE, false>(t), codes2<C::STORE, false>(l), codes2<C::STORE, true>(t), codes2<C::STORE, true>(l)};
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int p = 0; p < C::QP; ++p) mma<C::HALF>(s[mt][n], x, q[p][n][k * 4 + j][0], q[p][n][k * 4 + j][1]);
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (C::QP == 1) {
+                mma<C::HALF>(s[mt][n], x, q[0][n][k * 4 + j][0], q[0][n][k * 4 + j][1]);
+              } else {
+                mma_apart(s[mt][n], x, q[1][n][k * 4 + j], q[0][n][k * 4 + j]);
+              }
+            }
           }
         }
       }
@@ -1355,8 +1368,12 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
               const int t = j * 8 + 2 * k + h;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                mma<C::HALF>(sums[n].o[t], x, high[n][0], high[n][1]);
-                if (C::TWO_PARTS) mma<C::HALF>(sums[n].o[t], x, low[n][0], low[n][1]);
+                if constexpr (C::QP == 2) {
+                  mma_apart(sums[n].o[t], x, low[n], high[n]);
+                } else {
+                  mma<C::HALF>(sums[n].o[t], x, high[n][0], high[n][1]);
+                  if (C::TWO_PARTS) mma<C::HALF>(sums[n].o[t], x, low[n][0], low[n][1]);
+                }
               }
             }
           }

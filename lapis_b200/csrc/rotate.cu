@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_any_backward_kernel(const 
           sum = fmaf(x[i], x[i], sum);
         }
         __syncwarp();
-        const float r = 1.0f / sqrtf(warp_sum(sum) / (float)a.dim + a.eps);
+        const float mean = warp_sum(sum) / (float)a.dim, r = real ? 1.0f / sqrtf(mean + a.eps) : 0.0f;  // eps may be zero
 #pragma unroll
         for (int j = 0; j < PER_LANE; ++j) {
           const int i = lane + 32 * j;
@@ -789,7 +789,8 @@ __global__ void __launch_bounds__(ROW_THREADS, backward_blocks(sizeof(T))) rotat
           sum += __shfl_xor_sync(0xffffffffu, sum, d);
           inner += __shfl_xor_sync(0xffffffffu, inner, d);
         }
-        const float r = rsqrtf(fmaf(sum, by_dim, a.eps)), back = -inner * by_dim * r * r;
+        // What is no row, padding or beside the last head, adds nothing: with an eps of zero its 1 / sqrt(0) would.
+        const float r = real && head < a.heads[which] ? rsqrtf(fmaf(sum, by_dim, a.eps)) : 0.0f, back = -inner * by_dim * r * r;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           mul_all(x[k].x, x[k].x, r);

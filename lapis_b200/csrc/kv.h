@@ -43,6 +43,9 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 
 // Codes of a quantised row: x * (largest / amax) to the nearest code, ties to even; the row's scale is amax / largest.
 __device__ __forceinline__ float largest_code(int type) { return type == LAPIS_I8 ? 127.0f : 448.0f; }
+// A row whose largest magnitude is below SMALL_ROW is taken times RAISE, a power of two: 127 / amax is no number of 32 bits where amax
+// is below 3.7e-37, 448 / amax below 1.3e-36.  The products are the same numbers.
+constexpr float SMALL_ROW = 0x1p-63f, RAISE = 0x1p64f;
 // A row that is not finite reads as NaN, whatever its codes are.
 __device__ __forceinline__ float scale_of(float amax, float largest) { return amax < INFINITY ? amax / largest : NAN; }
 __device__ __forceinline__ int8_t to_i8(float x) {

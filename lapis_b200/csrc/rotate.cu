@@ -136,8 +136,14 @@ __global__ void __launch_bounds__(ROW_THREADS) rotate_any_kernel(const __grid_co
   for (int j = 0; j < PER_LANE; ++j) most = max_nan(most, fabsf(y[j]));
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-  const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+  const float big = largest_code(a.cache.type);
   if (lane == 0) (which == 1 ? a.cache.d_k_scale : a.cache.d_v_scale)[row] = scale_of(most, big);
+  if (most < SMALL_ROW) {
+    most *= RAISE;
+#pragma unroll
+    for (int j = 0; j < PER_LANE; ++j) y[j] *= RAISE;
+  }
+  const float by = most == 0.0f ? 0.0f : big / most;
 #pragma unroll
   for (int j = 0; j < PER_LANE; ++j) {
     if (lane + 32 * j >= a.dim) continue;
@@ -602,9 +608,15 @@ __device__ __forceinline__ void rotate_rows(const RotateArgs &a, const Pieces<T,
         for (int j = 0; j < V; ++j) most = max_nan(most, fabsf(x[k].x[j]));
 #pragma unroll
       for (int d = LANES / 2; d > 0; d /= 2) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-      const float big = largest_code(a.cache.type), by = most == 0.0f ? 0.0f : big / most;
+      const float big = largest_code(a.cache.type);
+      if (head < count && threadIdx.x % LANES == 0) *scales = scale_of(most, big);
+      if (most < SMALL_ROW) {
+        most *= RAISE;
+        mul_all(x[0].x, x[0].x, RAISE);
+        mul_all(x[1].x, x[1].x, RAISE);
+      }
+      const float by = most == 0.0f ? 0.0f : big / most;
       if (head < count) {
-        if (threadIdx.x % LANES == 0) *scales = scale_of(most, big);
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           if (p.in[k]) store_codes<V>(out + p.at[k] * PIECE, x[k].x, by, a.cache.type);

@@ -1309,7 +1309,8 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float p0 = power2(s[mt][n][2 * e] - (base[n][0] - C::OFFSET)), p1 = power2(s[mt][n][2 * e + 1] - (base[n][1] - C::OFFSET));
+          // The difference first: it is exact near the maximum, where base - OFFSET may be off by more than OFFSET (scores of 10^8).
+          float p0 = power2((s[mt][n][2 * e] - base[n][0]) + C::OFFSET), p1 = power2((s[mt][n][2 * e + 1] - base[n][1]) + C::OFFSET);
           sums[n].l[0] += p0;
           sums[n].l[1] += p1;
           if (C::CODES) {

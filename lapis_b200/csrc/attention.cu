@@ -886,7 +886,7 @@ static int launch_f32_of(const AttendArgs &a, int dev, cudaStream_t st) {
 // results from a quantised cache, whose own 8 bits are 2^-8 and the weights' 11 here) as two, high and low part, whose sum has
 // at least 16 bits.  Quantised caches: codes are exact in fp16, so are queries after a power of two is taken out of each; a
 // key's scale is multiplied to its score in 32 bits, a value's scale to its weight, relative to the largest power of two so
-// far.  Weights in fp16 are times 2^14, so that they are subnormal only below 2^-28.
+// far.
 // Measured, kernel alone: 1 x 131,072 tokens, 8 key heads of 128 in bf16, 32 query heads: 82 to 87 us, 6.2 to 6.5 TB/s, the rate of a copy; 128
 // requests of up to 8192, 64 query heads, int8: 194 us, 6.1 TB/s of DRAM, 870 instructions a step at 2.6 a cycle; called again and
 // again it falls to 215 to 235 us, as the power cap takes the clock.  Scores of int8 by whole-number products of three digits of the
@@ -918,7 +918,8 @@ struct MmaConfig {
   static constexpr int SMEM = MMA_WARPS * STAGES * STAGE;
   static_assert(STAGES >= 2, "one is copied while another is read");
   static_assert(PART * 4 <= STAGE, "a warp's sums fit where its last keys were");
-  static constexpr float OFFSET = HALF ? 14.0f : 0.0f;
+  // Weights in fp16 are times 2^14, so that they are subnormal only below 2^-28; the sums are without it.
+  static constexpr float OFFSET = HALF ? 0x1p14f : 1.0f;
   static __device__ __forceinline__ int k_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? 0 : r & 4; }
   static __device__ __forceinline__ int v_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? r & 2 : (r & 3) << 1; }
 };
@@ -1031,7 +1032,7 @@ __device__ __forceinline__ void give(const AttendArgs &a, const Sums<C::DT> &s, 
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (part == nullptr && a.lse != nullptr && 2 * c + i < heads)
-        a.lse[(int64_t)request * a.q_heads + first_head + 2 * c + i] = l[i] == 0.0f ? -INFINITY : (m[i] - C::OFFSET) * LN2 + logf(l[i]);
+        a.lse[(int64_t)request * a.q_heads + first_head + 2 * c + i] = l[i] == 0.0f ? -INFINITY : m[i] * LN2 + logf(l[i]);
   }
   const float by[2] = {l[0] == 0.0f ? 0.0f : 1.0f / l[0], l[1] == 0.0f ? 0.0f : 1.0f / l[1]};
   T *const out = static_cast<T *>(a.out) + ((int64_t)request * a.q_heads + first_head + 2 * c) * a.dim;
@@ -1089,7 +1090,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 
   uint32_t q[C::QP][NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
-  float value_by = 0.0f, values_in = 0.0f;  // codes: the power of two that the values' scales are relative to, and 1 / it
+  float value_by = 0.0f, values_in = 0.0f;  // codes: the power of two that the values' scales are relative to, and OFFSET / it
   Sums<DT> sums[NT];
   // The queries of unit `out` as they are; q takes them once the unit in front has been given out.  Four values of a lane: for
   // codes they are neighbours.
@@ -1276,11 +1277,11 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) most_value = fmaxf(most_value, __shfl_xor_sync(0xffffffffu, most_value, d));
         if (most_value > value_by) {  // the next power of two
-          const uint32_t exponent = (__float_as_uint(most_value) >> 23) + 1;
+          const uint32_t exponent = max((__float_as_uint(most_value) >> 23) + 1, 15u);
           const float now = exponent >= 255 ? most_value : __uint_as_float(exponent << 23);
           shrink = value_by / now;
           value_by = now;
-          values_in = 1.0f / now;
+          values_in = C::OFFSET / now;
         }
       }
 #pragma unroll
@@ -1309,12 +1310,11 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          // The difference first: it is exact near the maximum, where base - OFFSET may be off by more than OFFSET (scores of 10^8).
-          float p0 = power2((s[mt][n][2 * e] - base[n][0]) + C::OFFSET), p1 = power2((s[mt][n][2 * e + 1] - base[n][1]) + C::OFFSET);
+          float p0 = power2(s[mt][n][2 * e] - base[n][0]), p1 = power2(s[mt][n][2 * e + 1] - base[n][1]);
           sums[n].l[0] += p0;
           sums[n].l[1] += p1;
-          if (C::CODES) {
-            const float by = value_scale[mt][e] * values_in;
+          if (C::HALF) {
+            const float by = C::CODES ? value_scale[mt][e] * values_in : C::OFFSET;
             p0 *= by;
             p1 *= by;
           }
@@ -1398,11 +1398,12 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) sums[n].l[i] += __shfl_xor_sync(0xffffffffu, sums[n].l[i], d);
-      if (C::CODES) {
+      if (C::HALF) {
+        const float by = (C::CODES ? value_by : 1.0f) / C::OFFSET;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= value_by;
+          for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= by;
       }
       float *const part = a.partial + (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * NT + n) * C::PART;
       __syncwarp();
@@ -1469,7 +1470,7 @@ __device__ __forceinline__ void join_unit(const AttendArgs &a, const CutUnit &cu
       if (2 * c + i >= heads) continue;
       const int64_t head = (int64_t)cut.request * a.q_heads + first_head + head0 + 2 * c + i;
       const float m = i == 0 ? ml.x : ml.y, l = i == 0 ? ml.z : ml.w, by = l == 0.0f ? 0.0f : 1.0f / l;
-      if (t == 0 && g == 0 && a.lse != nullptr) a.lse[head] = l == 0.0f ? -INFINITY : (m - C::OFFSET) * LN2 + logf(l);
+      if (t == 0 && g == 0 && a.lse != nullptr) a.lse[head] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
       T *const out = static_cast<T *>(a.out) + head * a.dim;
       if (d0 < a.dim) out[d0] = from_f32<T>((i == 0 ? acc.x : acc.y) * by);
       if (d1 < a.dim) out[d1] = from_f32<T>((i == 0 ? acc.z : acc.w) * by);

@@ -5,9 +5,11 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_attention import BF16, DEV, E4M3, F16, F32, I8, U, WEIGHT, make_cache, normal, quantised, tokens_of
+from tests.test_gpu_attention import BF16, DEV, E4M3, F16, F32, I8, U, WEIGHT, attend64, holds, make_cache, normal, quantised, tokens_of
 
 pytestmark = pytest.mark.gpu
+
+CODES = [(BF16, I8, 128), (BF16, E4M3, 64), (F16, I8, 64), (F16, E4M3, 256), (F32, I8, 128), (F32, E4M3, 64), (F32, I8, 20)]
 
 
 @pytest.fixture(scope="module")
@@ -46,3 +48,22 @@ def test_one_key_far_above_all_others(A, dtype, store, dim, lens, heads):
         assert bool(((out[b].double() - want).abs() <= (U[dtype] + WEIGHT[dtype] + 2.0 ** -21) * want.abs() + 2.0 ** -24).all())
         score = (q[b].double() * k[j].double()).sum(-1) * dim ** -0.5
         assert bool(((lse[b].double() - score).abs() <= 4 * (dim + 8) * 2.0 ** -24 * score.abs()).all())
+
+
+# ---- values of 10^36 ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens", [[30, 5], [3000]])
+@pytest.mark.parametrize("dtype,store,dim", [c for c in CODES if c[0] != F16])
+def test_values_near_the_largest_number(A, dtype, store, dim, lens):
+    """Sums of the weights' products with values of up to 10^34 for 3000 tokens, 10^36 for 30, are numbers of 32 bits."""
+    cache, pos, crd = make_cache(A, (lens, 1, dim, 16, dtype, store, torch.int32))
+    row, place = tokens_of(lens)
+    k, v = normal(1, len(row), 1, dim).to(dtype), (normal(2, len(row), 1, dim) * (2e36 if lens[0] == 30 else 3e34)).to(dtype)
+    cache.append(k, v, pos, crd, row, place)
+    held, at = [], 0
+    for n in lens:
+        held.append(tuple(quantised(x[at:at + n].float(), store).double() for x in (k, v)))
+        at += n
+    q = normal(5, len(lens), 4, dim).to(dtype)
+    holds(q, A.paged_attention(q, cache, pos, crd, length_of(lens), return_lse=True), attend64(q, held, dim ** -0.5, 0))

@@ -1245,7 +1245,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         if (C::CODES) {
           by = load4(scales + r * 4);
           value_scale[mt][e] = load4(scales + (KEYS + r) * 4);
-          most_value = fmaxf(most_value, value_scale[mt][e]);
+          most_value = fmaxf(most_value, fabsf(value_scale[mt][e]));  // a caller's own scales may be negative
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {

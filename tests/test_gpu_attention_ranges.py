@@ -67,3 +67,23 @@ def test_values_near_the_largest_number(A, dtype, store, dim, lens):
         at += n
     q = normal(5, len(lens), 4, dim).to(dtype)
     holds(q, A.paged_attention(q, cache, pos, crd, length_of(lens), return_lse=True), attend64(q, held, dim ** -0.5, 0))
+
+
+# ---- scales of a caller's own cache ------------------------------------------
+
+
+@pytest.mark.parametrize("signs", ["mixed", "negative"])
+@pytest.mark.parametrize("dtype,store,dim", CODES)
+def test_negative_scales(A, dtype, store, dim, signs):
+    lens = [130, 7]
+    cache, pos, crd = make_cache(A, (lens, 2, dim, 16, dtype, store, torch.int32))
+    row, place = tokens_of(lens)
+    k, v = normal(1, len(row), 2, dim).to(dtype), normal(2, len(row), 2, dim).to(dtype)
+    cache.append(k, v, pos, crd, row, place)
+    sign = torch.where(normal(3, 2, *cache.k_scale.shape) < 0, -1.0, 1.0) if signs == "mixed" else torch.full((2, *cache.k_scale.shape), -1.0, device=DEV)
+    cache.k_scale *= sign[0]
+    cache.v_scale *= sign[1]
+    k, v = cache.read(pos, crd, row, place, dtype=F32)
+    held = [(k[:130].double(), v[:130].double()), (k[130:].double(), v[130:].double())]
+    q = normal(5, 2, 6, dim).to(dtype)
+    holds(q, A.paged_attention(q, cache, pos, crd, length_of(lens), return_lse=True), attend64(q, held, dim ** -0.5, 0))

@@ -885,8 +885,9 @@ static int launch_f32_of(const AttendArgs &a, int dev, cudaStream_t st) {
 // Weights go into the product with the values as a 16-bit number, and where that would show in the result (all but bf16
 // results from a quantised cache, whose own 8 bits are 2^-8 and the weights' 11 here) as two, high and low part, whose sum has
 // at least 16 bits.  Quantised caches: codes are exact in fp16, so are queries after a power of two is taken out of each; a
-// key's scale is multiplied to its score in 32 bits, a value's scale to its weight, relative to the largest power of two so
-// far.
+// key's scale is multiplied to its score in 32 bits, a value's scale to its weight, and the product is taken relative to the largest
+// one that the head has seen, carried along as the softmax's maximum is: a large scale counts for no more than its token's weight.
+// What fp16 leaves of weight * scale is off by at most 2^-38 of that largest one beside the rounding to its bits.
 // Measured, kernel alone: 1 x 131,072 tokens, 8 key heads of 128 in bf16, 32 query heads: 82 to 87 us, 6.2 to 6.5 TB/s, the rate of a copy; 128
 // requests of up to 8192, 64 query heads, int8: 194 us, 6.1 TB/s of DRAM, 870 instructions a step at 2.6 a cycle; called again and
 // again it falls to 215 to 235 us, as the power cap takes the clock.  Scores of int8 by whole-number products of three digits of the
@@ -920,6 +921,7 @@ struct MmaConfig {
   static_assert(PART * 4 <= STAGE, "a warp's sums fit where its last keys were");
   // Weights in fp16 are times 2^14, so that they are subnormal only below 2^-28; the sums are without it.
   static constexpr float OFFSET = HALF ? 0x1p14f : 1.0f;
+  static constexpr uint32_t LEAST_UNIT = 0x07800000;  // 2^-112: OFFSET / it is a number
   static __device__ __forceinline__ int k_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? 0 : r & 4; }
   static __device__ __forceinline__ int v_swizzle(int r) { return !CODES ? r & 7 : DP == 64 ? r & 2 : (r & 3) << 1; }
 };
@@ -1090,7 +1092,10 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 
   uint32_t q[C::QP][NT][DT][2];
   float score_by[NT][2];     // scale of the scores of heads 2c, 2c + 1
-  float value_by = 0.0f, values_in = 0.0f;  // codes: the power of two that the values' scales are relative to, and OFFSET / it
+  // Codes: the largest |weight * value's scale| of a head so far, relative to m, and the bits of the power of two above it that the
+  // sums of its values are relative to.  Both go down where m goes up, so that keys count by what they add to the result.
+  float peak[NT][2];
+  uint32_t unit[NT][2];
   Sums<DT> sums[NT];
   // The queries of unit `out` as they are; q takes them once the unit in front has been given out.  Four values of a lane: for
   // codes they are neighbours.
@@ -1127,10 +1132,11 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     }
   };
   auto take_q = [&]() {
-    value_by = values_in = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       sums[n].clear();
+      peak[n][0] = peak[n][1] = 0.0f;
+      unit[n][0] = unit[n][1] = C::LEAST_UNIT;
       if constexpr (!C::CODES) {
         score_by[n][0] = score_by[n][1] = a.scale2;
 #pragma unroll
@@ -1233,7 +1239,7 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
     // scores of keys (row g, row g + 8 of the tile) and heads (2c, 2c + 1)
     const int key0 = out.span.origin + out.tile * C::TILE + warp * KEYS;
     const bool all_seen = key0 >= out.span.lo && key0 + KEYS <= out.span.hi;
-    float value_scale[MT][2], most_value = 0.0f;
+    float value_scale[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -1245,7 +1251,6 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         if (C::CODES) {
           by = load4(scales + r * 4);
           value_scale[mt][e] = load4(scales + (KEYS + r) * 4);
-          most_value = fmaxf(most_value, fabsf(value_scale[mt][e]));  // a caller's own scales may be negative
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -1270,20 +1275,30 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         grows |= x > sums[n].m[i];
       }
     }
-    if (C::CODES) grows |= most_value > value_by;
-    if (__any_sync(0xffffffffu, grows)) {
-      float shrink = 1.0f;
-      if (C::CODES) {
+    // s becomes the weights, of codes times their scales
+    float added[NT][2], largest[NT][2];
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) most_value = fmaxf(most_value, __shfl_xor_sync(0xffffffffu, most_value, d));
-        if (most_value > value_by) {  // the next power of two
-          const uint32_t exponent = max((__float_as_uint(most_value) >> 23) + 1, 15u);
-          const float now = exponent >= 255 ? most_value : __uint_as_float(exponent << 23);
-          shrink = value_by / now;
-          value_by = now;
-          values_in = C::OFFSET / now;
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        added[n][i] = largest[n][i] = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float &p = s[mt][n][2 * e + i];
+            p = power2(p - base[n][i]);
+            added[n][i] += p;
+            if (C::CODES) {
+              p *= value_scale[mt][e];
+              largest[n][i] = fmaxf(largest[n][i], fabsf(p));  // a caller's own scales may be negative
+            }
+          }
         }
+        if (C::CODES) grows |= largest[n][i] > __uint_as_float(unit[n][i]);
       }
+    }
+    if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float f[2];
@@ -1292,7 +1307,15 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
           f[i] = power2(sums[n].m[i] - base[n][i]);
           sums[n].l[i] *= f[i];
           sums[n].m[i] = most[n][i];
-          f[i] *= shrink;
+          if (C::CODES) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) largest[n][i] = fmaxf(largest[n][i], __shfl_xor_sync(0xffffffffu, largest[n][i], d));
+            peak[n][i] = fmaxf(peak[n][i] * f[i], largest[n][i]);
+            const uint32_t now = min(max((__float_as_uint(peak[n][i]) & 0x7f800000u) + 0x800000u, C::LEAST_UNIT), 0x7f000000u);
+            // times unit / now, which is above 2^127 only where f is 0
+            f[i] *= __uint_as_float((uint32_t)min(max((int)(unit[n][i] >> 23) - (int)(now >> 23) + 127, 0), 254) << 23);
+            unit[n][i] = now;
+          }
         }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
@@ -1303,6 +1326,15 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
         }
       }
     }
+    float weight_by[NT][2];  // OFFSET, of codes over the unit
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sums[n].l[i] += added[n][i];
+        weight_by[n][i] = C::CODES ? __uint_as_float(__float_as_uint(C::OFFSET) + 0x3f800000u - unit[n][i]) : C::OFFSET;
+      }
+    }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint32_t high[NT][2], low[NT][2];
@@ -1310,13 +1342,10 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float p0 = power2(s[mt][n][2 * e] - base[n][0]), p1 = power2(s[mt][n][2 * e + 1] - base[n][1]);
-          sums[n].l[0] += p0;
-          sums[n].l[1] += p1;
+          float p0 = s[mt][n][2 * e], p1 = s[mt][n][2 * e + 1];
           if (C::HALF) {
-            const float by = C::CODES ? value_scale[mt][e] * values_in : C::OFFSET;
-            p0 *= by;
-            p1 *= by;
+            p0 *= weight_by[n][0];
+            p1 *= weight_by[n][1];
           }
           const uint32_t h = pack2<C::HALF>(p0, p1);
           high[n][e] = transposed(h);
@@ -1399,11 +1428,11 @@ __global__ void __launch_bounds__(ATT_THREADS, C::BLOCKS) attend_mma_kernel(cons
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) sums[n].l[i] += __shfl_xor_sync(0xffffffffu, sums[n].l[i], d);
       if (C::HALF) {
-        const float by = (C::CODES ? value_by : 1.0f) / C::OFFSET;
+        const float by[2] = {C::CODES ? __uint_as_float(unit[n][0]) / C::OFFSET : 1.0f / C::OFFSET, C::CODES ? __uint_as_float(unit[n][1]) / C::OFFSET : 1.0f / C::OFFSET};
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= by;
+          for (int i = 0; i < 4; ++i) sums[n].o[t][i] *= by[i & 1];
       }
       float *const part = a.partial + (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * NT + n) * C::PART;
       __syncwarp();

@@ -801,8 +801,9 @@ __global__ void __launch_bounds__(ROW_THREADS, backward_blocks(sizeof(T))) rotat
           sum += __shfl_xor_sync(0xffffffffu, sum, d);
           inner += __shfl_xor_sync(0xffffffffu, inner, d);
         }
-        // What is no row, padding or beside the last head, adds nothing: with an eps of zero its 1 / sqrt(0) would.
-        const float r = real && head < a.heads[which] ? rsqrtf(fmaf(sum, by_dim, a.eps)) : 0.0f, back = -inner * by_dim * r * r;
+        // What is no row, padding or beside the last head, is zeros and adds nothing; with an eps of zero its 1 / sqrt(0) would.
+        const float eps = real && head < a.heads[which] ? a.eps : 1.0f;
+        const float r = rsqrtf(fmaf(sum, by_dim, eps)), back = -inner * by_dim * r * r;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           mul_all(x[k].x, x[k].x, r);

@@ -62,8 +62,9 @@ struct Span {
   int64_t entry;
 };
 __device__ __forceinline__ Span span_of(const AttendArgs &a, int request) {
-  const int64_t first = load_index(a.lists.d_pos, request, a.lists.idx_bytes), last = load_index(a.lists.d_pos, request + 1, a.lists.idx_bytes);
-  const int64_t room = (last - first) * a.cache.page_size, n = load_index(a.length, request, a.lists.idx_bytes);
+  // A list ends where the lists do, whatever pos says: no walk is longer than they are.
+  const int64_t first = load_index(a.lists.d_pos, request, a.lists.idx_bytes), last = min(load_index(a.lists.d_pos, request + 1, a.lists.idx_bytes), a.lists.entries);
+  const int64_t room = first < 0 || last <= first ? 0 : (last - first) * a.cache.page_size, n = load_index(a.length, request, a.lists.idx_bytes);
   Span s;
   s.hi = (int)max((int64_t)0, min(min(n, room), (int64_t)MOST_TOKENS));
   s.lo = a.window > 0 && a.window < s.hi ? s.hi - (int)a.window : 0;

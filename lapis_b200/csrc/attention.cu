@@ -1581,7 +1581,8 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   if (requests > 65535 || q->heads > (1 << 16)) return fail(LAPIS_ETOOBIG, "%s: more than 65535 requests or 65536 heads", what);
   if (lists->rows != requests) return fail(LAPIS_EBADSHAPE, "%s: a page list for each request", what);
   if (window < 0) return fail(LAPIS_EBADARG, "%s: negative window", what);
-  if (!std::isfinite(scale)) return fail(LAPIS_EBADARG, "%s: scale must be finite", what);
+  const float scale2 = (float)(scale * 1.4426950408889634);
+  if (!std::isfinite(scale2)) return fail(LAPIS_EBADARG, "%s: scale must be finite, in 32 bits", what);
   if (requests == 0) return LAPIS_OK;
   if (q->d == nullptr || d_length == nullptr || d_out == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
   int dev = 0;
@@ -1595,7 +1596,7 @@ extern "C" int lapis_b200_paged_attention(int type, int64_t requests, const lapi
   a.q_heads = (int)q->heads;
   a.group = (int)(q->heads / cache->heads);
   a.dim = (int)cache->dim;
-  a.scale2 = (float)(scale * 1.4426950408889634);
+  a.scale2 = scale2;
   a.window = window;
   a.cache = *cache;
   a.lists = *lists;

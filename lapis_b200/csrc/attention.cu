@@ -578,7 +578,7 @@ struct F32Config {
   static constexpr int PART = HEADS * DP + 2 * HEADS;       // floats of a warp's sums: O, then m and l
   static constexpr int WEIGHTS = KEYS * HEADS + HEADS;      // floats of a warp's weights, and of the factors for older sums
   static constexpr int EXTRA = (HEADS * DP + ATT_THREADS / 32 * WEIGHTS) * 4;
-  // Wide heads of codes: one block an SM takes 168 us of 32 requests of up to 8192, two 119.
+  // As many as shared memory holds with two stages each: three, of heads of 256 one (with three).
   static constexpr int BLOCKS = DP == 256 ? 1 : 3;
   static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048 - EXTRA) / (ATT_THREADS / 32 * STAGE);
   static constexpr int SMEM = ATT_THREADS / 32 * STAGES * STAGE + EXTRA;
@@ -915,6 +915,7 @@ struct MmaConfig {
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW + (CODES ? 2 * KEYS * 4 : 0);
   static constexpr int DT = DP / 16, PART = DT * 128 + 16;  // floats of eight heads' sums: O, then m and l
+  // Wide heads of codes: one block an SM takes 168 us of 32 requests of up to 8192, two 119.
   static constexpr int BLOCKS = DP == 256 ? (CODES ? 2 : 1) : DP * NT * QP >= 256 ? 2 : 3;  // an SM, by registers and shared memory
   static constexpr int STAGES = (227 * 1024 / BLOCKS - 2048) / (MMA_WARPS * STAGE);
   static constexpr int SMEM = MMA_WARPS * STAGES * STAGE;

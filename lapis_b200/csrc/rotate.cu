@@ -847,7 +847,7 @@ template <typename T, int LANES, bool CODES>
 __global__ void __launch_bounds__(ROW_THREADS)
 kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_constant__ lapis_b200_page_lists lists, int64_t tokens, const void *row,
                const void *place, int page_shift, int parts, int each, T *k, T *v) {
-  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, ROUNDS = 1, SIZE = CODES ? 1 : sizeof(T);
+  constexpr int V = Piece<T>::V, GROUPS = 32 / LANES, SIZE = CODES ? 1 : sizeof(T);
   const int64_t task = (int64_t)blockIdx.x * ROW_WARPS + threadIdx.x / 32, token = task / parts;
   if (token >= tokens) return;
   const int lane = threadIdx.x % LANES, dim = (int)cache.dim, heads = (int)cache.heads;
@@ -861,70 +861,63 @@ kv_read_kernel(const __grid_constant__ lapis_b200_kv_cache cache, const __grid_c
   const char *rows[2] = {static_cast<const char *>(cache.d_k) + bytes, static_cast<const char *>(cache.d_v) + bytes};
   const float *scales[2] = {cache.d_k_scale + at, cache.d_v_scale + at};
   T *to_rows[2] = {k + out, v + out};
-  for (int round = from; round < to; round += ROUNDS) {
-    uint4 raw[ROUNDS][2][2];
-    float scale[ROUNDS][2];
+  for (int round = from; round < to; ++round) {
+    uint4 raw[2][2];
+    float scale[2];
+    const bool mine = head < heads, real = first >= 0 && mine;
 #pragma unroll
-    for (int u = 0; u < ROUNDS; ++u) {
-      const bool real = first >= 0 && round + u < to && head + u * GROUPS < heads;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        raw[u][w][0] = raw[u][w][1] = make_uint4(0, 0, 0, 0);
-        if (CODES) {
-          scale[u][w] = real ? *scales[w] : 0.0f;
-          scales[w] += step;
-          uint32_t c[4] = {0, 0, 0, 0};
-          if (real && wide && in[0]) {  // both pieces in one
-            if constexpr (V == 8) {
-              const uint4 x = *reinterpret_cast<const uint4 *>(rows[w]);
-              c[0] = x.x;
-              c[1] = x.y;
-              c[2] = x.z;
-              c[3] = x.w;
-            } else {
-              const uint2 x = *reinterpret_cast<const uint2 *>(rows[w]);
-              c[0] = x.x;
-              c[1] = x.y;
-            }
-          } else if (real) {  // a row that begins at a multiple of one piece only
-#pragma unroll
-            for (int i = 0; i < 2 * V / 4; ++i)
-              if (in[i / (V / 4)]) c[i] = reinterpret_cast<const uint32_t *>(rows[w])[i];
-          }
-          raw[u][w][0] = make_uint4(c[0], c[1], c[2], c[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (real && in[i]) raw[u][w][i] = reinterpret_cast<const uint4 *>(rows[w])[i];
-        }
-        rows[w] += byte_step;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < ROUNDS; ++u) {
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const bool real = round + u < to && head < heads;
-        if constexpr (CODES) {
-          const uint4 r = raw[u][w][0];
-          Piece<T> p[2];
+    for (int w = 0; w < 2; ++w) {
+      raw[w][0] = raw[w][1] = make_uint4(0, 0, 0, 0);
+      if (CODES) {
+        scale[w] = real ? *scales[w] : 0.0f;
+        scales[w] += step;
+        uint32_t c[4] = {0, 0, 0, 0};
+        if (real && wide && in[0]) {  // both pieces in one
           if constexpr (V == 8) {
-            values_of<V>(p[0].x, make_uint2(r.x, r.y), scale[u][w], cache.type);
-            values_of<V>(p[1].x, make_uint2(r.z, r.w), scale[u][w], cache.type);
+            const uint4 x = *reinterpret_cast<const uint4 *>(rows[w]);
+            c[0] = x.x;
+            c[1] = x.y;
+            c[2] = x.z;
+            c[3] = x.w;
           } else {
-            values_of<V>(p[0].x, make_uint2(r.x, 0), scale[u][w], cache.type);
-            values_of<V>(p[1].x, make_uint2(r.y, 0), scale[u][w], cache.type);
+            const uint2 x = *reinterpret_cast<const uint2 *>(rows[w]);
+            c[0] = x.x;
+            c[1] = x.y;
           }
-          raw[u][w][0] = p[0].get();
-          raw[u][w][1] = p[1].get();
+        } else if (real) {  // a row that begins at a multiple of one piece only
+#pragma unroll
+          for (int i = 0; i < 2 * V / 4; ++i)
+            if (in[i / (V / 4)]) c[i] = reinterpret_cast<const uint32_t *>(rows[w])[i];
         }
+        raw[w][0] = make_uint4(c[0], c[1], c[2], c[3]);
+      } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (real && in[i]) reinterpret_cast<uint4 *>(to_rows[w])[i] = raw[u][w][i];
-        to_rows[w] += GROUPS * dim;
+          if (real && in[i]) raw[w][i] = reinterpret_cast<const uint4 *>(rows[w])[i];
       }
-      head += GROUPS;
+      rows[w] += byte_step;
     }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if constexpr (CODES) {
+        const uint4 r = raw[w][0];
+        Piece<T> p[2];
+        if constexpr (V == 8) {
+          values_of<V>(p[0].x, make_uint2(r.x, r.y), scale[w], cache.type);
+          values_of<V>(p[1].x, make_uint2(r.z, r.w), scale[w], cache.type);
+        } else {
+          values_of<V>(p[0].x, make_uint2(r.x, 0), scale[w], cache.type);
+          values_of<V>(p[1].x, make_uint2(r.y, 0), scale[w], cache.type);
+        }
+        raw[w][0] = p[0].get();
+        raw[w][1] = p[1].get();
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (mine && in[i]) reinterpret_cast<uint4 *>(to_rows[w])[i] = raw[w][i];
+      to_rows[w] += GROUPS * dim;
+    }
+    head += GROUPS;
   }
   pdl_release();
 }

@@ -302,8 +302,8 @@ typedef struct {
 
 /* Keys and values in pages, [pages, heads, page_size, dim], of the rows' type, int8 or e4m3.  A quantised cache has a scale
  * for each head of each token, [pages, heads, page_size]: amax / 127 (448 for e4m3), and holds value * (127 / amax) to the
- * nearest code, ties to even; a row that holds a NaN or an infinity reads as NaN.  At most 256 values a head and 2^32 - 1
- * rows (pages * heads * page_size). */
+ * nearest code, ties to even; a row that holds a NaN or an infinity reads as NaN.  A caller's own scales may be negative.  At
+ * most 256 values a head and 2^32 - 1 rows (pages * heads * page_size). */
 typedef struct {
   int type;
   int64_t pages, heads, page_size, dim;
@@ -345,7 +345,8 @@ int lapis_b200_kv_read(const lapis_b200_kv_cache *cache, const lapis_b200_page_l
  * 0), which hold its own key and value too: softmax(scale q.k) v for each query head, query heads h with h / (q heads / cache
  * heads) sharing a key head.  q [requests, heads, dim]; out the same, contiguous; d_lse (may be null) [requests, heads] gets
  * the natural logarithm of the sum of the exponentials.  A request of length 0 gets zeros and -infinity.  A length beyond the
- * listed pages counts as their end, as does a pos beyond `entries`; a list that begins before entry 0 is empty.  At most 65,535 requests of at most 2^31 - 2^16 tokens. */
+ * listed pages counts as their end, as does a pos beyond `entries`; a list that begins before entry 0 is empty.  At most
+ * 65,535 requests of at most 2^31 - 2^16 tokens. */
 int lapis_b200_paged_attention(int type, int64_t requests, const lapis_b200_heads *q, const lapis_b200_kv_cache *cache,
                                const lapis_b200_page_lists *lists, const void *d_length, double scale, int64_t window, void *d_out,
                                float *d_lse, void *stream);

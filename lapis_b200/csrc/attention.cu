@@ -890,7 +890,7 @@ static int launch_f32_of(const AttendArgs &a, int dev, cudaStream_t st) {
 // one that the head has seen, carried along as the softmax's maximum is: a large scale counts for no more than its token's weight.
 // What fp16 leaves of weight * scale is off by at most 2^-38 of that largest one beside the rounding to its bits.
 // Measured, kernel alone: 1 x 131,072 tokens, 8 key heads of 128 in bf16, 32 query heads: 82 to 87 us, 6.2 to 6.5 TB/s, the rate of a copy; 128
-// requests of up to 8192, 64 query heads, int8: 194 us, 6.1 TB/s of DRAM, 870 instructions a step at 2.6 a cycle; called again and
+// requests of up to 8192, 64 query heads, int8: 197 us, 6.0 TB/s of DRAM, 881 instructions a step at 2.5 a cycle; called again and
 // again it falls to 215 to 235 us, as the power cap takes the clock.  Scores of int8 by whole-number products of three digits of the
 // queries (no conversion of the keys, 14 % fewer instructions) took 229 us where this took 231, and 62 where this took 59 on 32
 // requests.  Four warps of 168 registers, three blocks an SM: two blocks of 250 registers took 274 us of the second where three took

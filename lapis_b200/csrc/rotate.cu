@@ -269,7 +269,7 @@ kv_read_any_kernel(lapis_b200_kv_cache cache, lapis_b200_page_lists lists, int64
 // lane uses for itself: what is on its way takes no registers.  Weight and rotation are one product each with a value and
 // its partner, y = r (x wc + x' ws), wc = w cos, ws = -+ w' sin, two values an instruction.
 // Measured, bf16 heads of 128: 8192 tokens of 32 + 8 heads 31 us (5.5 TB/s; 40 us with the partner in another lane, 180
-// instructions for two rows; 33 with six blocks an SM, which spill), backward of 16,384 83 us (6.2 TB/s) and 4 to add up the
+// instructions for two rows; 33 with six blocks an SM, which spill), backward of 16,384 85 us (6.0 TB/s) and 4.6 to add up the
 // weights' gradients, 32,768 tokens of 32 + 8 + 8 normalised and written as int8 139 us (5.3 TB/s), read back 40 (5.0 TB/s).
 
 __device__ __forceinline__ uint32_t shared_at(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -996,7 +996,7 @@ static bool aligned(const Rows &r, int size) {
   return aligned(r.d, 16) && r.token_stride * size % 16 == 0 && r.head_stride * size % 16 == 0;
 }
 // Whether 16-byte pieces fit the rows of a type, the pairs of their rotation and all arrays; rows that they do not fit are taken
-// value by value (8192 tokens of 32 + 8 heads of 128: 196 us, not 31; backward of 16,384 669, not 86).
+// value by value (8192 tokens of 32 + 8 heads of 128: 196 us, not 31; backward of 16,384 669, not 85).
 static bool pieces_fit(int type, const RotateArgs &a, bool backward) {
   const int size = type_bytes(type), v = 16 / size;
   if (a.dim % v != 0) return false;

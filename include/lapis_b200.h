@@ -351,6 +351,70 @@ int lapis_b200_paged_attention(int type, int64_t requests, const lapis_b200_head
                                const lapis_b200_page_lists *lists, const void *d_length, double scale, int64_t window, void *d_out,
                                float *d_lse, void *stream);
 
+/* ---- a layer of experts: router, lists, rows there and back, 4-bit weights --------------------------------- */
+
+/* The k largest of each token's logits, [tokens, experts] with rows token_stride elements apart: d_expert their numbers, the largest
+ * first, of equal ones the lowest first; d_weights their share of the softmax of all logits, or, with `normalise`, of the k
+ * chosen ones.  Both [tokens, k].  A logit of -infinity is never chosen: where too few are left the expert is -1 and the weight
+ * zero.  NaN counts as the largest, and makes the token's weights NaN, as does +infinity.  experts at most 1024, k at most 32. */
+int lapis_b200_route(int type, int64_t tokens, int64_t experts, const void *d_logits, int64_t token_stride, int64_t k, int normalise,
+                     float *d_weights, int32_t *d_expert, void *stream);
+/* Gradient of the logits, [tokens, experts] contiguous, of their type.  d_expert as it came out (numbers outside [0, experts)
+ * are no one's). */
+int lapis_b200_route_backward(int type, int64_t tokens, int64_t experts, const void *d_logits, int64_t token_stride, int64_t k, int normalise,
+                              const int32_t *d_expert, const float *d_dweights, void *d_dlogits, void *stream);
+
+/* Which slots belong to an expert, as the rows of a CSR pattern.  Slot token * k + j is the token's j-th expert; crd holds the slots
+ * sorted by expert, in ascending order within each, those of experts pos[e] .. pos[e + 1]; pos has experts + 1 entries.  Slots
+ * whose expert is outside [0, experts) (padding, or experts of another process) follow behind pos[experts].  place[slot] is where
+ * a slot stands in crd.  Entries that are not such a permutation are never followed out of the arrays. */
+typedef struct {
+  int64_t tokens, k, experts;
+  const int32_t *d_pos, *d_crd, *d_place;
+} lapis_b200_expert_lists;
+
+/* Fills the three arrays from d_expert [tokens, k], idx_bytes wide.  tokens * k below 2^31, experts at most 1024. */
+int lapis_b200_expert_lists_make(int idx_bytes, int64_t tokens, int64_t k, int64_t experts, const void *d_expert, int32_t *d_pos, int32_t *d_crd,
+                                 int32_t *d_place, void *stream);
+/* Rows of the tokens in the order of the lists: rows[place[t, j]] = x[t], zeros behind pos[experts].  x [tokens, dim], rows
+ * x_stride elements apart; d_rows [tokens * k, dim] contiguous. */
+int lapis_b200_expert_gather(int type, int64_t dim, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists, void *d_rows, void *stream);
+/* out[t] = sum over j of weights[t, j] * rows[place[t, j]], of the slots in front of pos[experts], in 32 bits, in the order of j.
+ * d_weights [tokens, k], or null: without weights, which is the gradient of expert_gather.  d_out [tokens, dim] contiguous. */
+int lapis_b200_expert_combine(int type, int64_t dim, const void *d_rows, int64_t row_stride, const lapis_b200_expert_lists *lists, const float *d_weights,
+                              void *d_out, void *stream);
+/* Its gradients: d_drows [tokens * k, dim] contiguous, zeros behind pos[experts], and d_dweights [tokens, k], zeros for the
+ * slots that are there. */
+int lapis_b200_expert_combine_backward(int type, int64_t dim, const void *d_dout, int64_t dout_stride, const void *d_rows, int64_t row_stride,
+                                       const lapis_b200_expert_lists *lists, const float *d_weights, void *d_drows, float *d_dweights, void *stream);
+
+/* Weights of 4 bits: w[e, n, c] = (code - zero) * scale, code 0 to 15, with a scale and a zero (0 to 15; 8 without zeros) for
+ * every `group` (32, 64 or 128) of an output's columns; `experts` matrices of [outputs, columns].  The library keeps them in
+ * an order of its own: `d_packed` from lapis_b200_int4_pack, of lapis_b200_int4_bytes.  gated: the first half of the outputs are
+ * gates, and a product is silu(gate) * the other half. */
+typedef struct {
+  int64_t experts, outputs, columns;
+  int group, scale_type, zeros, gated;
+  const void *d_packed;
+} lapis_b200_int4;
+/* Bytes of d_packed, or -1 for a description that is refused. */
+int64_t lapis_b200_int4_bytes(const lapis_b200_int4 *w);
+/* d_codes [experts, outputs, ceil(columns / 2)], the even column in the low half of a byte; d_scale [experts, outputs,
+ * ceil(columns / group)] of scale_type; d_zero the same of bytes, of which the low 4 bits count, or null where w->zeros is 0.
+ * Contiguous.  Returns when d_packed is filled: products may fetch weights before the launch in front of them has ended. */
+int lapis_b200_int4_pack(const lapis_b200_int4 *w, const void *d_codes, const void *d_scale, const void *d_zero, void *d_packed, void *stream);
+/* Codes, scales and zeros of dense weights [experts * outputs, columns] of `type`, rows w_stride elements apart, to nearest: without zeros
+ * (d_zero null) scale = amax / 7, codes 1 to 15; with them scale = (max - min) / 15 over the group and 0, zero = -min / scale.  The scale is
+ * rounded to scale_type first.  A group of zeros gets scale 0; one that is not finite a scale of NaN. */
+int lapis_b200_int4_quantise(int type, int64_t rows, int64_t columns, const void *d_w, int64_t w_stride, int group, int scale_type, void *d_codes,
+                             void *d_scale, void *d_zero, void *stream);
+/* y = x w^T of `rows` rows [rows, columns], x_stride elements apart: codes and x are exact (x of 32 bits as three parts of bf16), sums
+ * are in 32 bits, one rounding.  d_y [rows, outputs], or half as many if gated, contiguous.  With lists (may be null) the rows of
+ * y are the lists' slots, those of expert e times its matrix, zeros behind pos[experts]; row i of x is the slot's own, or, with
+ * `fetch`, that of its token: x [tokens, columns].  Made for few rows, of each expert: beyond 64 of them weights are fetched again. */
+int lapis_b200_int4_matmul(int type, const lapis_b200_int4 *w, int64_t rows, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists,
+                           int fetch, void *d_y, void *stream);
+
 /* Step-level PCG entry points: the three passes of one iteration, for callers that
  * put an exchange between them (row-block partitioned solves put a halo copy of p in
  * front of pass A and an allreduce of the scalar block behind passes A and B).

@@ -91,6 +91,16 @@ _PROTOS = {
     "lapis_b200_kv_append": (c_int, [c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "lapis_b200_kv_read": (c_int, [c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
     "lapis_b200_paged_attention": (c_int, [c_int, c_i64, c_vp, c_vp, c_vp, c_vp, c_dbl, c_i64, c_vp, c_vp, c_vp]),
+    "lapis_b200_route": (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]),
+    "lapis_b200_route_backward": (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_expert_lists_make": (c_int, [c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_expert_gather": (c_int, [c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "lapis_b200_expert_combine": (c_int, [c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_expert_combine_backward": (c_int, [c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_int4_bytes": (c_i64, [c_vp]),
+    "lapis_b200_int4_pack": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_int4_quantise": (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "lapis_b200_int4_matmul": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_int, c_vp, c_vp]),
     "lapis_b200_validate_csr_host": (c_int, [c_int, c_i64, c_i64, c_i64, c_vp, c_vp]),
 }
 
@@ -106,6 +116,17 @@ class KvCache(ctypes.Structure):
     """``lapis_b200_kv_cache`` of include/lapis_b200.h."""
     _fields_ = [("type", c_int), ("pages", c_i64), ("heads", c_i64), ("page_size", c_i64), ("dim", c_i64), ("d_k", c_vp), ("d_v", c_vp),
                 ("d_k_scale", c_vp), ("d_v_scale", c_vp)]
+
+
+class ExpertLists(ctypes.Structure):
+    """``lapis_b200_expert_lists`` of include/lapis_b200.h."""
+    _fields_ = [("tokens", c_i64), ("k", c_i64), ("experts", c_i64), ("d_pos", c_vp), ("d_crd", c_vp), ("d_place", c_vp)]
+
+
+class Int4(ctypes.Structure):
+    """``lapis_b200_int4`` of include/lapis_b200.h."""
+    _fields_ = [("experts", c_i64), ("outputs", c_i64), ("columns", c_i64), ("group", c_int), ("scale_type", c_int), ("zeros", c_int), ("gated", c_int),
+                ("d_packed", c_vp)]
 
 
 _LIB = None

@@ -1,0 +1,665 @@
+// A layer of experts: the router, the slots of each expert as CSR rows, tokens copied into that order and summed back.
+//
+//   route     the k largest logits of a token and their softmax, w_j = exp(l_j - m) / sum exp(l_i - m), and the logits' gradient:
+//             over the chosen ones dl_e = w_e (g_e - sum_i w_i g_i), over all dl_i = [i chosen] w_i g_i - p_i sum_j w_j g_j
+//   lists     a stable counting sort of the slots (token * k + j) by expert
+//   gather    rows[place[t, j]] = x[t]
+//   combine   out[t] = sum_j w[t, j] rows[place[t, j]]; backward: drows[place[t, j]] = w[t, j] dout[t], dw[t, j] = rows[..] . dout[t]
+//
+// Everything is computed in 32 bits and rounded once, sums in a fixed order.  Places, offsets and experts are looked at before
+// they are followed.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "experts.h"
+
+namespace lapis_b200 {
+
+// ---- router ---------------------------------------------------------------------
+
+constexpr int ROUTE_THREADS = 128;
+
+struct RouteArgs {
+  const void *logits;
+  int64_t tokens, token_stride;
+  int experts, k, normalise;
+  float *weights;
+  int32_t *expert;
+  const float *dweights;
+  void *dlogits;
+};
+
+// Numbers in the order of the logits: NaN above all, -0 as 0.  0 is below all of them: no logit, or one already taken.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+constexpr uint32_t KEY_NEVER = 0x007fffffu;  // of -infinity
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
+
+// A warp a token; lane l holds logits l, l + 32, ... (32 R of them at most).
+template <typename T, int R>
+__global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const __grid_constant__ RouteArgs a) {
+  const int lane = threadIdx.x % 32;
+  const int64_t token = (int64_t)blockIdx.x * (ROUTE_THREADS / 32) + threadIdx.x / 32;
+  pdl_wait();
+  pdl_release();
+  if (token >= a.tokens) return;
+  const T *const logits = static_cast<const T *>(a.logits) + token * a.token_stride;
+  uint32_t key[R], most = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    key[i] = lane + 32 * i < a.experts ? key_of(to_f32(logits[lane + 32 * i])) : 0;
+    most = max(most, key[i]);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  const float top = logit_of(most);
+  float total = 0.0f;
+  if (!a.normalise) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) total += key[i] > KEY_NEVER ? expf(logit_of(key[i]) - top) : 0.0f;
+    total = warp_sum(total);
+  }
+  float mine = 0.0f;  // of the lane's choice, the lane-th largest
+  int expert = -1;
+  for (int j = 0; j < a.k && most > KEY_NEVER; ++j) {
+    int at = 32 * R;
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i)
+      if (key[i] == most) at = lane + 32 * i;
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == j) {
+      mine = expf(logit_of(most) - top);
+      expert = at;
+    }
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (at == lane + 32 * i) key[i] = 0;
+      most = max(most, key[i]);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+  }
+  if (a.normalise) total = warp_sum(mine);
+  if (lane < a.k) {
+    a.weights[token * a.k + lane] = expert < 0 ? 0.0f : mine / total;
+    a.expert[token * a.k + lane] = expert;
+  }
+}
+
+// A warp a token: its row is written as it would be without the chosen ones, and then theirs.
+template <typename T, int R>
+__global__ void __launch_bounds__(ROUTE_THREADS) route_backward_kernel(const __grid_constant__ RouteArgs a) {
+  const int lane = threadIdx.x % 32;
+  const int64_t token = (int64_t)blockIdx.x * (ROUTE_THREADS / 32) + threadIdx.x / 32;
+  pdl_wait();
+  pdl_release();
+  if (token >= a.tokens) return;
+  const T *const logits = static_cast<const T *>(a.logits) + token * a.token_stride;
+  T *const out = static_cast<T *>(a.dlogits) + token * a.experts;
+  int expert = -1;
+  float mine = -INFINITY, g = 0.0f;
+  if (lane < a.k) {
+    expert = a.expert[token * a.k + lane];
+    if ((uint32_t)expert >= (uint32_t)a.experts) expert = -1;
+    if (expert >= 0) {
+      mine = to_f32(logits[expert]);
+      g = a.dweights[token * a.k + lane];
+    }
+  }
+  float l[R], most, total;
+  if (a.normalise) {
+    most = warp_max(mine);
+    if (most == -INFINITY) most = 0.0f;
+    mine = expf(mine - most);
+    total = warp_sum(mine);
+  } else {
+    most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      l[i] = lane + 32 * i < a.experts ? to_f32(logits[lane + 32 * i]) : -INFINITY;
+      most = fmaxf(most, l[i]);
+    }
+    most = warp_max(most);
+    if (most == -INFINITY) most = 0.0f;
+    total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) total += l[i] = expf(l[i] - most);
+    total = warp_sum(total);
+    mine = expf(mine - most);
+  }
+  if (total == 0.0f) total = 1.0f;
+  const float w = mine / total, inner = warp_sum(expert >= 0 ? w * g : 0.0f);
+  const float own = a.normalise ? w * (g - inner) : w * g;
+  float sum = a.normalise ? 0.0f : -(w * inner);  // of the lane's expert, which a caller may name twice
+  for (int j = 0; j < a.k; ++j) {
+    const int e = __shfl_sync(0xffffffffu, expert, j);
+    const float x = __shfl_sync(0xffffffffu, own, j);
+    if (e == expert) sum += x;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (lane + 32 * i < a.experts) out[lane + 32 * i] = from_f32<T>(a.normalise ? 0.0f : -(l[i] / total * inner));
+  __syncwarp();
+  if (expert >= 0) out[expert] = from_f32<T>(sum);
+}
+
+template <typename T, int R>
+static int launch_route_as(const RouteArgs &a, cudaStream_t st) {
+  const dim3 grid((unsigned)((a.tokens + ROUTE_THREADS / 32 - 1) / (ROUTE_THREADS / 32)));
+  LAPIS_CUDA_TRY(a.dlogits != nullptr ? launch_pdl(route_backward_kernel<T, R>, grid, ROUTE_THREADS, 0, st, a)
+                                      : launch_pdl(route_kernel<T, R>, grid, ROUTE_THREADS, 0, st, a));
+  return LAPIS_OK;
+}
+template <typename T>
+static int launch_route_of(const RouteArgs &a, cudaStream_t st) {
+  if (a.experts <= 32) return launch_route_as<T, 1>(a, st);
+  if (a.experts <= 64) return launch_route_as<T, 2>(a, st);
+  if (a.experts <= 128) return launch_route_as<T, 4>(a, st);
+  if (a.experts <= 256) return launch_route_as<T, 8>(a, st);
+  if (a.experts <= 512) return launch_route_as<T, 16>(a, st);
+  return launch_route_as<T, 32>(a, st);
+}
+static int launch_route(int type, const RouteArgs &a, cudaStream_t st) {
+  switch (type) {
+    case LAPIS_F32: return launch_route_of<float>(a, st);
+    case LAPIS_F16: return launch_route_of<__half>(a, st);
+    default: return launch_route_of<__nv_bfloat16>(a, st);
+  }
+}
+
+// ---- lists ----------------------------------------------------------------------
+
+constexpr int LIST_THREADS = 512, LIST_WARPS = LIST_THREADS / 32;
+
+struct ListArgs {
+  const void *expert;
+  int idx_bytes, experts, blocks;
+  int64_t slots;
+  uint32_t *counts;  // [blocks, experts + 1], or null for one block
+  int32_t *pos, *crd, *place;
+};
+// The list of a slot; `experts` for those that are no one's.
+__device__ __forceinline__ int bucket_of(const ListArgs &a, int64_t slot) {
+  const int64_t e = load_index(a.expert, slot, a.idx_bytes);
+  return (uint64_t)e < (uint64_t)a.experts ? (int)e : a.experts;
+}
+
+// What each block's slots add to each list.
+template <int S>
+__global__ void __launch_bounds__(LIST_THREADS) list_count_kernel(const __grid_constant__ ListArgs a) {
+  extern __shared__ uint32_t hist[];
+  const int buckets = a.experts + 1;
+  for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) hist[b] = 0;
+  pdl_wait();
+  pdl_release();
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * LIST_THREADS * S;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int64_t slot = first + s * LIST_THREADS + threadIdx.x;
+    if (slot < a.slots) atomicAdd(&hist[bucket_of(a, slot)], 1u);
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) a.counts[(int64_t)blockIdx.x * buckets + b] = hist[b];
+}
+
+// Every warp numbers its slots within each list (peers in a step of 32 by match), the block adds up its warps and the blocks in
+// front of it, and the lists' beginnings are a scan over all lists' lengths.
+template <int S>
+__global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_constant__ ListArgs a) {
+  extern __shared__ uint32_t smem[];
+  __shared__ uint32_t warp_sums[LIST_WARPS];
+  const int buckets = a.experts + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  uint32_t *const of_warp = smem, *const length = smem + LIST_WARPS * buckets, *const in_front = length + buckets;
+  for (int i = threadIdx.x; i < (LIST_WARPS + 2) * buckets; i += LIST_THREADS) smem[i] = 0;
+  pdl_wait();
+  pdl_release();
+  const int64_t first = ((int64_t)blockIdx.x * LIST_WARPS + warp) * 32 * S;
+  int bucket[S];
+  uint32_t rank[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int64_t slot = first + s * 32 + lane;
+    bucket[s] = slot < a.slots ? bucket_of(a, slot) : -1;
+  }
+  __syncthreads();
+  uint32_t *const mine = of_warp + warp * buckets;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const uint32_t peers = __match_any_sync(0xffffffffu, bucket[s]);
+    const uint32_t before = bucket[s] >= 0 ? mine[bucket[s]] : 0;
+    rank[s] = before + __popc(peers & ((1u << lane) - 1));
+    __syncwarp();
+    if (bucket[s] >= 0 && lane == __ffs(peers) - 1) mine[bucket[s]] = before + __popc(peers);
+    __syncwarp();
+  }
+  if (a.counts != nullptr) {
+    const int share = max(1, LIST_THREADS / buckets);  // threads that add up one list's counts
+    for (int i = threadIdx.x; i < share * buckets; i += LIST_THREADS) {
+      const int b = i % buckets;
+      uint32_t all = 0, before = 0;
+#pragma unroll 8
+      for (int n = i / buckets; n < a.blocks; n += share) {
+        const uint32_t c = a.counts[(int64_t)n * buckets + b];
+        all += c;
+        before += n < (int)blockIdx.x ? c : 0;
+      }
+      atomicAdd(&length[b], all);
+      atomicAdd(&in_front[b], before);
+    }
+  }
+  __syncthreads();
+  for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) {
+    uint32_t upto = 0;
+#pragma unroll
+    for (int w = 0; w < LIST_WARPS; ++w) {
+      const uint32_t n = of_warp[w * buckets + b];
+      of_warp[w * buckets + b] = upto;
+      upto += n;
+    }
+    if (a.counts == nullptr) length[b] = upto;
+  }
+  __syncthreads();
+  // Where the lists begin: a thread takes `run` lists that lie next to one another.
+  const int run = (buckets + LIST_THREADS - 1) / LIST_THREADS, from = threadIdx.x * run;
+  uint32_t sum = 0;
+  for (int b = from; b < min(from + run, buckets); ++b) sum += length[b];
+  uint32_t upto = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += below;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  uint32_t begin = upto - sum;
+  for (int w = 0; w < warp; ++w) begin += warp_sums[w];
+  for (int b = from; b < min(from + run, buckets); ++b) {
+    if (blockIdx.x == 0) a.pos[b] = (int32_t)begin;
+    in_front[b] += begin;
+    begin += length[b];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if (bucket[s] < 0) continue;
+    const int64_t slot = first + s * 32 + lane;
+    const uint32_t at = in_front[bucket[s]] + mine[bucket[s]] + rank[s];
+    a.place[slot] = (int32_t)at;
+    a.crd[at] = (int32_t)slot;
+  }
+}
+
+template <int S>
+static int launch_lists_as(ListArgs &a, cudaStream_t st) {
+  const int buckets = a.experts + 1;
+  a.blocks = (int)((a.slots + LIST_THREADS * S - 1) / (LIST_THREADS * S));
+  a.blocks = std::max(a.blocks, 1);
+  PoolBuf counts;
+  if (a.blocks > 1) {
+    LAPIS_TRY(counts.alloc((size_t)a.blocks * buckets * sizeof(uint32_t), st));
+    a.counts = static_cast<uint32_t *>(counts.p);
+    LAPIS_CUDA_TRY(launch_pdl(list_count_kernel<S>, dim3(a.blocks), LIST_THREADS, buckets * sizeof(uint32_t), st, a));
+  }
+  const size_t smem = (LIST_WARPS + 2) * buckets * sizeof(uint32_t);
+  LAPIS_CUDA_TRY(cudaFuncSetAttribute(list_place_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((LIST_WARPS + 2) * (MAX_EXPERTS + 1) * sizeof(uint32_t))));
+  LAPIS_CUDA_TRY(launch_pdl(list_place_kernel<S>, dim3(a.blocks), LIST_THREADS, smem, st, a));
+  return LAPIS_OK;
+}
+static int launch_lists(ListArgs &a, cudaStream_t st) {
+  const int64_t all = a.slots / sm_count();
+  if (a.slots <= LIST_THREADS || all <= LIST_THREADS) return launch_lists_as<1>(a, st);
+  if (all <= 2 * LIST_THREADS) return launch_lists_as<2>(a, st);
+  if (all <= 4 * LIST_THREADS) return launch_lists_as<4>(a, st);
+  if (all <= 8 * LIST_THREADS) return launch_lists_as<8>(a, st);
+  return launch_lists_as<32>(a, st);
+}
+
+// ---- rows there and back ----------------------------------------------------------
+
+constexpr int ROWS_THREADS = 256;
+
+struct RowsArgs {
+  const void *x, *rows;
+  int64_t x_stride, row_stride, dim;  // strides in elements
+  int64_t tokens, slots;
+  int k, experts;
+  int64_t items;
+  uint32_t chunks;  // items of a row
+  const int32_t *pos, *place;
+  const float *weights;
+  void *out;
+  float *dweights;
+};
+// A slot's place, or -1 where the list names none, and whether there is an expert at it.
+struct Place {
+  int32_t at;
+  bool here;
+};
+__device__ __forceinline__ Place place_of(const RowsArgs &a, int64_t slot, int32_t end) {
+  const int32_t at = a.place[slot];
+  return {(uint32_t)at < (uint64_t)a.slots ? at : -1, (uint32_t)at < (uint64_t)a.slots && at < end};
+}
+__device__ __forceinline__ int64_t divided(int64_t item, uint32_t by, int64_t items) {
+  return items <= 0xffffffffll ? (int64_t)((uint32_t)item / by) : item / by;
+}
+
+// A piece of a row: V elements, 16 bytes where rows allow it.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Piece {
+  T v[V];
+};
+
+// A warp an item: GATHER_PIECES pieces a lane of a token's row, read once and written k times.
+constexpr int GATHER_PIECES = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) gather_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  const int lane = threadIdx.x % 32;
+  const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
+  pdl_wait();
+  pdl_release();
+  if (item >= a.items) return;
+  const int64_t token = divided(item, a.chunks, a.items);
+  const int64_t first = (item - token * a.chunks) * (32 * GATHER_PIECES) + lane, pieces = a.dim / V;
+  const P *const from = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + token * a.x_stride);
+  const int32_t end = a.pos[a.experts];
+  P got[GATHER_PIECES] = {};
+#pragma unroll
+  for (int u = 0; u < GATHER_PIECES; ++u)
+    if (first + u * 32 < pieces) got[u] = from[first + u * 32];
+  for (int j0 = 0; j0 < a.k; j0 += 32) {
+    const Place p = j0 + lane < a.k ? place_of(a, token * a.k + j0 + lane, end) : Place{-1, false};
+    for (int j = 0; j < min(32, a.k - j0); ++j) {
+      const int32_t at = __shfl_sync(0xffffffffu, p.at, j);
+      const bool here = __shfl_sync(0xffffffffu, p.here, j);
+      if (at < 0) continue;
+      P *const to = reinterpret_cast<P *>(static_cast<T *>(a.out) + at * a.dim);
+#pragma unroll
+      for (int u = 0; u < GATHER_PIECES; ++u)
+        if (first + u * 32 < pieces) to[first + u * 32] = here ? got[u] : P{};
+    }
+  }
+}
+
+// A warp an item: a piece a lane of a token's row, COMBINE_ROWS rows asked for at a time.
+constexpr int COMBINE_ROWS = 8;
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) combine_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  const int lane = threadIdx.x % 32;
+  const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
+  pdl_wait();
+  pdl_release();
+  if (item >= a.items) return;
+  const int64_t token = divided(item, a.chunks, a.items);
+  const int64_t piece = (item - token * a.chunks) * 32 + lane, pieces = a.dim / V;
+  const int32_t end = a.pos[a.experts];
+  float sum[V] = {};
+  for (int j0 = 0; j0 < a.k; j0 += 32) {
+    const Place p = j0 + lane < a.k ? place_of(a, token * a.k + j0 + lane, end) : Place{-1, false};
+    const float weight = a.weights != nullptr && p.here ? a.weights[token * a.k + j0 + lane] : 1.0f;
+    for (int j1 = 0; j1 < min(32, a.k - j0); j1 += COMBINE_ROWS) {
+      P got[COMBINE_ROWS];
+#pragma unroll
+      for (int j = 0; j < COMBINE_ROWS; ++j) {
+        const int32_t at = __shfl_sync(0xffffffffu, p.here ? p.at : -1, j1 + j);
+        if (at >= 0 && piece < pieces) got[j] = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + at * a.row_stride)[piece];
+      }
+#pragma unroll
+      for (int j = 0; j < COMBINE_ROWS; ++j) {
+        const bool here = __shfl_sync(0xffffffffu, p.here, j1 + j);
+        const float w = __shfl_sync(0xffffffffu, weight, j1 + j);
+        if (!here || piece >= pieces) continue;
+#pragma unroll
+        for (int v = 0; v < V; ++v) sum[v] = fmaf(w, to_f32(got[j].v[v]), sum[v]);
+      }
+    }
+  }
+  if (piece >= pieces) return;
+  P done;
+#pragma unroll
+  for (int v = 0; v < V; ++v) done.v[v] = from_f32<T>(sum[v]);
+  reinterpret_cast<P *>(static_cast<T *>(a.out) + token * a.dim)[piece] = done;
+}
+
+// A warp a slot: its row's product with dout of its token, and its weight times dout.
+constexpr int BACK_PIECES = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) combine_backward_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  const int lane = threadIdx.x % 32;
+  const int64_t slot = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
+  pdl_wait();
+  pdl_release();
+  if (slot >= a.slots) return;
+  const int64_t token = divided(slot, a.k, a.slots), pieces = a.dim / V;
+  const Place p = place_of(a, slot, a.pos[a.experts]);
+  const P *const dout = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + token * a.x_stride);
+  const P *const row = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + p.at * a.row_stride);
+  P *const to = reinterpret_cast<P *>(static_cast<T *>(a.out) + p.at * a.dim);
+  float dot = 0.0f;
+  if (p.here) {
+    const float w = a.weights[slot];
+    for (int64_t first = lane; first < pieces; first += 32 * BACK_PIECES) {
+      P d[BACK_PIECES], r[BACK_PIECES];
+#pragma unroll
+      for (int u = 0; u < BACK_PIECES; ++u)
+        if (first + u * 32 < pieces) {
+          d[u] = dout[first + u * 32];
+          r[u] = row[first + u * 32];
+        }
+#pragma unroll
+      for (int u = 0; u < BACK_PIECES; ++u)
+        if (first + u * 32 < pieces) {
+          P done;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float x = to_f32(d[u].v[v]);
+            dot = fmaf(x, to_f32(r[u].v[v]), dot);
+            done.v[v] = from_f32<T>(w * x);
+          }
+          to[first + u * 32] = done;
+        }
+    }
+  } else if (p.at >= 0) {
+    for (int64_t i = lane; i < pieces; i += 32) to[i] = P{};
+  }
+  dot = warp_sum(dot);
+  if (lane == 0) a.dweights[slot] = dot;
+}
+
+enum RowsOp { GATHER, COMBINE, COMBINE_BACKWARD };
+
+template <typename T, int V>
+static int launch_rows_as(RowsOp op, RowsArgs &a, cudaStream_t st) {
+  constexpr int WARPS = ROWS_THREADS / 32;
+  const int64_t lanes = (a.dim / V + 31) / 32;
+  a.chunks = (uint32_t)(op == GATHER ? (lanes + GATHER_PIECES - 1) / GATHER_PIECES : lanes);
+  a.items = op == COMBINE_BACKWARD ? a.slots : a.tokens * a.chunks;
+  const int64_t blocks = (a.items + WARPS - 1) / WARPS;
+  if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
+  const dim3 grid((unsigned)blocks);
+  LAPIS_CUDA_TRY(op == GATHER ? launch_pdl(gather_kernel<T, V>, grid, ROWS_THREADS, 0, st, a)
+                 : op == COMBINE ? launch_pdl(combine_kernel<T, V>, grid, ROWS_THREADS, 0, st, a)
+                                 : launch_pdl(combine_backward_kernel<T, V>, grid, ROWS_THREADS, 0, st, a));
+  return LAPIS_OK;
+}
+static bool fits(const void *p, int64_t stride, int bytes, int align) { return reinterpret_cast<uintptr_t>(p) % align == 0 && stride * bytes % align == 0; }
+template <typename T>
+static int launch_rows_of(RowsOp op, RowsArgs &a, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = fits(a.x, a.x_stride, sizeof(T), 16) && fits(a.rows, a.row_stride, sizeof(T), 16) && fits(a.out, a.dim, sizeof(T), 16);
+  return wide ? launch_rows_as<T, V>(op, a, st) : launch_rows_as<T, 1>(op, a, st);
+}
+static int launch_rows(int type, RowsOp op, RowsArgs &a, cudaStream_t st) {
+  switch (type) {
+    case LAPIS_F32: return launch_rows_of<float>(op, a, st);
+    case LAPIS_F16: return launch_rows_of<__half>(op, a, st);
+    default: return launch_rows_of<__nv_bfloat16>(op, a, st);
+  }
+}
+
+// ---- checks -----------------------------------------------------------------------
+
+int check_expert_lists(const char *what, const lapis_b200_expert_lists *l) {
+  if (l == nullptr) return fail(LAPIS_EBADARG, "%s: null lists", what);
+  if (l->tokens < 0 || l->k < 0 || l->experts < 0) return fail(LAPIS_EBADSHAPE, "%s: negative size", what);
+  if (l->experts > MAX_EXPERTS) return fail(LAPIS_ETOOBIG, "%s: more than %d experts", what, MAX_EXPERTS);
+  if (l->k > 0 && l->tokens > 0x7fffffff / l->k) return fail(LAPIS_ETOOBIG, "%s: 2^31 slots or more", what);
+  if (l->d_pos == nullptr || (l->tokens * l->k > 0 && (l->d_crd == nullptr || l->d_place == nullptr))) return fail(LAPIS_EBADARG, "%s: null list", what);
+  return LAPIS_OK;
+}
+static int check_rows(const char *what, int type, int64_t dim, const lapis_b200_expert_lists *lists) {
+  if (!is_float_type(type)) return fail(LAPIS_EBADARG, "%s: type must be LAPIS_F32, LAPIS_F16 or LAPIS_BF16", what);
+  LAPIS_TRY(check_expert_lists(what, lists));
+  if (dim < 0) return fail(LAPIS_EBADSHAPE, "%s: negative size", what);
+  if (dim > 0x7fffffff) return fail(LAPIS_ETOOBIG, "%s: rows of 2^31 elements or more", what);
+  return LAPIS_OK;
+}
+static RowsArgs rows_args(int64_t dim, const lapis_b200_expert_lists *l) {
+  RowsArgs a = {};
+  a.dim = dim;
+  a.tokens = l->tokens;
+  a.slots = l->tokens * l->k;
+  a.k = (int)l->k;
+  a.experts = (int)l->experts;
+  a.pos = l->d_pos;
+  a.place = l->d_place;
+  return a;
+}
+static int check_route(const char *what, int type, int64_t tokens, int64_t experts, const void *d_logits, int64_t k) {
+  if (!is_float_type(type)) return fail(LAPIS_EBADARG, "%s: type must be LAPIS_F32, LAPIS_F16 or LAPIS_BF16", what);
+  if (tokens < 0 || experts < 0 || k < 0) return fail(LAPIS_EBADSHAPE, "%s: negative size", what);
+  if (k > experts) return fail(LAPIS_EBADSHAPE, "%s: more choices than experts", what);
+  if (experts > MAX_EXPERTS) return fail(LAPIS_ETOOBIG, "%s: more than %d experts", what, MAX_EXPERTS);
+  if (k > MAX_CHOSEN) return fail(LAPIS_ETOOBIG, "%s: more than %d choices", what, MAX_CHOSEN);
+  if (tokens > 0x7fffffff) return fail(LAPIS_ETOOBIG, "%s: 2^31 tokens or more", what);
+  if (tokens > 0 && experts > 0 && d_logits == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  return LAPIS_OK;
+}
+
+}  // namespace lapis_b200
+
+using namespace lapis_b200;
+
+extern "C" int lapis_b200_route(int type, int64_t tokens, int64_t experts, const void *d_logits, int64_t token_stride, int64_t k, int normalise,
+                                float *d_weights, int32_t *d_expert, void *stream) {
+  clear_error();
+  const char *what = "route";
+  LAPIS_TRY(check_route(what, type, tokens, experts, d_logits, k));
+  if (tokens == 0 || k == 0) return LAPIS_OK;
+  if (d_weights == nullptr || d_expert == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  RouteArgs a = {};
+  a.logits = d_logits;
+  a.tokens = tokens;
+  a.token_stride = token_stride;
+  a.experts = (int)experts;
+  a.k = (int)k;
+  a.normalise = normalise != 0;
+  a.weights = d_weights;
+  a.expert = d_expert;
+  return launch_route(type, a, as_stream(stream));
+}
+
+extern "C" int lapis_b200_route_backward(int type, int64_t tokens, int64_t experts, const void *d_logits, int64_t token_stride, int64_t k, int normalise,
+                                         const int32_t *d_expert, const float *d_dweights, void *d_dlogits, void *stream) {
+  clear_error();
+  const char *what = "route_backward";
+  LAPIS_TRY(check_route(what, type, tokens, experts, d_logits, k));
+  if (tokens == 0 || experts == 0) return LAPIS_OK;
+  if (d_dlogits == nullptr || (k > 0 && (d_expert == nullptr || d_dweights == nullptr))) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  RouteArgs a = {};
+  a.logits = d_logits;
+  a.tokens = tokens;
+  a.token_stride = token_stride;
+  a.experts = (int)experts;
+  a.k = (int)k;
+  a.normalise = normalise != 0;
+  a.expert = const_cast<int32_t *>(d_expert);
+  a.dweights = d_dweights;
+  a.dlogits = d_dlogits;
+  return launch_route(type, a, as_stream(stream));
+}
+
+extern "C" int lapis_b200_expert_lists_make(int idx_bytes, int64_t tokens, int64_t k, int64_t experts, const void *d_expert, int32_t *d_pos, int32_t *d_crd,
+                                            int32_t *d_place, void *stream) {
+  clear_error();
+  const char *what = "expert_lists";
+  const lapis_b200_expert_lists l = {tokens, k, experts, d_pos, d_crd, d_place};
+  if (idx_bytes != 4 && idx_bytes != 8) return fail(LAPIS_EBADARG, "%s: idx_bytes must be 4 or 8", what);
+  LAPIS_TRY(check_expert_lists(what, &l));
+  if (tokens * k > 0 && d_expert == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  ListArgs a = {};
+  a.expert = d_expert;
+  a.idx_bytes = idx_bytes;
+  a.experts = (int)experts;
+  a.slots = tokens * k;
+  a.pos = d_pos;
+  a.crd = d_crd;
+  a.place = d_place;
+  return launch_lists(a, as_stream(stream));
+}
+
+extern "C" int lapis_b200_expert_gather(int type, int64_t dim, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists, void *d_rows,
+                                        void *stream) {
+  clear_error();
+  const char *what = "expert_gather";
+  LAPIS_TRY(check_rows(what, type, dim, lists));
+  RowsArgs a = rows_args(dim, lists);
+  if (a.slots == 0 || dim == 0) return LAPIS_OK;
+  if (d_x == nullptr || d_rows == nullptr) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  a.x = d_x;
+  a.x_stride = x_stride;
+  a.out = d_rows;
+  return launch_rows(type, GATHER, a, as_stream(stream));
+}
+
+extern "C" int lapis_b200_expert_combine(int type, int64_t dim, const void *d_rows, int64_t row_stride, const lapis_b200_expert_lists *lists,
+                                         const float *d_weights, void *d_out, void *stream) {
+  clear_error();
+  const char *what = "expert_combine";
+  LAPIS_TRY(check_rows(what, type, dim, lists));
+  RowsArgs a = rows_args(dim, lists);
+  if (a.tokens == 0 || dim == 0) return LAPIS_OK;
+  if (d_out == nullptr || (a.slots > 0 && d_rows == nullptr)) return fail(LAPIS_EBADARG, "%s: null operand", what);
+  a.rows = d_rows;
+  a.row_stride = row_stride;
+  a.weights = d_weights;
+  a.out = d_out;
+  return launch_rows(type, COMBINE, a, as_stream(stream));
+}
+
+extern "C" int lapis_b200_expert_combine_backward(int type, int64_t dim, const void *d_dout, int64_t dout_stride, const void *d_rows, int64_t row_stride,
+                                                  const lapis_b200_expert_lists *lists, const float *d_weights, void *d_drows, float *d_dweights,
+                                                  void *stream) {
+  clear_error();
+  const char *what = "expert_combine_backward";
+  LAPIS_TRY(check_rows(what, type, dim, lists));
+  RowsArgs a = rows_args(dim, lists);
+  if (a.slots == 0) return LAPIS_OK;
+  if (d_weights == nullptr || d_dweights == nullptr || (dim > 0 && (d_dout == nullptr || d_rows == nullptr || d_drows == nullptr)))
+    return fail(LAPIS_EBADARG, "%s: null operand", what);
+  a.x = d_dout;
+  a.x_stride = dout_stride;
+  a.rows = d_rows;
+  a.row_stride = row_stride;
+  a.weights = d_weights;
+  a.out = d_drows;
+  a.dweights = d_dweights;
+  return launch_rows(type, COMBINE_BACKWARD, a, as_stream(stream));
+}

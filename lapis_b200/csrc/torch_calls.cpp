@@ -4,7 +4,7 @@
 // A small call is bound by the host: at 10,000 rows the SpMV kernel takes 2-3 us and the launch 2 us, while the same
 // checks written in Python with a ctypes call took 11 us (3.5 us of it torch.cuda.current_stream()).
 // Every function returns the library's status, or -1 when an operand is not the kind of tensor it takes; the caller
-// (lapis_b200/device.py) then names the operand in the exception it raises.  Those of lapis_b200/attention.py make their results
+// (lapis_b200/device.py) then names the operand in the exception it raises.  Those of lapis_b200/attention.py and experts.py make their results
 // here (torch.empty took 3.3 us where it was measured, at::empty 0.8) and return them where all went well.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -312,6 +312,138 @@ PyObject *py_paged_attention(PyObject *const *a) {
                  out, lse);
 }
 
+// ---- a layer of experts (lapis_b200/experts.py) ----
+
+// Rows [rows, dim] of a type whose values lie next to one another.
+bool rows_of(const at::Tensor *t, int type, int64_t rows, int64_t dim) {
+  if (t == nullptr || t->dim() != 2 || !on_device(t) || type_of(t) != type || t->size(0) != rows || t->size(1) != dim) return false;
+  return dim <= 1 || t->stride(1) == 1 || t->numel() == 0;
+}
+bool matrix_of(PyObject *o, at::ScalarType type, int64_t rows, int64_t columns, const at::Tensor **t) {
+  *t = tensor(o);
+  return is(*t, type) && on_device(*t) && (*t)->dim() == 2 && (*t)->size(0) == rows && (*t)->size(1) == columns;
+}
+// a: pos, crd, place
+bool expert_lists_of(PyObject *const *a, lapis_b200_expert_lists *l) {
+  const at::Tensor *pos = tensor(a[0]), *crd = tensor(a[1]), *place = tensor(a[2]);
+  for (const at::Tensor *t : {pos, crd, place})
+    if (!is(t, at::kInt) || !on_device(t)) return false;
+  if (pos->dim() != 1 || pos->numel() < 1 || crd->dim() != 1 || place->dim() != 2 || crd->numel() != place->numel()) return false;
+  *l = {place->size(0), place->size(1), pos->numel() - 1, addr_of<int32_t>(pos), addr_of<int32_t>(crd), addr_of<int32_t>(place)};
+  return true;
+}
+
+// route(logits, k, normalise) -> weights, expert
+PyObject *py_route(PyObject *const *a) {
+  const at::Tensor *logits = tensor(a[0]);
+  const long long k = PyLong_AsLongLong(a[1]);
+  const int normalise = PyObject_IsTrue(a[2]);
+  if (PyErr_Occurred()) return nullptr;
+  if (logits == nullptr || logits->dim() != 2 || k < 0 || k > logits->size(1)) return status(-1);
+  const int64_t tokens = logits->size(0), experts = logits->size(1);
+  const int type = type_of(logits);
+  if (type < 0 || !rows_of(logits, type, tokens, experts)) return status(-1);
+  const at::Tensor weights = result(logits, at::kFloat, {tokens, k}), expert = result(logits, at::kInt, {tokens, k});
+  return results(call(lapis_b200_route, type, tokens, experts, addr(logits), logits->stride(0), k, normalise, addr_of<float>(&weights),
+                      addr_of<int32_t>(&expert), stream()),
+                 weights, expert);
+}
+
+// route_backward(dweights, logits, expert, normalise) -> of the logits
+PyObject *py_route_backward(PyObject *const *a) {
+  const at::Tensor *logits = tensor(a[1]), *dweights, *expert;
+  const int normalise = PyObject_IsTrue(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (logits == nullptr || logits->dim() != 2) return status(-1);
+  const int64_t tokens = logits->size(0), experts = logits->size(1);
+  const int type = type_of(logits);
+  const at::Tensor *chosen = tensor(a[2]);
+  if (chosen == nullptr || chosen->dim() != 2 || chosen->size(1) > experts) return status(-1);
+  const int64_t k = chosen->size(1);
+  if (type < 0 || !rows_of(logits, type, tokens, experts) || !matrix_of(a[0], at::kFloat, tokens, k, &dweights) ||
+      !matrix_of(a[2], at::kInt, tokens, k, &expert))
+    return status(-1);
+  const at::Tensor dlogits = result(logits, {tokens, experts});
+  return results(call(lapis_b200_route_backward, type, tokens, experts, addr(logits), logits->stride(0), k, normalise, addr_of<int32_t>(expert),
+                      addr_of<float>(dweights), addr(&dlogits), stream()),
+                 dlogits);
+}
+
+// expert_lists(expert, experts) -> pos, crd, place
+PyObject *py_expert_lists(PyObject *const *a) {
+  const at::Tensor *expert = tensor(a[0]);
+  const long long experts = PyLong_AsLongLong(a[1]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!is_index(expert) || !on_device(expert) || expert->dim() != 2 || experts < 0 || experts > (1 << 20)) return status(-1);
+  const int64_t tokens = expert->size(0), k = expert->size(1);
+  const at::Tensor pos = result(expert, at::kInt, {experts + 1}), crd = result(expert, at::kInt, {tokens * k}), place = result(expert, at::kInt, {tokens, k});
+  return results(call(lapis_b200_expert_lists_make, (int)expert->element_size(), tokens, k, experts, addr(expert), addr_of<int32_t>(&pos),
+                      addr_of<int32_t>(&crd), addr_of<int32_t>(&place), stream()),
+                 pos, crd, place);
+}
+
+// expert_gather(x, pos, crd, place) -> rows
+PyObject *py_expert_gather(PyObject *const *a) {
+  const at::Tensor *x = tensor(a[0]);
+  lapis_b200_expert_lists l;
+  if (x == nullptr || x->dim() != 2 || !expert_lists_of(a + 1, &l)) return status(-1);
+  const int type = type_of(x);
+  const int64_t dim = x->size(1);
+  if (type < 0 || !rows_of(x, type, l.tokens, dim)) return status(-1);
+  const at::Tensor rows = result(x, {l.tokens * l.k, dim});
+  return results(call(lapis_b200_expert_gather, type, dim, addr(x), x->stride(0), &l, addr(&rows), stream()), rows);
+}
+
+// expert_combine(rows, weights or None, pos, crd, place) -> out
+PyObject *py_expert_combine(PyObject *const *a) {
+  const at::Tensor *rows = tensor(a[0]), *weights = nullptr;
+  lapis_b200_expert_lists l;
+  if (rows == nullptr || rows->dim() != 2 || !expert_lists_of(a + 2, &l)) return status(-1);
+  const int type = type_of(rows);
+  const int64_t dim = rows->size(1);
+  if (type < 0 || !rows_of(rows, type, l.tokens * l.k, dim) || (a[1] != Py_None && !matrix_of(a[1], at::kFloat, l.tokens, l.k, &weights))) return status(-1);
+  const at::Tensor out = result(rows, {l.tokens, dim});
+  return results(call(lapis_b200_expert_combine, type, dim, addr(rows), rows->stride(0), &l, weights == nullptr ? nullptr : addr_of<float>(weights),
+                      addr(&out), stream()),
+                 out);
+}
+
+// expert_combine_backward(dout, rows, weights, pos, crd, place) -> of rows, of weights
+PyObject *py_expert_combine_backward(PyObject *const *a) {
+  const at::Tensor *dout = tensor(a[0]), *rows = tensor(a[1]), *weights;
+  lapis_b200_expert_lists l;
+  if (rows == nullptr || rows->dim() != 2 || !expert_lists_of(a + 3, &l)) return status(-1);
+  const int type = type_of(rows);
+  const int64_t dim = rows->size(1);
+  if (type < 0 || !rows_of(rows, type, l.tokens * l.k, dim) || !rows_of(dout, type, l.tokens, dim) || !matrix_of(a[2], at::kFloat, l.tokens, l.k, &weights))
+    return status(-1);
+  const at::Tensor drows = result(rows, rows->sizes()), dweights = result(weights, weights->sizes());
+  return results(call(lapis_b200_expert_combine_backward, type, dim, addr(dout), dout->stride(0), addr(rows), rows->stride(0), &l, addr_of<float>(weights),
+                      addr(&drows), addr_of<float>(&dweights), stream()),
+                 drows, dweights);
+}
+
+// int4_matmul(weights, x) -> y, int4_matmul_lists(weights, x, fetch, pos, crd, place) -> y
+const lapis_b200_int4 *int4_of(PyObject *o) { return static_cast<const lapis_b200_int4 *>(PyLong_AsVoidPtr(o)); }
+PyObject *int4_product(const lapis_b200_int4 *w, PyObject *rows, int fetch, const lapis_b200_expert_lists *l) {
+  const at::Tensor *x = tensor(rows);
+  if (PyErr_Occurred()) return nullptr;
+  if (w == nullptr || x == nullptr || x->dim() != 2) return status(-1);
+  const int type = type_of(x);
+  const int64_t given = x->size(0);
+  if (type < 0 || !rows_of(x, type, given, w->columns)) return status(-1);
+  const at::Tensor y = result(x, {l == nullptr ? given : l->tokens * l->k, w->gated ? w->outputs / 2 : w->outputs});
+  return results(call(lapis_b200_int4_matmul, type, w, given, addr(x), x->stride(0), l, fetch, addr(&y), stream()), y);
+}
+PyObject *py_int4_matmul(PyObject *const *a) { return int4_product(int4_of(a[0]), a[1], 0, nullptr); }
+PyObject *py_int4_matmul_lists(PyObject *const *a) {
+  const int fetch = PyObject_IsTrue(a[2]);
+  lapis_b200_expert_lists l;
+  if (PyErr_Occurred()) return nullptr;
+  if (!expert_lists_of(a + 3, &l)) return status(-1);
+  return int4_product(int4_of(a[0]), a[1], fetch, &l);
+}
+
 template <PyObject *(*CALL)(PyObject *const *), Py_ssize_t ARGS>
 PyMethodDef method(const char *name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<CALL, ARGS>)), METH_FASTCALL, nullptr};
@@ -320,7 +452,11 @@ PyMethodDef methods[] = {method<py_spmv, 6>("spmv"),   method<py_spmm, 6>("spmm"
                          method<py_bspmm, 7>("bspmm"), method<py_bgemm, 3>("bgemm"),
                          method<py_qk_norm_rope, 9>("qk_norm_rope"), method<py_qk_norm_rope_backward, 11>("qk_norm_rope_backward"),
                          method<py_kv_append, 7>("kv_append"), method<py_kv_append_norm_rope, 14>("kv_append_norm_rope"),
-                         method<py_kv_read, 6>("kv_read"), method<py_paged_attention, 8>("paged_attention"), {nullptr, nullptr, 0, nullptr}};
+                         method<py_kv_read, 6>("kv_read"), method<py_paged_attention, 8>("paged_attention"),
+                         method<py_route, 3>("route"), method<py_route_backward, 4>("route_backward"), method<py_expert_lists, 2>("expert_lists"),
+                         method<py_expert_gather, 4>("expert_gather"), method<py_expert_combine, 5>("expert_combine"),
+                         method<py_expert_combine_backward, 6>("expert_combine_backward"), method<py_int4_matmul, 2>("int4_matmul"),
+                         method<py_int4_matmul_lists, 6>("int4_matmul_lists"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "experts.h"
 
@@ -340,6 +341,7 @@ struct RowsArgs {
   int k, experts;
   int64_t items;
   uint32_t chunks;  // items of a row
+  int run;          // of combine: what an item has of them, in turns of its loop
   const int32_t *pos, *place;
   const float *weights;
   void *out;
@@ -396,45 +398,77 @@ __global__ void __launch_bounds__(ROWS_THREADS) gather_kernel(const __grid_const
   }
 }
 
-// A warp an item: a piece a lane of a token's row, COMBINE_ROWS rows asked for at a time.
-constexpr int COMBINE_ROWS = 8;
+// sum += w * piece, and the piece that a sum is rounded to: by words of 32 bits, so that 16-bit elements are taken apart as late as
+// they are used (as members of an array of their own they took 119 registers in place of 64, and half of the rows in flight).
 template <typename T, int V>
-__global__ void __launch_bounds__(ROWS_THREADS) combine_kernel(const __grid_constant__ RowsArgs a) {
+__device__ __forceinline__ void add_piece(float (&sum)[V], float w, const Piece<T, V> &p) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum[v] = fmaf(w, to_f32(p.v[v]), sum[v]);
+}
+__device__ __forceinline__ float2 pair_of(uint32_t word, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&word)); }
+__device__ __forceinline__ float2 pair_of(uint32_t word, __nv_bfloat16) { return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u)); }
+
+// A warp an item: `run` chunks of 32 U pieces of a token's row, J rows asked for at a time.
+template <typename T, int V, int U, int J>
+__global__ void __launch_bounds__(ROWS_THREADS, 4) combine_kernel(const __grid_constant__ RowsArgs a) {
   using P = Piece<T, V>;
+  constexpr int WORDS = sizeof(P) >= 4 ? sizeof(P) / 4 : 1;
+  using W = typename std::conditional<sizeof(P) == 16, uint4, typename std::conditional<sizeof(P) == 4, uint32_t, uint16_t>::type>::type;
   const int lane = threadIdx.x % 32;
   const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
   pdl_release();
   if (item >= a.items) return;
   const int64_t token = divided(item, a.chunks, a.items);
-  const int64_t piece = (item - token * a.chunks) * 32 + lane, pieces = a.dim / V;
+  const int chunk = (int)(item - token * a.chunks), pieces = (int)(a.dim / V);
   const int32_t end = a.pos[a.experts];
-  float sum[V] = {};
-  for (int j0 = 0; j0 < a.k; j0 += 32) {
-    const Place p = j0 + lane < a.k ? place_of(a, token * a.k + j0 + lane, end) : Place{-1, false};
-    const float weight = a.weights != nullptr && p.here ? a.weights[token * a.k + j0 + lane] : 1.0f;
-    for (int j1 = 0; j1 < min(32, a.k - j0); j1 += COMBINE_ROWS) {
-      P got[COMBINE_ROWS];
+  for (int first = chunk * a.run * 32 * U + lane; first - lane < min(pieces, (chunk + 1) * a.run * 32 * U); first += 32 * U) {
+    float sum[U][V] = {};
+    for (int j0 = 0; j0 < a.k; j0 += 32) {
+      const Place p = j0 + lane < a.k ? place_of(a, token * a.k + j0 + lane, end) : Place{-1, false};
+      const int32_t mine = p.here ? p.at : -1;
+      const float weight = a.weights != nullptr && p.here ? a.weights[token * a.k + j0 + lane] : 1.0f;
+      for (int j1 = 0; j1 < min(32, a.k - j0); j1 += J) {
+        W got[J][U];
 #pragma unroll
-      for (int j = 0; j < COMBINE_ROWS; ++j) {
-        const int32_t at = __shfl_sync(0xffffffffu, p.here ? p.at : -1, j1 + j);
-        if (at >= 0 && piece < pieces) got[j] = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + at * a.row_stride)[piece];
-      }
+        for (int j = 0; j < J; ++j) {
+          const int32_t at = __shfl_sync(0xffffffffu, mine, j1 + j);
+          const W *const row = reinterpret_cast<const W *>(static_cast<const T *>(a.rows) + at * a.row_stride);
 #pragma unroll
-      for (int j = 0; j < COMBINE_ROWS; ++j) {
-        const bool here = __shfl_sync(0xffffffffu, p.here, j1 + j);
-        const float w = __shfl_sync(0xffffffffu, weight, j1 + j);
-        if (!here || piece >= pieces) continue;
+          for (int u = 0; u < U; ++u)
+            if (at >= 0 && first + u * 32 < pieces) got[j][u] = row[first + u * 32];
+        }
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] = fmaf(w, to_f32(got[j].v[v]), sum[v]);
+        for (int j = 0; j < J; ++j) {
+          const bool here = __shfl_sync(0xffffffffu, mine, j1 + j) >= 0;
+          const float w = __shfl_sync(0xffffffffu, weight, j1 + j);
+          if (!here) continue;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if constexpr (sizeof(T) == 2 && V > 1) {
+              uint32_t word[WORDS];
+              *reinterpret_cast<W *>(word) = got[j][u];
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) {
+                const float2 x = pair_of(word[i], T());
+                const float2 s = fma2(make_float2(w, w), x, make_float2(sum[u][2 * i], sum[u][2 * i + 1]));
+                sum[u][2 * i] = s.x, sum[u][2 * i + 1] = s.y;
+              }
+            } else {
+              add_piece<T, V>(sum[u], w, *reinterpret_cast<const P *>(&got[j][u]));
+            }
+          }
+        }
       }
     }
-  }
-  if (piece >= pieces) return;
-  P done;
 #pragma unroll
-  for (int v = 0; v < V; ++v) done.v[v] = from_f32<T>(sum[v]);
-  reinterpret_cast<P *>(static_cast<T *>(a.out) + token * a.dim)[piece] = done;
+    for (int u = 0; u < U; ++u) {
+      P done;
+#pragma unroll
+      for (int v = 0; v < V; ++v) done.v[v] = from_f32<T>(sum[u][v]);
+      if (first + u * 32 < pieces) reinterpret_cast<P *>(static_cast<T *>(a.out) + token * a.dim)[first + u * 32] = done;
+    }
+  }
 }
 
 // A warp a slot: its row's product with dout of its token, and its weight times dout.
@@ -485,18 +519,33 @@ __global__ void __launch_bounds__(ROWS_THREADS) combine_backward_kernel(const __
 
 enum RowsOp { GATHER, COMBINE, COMBINE_BACKWARD };
 
+template <typename T, int V, int U, int J>
+static int launch_combine(RowsArgs &a, cudaStream_t st) {
+  constexpr int WARPS = ROWS_THREADS / 32;
+  // A warp looks up a token's places once for several pieces, where there are warps enough for that.
+  const int64_t turns = (a.dim / V + 32 * U - 1) / (32 * U), warps = (int64_t)sm_count() * 128;
+  a.run = (int)std::min<int64_t>(turns, std::max<int64_t>(1, a.tokens * turns / warps));
+  a.chunks = (uint32_t)((turns + a.run - 1) / a.run);
+  a.items = a.tokens * a.chunks;
+  const int64_t blocks = (a.items + WARPS - 1) / WARPS;
+  if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
+  LAPIS_CUDA_TRY(launch_pdl(combine_kernel<T, V, U, J>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
+  return LAPIS_OK;
+}
 template <typename T, int V>
 static int launch_rows_as(RowsOp op, RowsArgs &a, cudaStream_t st) {
   constexpr int WARPS = ROWS_THREADS / 32;
+  if (op == COMBINE) {
+    if constexpr (V == 1) return launch_combine<T, V, 4, 4>(a, st);
+    else return launch_combine<T, V, 4, 1>(a, st);
+  }
   const int64_t lanes = (a.dim / V + 31) / 32;
-  a.chunks = (uint32_t)(op == GATHER ? (lanes + GATHER_PIECES - 1) / GATHER_PIECES : lanes);
+  a.chunks = (uint32_t)((lanes + GATHER_PIECES - 1) / GATHER_PIECES);
   a.items = op == COMBINE_BACKWARD ? a.slots : a.tokens * a.chunks;
   const int64_t blocks = (a.items + WARPS - 1) / WARPS;
   if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
-  const dim3 grid((unsigned)blocks);
-  LAPIS_CUDA_TRY(op == GATHER ? launch_pdl(gather_kernel<T, V>, grid, ROWS_THREADS, 0, st, a)
-                 : op == COMBINE ? launch_pdl(combine_kernel<T, V>, grid, ROWS_THREADS, 0, st, a)
-                                 : launch_pdl(combine_backward_kernel<T, V>, grid, ROWS_THREADS, 0, st, a));
+  LAPIS_CUDA_TRY(op == GATHER ? launch_pdl(gather_kernel<T, V>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a)
+                              : launch_pdl(combine_backward_kernel<T, V>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
   return LAPIS_OK;
 }
 static bool fits(const void *p, int64_t stride, int bytes, int align) { return reinterpret_cast<uintptr_t>(p) % align == 0 && stride * bytes % align == 0; }

@@ -31,14 +31,33 @@ struct RouteArgs {
   void *dlogits;
 };
 
-// Numbers in the order of the logits: NaN above all, -0 as 0.  0 is below all of them: no logit, or one already taken.
+// Numbers in the order of the logits: NaN above all, -0 as 0.  0 is below all of them: no logit.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = x != x ? 0x7fffffffu : __float_as_uint(x + 0.0f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
-constexpr uint32_t KEY_NEVER = 0x007fffffu;  // of -infinity
+template <typename T>
+__device__ __forceinline__ uint32_t key16_of(T x) {
+  if (x != x) return 0xffffu;
+  const uint32_t u = *reinterpret_cast<const uint16_t *>(&x) == 0x8000u ? 0 : *reinterpret_cast<const uint16_t *>(&x);
+  return u & 0x8000u ? u ^ 0xffffu : u | 0x8000u;
+}
+// The logit of a key (of 16-bit ones the upper half), and whether it is one that may be chosen: above -infinity.
+template <typename T>
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  } else {
+    const uint32_t k = key >> 16;
+    const uint16_t u = (uint16_t)(k & 0x8000u ? k ^ 0x8000u : k ^ 0xffffu);
+    return to_f32(*reinterpret_cast<const T *>(&u));
+  }
+}
+template <typename T>
+__device__ __forceinline__ bool is_logit(uint32_t key) {
+  constexpr uint32_t NEVER = sizeof(T) == 4 ? 0x007fffffu : std::is_same<T, __half>::value ? 0x03ffffffu : 0x007fffffu;  // of -infinity, with any number
+  return key > NEVER;
+}
 
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
@@ -51,52 +70,97 @@ __device__ __forceinline__ float warp_max(float x) {
   return x;
 }
 
-// A warp a token; lane l holds logits l, l + 32, ... (32 R of them at most).
+// The two largest keys of a lane that follow the last one taken from it, and their places i (of logits lane + 32 i); of equal keys the
+// lower place comes first.  16-bit logits and their numbers make one key of 32 bits, no two of which are equal.
+template <bool PACKED, int R>
+struct Largest {
+  uint32_t key[2];
+  int at[2];
+  // Those of `all` behind key `last` at place `last_at`, packed ones up to `last`; 0 where there are no more.
+  template <bool FROM_START>
+  __device__ __forceinline__ void find(const uint32_t (&all)[R], uint32_t last, int last_at) {
+    key[0] = key[1] = 0;
+    at[0] = at[1] = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      uint32_t x = all[i];
+      if (!FROM_START && (PACKED ? x > last : x > last || (x == last && i <= last_at))) x = 0;
+      if constexpr (!PACKED) {
+        const bool first = x > key[0], second = x > key[1];
+        at[1] = first ? at[0] : second ? i : at[1];
+        at[0] = first ? i : at[0];
+      }
+      key[1] = max(key[1], min(key[0], x));
+      key[0] = max(key[0], x);
+    }
+  }
+};
+
+// A warp a token; lane l holds logits l, l + 32, ... (32 R of them at most).  A turn takes the largest key of the warp; its lane goes on to
+// its second, and only when that is taken too looks through its logits again, which of 8 among 256 happens about once a token.
+// Bound by the instructions on 32 bits, one every two cycles: 16,384 x 256 with a look in every turn took 15.4 us.
 template <typename T, int R>
 __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const __grid_constant__ RouteArgs a) {
+  constexpr bool PACKED = sizeof(T) == 2;
   const int lane = threadIdx.x % 32;
   const int64_t token = (int64_t)blockIdx.x * (ROUTE_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
   pdl_release();
   if (token >= a.tokens) return;
   const T *const logits = static_cast<const T *>(a.logits) + token * a.token_stride;
-  uint32_t key[R], most = 0;
+  T given[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) given[i] = lane + 32 * i < a.experts ? logits[lane + 32 * i] : from_f32<T>(0.0f);
+  uint32_t key[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    key[i] = lane + 32 * i < a.experts ? key_of(to_f32(logits[lane + 32 * i])) : 0;
-    most = max(most, key[i]);
+    if constexpr (PACKED) key[i] = key16_of<T>(given[i]) << 16 | (0xffffu - (lane + 32 * i));
+    else key[i] = key_of(given[i]);
+    if (lane + 32 * i >= a.experts) key[i] = 0;
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  const float top = logit_of(most);
+  Largest<PACKED, R> mine;
+  mine.template find<true>(key, 0, 0);
+  int left = 2;  // of `mine`
+  uint32_t most = __reduce_max_sync(0xffffffffu, mine.key[0]);
+  const float top = logit_of<T>(most);
   float total = 0.0f;
   if (!a.normalise) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) total += key[i] > KEY_NEVER ? expf(logit_of(key[i]) - top) : 0.0f;
+    for (int i = 0; i < R; ++i) total += is_logit<T>(key[i]) ? expf(to_f32(given[i]) - top) : 0.0f;
     total = warp_sum(total);
   }
-  float mine = 0.0f;  // of the lane's choice, the lane-th largest
+  uint32_t taken = 0;  // the key of the lane's choice, the lane-th largest
   int expert = -1;
-  for (int j = 0; j < a.k && most > KEY_NEVER; ++j) {
-    int at = 32 * R;
-#pragma unroll
-    for (int i = R - 1; i >= 0; --i)
-      if (key[i] == most) at = lane + 32 * i;
-    at = __reduce_min_sync(0xffffffffu, at);
+  for (int j = 0; j < a.k && is_logit<T>(most); ++j) {
+    int number;
+    if constexpr (PACKED) {
+      number = 0xffff - (int)(most & 0xffffu);
+    } else {
+      const uint32_t lanes = __ballot_sync(0xffffffffu, mine.key[0] == most);
+      const int here = lane + 32 * mine.at[0];
+      number = (lanes & (lanes - 1)) == 0 ? __shfl_sync(0xffffffffu, here, __ffs(lanes) - 1) : __reduce_min_sync(0xffffffffu, mine.key[0] == most ? here : 32 * R);
+    }
     if (lane == j) {
-      mine = expf(logit_of(most) - top);
-      expert = at;
+      taken = most;
+      expert = number;
     }
-    most = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (at == lane + 32 * i) key[i] = 0;
-      most = max(most, key[i]);
+    const bool won = number % 32 == lane;
+    if (won) --left;
+    if (__any_sync(0xffffffffu, left == 0)) {
+      if (left == 0) {
+        mine.template find<false>(key, PACKED ? most - 1 : most, number / 32);
+        left = 2;
+      }
+    } else if (won) {
+      mine.key[0] = mine.key[1];
+      mine.at[0] = mine.at[1];
     }
-    most = __reduce_max_sync(0xffffffffu, most);
+    most = __reduce_max_sync(0xffffffffu, mine.key[0]);
   }
-  if (a.normalise) total = warp_sum(mine);
+  const float weight = expert < 0 ? 0.0f : expf(logit_of<T>(taken) - top);
+  if (a.normalise) total = warp_sum(weight);
   if (lane < a.k) {
-    a.weights[token * a.k + lane] = expert < 0 ? 0.0f : mine / total;
+    a.weights[token * a.k + lane] = expert < 0 ? 0.0f : weight / total;
     a.expert[token * a.k + lane] = expert;
   }
 }
@@ -317,13 +381,18 @@ static int launch_lists_as(ListArgs &a, cudaStream_t st) {
     LAPIS_CUDA_TRY(launch_pdl(list_count_kernel<S>, dim3(a.blocks), LIST_THREADS, buckets * sizeof(uint32_t), st, a));
   }
   const size_t smem = (LIST_WARPS + 2) * buckets * sizeof(uint32_t);
-  LAPIS_CUDA_TRY(cudaFuncSetAttribute(list_place_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)((LIST_WARPS + 2) * (MAX_EXPERTS + 1) * sizeof(uint32_t))));
+  LAPIS_TRY(allow_smem<list_place_kernel<S>>((int)((LIST_WARPS + 2) * (MAX_EXPERTS + 1) * sizeof(uint32_t))));
   LAPIS_CUDA_TRY(launch_pdl(list_place_kernel<S>, dim3(a.blocks), LIST_THREADS, smem, st, a));
   return LAPIS_OK;
 }
 static int launch_lists(ListArgs &a, cudaStream_t st) {
+  // One block, where its turns take less than a second launch.
+  if (a.slots <= LIST_THREADS) return launch_lists_as<1>(a, st);
+  if (a.slots <= 2 * LIST_THREADS) return launch_lists_as<2>(a, st);
+  if (a.slots <= 4 * LIST_THREADS) return launch_lists_as<4>(a, st);
+  if (a.slots <= 8 * LIST_THREADS) return launch_lists_as<8>(a, st);
   const int64_t all = a.slots / sm_count();
-  if (a.slots <= LIST_THREADS || all <= LIST_THREADS) return launch_lists_as<1>(a, st);
+  if (all <= LIST_THREADS) return launch_lists_as<1>(a, st);
   if (all <= 2 * LIST_THREADS) return launch_lists_as<2>(a, st);
   if (all <= 4 * LIST_THREADS) return launch_lists_as<4>(a, st);
   if (all <= 8 * LIST_THREADS) return launch_lists_as<8>(a, st);
@@ -398,45 +467,149 @@ __global__ void __launch_bounds__(ROWS_THREADS) gather_kernel(const __grid_const
   }
 }
 
-// sum += w * piece, and the piece that a sum is rounded to: by words of 32 bits, so that 16-bit elements are taken apart as late as
-// they are used (as members of an array of their own they took 119 registers in place of 64, and half of the rows in flight).
-template <typename T, int V>
-__device__ __forceinline__ void add_piece(float (&sum)[V], float w, const Piece<T, V> &p) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum[v] = fmaf(w, to_f32(p.v[v]), sum[v]);
-}
 __device__ __forceinline__ float2 pair_of(uint32_t word, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&word)); }
 __device__ __forceinline__ float2 pair_of(uint32_t word, __nv_bfloat16) { return make_float2(__uint_as_float(word << 16), __uint_as_float(word & 0xffff0000u)); }
 
-// A warp an item: `run` chunks of 32 U pieces of a token's row, J rows asked for at a time.
-template <typename T, int V, int U, int J>
+// Rows of 16-byte pieces.  A warp takes (token, chunk) after (token, chunk); for each it needs J rows at a time, C pieces a lane of each,
+// which come by cp.async into a ring of its own: every lane copies what it will add, so that nothing but its own copies is waited for.
+// Bound by memory.  What it takes is bytes in flight: rows of eight places a token, 16 warps an SM with 8 KB each on their way.
+constexpr int RING_STAGES = 3, RING_WARPS = 8;
+template <typename T, int J>
+__global__ void __launch_bounds__(32 * RING_WARPS, 2) combine_ring_kernel(const __grid_constant__ RowsArgs a) {
+  constexpr int C = 8 / J, V = 16 / sizeof(T), STAGE = 32 * 8 * 16;
+  extern __shared__ __align__(16) uint8_t rings[];
+  __shared__ float weight_of[RING_WARPS][RING_STAGES][J];
+  __shared__ uint32_t here_of[RING_WARPS][RING_STAGES];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  uint8_t *const ring = rings + warp * RING_STAGES * STAGE + lane * 16;
+  const int64_t step = (int64_t)gridDim.x * RING_WARPS;
+  const int pieces = (int)(a.dim / V);
+  pdl_wait();
+  pdl_release();
+  const int32_t end = a.pos[a.experts];
+
+  struct Unit {  // rows j0 to j0 + J - 1 of a token's chunk
+    int64_t item, token;
+    int j0, first;
+  };
+  const auto place = [&](Unit &u) {
+    if (u.item >= a.items) return;
+    u.token = divided(u.item, a.chunks, a.items);
+    u.first = (int)(u.item - u.token * a.chunks) * (32 * C) + lane;
+  };
+  const auto advance = [&](Unit &u) {
+    u.j0 += J;
+    if (u.j0 < a.k) return;
+    u.j0 = 0;
+    u.item += step;
+    place(u);
+  };
+  Unit next = {(int64_t)blockIdx.x * RING_WARPS + warp, 0, 0, 0}, now = next;
+  place(next);
+  now = next;
+  int32_t at = -1;  // of the next unit: the lane's row, or -1, and its weight
+  float w = 1.0f;
+  const auto look = [&] {
+    at = -1;
+    if (next.item >= a.items || lane >= J || next.j0 + lane >= a.k) return;
+    const int64_t slot = next.token * a.k + next.j0 + lane;
+    const Place p = place_of(a, slot, end);
+    at = p.here ? p.at : -1;
+    if (a.weights != nullptr) w = a.weights[slot];
+  };
+  const auto ask = [&](int stage) {
+    if (next.item < a.items) {
+      const uint32_t here = __ballot_sync(0xffffffffu, at >= 0);
+      if (lane < J) weight_of[warp][stage][lane] = w;
+      if (lane == 0) here_of[warp][stage] = here;
+      const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + stage * STAGE);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int32_t row = __shfl_sync(0xffffffffu, at, j);
+        const uint4 *const from = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.rows) + row * a.row_stride) + next.first;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (row >= 0 && next.first + c * 32 < pieces)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (j * C + c) * 512), "l"(from + c * 32) : "memory");
+      }
+      advance(next);
+      look();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look();
+#pragma unroll
+  for (int s = 0; s < RING_STAGES - 1; ++s) ask(s);
+  float2 sum[C][V / 2] = {};
+  for (int stage = 0; now.item < a.items; stage = stage == RING_STAGES - 1 ? 0 : stage + 1) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING_STAGES - 2) : "memory");
+    __syncwarp();
+    const uint32_t here = here_of[warp][stage];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (!(here >> j & 1)) continue;
+      const float wj = weight_of[warp][stage][j];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(ring + stage * STAGE + (j * C + c) * 512);
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          float2 x;
+          if constexpr (sizeof(T) == 2) x = pair_of(words[i], T());
+          else x = make_float2(__uint_as_float(words[2 * i]), __uint_as_float(words[2 * i + 1]));
+          sum[c][i] = fma2(make_float2(wj, wj), x, sum[c][i]);
+        }
+      }
+    }
+    if (now.j0 + J >= a.k) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        Piece<T, V> done;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          done.v[2 * i] = from_f32<T>(sum[c][i].x);
+          done.v[2 * i + 1] = from_f32<T>(sum[c][i].y);
+          sum[c][i] = make_float2(0.0f, 0.0f);
+        }
+        if (now.first + c * 32 < pieces) reinterpret_cast<Piece<T, V> *>(static_cast<T *>(a.out) + now.token * a.dim)[now.first + c * 32] = done;
+      }
+    }
+    advance(now);
+    __syncwarp();  // here_of and weight_of of the stage in front, which is asked into now, have been read
+    ask(stage == 0 ? RING_STAGES - 1 : stage - 1);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Rows of any alignment.  A warp an item: `run` chunks of 32 U elements of a token's row, J rows asked for at a time.
+template <typename T, int U, int J>
 __global__ void __launch_bounds__(ROWS_THREADS, 4) combine_kernel(const __grid_constant__ RowsArgs a) {
-  using P = Piece<T, V>;
-  constexpr int WORDS = sizeof(P) >= 4 ? sizeof(P) / 4 : 1;
-  using W = typename std::conditional<sizeof(P) == 16, uint4, typename std::conditional<sizeof(P) == 4, uint32_t, uint16_t>::type>::type;
   const int lane = threadIdx.x % 32;
   const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
   pdl_release();
   if (item >= a.items) return;
   const int64_t token = divided(item, a.chunks, a.items);
-  const int chunk = (int)(item - token * a.chunks), pieces = (int)(a.dim / V);
+  const int chunk = (int)(item - token * a.chunks), dim = (int)a.dim;
   const int32_t end = a.pos[a.experts];
-  for (int first = chunk * a.run * 32 * U + lane; first - lane < min(pieces, (chunk + 1) * a.run * 32 * U); first += 32 * U) {
-    float sum[U][V] = {};
+  const uint32_t upto = min((uint32_t)dim, (uint32_t)(chunk + 1) * a.run * 32 * U);
+  for (uint32_t from = (uint32_t)chunk * a.run * 32 * U; from < upto; from += 32 * U) {
+    const int first = (int)from + lane;
+    float sum[U] = {};
     for (int j0 = 0; j0 < a.k; j0 += 32) {
       const Place p = j0 + lane < a.k ? place_of(a, token * a.k + j0 + lane, end) : Place{-1, false};
       const int32_t mine = p.here ? p.at : -1;
       const float weight = a.weights != nullptr && p.here ? a.weights[token * a.k + j0 + lane] : 1.0f;
       for (int j1 = 0; j1 < min(32, a.k - j0); j1 += J) {
-        W got[J][U];
+        T got[J][U];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const int32_t at = __shfl_sync(0xffffffffu, mine, j1 + j);
-          const W *const row = reinterpret_cast<const W *>(static_cast<const T *>(a.rows) + at * a.row_stride);
+          const T *const row = static_cast<const T *>(a.rows) + at * a.row_stride;
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (at >= 0 && first + u * 32 < pieces) got[j][u] = row[first + u * 32];
+            if (at >= 0 && first + u * 32 < dim) got[j][u] = row[first + u * 32];
         }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -444,30 +617,13 @@ __global__ void __launch_bounds__(ROWS_THREADS, 4) combine_kernel(const __grid_c
           const float w = __shfl_sync(0xffffffffu, weight, j1 + j);
           if (!here) continue;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if constexpr (sizeof(T) == 2 && V > 1) {
-              uint32_t word[WORDS];
-              *reinterpret_cast<W *>(word) = got[j][u];
-#pragma unroll
-              for (int i = 0; i < WORDS; ++i) {
-                const float2 x = pair_of(word[i], T());
-                const float2 s = fma2(make_float2(w, w), x, make_float2(sum[u][2 * i], sum[u][2 * i + 1]));
-                sum[u][2 * i] = s.x, sum[u][2 * i + 1] = s.y;
-              }
-            } else {
-              add_piece<T, V>(sum[u], w, *reinterpret_cast<const P *>(&got[j][u]));
-            }
-          }
+          for (int u = 0; u < U; ++u) sum[u] = fmaf(w, to_f32(got[j][u]), sum[u]);
         }
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      P done;
-#pragma unroll
-      for (int v = 0; v < V; ++v) done.v[v] = from_f32<T>(sum[u][v]);
-      if (first + u * 32 < pieces) reinterpret_cast<P *>(static_cast<T *>(a.out) + token * a.dim)[first + u * 32] = done;
-    }
+    for (int u = 0; u < U; ++u)
+      if (first + u * 32 < dim) static_cast<T *>(a.out)[token * a.dim + first + u * 32] = from_f32<T>(sum[u]);
   }
 }
 
@@ -519,26 +675,35 @@ __global__ void __launch_bounds__(ROWS_THREADS) combine_backward_kernel(const __
 
 enum RowsOp { GATHER, COMBINE, COMBINE_BACKWARD };
 
-template <typename T, int V, int U, int J>
+template <typename T, int J>
+static int launch_ring(RowsArgs &a, cudaStream_t st) {
+  const int64_t lanes = (a.dim * (int)sizeof(T) / 16 + 31) / 32;
+  a.chunks = (uint32_t)((lanes + 8 / J - 1) / (8 / J));
+  a.items = a.tokens * a.chunks;
+  const int smem = RING_WARPS * RING_STAGES * 32 * 8 * 16;
+  LAPIS_TRY((allow_smem<combine_ring_kernel<T, J>>(smem)));
+  const int64_t blocks = std::min<int64_t>(2 * sm_count(), (a.items + RING_WARPS - 1) / RING_WARPS);
+  LAPIS_CUDA_TRY(launch_pdl(combine_ring_kernel<T, J>, dim3((unsigned)blocks), 32 * RING_WARPS, smem, st, a));
+  return LAPIS_OK;
+}
+template <typename T, int V>
 static int launch_combine(RowsArgs &a, cudaStream_t st) {
-  constexpr int WARPS = ROWS_THREADS / 32;
+  if constexpr (V > 1) return a.k <= 1 ? launch_ring<T, 1>(a, st) : a.k <= 2 ? launch_ring<T, 2>(a, st) : launch_ring<T, 4>(a, st);
+  constexpr int WARPS = ROWS_THREADS / 32, U = 4;
   // A warp looks up a token's places once for several pieces, where there are warps enough for that.
-  const int64_t turns = (a.dim / V + 32 * U - 1) / (32 * U), warps = (int64_t)sm_count() * 128;
+  const int64_t turns = (a.dim + 32 * U - 1) / (32 * U), warps = (int64_t)sm_count() * 128;
   a.run = (int)std::min<int64_t>(turns, std::max<int64_t>(1, a.tokens * turns / warps));
   a.chunks = (uint32_t)((turns + a.run - 1) / a.run);
   a.items = a.tokens * a.chunks;
   const int64_t blocks = (a.items + WARPS - 1) / WARPS;
   if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
-  LAPIS_CUDA_TRY(launch_pdl(combine_kernel<T, V, U, J>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
+  LAPIS_CUDA_TRY(launch_pdl(combine_kernel<T, U, 4>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
   return LAPIS_OK;
 }
 template <typename T, int V>
 static int launch_rows_as(RowsOp op, RowsArgs &a, cudaStream_t st) {
   constexpr int WARPS = ROWS_THREADS / 32;
-  if (op == COMBINE) {
-    if constexpr (V == 1) return launch_combine<T, V, 4, 4>(a, st);
-    else return launch_combine<T, V, 4, 1>(a, st);
-  }
+  if (op == COMBINE) return launch_combine<T, V>(a, st);
   const int64_t lanes = (a.dim / V + 31) / 32;
   a.chunks = (uint32_t)((lanes + GATHER_PIECES - 1) / GATHER_PIECES);
   a.items = op == COMBINE_BACKWARD ? a.slots : a.tokens * a.chunks;

@@ -436,7 +436,7 @@ struct alignas(sizeof(T) * V) Piece {
 };
 
 // A warp an item: GATHER_PIECES pieces a lane of a token's row, read once and written k times.
-constexpr int GATHER_PIECES = 4;
+constexpr int GATHER_PIECES = 2;  // 16,384 x 8 rows of 2048 106.9 us, with 4 108.5, with 8 108.8; 40 x 4 rows 2.7 us, 3.3, 4.3
 template <typename T, int V>
 __global__ void __launch_bounds__(ROWS_THREADS) gather_kernel(const __grid_constant__ RowsArgs a) {
   using P = Piece<T, V>;
@@ -627,25 +627,36 @@ __global__ void __launch_bounds__(ROWS_THREADS, 4) combine_kernel(const __grid_c
   }
 }
 
-// A warp a slot: its row's product with dout of its token, and its weight times dout.
-constexpr int BACK_PIECES = 4;
+__device__ __forceinline__ uint32_t word_of(float2 x, __half) {
+  const __half2 h = __float22half2_rn(x);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t word_of(float2 x, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(x);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// A warp a slot: its row's product with dout of its token, and its weight times dout.  16-bit pieces stay words until they are used: as
+// arrays of elements they took 89 registers, and the warps that memory needs did not fit.
+constexpr int BACK_PIECES = 4, BACK_BLOCKS = 4;  // 8192 x 6 rows of 5120 164 us; 5 blocks an SM (spills) 169, 2 pieces 167
 template <typename T, int V>
-__global__ void __launch_bounds__(ROWS_THREADS) combine_backward_kernel(const __grid_constant__ RowsArgs a) {
-  using P = Piece<T, V>;
+__global__ void __launch_bounds__(ROWS_THREADS, BACK_BLOCKS) combine_backward_kernel(const __grid_constant__ RowsArgs a) {
+  using P = typename std::conditional<V == 1, T, uint4>::type;
   const int lane = threadIdx.x % 32;
   const int64_t slot = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
   pdl_release();
   if (slot >= a.slots) return;
-  const int64_t token = divided(slot, a.k, a.slots), pieces = a.dim / V;
+  const int64_t token = divided(slot, a.k, a.slots);
+  const int pieces = (int)(a.dim / V);
   const Place p = place_of(a, slot, a.pos[a.experts]);
-  const P *const dout = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + token * a.x_stride);
-  const P *const row = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + p.at * a.row_stride);
-  P *const to = reinterpret_cast<P *>(static_cast<T *>(a.out) + p.at * a.dim);
-  float dot = 0.0f;
+  P *const to = reinterpret_cast<P *>(static_cast<T *>(a.out) + max(p.at, 0) * a.dim);
+  float2 dot = make_float2(0.0f, 0.0f);
   if (p.here) {
+    const P *const dout = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + token * a.x_stride);
+    const P *const row = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + p.at * a.row_stride);
     const float w = a.weights[slot];
-    for (int64_t first = lane; first < pieces; first += 32 * BACK_PIECES) {
+    for (int first = lane; first < pieces; first += 32 * BACK_PIECES) {
       P d[BACK_PIECES], r[BACK_PIECES];
 #pragma unroll
       for (int u = 0; u < BACK_PIECES; ++u)
@@ -654,23 +665,39 @@ __global__ void __launch_bounds__(ROWS_THREADS) combine_backward_kernel(const __
           r[u] = row[first + u * 32];
         }
 #pragma unroll
-      for (int u = 0; u < BACK_PIECES; ++u)
-        if (first + u * 32 < pieces) {
-          P done;
+      for (int u = 0; u < BACK_PIECES; ++u) {
+        if (first + u * 32 >= pieces) continue;
+        if constexpr (V == 1) {
+          dot.x = fmaf(to_f32(d[u]), to_f32(r[u]), dot.x);
+          to[first + u * 32] = from_f32<T>(w * to_f32(d[u]));
+        } else {
+          const uint32_t dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w}, rw[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+          uint32_t out[4];
+          if constexpr (sizeof(T) == 2) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float x = to_f32(d[u].v[v]);
-            dot = fmaf(x, to_f32(r[u].v[v]), dot);
-            done.v[v] = from_f32<T>(w * x);
+            for (int i = 0; i < 4; ++i) {
+              const float2 x = pair_of(dw[i], T());
+              dot = fma2(x, pair_of(rw[i], T()), dot);
+              out[i] = word_of(mul2(make_float2(w, w), x), T());
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const float2 x = make_float2(__uint_as_float(dw[i]), __uint_as_float(dw[i + 1]));
+              dot = fma2(x, make_float2(__uint_as_float(rw[i]), __uint_as_float(rw[i + 1])), dot);
+              const float2 y = mul2(make_float2(w, w), x);
+              out[i] = __float_as_uint(y.x), out[i + 1] = __float_as_uint(y.y);
+            }
           }
-          to[first + u * 32] = done;
+          to[first + u * 32] = make_uint4(out[0], out[1], out[2], out[3]);
         }
+      }
     }
   } else if (p.at >= 0) {
-    for (int64_t i = lane; i < pieces; i += 32) to[i] = P{};
+    for (int i = lane; i < pieces; i += 32) to[i] = P{};
   }
-  dot = warp_sum(dot);
-  if (lane == 0) a.dweights[slot] = dot;
+  const float all = warp_sum(dot.x + dot.y);
+  if (lane == 0) a.dweights[slot] = all;
 }
 
 enum RowsOp { GATHER, COMBINE, COMBINE_BACKWARD };
@@ -742,7 +769,7 @@ static int check_rows(const char *what, int type, int64_t dim, const lapis_b200_
   if (!is_float_type(type)) return fail(LAPIS_EBADARG, "%s: type must be LAPIS_F32, LAPIS_F16 or LAPIS_BF16", what);
   LAPIS_TRY(check_expert_lists(what, lists));
   if (dim < 0) return fail(LAPIS_EBADSHAPE, "%s: negative size", what);
-  if (dim > 0x7fffffff) return fail(LAPIS_ETOOBIG, "%s: rows of 2^31 elements or more", what);
+  if (dim > 1 << 30) return fail(LAPIS_ETOOBIG, "%s: rows of more than 2^30 elements", what);
   return LAPIS_OK;
 }
 static RowsArgs rows_args(int64_t dim, const lapis_b200_expert_lists *l) {

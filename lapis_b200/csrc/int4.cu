@@ -7,9 +7,9 @@
 // is rounded once.  With `gated` outputs the two halves of the result meet in a lane, silu(gate) * up, in 32 bits.
 //
 // The work is to read the weights once.  They lie in the order in which a warp takes them: a strip of 16 outputs, 64 columns of
-// it in one 16-byte load a lane, which is the A operand of four products of 16 x 8 x 16.  The rows x are the B operand, from
-// shared memory.  The columns of a product may come in any order, the same for A and B: the lane of a row takes 8 that lie
-// next to one another in each half of the 64, so that it has its part of x in two 16-byte loads.
+// it in one 16-byte load a lane, which is the A operand of four products of 16 x 8 x 16 (int4_few.cu) or, converted, of a warp's store to
+// tensor memory (int4_many.cu).  The columns of a product may come in any order, the same for A and B: the lane of a row takes 8 that
+// lie next to one another in each half of the 64.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -305,5 +305,5 @@ extern "C" int lapis_b200_int4_matmul(int type, const lapis_b200_int4 *w, int64_
   // Lists are ragged: most have no more than twice the mean.
   const int64_t expected = lists == nullptr ? a.rows : std::min(a.rows, 2 * ((a.rows + a.experts - 1) / a.experts));
   const bool few = expected * (type == LAPIS_F32 ? 3 : 1) <= FEW_COLUMNS;
-  return few ? launch_few(type, a, w->group, matrices, expected, st) : launch_many(type, a, w->group, matrices, expected, st);
+  return few ? launch_few(type, a, w->group, matrices, st) : launch_many(type, a, w->group, matrices, expected, st);
 }

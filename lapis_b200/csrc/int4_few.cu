@@ -1,4 +1,10 @@
-// Products of few rows with 4-bit weights (int4.cu) on mma.sync: the weights as fast as they come from memory.
+// Products of few rows with 4-bit weights (int4.cu) on mma.sync: 8 columns of the product, 16 outputs a warp.
+//
+// The weights go from memory to registers, a batch ahead, and need nothing but their own warp; the rows x, the B operand, are in shared
+// memory.  What bounds it are the instructions on 32 bits that make numbers of codes: of one every two cycles a batch of 16 x 256 takes 150 to
+// 190, its bytes as long as 170.  48 x 8 rows over 128 experts (2048 x 2048, groups of 32, gated) 79 us, 3.7 TB/s; one row times 14,336 x 4096 12.1 us,
+// 2.5 TB/s; 4096 x 4096 7.2 us, most of it launch and latency.  tcgen05 (int4_many.cu) with 8 columns would convert as many codes and add its
+// hand-overs: 16 rows take it 23 us where 8 take this 18.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -10,11 +16,11 @@ namespace lapis_b200 {
 template <typename T>
 __device__ __forceinline__ void multiply(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -22,11 +28,11 @@ __device__ __forceinline__ void multiply(float (&d)[4], uint32_t a0, uint32_t a1
 template <typename T>
 __device__ __forceinline__ void multiply_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
@@ -75,7 +81,9 @@ struct Batch {
 constexpr int SUM_PITCH = STRIP + 1;
 
 constexpr int FEW_WARPS_LOG = 2, FEW_WARPS = 1 << FEW_WARPS_LOG, FEW_THREADS = 32 * FEW_WARPS;
-constexpr int FEW_BLOCKS = 5, FEW_ROOM = 40 << 10;  // blocks of an SM, and the rows x of each in shared memory
+// Blocks of an SM, and the rows x of each in shared memory.  The registers of a sixth block are missing in the loop: 48 x 8 rows over 128
+// experts take 79 us with 5 blocks, 82 with 4, 99 with 6; with two of eight warps 87.
+constexpr int FEW_BLOCKS = 5, FEW_ROOM = 40 << 10;
 
 // Bytes of a row of x in shared memory: neighbouring rows' pieces of a phase lie on different banks.
 __host__ __device__ constexpr int few_pitch(int columns) { return columns * 2 + 64; }
@@ -173,11 +181,10 @@ struct Way {
   }
 };
 
-// sum += the product of the batch that `way` is at with the rows x, whose lane's pieces begin at x_at.
-template <typename T, int GROUP, int NT, bool ZEROS>
-__device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum)[NT][4], Way<GROUP, ZEROS> &way, const uint8_t *x, const int (&x_at)[NT], int tiles,
-                                               int lane) {
-  float part[NT][4];
+// sum += the product of the batch that `way` is at with the rows x, of which the lane's pieces begin at x.
+template <typename T, int GROUP, bool ZEROS>
+__device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum)[4], Way<GROUP, ZEROS> &way, const uint8_t *x, int lane) {
+  float part[4];
   way.enter(a, lane);
 #pragma unroll
   for (int half = 0; half < 2 * BATCH / BLOCK; ++half) {
@@ -190,32 +197,24 @@ __device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum
     pairs_of(p0, half % 2 ? c.y : c.x, z0);
     pairs_of(p1, half % 2 ? c.w : c.z, z1);
     if (half % 2 == 1) way.ask(half / 2);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (t > 0 && t >= tiles) break;
-      const uint4 v = *reinterpret_cast<const uint4 *>(x + x_at[t] + half * 64);
-      if (half * 32 % GROUP == 0) multiply_first<T>(part[t], p0[0], p1[0], p0[1], p1[1], v.x, v.y);
-      else multiply<T>(part[t], p0[0], p1[0], p0[1], p1[1], v.x, v.y);
-      multiply<T>(part[t], p0[2], p1[2], p0[3], p1[3], v.z, v.w);
-    }
+    const uint4 v = *reinterpret_cast<const uint4 *>(x + half * 64);
+    if (half * 32 % GROUP == 0) multiply_first<T>(part, p0[0], p1[0], p0[1], p1[1], v.x, v.y);
+    else multiply<T>(part, p0[0], p1[0], p0[1], p1[1], v.x, v.y);
+    multiply<T>(part, p0[2], p1[2], p0[3], p1[3], v.z, v.w);
     if ((half + 1) * 32 % GROUP == 0) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if (t > 0 && t >= tiles) break;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[t][i] = fmaf(way.scale[i / 2][g], part[t][i], sum[t][i]);
-      }
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(way.scale[i / 2][g], part[i], sum[i]);
     }
   }
   way.advance();
 }
 
 // A block's warps are strips times shares of the columns, both powers of two.  A warp takes its batches of a strip one after the
-// other, two more on their way to its registers; the rows x are in shared memory, all of their columns where they fit.
-template <typename X, int GROUP, int NT, bool ZEROS>
+// other, the next on its way to its registers; the rows x are in shared memory, all of their columns where they fit.
+template <typename X, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const __grid_constant__ ProductArgs a) {
   using T = typename std::conditional<std::is_same<X, float>::value, __nv_bfloat16, X>::type;
-  constexpr int A_ROW = std::is_same<X, float>::value ? 3 : 1, ROWS = 8 * NT / A_ROW;
+  constexpr int A_ROW = std::is_same<X, float>::value ? 3 : 1, ROWS = FEW_COLUMNS / A_ROW;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ const X *row_at[ROWS];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
     }
   }
   for (int64_t row0 = begin; row0 < end; row0 += a.rows_a_pass) {
-    const int rows = (int)min((int64_t)a.rows_a_pass, end - row0), tiles = (rows * A_ROW + 7) / 8;
+    const int rows = (int)min((int64_t)a.rows_a_pass, end - row0);
     if (!early || row0 != begin) way.begin(a, of_all, my_share, shares, lane);
     if (threadIdx.x < rows) {
       int64_t from = row0 + threadIdx.x;
@@ -253,34 +252,27 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
       row_at[threadIdx.x] = (uint64_t)from < (uint64_t)a.x_rows ? static_cast<const X *>(a.x) + from * a.x_stride : nullptr;
     }
     // Columns of the product beyond the rows take the first row's values: nobody looks at them.
-    int x_at[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int n = t * 8 + lane / 4;
-      x_at[t] = (n < rows * A_ROW ? n : 0) * pitch + lane % 4 * 16;
-    }
-    float sum[NT][4] = {};
+    const uint8_t *const x = smem + (lane / 4 < rows * A_ROW ? lane / 4 : 0) * pitch + lane % 4 * 16;
+    float sum[4] = {};
     const int step = a.chunk / BATCH;  // a multiple of the shares
     for (int b0 = 0; b0 < a.batches; b0 += step) {
       __syncthreads();
       stage_few<X>(a, smem, row_at, rows, b0 * BATCH, min(a.chunk, (a.batches - b0) * BATCH), pitch);
       __syncthreads();
       for (int b = b0 + my_share; b < min(b0 + step, batches); b += shares)
-        multiply_batch<T, GROUP, NT, ZEROS>(a, sum, way, smem + (b - b0) * (BATCH * 2), x_at, tiles, lane);
+        multiply_batch<T, GROUP, ZEROS>(a, sum, way, x + (b - b0) * (BATCH * 2), lane);
     }
     // The shares' sums meet in shared memory: [share][strip][column][row].
     float *const sums = reinterpret_cast<float *>(smem);
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[(warp * 8 * NT + t * 8 + lane % 4 * 2 + i % 2) * SUM_PITCH + lane / 4 + i / 2 * 8] = sum[t][i];
+    for (int i = 0; i < 4; ++i) sums[(warp * FEW_COLUMNS + lane % 4 * 2 + i % 2) * SUM_PITCH + lane / 4 + i / 2 * 8] = sum[i];
     __syncthreads();
     const auto total = [&](int s, int r, int n) {
       float v = 0.0f;
 #pragma unroll
       for (int p = A_ROW - 1; p >= 0; --p)  // the small parts first
-        for (int share = 0; share < shares; ++share) v += sums[(((share << strips_log) + s) * 8 * NT + r * A_ROW + p) * SUM_PITCH + n];
+        for (int share = 0; share < shares; ++share) v += sums[(((share << strips_log) + s) * FEW_COLUMNS + r * A_ROW + p) * SUM_PITCH + n];
       return v;
     };
     for (int i = threadIdx.x; i < rows << (strips_log + outs_log); i += FEW_THREADS) {
@@ -294,35 +286,37 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
   }
 }
 
-template <typename X, int GROUP, int NT>
+template <typename X, int GROUP>
 static int launch_few_as(ProductArgs &a, int matrices, cudaStream_t st) {
   constexpr int A_ROW = std::is_same<X, float>::value ? 3 : 1;
-  a.rows_a_pass = (int)std::min<int64_t>(a.rows, 8 * NT / A_ROW);
+  a.rows_a_pass = (int)std::min<int64_t>(a.rows, FEW_COLUMNS / A_ROW);
   a.strips_log = 0;
+  // Warps that take whole strips share the rows x, warps that share a strip fill the GPU: as many strips as leave four blocks an SM.  14,336 x
+  // 4096 (896 strips), one row: a strip a block 12.4 us, two 15.0; 128 experts of 128 strips: a strip 127 us, two 95, four 85.
   while (a.strips_log < FEW_WARPS_LOG && (int64_t)(a.strips >> (1 + a.strips_log)) * a.experts >= 4 * sm_count()) ++a.strips_log;
-  const int strips = 1 << a.strips_log, turn = BATCH * (FEW_WARPS >> a.strips_log), room = FEW_ROOM;
-  a.chunk = std::max(turn, (room / (a.rows_a_pass * A_ROW) - 64) / 2 / turn * turn);
+  const int strips = 1 << a.strips_log, turn = BATCH * (FEW_WARPS >> a.strips_log);
+  a.chunk = std::max(turn, (FEW_ROOM / (a.rows_a_pass * A_ROW) - 64) / 2 / turn * turn);
   a.chunk = (int)std::min<int64_t>(a.chunk, (a.columns + turn - 1) / turn * turn);
-  const int smem = std::max(a.rows_a_pass * A_ROW * few_pitch(a.chunk), FEW_WARPS * 8 * NT * SUM_PITCH * 4);
+  const int smem = std::max(a.rows_a_pass * A_ROW * few_pitch(a.chunk), FEW_WARPS * FEW_COLUMNS * SUM_PITCH * 4);
   const dim3 grid((a.strips + strips - 1) / strips, matrices);
-  LAPIS_TRY(a.zeros_at ? (allow_smem<int4_few_kernel<X, GROUP, NT, true>>(160 << 10)) : (allow_smem<int4_few_kernel<X, GROUP, NT, false>>(160 << 10)));
-  LAPIS_CUDA_TRY(launch_pdl(a.zeros_at ? int4_few_kernel<X, GROUP, NT, true> : int4_few_kernel<X, GROUP, NT, false>, grid, FEW_THREADS, smem, st, a));
+  LAPIS_TRY(a.zeros_at ? (allow_smem<int4_few_kernel<X, GROUP, true>>(160 << 10)) : (allow_smem<int4_few_kernel<X, GROUP, false>>(160 << 10)));
+  LAPIS_CUDA_TRY(launch_pdl(a.zeros_at ? int4_few_kernel<X, GROUP, true> : int4_few_kernel<X, GROUP, false>, grid, FEW_THREADS, smem, st, a));
   return LAPIS_OK;
 }
 
 template <typename X>
-static int launch_few_of(ProductArgs &a, int group, int matrices, int64_t expected, cudaStream_t st) {
+static int launch_few_of(ProductArgs &a, int group, int matrices, cudaStream_t st) {
   switch (group) {
-    case 32: return launch_few_as<X, 32, 1>(a, matrices, st);
-    case 64: return launch_few_as<X, 64, 1>(a, matrices, st);
-    default: return launch_few_as<X, 128, 1>(a, matrices, st);
+    case 32: return launch_few_as<X, 32>(a, matrices, st);
+    case 64: return launch_few_as<X, 64>(a, matrices, st);
+    default: return launch_few_as<X, 128>(a, matrices, st);
   }
 }
-int launch_few(int type, ProductArgs &a, int group, int matrices, int64_t expected, cudaStream_t st) {
+int launch_few(int type, ProductArgs &a, int group, int matrices, cudaStream_t st) {
   switch (type) {
-    case LAPIS_F32: return launch_few_of<float>(a, group, matrices, expected, st);
-    case LAPIS_F16: return launch_few_of<__half>(a, group, matrices, expected, st);
-    default: return launch_few_of<__nv_bfloat16>(a, group, matrices, expected, st);
+    case LAPIS_F32: return launch_few_of<float>(a, group, matrices, st);
+    case LAPIS_F16: return launch_few_of<__half>(a, group, matrices, st);
+    default: return launch_few_of<__nv_bfloat16>(a, group, matrices, st);
   }
 }
 

@@ -20,17 +20,21 @@
 namespace lapis_b200 {
 
 constexpr int MANY_WARPS = 8, MANY_THREADS = 32 * (MANY_WARPS + 2);  // a warp copies, a warp issues
-constexpr int X_STAGES = 4;  // of x: a copy takes about 1 us
+constexpr int X_STAGES = 4;  // of x, of two blocks at most: a copy takes about 1 us
 constexpr int MANY_TILE = 128, MANY_STRIPS = MANY_TILE / STRIP;
 
-// Shared memory: the stages of x, or the sums of a tile as [column][output] with a float between columns.
 // Blocks of a stage, and columns of tensor memory: sums of two stages and their codes, a power of two.
 __host__ __device__ constexpr int stage_blocks(int group) { return group == 32 ? 1 : 2; }
 __host__ __device__ constexpr int many_tmem(int group, int nc) {
-  return 2 * stage_blocks(group) * (BLOCK / (group < BLOCK ? group : BLOCK)) * nc / (group == 128 ? 2 : 1) + 64 * stage_blocks(group) <= 256 ? 256 : 512;
+  return 2 * stage_blocks(group) * BLOCK / group * nc + 64 * stage_blocks(group) <= 256 ? 256 : 512;
 }
+// Shared memory: the stages of x, or the sums of a tile as [column][output] with a float between columns.  A cluster asks for more than that,
+// in proportion to tensor memory: its CTAs wait for one another, so none may be resident whose tensor memory a CTA of another such
+// cluster holds, of a launch on another stream, that waits in the same way.  Two of 76 KB fit an SM, or one of 152.  CTAs that share
+// nothing end by themselves, and the next launch's may come in beside them (64 rows x 14,336 x 4096 in groups of 64: 31 us, else 38).
 constexpr int MANY_SUM_PITCH = MANY_TILE + 1;
 constexpr int many_smem(int nc) { return 1024 + std::max(X_STAGES * 2 * nc * 128, nc * MANY_SUM_PITCH * 4); }
+constexpr int many_cluster_smem(int group, int nc) { return std::max(many_tmem(group, nc) == 256 ? 76 << 10 : 152 << 10, many_smem(nc)); }
 
 __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]), "r"(r[1]),
@@ -444,11 +448,11 @@ static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   const int64_t each = (a.rows + a.experts - 1) / a.experts * 2 * a.blocks;
   LAPIS_CUDA_TRY(launch_pdl(arrange_kernel<X, NC>, dim3((unsigned)std::min<int64_t>(4 * sm_count(), (each + 255) / 256), a.experts), 256, 0, st, a));
   const auto kernel = a.zeros_at ? int4_many_kernel<X, GROUP, NC, true> : int4_many_kernel<X, GROUP, NC, false>;
-  LAPIS_TRY(a.zeros_at ? (allow_smem<int4_many_kernel<X, GROUP, NC, true>>(many_smem(NC))) : (allow_smem<int4_many_kernel<X, GROUP, NC, false>>(many_smem(NC))));
+  LAPIS_TRY(a.zeros_at ? (allow_smem<int4_many_kernel<X, GROUP, NC, true>>(many_cluster_smem(GROUP, NC))) : (allow_smem<int4_many_kernel<X, GROUP, NC, false>>(many_cluster_smem(GROUP, NC))));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles << a.shares_log, matrices);
   cfg.blockDim = dim3(MANY_THREADS);
-  cfg.dynamicSmemBytes = many_smem(NC);
+  cfg.dynamicSmemBytes = a.shares_log > 0 ? many_cluster_smem(GROUP, NC) : many_smem(NC);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -405,13 +405,15 @@ int64_t lapis_b200_int4_bytes(const lapis_b200_int4 *w);
 int lapis_b200_int4_pack(const lapis_b200_int4 *w, const void *d_codes, const void *d_scale, const void *d_zero, void *d_packed, void *stream);
 /* Codes, scales and zeros of dense weights [experts * outputs, columns] of `type`, rows w_stride elements apart, to nearest: without zeros
  * (d_zero null) scale = amax / 7, codes 1 to 15; with them scale = (max - min) / 15 over the group and 0, zero = -min / scale.  The scale is
- * rounded to scale_type first.  A group of zeros gets scale 0; one that is not finite a scale of NaN. */
+ * rounded to scale_type first (a number beyond that is infinite).  A group of zeros gets scale 0; one that is not finite a scale of NaN. */
 int lapis_b200_int4_quantise(int type, int64_t rows, int64_t columns, const void *d_w, int64_t w_stride, int group, int scale_type, void *d_codes,
                              void *d_scale, void *d_zero, void *stream);
 /* y = x w^T of `rows` rows [rows, columns], x_stride elements apart: codes and x are exact (x of 32 bits as three parts of bf16), sums
  * are in 32 bits, one rounding.  d_y [rows, outputs], or half as many if gated, contiguous.  With lists (may be null) the rows of
  * y are the lists' slots, those of expert e times its matrix, zeros behind pos[experts]; row i of x is the slot's own, or, with
- * `fetch`, that of its token: x [tokens, columns].  Made for few rows, of each expert: beyond 64 of them weights are fetched again. */
+ * `fetch`, that of its token: x [tokens, columns].  Made for few rows, of each expert: up to 128 of them (64 with groups smaller than 128; one
+ * of 32 bits counts three) share a pass over the weights.  Above 8 a copy of the rows is laid out in memory of the library's pool, and a
+ * failed wait of the kernel is reported by lapis_b200_bgemm_status. */
 int lapis_b200_int4_matmul(int type, const lapis_b200_int4 *w, int64_t rows, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists,
                            int fetch, void *d_y, void *stream);
 

@@ -212,7 +212,8 @@ class Int4Matrix:
 
         With ``lists`` row i of the result is that of slot ``lists.crd[i]``, times its expert's weights, zeros for slots of no
         expert; ``x`` holds the slots' rows in the same order, or with ``fetch`` those of the tokens [tokens, columns].  Made for
-        few rows (of each expert): beyond 64 the weights are read again."""
+        few rows (of each expert): up to 128 share a pass over the weights, 64 with groups smaller than 128, a third of that
+        where they are float32."""
         if self._device != torch.cuda.current_device():
             raise TypeError("matmul: the weights must be on the current device")
         if lists is None:

@@ -76,6 +76,12 @@ __device__ __forceinline__ void many_mma(uint32_t d, uint32_t a, uint64_t b, uin
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
+// One lane of the warp, the same every time.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void workers_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * MANY_WARPS) : "memory"); }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -162,8 +168,8 @@ struct Record {
   __device__ __forceinline__ void ask(const uint8_t *zeros, const uint8_t *at, int type) {
     if constexpr (ZEROS) {
       if constexpr (GROUPS == 8) zero[0] = reinterpret_cast<const uint32_t *>(zeros)[0], zero[1] = reinterpret_cast<const uint32_t *>(zeros)[1];
-      else if constexpr (GROUPS == 4) zero[0] = reinterpret_cast<const uint32_t *>(zeros)[0], zero[1] = zero[0] >> 16;
-      else zero[0] = reinterpret_cast<const uint16_t *>(zeros)[0], zero[1] = zero[0] >> 8;
+      else if constexpr (GROUPS == 4) zero[0] = reinterpret_cast<const uint32_t *>(zeros)[0];
+      else zero[0] = reinterpret_cast<const uint16_t *>(zeros)[0];
     }
     if (type == LAPIS_F32) {
 #pragma unroll
@@ -277,17 +283,23 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
       }
       __syncwarp();
     } else if (warp == MANY_WARPS) {
-      if (lane == 0) {
-        for (int i = 0; i < stages && ok; ++i) {
-          const uint32_t s = i & 1;
-          ok = tc::mbar_wait(&ready[s], parity >> s & 1);
-          parity ^= 1u << s;
-          fence_after();
-          const uint64_t x = rows_desc(tc::smem_u32(smem) + x_turn++ % X_STAGES * SB * NC * 128);
-          const uint32_t d = tmem + s * SG * NC, codes = tmem + SUMS + s * SB * 32;
+      // All lanes go through the stages, and one issues: what the products are given is then computed once for the warp, in uniform registers.
+      // By a thread of its own a product took 100 cycles.
+      const bool leader = elected();
+      const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t x0 = rows_desc(__shfl_sync(0xffffffffu, tc::smem_u32(smem), 0));
+      for (int i = 0; i < stages && ok; ++i) {
+        const uint32_t s = i & 1;
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(&ready[s], parity >> s & 1));
+        parity ^= 1u << s;
+        fence_after();
+        const uint64_t x = x0 + x_turn++ % X_STAGES * (SB * NC * 128 / 16);
+        const uint32_t d = d0 + s * SG * NC, codes = d0 + SUMS + s * SB * 32;
+        const int here = ok ? blocks - i * SB : 0;
+        if (leader) {
 #pragma unroll
           for (int b = 0; b < SB; ++b) {
-            if (!ok || i * SB + b >= blocks) break;
+            if (b >= here) break;
 #pragma unroll
             for (int ks = 0; ks < BLOCK / 16; ++ks) {
               const int at = b * BLOCK + ks * 16;
@@ -295,10 +307,10 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
               else many_mma<false>(d + at / GROUP * NC, codes + b * 32 + ks * 8, x + b * (NC * 128 / 16) + ks * 2, IDESC);
             }
           }
-          if (ok) many_commit(&done[s]);
+          if (here > 0) many_commit(&done[s]);
         }
+        __syncwarp();
       }
-      __syncwarp();
     } else {
       // A warp converts the strip that lies in its half of its quarter of tensor memory, and adds half of the columns of that quarter.
       const int quarter = warp % 4, half = warp / 4;
@@ -344,7 +356,7 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
       for (int i0 = 0; i0 < blocks; i0 += BATCH / BLOCK) {
         float scale[GROUPS];
         record.scales(scale, a.scale_type);
-        const uint32_t zero[2] = {record.zero[0], record.zero[1]};
+        const uint32_t zero[2] = {record.zero[0], ZEROS && GROUPS < 8 ? record.zero[0] >> 4 * GROUPS : record.zero[1]};
         zeros += a.record_bytes;
         scales += a.record_bytes;
         if (i0 + BATCH / BLOCK < blocks) record.ask(zeros, scales, a.scale_type);

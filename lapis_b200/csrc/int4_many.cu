@@ -31,7 +31,7 @@ __host__ __device__ constexpr int many_tmem(int group, int nc) {
 // Shared memory: the stages of x, or the sums of a tile as [column][output] with a float between columns.  A cluster asks for more than that,
 // in proportion to tensor memory: its CTAs wait for one another, so none may be resident whose tensor memory a CTA of another such
 // cluster holds, of a launch on another stream, that waits in the same way.  Two of 76 KB fit an SM, or one of 152.  CTAs that share
-// nothing end by themselves, and the next launch's may come in beside them (64 rows x 14,336 x 4096 in groups of 64: 31 us, else 38).
+// nothing end by themselves, and the next launch's may come in beside them (64 rows x 14,336 x 4096 in groups of 64: 30 us, else 37).
 constexpr int MANY_SUM_PITCH = MANY_TILE + 1;
 constexpr int many_smem(int nc) { return 1024 + std::max(X_STAGES * 2 * nc * 128, nc * MANY_SUM_PITCH * 4); }
 constexpr int many_cluster_smem(int group, int nc) { return std::max(many_tmem(group, nc) == 256 ? 76 << 10 : 152 << 10, many_smem(nc)); }
@@ -446,9 +446,9 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
 template <typename X, int GROUP, int NC>
 static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   const int tiles = (a.strips + MANY_STRIPS - 1) / MANY_STRIPS;
-  // As many CTAs to a tile as keep all of them resident, two an SM where tensor memory has room for two: 14,336 x 4096 (112 tiles), 64 rows,
-  // groups of 128 take 33.7 us with one CTA a tile, 31.0 with two, 35.9 with four; 4096 x 4096 (32 tiles), 32 rows 28.7, 19.6 with two, 13.9 with
-  // four, 14.1 with eight.
+  // As many CTAs to a tile as keep all of them resident, two an SM where tensor memory has room for two.  Measured (with a slower issuing
+  // thread): 14,336 x 4096 (112 tiles), 64 rows, groups of 128 33.7 us with one CTA a tile, 31.0 with two, 35.9 with four; 4096 x 4096 (32
+  // tiles), 32 rows 28.7, 19.6 with two, 13.9 with four, 14.1 with eight.
   const int64_t slots = (int64_t)sm_count() * (512 / many_tmem(GROUP, NC));
   a.shares_log = 0;
   while (a.shares_log < 3 && (2 << a.shares_log) <= a.batches && (int64_t)(tiles << (a.shares_log + 1)) * a.experts <= slots) ++a.shares_log;

@@ -376,7 +376,7 @@ static int launch_lists_as(ListArgs &a, cudaStream_t st) {
   a.blocks = std::max(a.blocks, 1);
   PoolBuf counts;
   if (a.blocks > 1) {
-    LAPIS_TRY(counts.alloc((size_t)a.blocks * buckets * sizeof(uint32_t), st));
+    LAPIS_TRY(scratch(&counts, (size_t)a.blocks * buckets * sizeof(uint32_t), st));
     a.counts = static_cast<uint32_t *>(counts.p);
     LAPIS_CUDA_TRY(launch_pdl(list_count_kernel<S>, dim3(a.blocks), LIST_THREADS, buckets * sizeof(uint32_t), st, a));
   }

@@ -21,6 +21,21 @@ int allow_smem(int bytes) {
   return LAPIS_OK;
 }
 
+// Scratch memory of a call.  The first one of a process makes the pool that it comes from, which a stream that is captured allows in this mode
+// only.  What the pool does not serve is freed when the call returns, so a graph may not have it.
+inline int scratch(PoolBuf *buf, size_t bytes, cudaStream_t st) {
+  if (bytes > POOL_LARGEST) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    LAPIS_CUDA_TRY(cudaStreamIsCapturing(st, &capture));
+    if (capture != cudaStreamCaptureStatusNone) return fail(LAPIS_ETOOBIG, "%zu bytes of scratch memory under stream capture", bytes);
+  }
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  LAPIS_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+  const int status = buf->alloc(bytes, st);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return status;
+}
+
 int check_expert_lists(const char *what, const lapis_b200_expert_lists *lists);  // experts.cu; 0 or a recorded error
 
 }  // namespace lapis_b200

@@ -140,6 +140,24 @@ def test_layers_in_two_graphs(X, tokens):
             assert torch.equal(out, want)
 
 
+def test_scratch_that_a_graph_cannot_keep_is_refused(X):
+    """70,000 rows of 2048 columns are 287 MB as they are laid out, more than the library's pool holds."""
+    from lapis_b200._lib import LapisError
+    matrix = random_matrix(X, 1, None, 16, 2048, 128)
+    x = torch.ones(70_000, 2048, dtype=BF16, device=DEV)
+    want = matrix.matmul(x)
+    assert torch.equal(want, matrix.matmul(x[:1]).expand(70_000, 16))
+    few = matrix.matmul(x[:100])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(LapisError, match="under stream capture"):
+            matrix.matmul(x)
+        y = matrix.matmul(x[:100])
+    y.zero_()
+    g.replay()
+    assert torch.equal(y, few)
+
+
 def test_operands_of_the_wrong_kind_on_the_device(X):
     lists = X.ExpertLists(torch.zeros(3, 2, dtype=torch.int32, device=DEV), 4)
     x = torch.zeros(3, 16, dtype=BF16, device=DEV)

@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_c
     const int64_t slot = first + s * 32 + lane;
     const uint32_t at = in_front[bucket[s]] + mine[bucket[s]] + rank[s];
     a.place[slot] = (int32_t)at;
-    a.crd[at] = (int32_t)slot;
+    if (at < a.slots) a.crd[at] = (int32_t)slot;  // not so only where somebody writes the experts meanwhile, which are read twice
   }
 }
 

@@ -2,8 +2,8 @@
 //
 // The weights go from memory to registers, a batch ahead, and need nothing but their own warp; the rows x, the B operand, are in shared
 // memory.  What bounds it are the instructions on 32 bits that make numbers of codes: of one every two cycles a batch of 16 x 256 takes 150 to
-// 190, its bytes as long as 170.  48 x 8 rows over 128 experts (2048 x 2048, groups of 32, gated) 79 us, 3.7 TB/s; one row times 14,336 x 4096 12.1 us,
-// 2.5 TB/s; 4096 x 4096 7.2 us, most of it launch and latency.  tcgen05 (int4_many.cu) with 8 columns would convert as many codes and add its
+// 190, its bytes as long as 170.  48 x 8 rows over 128 experts (2048 x 2048, groups of 32, gated) 79 us, 3.7 TB/s; one row times 14,336 x 4096 11.3 us,
+// 2.7 TB/s; 4096 x 4096 6.6 us, most of it launch and latency.  tcgen05 (int4_many.cu) with 8 columns would convert as many codes and add its
 // hand-overs: 16 rows take it 23 us where 8 take this 18.
 #include <algorithm>
 #include <cstdint>
@@ -38,11 +38,11 @@ __device__ __forceinline__ void multiply_first(float (&d)[4], uint32_t a0, uint3
 }
 
 // What a lane holds of a batch: 16 columns of rows r and r + 8 in each of four blocks, their scales and zeros.
-template <int GROUP>
+template <int GROUP, bool FULL>
 struct Batch {
-  static constexpr int GROUPS = BATCH / GROUP;
+  static constexpr int GROUPS = BATCH / GROUP, SCALES = FULL ? 2 * GROUPS : GROUPS;  // words of scales: FULL those of 32 bits, else two in a word
   uint4 code[BATCH / BLOCK];
-  uint32_t scale[2 * GROUPS];  // 16-bit ones two in a word, in the first half
+  uint32_t scale[SCALES];
   uint32_t zero[2];
 
   template <int N>
@@ -61,8 +61,7 @@ struct Batch {
   template <bool ZEROS>
   __device__ __forceinline__ void load_record(const ProductArgs &a, const uint8_t *record, int lane) {
     const int row = lane / 4;
-    if (a.scale_type == LAPIS_F32) fetch<2 * GROUPS>(scale, record + row * GROUPS * 8);
-    else fetch<GROUPS>(scale, record + row * GROUPS * 4);
+    fetch<SCALES>(scale, record + row * SCALES * 4);
     if constexpr (!ZEROS) {
       zero[0] = zero[1] = 0x88888888u;
     } else if constexpr (GROUPS == 8) {
@@ -81,8 +80,8 @@ struct Batch {
 constexpr int SUM_PITCH = STRIP + 1;
 
 constexpr int FEW_WARPS_LOG = 2, FEW_WARPS = 1 << FEW_WARPS_LOG, FEW_THREADS = 32 * FEW_WARPS;
-// Blocks of an SM, and the rows x of each in shared memory.  The registers of a sixth block are missing in the loop: 48 x 8 rows over 128
-// experts take 79 us with 5 blocks, 82 with 4, 99 with 6; with two of eight warps 87.
+// Blocks of an SM, and the rows x of each in shared memory.  48 x 8 rows over 128 experts take 79 us with 5 blocks, 82 with 4, 78 with 6, for
+// which scales of 32 bits have to be spilled; with two of eight warps 87.
 constexpr int FEW_BLOCKS = 5, FEW_ROOM = 40 << 10;
 
 // Bytes of a row of x in shared memory: neighbouring rows' pieces of a phase lie on different banks.
@@ -131,11 +130,11 @@ __device__ __forceinline__ void stage_few(const ProductArgs &a, uint8_t *xs, con
 }
 
 // A warp's way through a strip: the batch that it multiplies, whose blocks give way to the next one's as they are used.
-template <int GROUP, bool ZEROS>
+template <int GROUP, bool ZEROS, bool FULL>
 struct Way {
-  static constexpr int GROUPS = BATCH / GROUP;
-  Batch<GROUP> next;   // codes: of this batch until they are used, then of the next
-  float scale[2][GROUPS];
+  static constexpr int GROUPS = BATCH / GROUP, SCALES = Batch<GROUP, FULL>::SCALES;
+  Batch<GROUP, FULL> next;  // codes: of this batch until they are used, then of the next
+  uint32_t scale[SCALES];
   uint32_t zero[2];
   const uint4 *codes;  // of the lane, of the next batch
   const uint8_t *record;
@@ -163,27 +162,24 @@ struct Way {
   }
   // Takes over the record of the batch whose codes are there, and asks for the next one's.
   __device__ __forceinline__ void enter(const ProductArgs &a, int lane) {
-    if (a.scale_type == LAPIS_F32) {
 #pragma unroll
-      for (int i = 0; i < 2 * GROUPS; ++i) scale[i / GROUPS][i % GROUPS] = __uint_as_float(next.scale[i]);
-    } else if (a.scale_type == LAPIS_BF16) {
-#pragma unroll
-      for (int i = 0; i < 2 * GROUPS; ++i) scale[i / GROUPS][i % GROUPS] = __uint_as_float(i % 2 ? next.scale[i / 2] & 0xffff0000u : next.scale[i / 2] << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2 * GROUPS; i += 2) {
-        const float2 s = __half22float2(*reinterpret_cast<const __half2 *>(&next.scale[i / 2]));
-        scale[i / GROUPS][i % GROUPS] = s.x, scale[(i + 1) / GROUPS][(i + 1) % GROUPS] = s.y;
-      }
-    }
+    for (int i = 0; i < SCALES; ++i) scale[i] = next.scale[i];
     zero[0] = next.zero[0], zero[1] = next.zero[1];
     if (left > 0) next.template load_record<ZEROS>(a, record, lane);
+  }
+  // Scale of group g of row r (0) or r + 8 (1).
+  __device__ __forceinline__ float scale_of(int row, int g, bool bf16) const {
+    const int i = row * GROUPS + g;
+    if constexpr (FULL) return __uint_as_float(scale[i]);
+    const uint32_t w = scale[i / 2];
+    if (bf16) return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+    return __half2float(__ushort_as_half((unsigned short)(i % 2 ? w >> 16 : w & 0xffffu)));
   }
 };
 
 // sum += the product of the batch that `way` is at with the rows x, of which the lane's pieces begin at x.
-template <typename T, int GROUP, bool ZEROS>
-__device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum)[4], Way<GROUP, ZEROS> &way, const uint8_t *x, int lane) {
+template <typename T, int GROUP, bool ZEROS, bool FULL>
+__device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum)[4], Way<GROUP, ZEROS, FULL> &way, const uint8_t *x, int lane) {
   float part[4];
   way.enter(a, lane);
 #pragma unroll
@@ -202,8 +198,9 @@ __device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum
     else multiply<T>(part, p0[0], p1[0], p0[1], p1[1], v.x, v.y);
     multiply<T>(part, p0[2], p1[2], p0[3], p1[3], v.z, v.w);
     if ((half + 1) * 32 % GROUP == 0) {
+      const float s0 = way.scale_of(0, g, a.scale_type == LAPIS_BF16), s1 = way.scale_of(1, g, a.scale_type == LAPIS_BF16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = fmaf(way.scale[i / 2][g], part[i], sum[i]);
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(i < 2 ? s0 : s1, part[i], sum[i]);
     }
   }
   way.advance();
@@ -211,7 +208,7 @@ __device__ __forceinline__ void multiply_batch(const ProductArgs &a, float (&sum
 
 // A block's warps are strips times shares of the columns, both powers of two.  A warp takes its batches of a strip one after the
 // other, the next on its way to its registers; the rows x are in shared memory, all of their columns where they fit.
-template <typename X, int GROUP, bool ZEROS>
+template <typename X, int GROUP, bool ZEROS, bool FULL>
 __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const __grid_constant__ ProductArgs a) {
   using T = typename std::conditional<std::is_same<X, float>::value, __nv_bfloat16, X>::type;
   constexpr int A_ROW = std::is_same<X, float>::value ? 3 : 1, ROWS = FEW_COLUMNS / A_ROW;
@@ -225,7 +222,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
   X *const y = static_cast<X *>(a.y);
   const int batches = strip < a.strips ? a.batches : 0;
   const int64_t of_all = (int64_t)expert * a.strips + min(strip, a.strips - 1);  // the strip's number among all matrices'
-  Way<GROUP, ZEROS> way;
+  Way<GROUP, ZEROS, FULL> way;
 
   // Weights are nobody's result (int4_pack waits for them), so they are asked for in front of pdl_wait(), unless lists say whose.
   const bool early = a.pos == nullptr;
@@ -260,7 +257,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
       stage_few<X>(a, smem, row_at, rows, b0 * BATCH, min(a.chunk, (a.batches - b0) * BATCH), pitch);
       __syncthreads();
       for (int b = b0 + my_share; b < min(b0 + step, batches); b += shares)
-        multiply_batch<T, GROUP, ZEROS>(a, sum, way, x + (b - b0) * (BATCH * 2), lane);
+        multiply_batch<T, GROUP, ZEROS, FULL>(a, sum, way, x + (b - b0) * (BATCH * 2), lane);
     }
     // The shares' sums meet in shared memory: [share][strip][column][row].
     float *const sums = reinterpret_cast<float *>(smem);
@@ -286,7 +283,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
   }
 }
 
-template <typename X, int GROUP>
+template <typename X, int GROUP, bool ZEROS, bool FULL>
 static int launch_few_as(ProductArgs &a, int matrices, cudaStream_t st) {
   constexpr int A_ROW = std::is_same<X, float>::value ? 3 : 1;
   a.rows_a_pass = (int)std::min<int64_t>(a.rows, FEW_COLUMNS / A_ROW);
@@ -299,11 +296,16 @@ static int launch_few_as(ProductArgs &a, int matrices, cudaStream_t st) {
   a.chunk = (int)std::min<int64_t>(a.chunk, (a.columns + turn - 1) / turn * turn);
   const int smem = std::max(a.rows_a_pass * A_ROW * few_pitch(a.chunk), FEW_WARPS * FEW_COLUMNS * SUM_PITCH * 4);
   const dim3 grid((a.strips + strips - 1) / strips, matrices);
-  LAPIS_TRY(a.zeros_at ? (allow_smem<int4_few_kernel<X, GROUP, true>>(160 << 10)) : (allow_smem<int4_few_kernel<X, GROUP, false>>(160 << 10)));
-  LAPIS_CUDA_TRY(launch_pdl(a.zeros_at ? int4_few_kernel<X, GROUP, true> : int4_few_kernel<X, GROUP, false>, grid, FEW_THREADS, smem, st, a));
+  LAPIS_TRY((allow_smem<int4_few_kernel<X, GROUP, ZEROS, FULL>>(160 << 10)));
+  LAPIS_CUDA_TRY(launch_pdl(int4_few_kernel<X, GROUP, ZEROS, FULL>, grid, FEW_THREADS, smem, st, a));
   return LAPIS_OK;
 }
 
+template <typename X, int GROUP>
+static int launch_few_as(ProductArgs &a, int matrices, cudaStream_t st) {
+  if (a.scale_type == LAPIS_F32) return a.zeros_at ? launch_few_as<X, GROUP, true, true>(a, matrices, st) : launch_few_as<X, GROUP, false, true>(a, matrices, st);
+  return a.zeros_at ? launch_few_as<X, GROUP, true, false>(a, matrices, st) : launch_few_as<X, GROUP, false, false>(a, matrices, st);
+}
 template <typename X>
 static int launch_few_of(ProductArgs &a, int group, int matrices, cudaStream_t st) {
   switch (group) {

@@ -700,6 +700,102 @@ __global__ void __launch_bounds__(ROWS_THREADS, BACK_BLOCKS) combine_backward_ke
   if (lane == 0) a.dweights[slot] = all;
 }
 
+// ---- the same for narrow rows -----------------------------------------------------
+
+// Rows of up to so many pieces leave lanes of a warp without work where a warp takes a row: there a thread takes a piece.  38,933 x 4 rows of
+// bf16, us, a warp a row and a thread a piece: combined 128 wide 29.7 and 12.2, 256 wide 31.9 and 23.9; gradients 70 and 25, 76 and 51;
+// copied 128 wide 25.5 and 24.4 with the lists, 256 wide 27.2 and 38.8, as a thread reads its piece for every slot.
+constexpr int NARROW = 32, NARROW_GATHER = 16;
+
+template <typename T, int V>
+__device__ __forceinline__ void to_floats(float (&x)[V], const Piece<T, V> &p) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) gather_narrow_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  const int64_t item = (int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x;
+  pdl_wait();
+  pdl_release();
+  if (item >= a.items) return;
+  const int64_t slot = divided(item, a.chunks, a.items), token = divided(slot, a.k, a.slots);
+  const int piece = (int)(item - slot * a.chunks);
+  const Place p = place_of(a, slot, a.pos[a.experts]);
+  if (p.at < 0) return;
+  P got = {};
+  if (p.here) got = reinterpret_cast<const P *>(static_cast<const T *>(a.x) + token * a.x_stride)[piece];
+  reinterpret_cast<P *>(static_cast<T *>(a.out) + p.at * a.dim)[piece] = got;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) combine_narrow_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  constexpr int J = 4;  // rows asked for at a time
+  const int64_t item = (int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x;
+  pdl_wait();
+  pdl_release();
+  if (item >= a.items) return;
+  const int64_t token = divided(item, a.chunks, a.items);
+  const int piece = (int)(item - token * a.chunks);
+  const int32_t end = a.pos[a.experts];
+  float sum[V] = {};
+  for (int j0 = 0; j0 < a.k; j0 += J) {
+    Place p[J];
+    P got[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) p[j] = j0 + j < a.k ? place_of(a, token * a.k + j0 + j, end) : Place{-1, false};
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (p[j].here) got[j] = reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + p[j].at * a.row_stride)[piece];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if (!p[j].here) continue;
+      const float w = a.weights != nullptr ? a.weights[token * a.k + j0 + j] : 1.0f;
+      float x[V];
+      to_floats<T, V>(x, got[j]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] = fmaf(w, x[v], sum[v]);
+    }
+  }
+  P done;
+#pragma unroll
+  for (int v = 0; v < V; ++v) done.v[v] = from_f32<T>(sum[v]);
+  reinterpret_cast<P *>(static_cast<T *>(a.out) + token * a.dim)[piece] = done;
+}
+
+// a.run lanes, a power of two, take a slot.
+template <typename T, int V>
+__global__ void __launch_bounds__(ROWS_THREADS) combine_backward_narrow_kernel(const __grid_constant__ RowsArgs a) {
+  using P = Piece<T, V>;
+  const int64_t slot = ((int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x) / a.run;
+  const int piece = threadIdx.x & (a.run - 1);
+  pdl_wait();
+  pdl_release();
+  float dot = 0.0f;
+  if (slot < a.slots) {
+    const Place p = place_of(a, slot, a.pos[a.experts]);
+    if (piece < (int)a.chunks && p.at >= 0) {
+      P done = {};
+      if (p.here) {
+        const float w = a.weights[slot];
+        float d[V], r[V];
+        to_floats<T, V>(d, reinterpret_cast<const P *>(static_cast<const T *>(a.x) + divided(slot, a.k, a.slots) * a.x_stride)[piece]);
+        to_floats<T, V>(r, reinterpret_cast<const P *>(static_cast<const T *>(a.rows) + p.at * a.row_stride)[piece]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          dot = fmaf(d[v], r[v], dot);
+          done.v[v] = from_f32<T>(w * d[v]);
+        }
+      }
+      reinterpret_cast<P *>(static_cast<T *>(a.out) + p.at * a.dim)[piece] = done;
+    }
+  }
+  for (int d = a.run / 2; d > 0; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+  if (slot < a.slots && piece == 0) a.dweights[slot] = dot;
+}
+
 enum RowsOp { GATHER, COMBINE, COMBINE_BACKWARD };
 
 template <typename T, int J>
@@ -728,8 +824,21 @@ static int launch_combine(RowsArgs &a, cudaStream_t st) {
   return LAPIS_OK;
 }
 template <typename T, int V>
+static int launch_narrow(RowsOp op, RowsArgs &a, cudaStream_t st) {
+  a.chunks = (uint32_t)(a.dim / V);  // pieces
+  for (a.run = 1; a.run < (int)a.chunks;) a.run *= 2;
+  a.items = op == GATHER ? a.slots * a.chunks : op == COMBINE ? a.tokens * a.chunks : a.slots * a.run;
+  const int64_t blocks = (a.items + ROWS_THREADS - 1) / ROWS_THREADS;
+  if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
+  LAPIS_CUDA_TRY(op == GATHER ? launch_pdl(gather_narrow_kernel<T, V>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a)
+                 : op == COMBINE ? launch_pdl(combine_narrow_kernel<T, V>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a)
+                                 : launch_pdl(combine_backward_narrow_kernel<T, V>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
+  return LAPIS_OK;
+}
+template <typename T, int V>
 static int launch_rows_as(RowsOp op, RowsArgs &a, cudaStream_t st) {
   constexpr int WARPS = ROWS_THREADS / 32;
+  if (a.dim / V <= (op == GATHER ? NARROW_GATHER : NARROW)) return launch_narrow<T, V>(op, a, st);
   if (op == COMBINE) return launch_combine<T, V>(a, st);
   const int64_t lanes = (a.dim / V + 31) / 32;
   a.chunks = (uint32_t)((lanes + GATHER_PIECES - 1) / GATHER_PIECES);

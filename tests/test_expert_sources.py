@@ -22,7 +22,7 @@ def test_no_read_only_loads(name):
 
 @pytest.mark.parametrize("name,kernels", [
     ("experts.cu", {"route_kernel", "route_backward_kernel", "list_count_kernel", "list_place_kernel", "gather_kernel", "combine_ring_kernel", "combine_kernel",
-                    "combine_backward_kernel"}),
+                    "combine_backward_kernel", "gather_narrow_kernel", "combine_narrow_kernel", "combine_backward_narrow_kernel"}),
     ("int4_few.cu", {"int4_few_kernel"}),
     ("int4_many.cu", {"arrange_kernel", "int4_many_kernel"}),
 ])

@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
   if (a.pos != nullptr) {
     begin = min((int64_t)max(a.pos[expert], 0), a.rows);
     end = expert < a.experts ? min((int64_t)a.pos[expert + 1], a.rows) : a.rows;
-    if (expert == a.experts || begin >= end) {  // rows of no expert
+    if (expert == a.experts || begin >= end) {  // rows of no expert (with lists the grid has one layer)
       pdl_release();
       const int n = min(outs, a.outputs - first_out);
       if (expert == a.experts && my_share == 0)
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
   bool ok = true;
   uint32_t parity = 0, x_turn = 0;  // of the next wait for each half's barrier; stages of x so far, of all passes
 
-  for (int64_t row0 = begin; row0 < end; row0 += ROWS) {
+  for (int64_t row0 = begin + (int64_t)blockIdx.z * ROWS; row0 < end; row0 += (int64_t)gridDim.z * ROWS) {  // every CTA has a pass at least
     const int rows = (int)min((int64_t)ROWS, end - row0);
     if (warp == MANY_WARPS + 1) {
       // Copies X_STAGES stages of x ahead, and says of each that it is there: what else is ready is said by the converting warps.
@@ -453,9 +453,11 @@ static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   // thread): 14,336 x 4096 (112 tiles), 64 rows, groups of 128 33.7 us with one CTA a tile, 31.0 with two, 35.9 with four; 4096 x 4096 (32
   // tiles), 32 rows 28.7, 19.6 with two, 13.9 with four, 14.1 with eight.
   const int64_t slots = (int64_t)sm_count() * (512 / many_tmem(GROUP, NC));
-  a.shares_log = 0;
-  while (a.shares_log < 3 && (2 << a.shares_log) <= a.batches && (int64_t)(tiles << (a.shares_log + 1)) * a.experts <= slots) ++a.shares_log;
+  // Passes of one matrix come before that: they need no join (126 rows of 32 bits x 256 x 1536, groups of 32: six passes one after the other 60 us, at once 16).
   constexpr int ROWS = NC / (std::is_same<X, float>::value ? 3 : 1);
+  const int64_t passes = a.pos != nullptr ? 1 : std::max<int64_t>(1, std::min({(a.rows + ROWS - 1) / ROWS, slots / tiles, (int64_t)65535}));
+  a.shares_log = 0;
+  while (a.shares_log < 3 && (2 << a.shares_log) <= a.batches && (tiles * passes << (a.shares_log + 1)) * a.experts <= slots) ++a.shares_log;
   // All passes of all experts (arranged_at).
   PoolBuf arranged;
   LAPIS_TRY(scratch(&arranged, (size_t)(a.rows / ROWS + a.experts + 1) * a.blocks * (NC * 128), st));
@@ -465,7 +467,7 @@ static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   const auto kernel = a.zeros_at ? int4_many_kernel<X, GROUP, NC, true> : int4_many_kernel<X, GROUP, NC, false>;
   LAPIS_TRY(a.zeros_at ? (allow_smem<int4_many_kernel<X, GROUP, NC, true>>(many_cluster_smem(GROUP, NC))) : (allow_smem<int4_many_kernel<X, GROUP, NC, false>>(many_cluster_smem(GROUP, NC))));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles << a.shares_log, matrices);
+  cfg.gridDim = dim3(tiles << a.shares_log, matrices, (unsigned)passes);
   cfg.blockDim = dim3(MANY_THREADS);
   cfg.dynamicSmemBytes = a.shares_log > 0 ? many_cluster_smem(GROUP, NC) : many_smem(NC);
   cfg.stream = st;

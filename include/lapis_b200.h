@@ -412,8 +412,9 @@ int lapis_b200_int4_quantise(int type, int64_t rows, int64_t columns, const void
  * are in 32 bits, one rounding.  d_y [rows, outputs], or half as many if gated, contiguous.  With lists (may be null) the rows of
  * y are the lists' slots, those of expert e times its matrix, zeros behind pos[experts]; row i of x is the slot's own, or, with
  * `fetch`, that of its token: x [tokens, columns].  Made for few rows, of each expert: up to 128 of them (64 with groups smaller than 128; one
- * of 32 bits counts three) share a pass over the weights.  Above 8 a copy of the rows is laid out in memory of the library's pool, and a
- * failed wait of the kernel is reported by lapis_b200_bgemm_status. */
+ * of 32 bits counts three) share a pass over the weights.  Above 8 a copy of the rows (6 bytes a value where they are of 32 bits), and up
+ * to 8 columns of the product more for each expert, is laid out in memory of the library's pool, or, beyond 256 MiB, in memory of its own, which stream
+ * capture refuses.  A failed wait of the kernel is reported by lapis_b200_bgemm_status. */
 int lapis_b200_int4_matmul(int type, const lapis_b200_int4 *w, int64_t rows, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists,
                            int fetch, void *d_y, void *stream);
 

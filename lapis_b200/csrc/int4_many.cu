@@ -96,9 +96,15 @@ __device__ __forceinline__ float peer_float(const float *p, int rank) {
   return v;
 }
 
-// Blocks of a matrix's rows: pass p of expert e has the blocks from arranged_at(pos[e], e, rows of a pass) + p on, in passes.  No two
-// experts' overlap: those in front have at most pos[e] / ROWS + e passes.
-__device__ __forceinline__ int64_t arranged_at(int64_t begin, int expert, int rows) { return begin / rows + expert; }
+// Where an expert's rows lie as they are laid out, in groups of 8 columns of the product (times a.blocks, of 1024 bytes): pass p of it begins
+// p * NC / 8 groups behind arranged_at(pos[e], e), and its blocks of 64 columns of x follow one another, each with the groups that the pass
+// has rows for.  No two experts overlap: n rows take less than n * (NC / 8) / ROWS + 1 groups, and from pos[e] to pos[e] + n and the next expert
+// there are more than n * (NC / 8) / ROWS of them.
+template <int NC, int ROWS>
+__host__ __device__ constexpr int64_t arranged_at(int64_t begin, int expert) { return begin * (NC / 8) / ROWS + expert; }
+// Bytes of a block of 64 columns for `rows` rows of a pass.
+template <int A_ROW>
+__device__ __forceinline__ int block_bytes(int rows) { return (rows * A_ROW + 7) / 8 * 1024; }
 
 // A thread half a row's block: 32 columns, of which lane c's operand has 8 c to 8 c + 7.  The columns of the product come in the order of the
 // codes in tensor memory, pair p of lane c at 4 p + c, so that pair p of the four lanes makes 16 bytes.
@@ -114,7 +120,7 @@ __global__ void __launch_bounds__(256) arrange_kernel(const __grid_constant__ Pr
     begin = min((int64_t)max(a.pos[expert], 0), a.rows);
     end = min((int64_t)a.pos[expert + 1], a.rows);
   }
-  uint8_t *const blocks = a.arranged + arranged_at(begin, expert, ROWS) * a.blocks * (NC * 128);
+  uint8_t *const passes = a.arranged + arranged_at<NC, ROWS>(begin, expert) * a.blocks * 1024;
   const int halves = 2 * a.blocks;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < (end - begin) * halves; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t row = i / halves;
@@ -131,7 +137,7 @@ __global__ void __launch_bounds__(256) arrange_kernel(const __grid_constant__ Pr
 #pragma unroll
       for (int k = 0; k < 32; ++k) v[k] = there && c0 + k < columns ? x[c0 + k] : from_f32<X>(0.0f);
     }
-    uint8_t *const block = blocks + ((row / ROWS) * a.blocks + half / 2) * (NC * 128);
+    uint8_t *const block = passes + (row / ROWS) * a.blocks * (NC * 128) + (int64_t)(half / 2) * block_bytes<A_ROW>((int)min((int64_t)ROWS, end - begin - (row - r)));
 #pragma unroll
     for (int p = 0; p < A_ROW; ++p) {
       uint32_t word[16];  // pair by pair
@@ -253,17 +259,18 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
   uint32_t parity = 0, x_turn = 0;  // of the next wait for each half's barrier; stages of x so far, of all passes
 
   for (int64_t row0 = begin + (int64_t)blockIdx.z * ROWS; row0 < end; row0 += (int64_t)gridDim.z * ROWS) {  // every CTA has a pass at least
-    const int rows = (int)min((int64_t)ROWS, end - row0);
+    const int rows = (int)min((int64_t)ROWS, end - row0), block_size = block_bytes<A_ROW>(rows);
     if (warp == MANY_WARPS + 1) {
       // Copies X_STAGES stages of x ahead, and says of each that it is there: what else is ready is said by the converting warps.
       if (lane == 0) {
         asm volatile("fence.proxy.async;" ::: "memory");  // blocks, and the sums where they come, were written by ordinary stores
-        const uint8_t *const from = a.arranged + ((arranged_at(begin, expert, ROWS) + (row0 - begin) / ROWS) * a.blocks + batch0 * (BATCH / BLOCK)) * (NC * 128);
+        const uint8_t *const from = a.arranged + (arranged_at<NC, ROWS>(begin, expert) + (row0 - begin) / ROWS * (NC / 8)) * a.blocks * 1024 +
+                                    (int64_t)batch0 * (BATCH / BLOCK) * block_size;
         const auto copy = [&](int i) {
-          const uint32_t s = (x_turn + i) % X_STAGES, bytes = min(SB, blocks - i * SB) * (NC * 128);
+          const uint32_t s = (x_turn + i) % X_STAGES, bytes = min(SB, blocks - i * SB) * block_size;
           tc::mbar_expect_tx(&copied[s], bytes);
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(smem) + s * SB * NC * 128),
-                       "l"(from + (int64_t)i * SB * NC * 128), "r"(bytes), "r"(tc::smem_u32(&copied[s]))
+                       "l"(from + (int64_t)i * SB * block_size), "r"(bytes), "r"(tc::smem_u32(&copied[s]))
                        : "memory");
         };
         const auto arrived = [&](int i) { return tc::mbar_wait(&copied[(x_turn + i) % X_STAGES], (x_turn + i) / X_STAGES & 1); };
@@ -290,6 +297,9 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
       const bool leader = elected();
       const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t x0 = rows_desc(__shfl_sync(0xffffffffu, tc::smem_u32(smem), 0));
+      // A stage's second block lies right behind the first.  Columns of the product beyond the rows are whatever lies in the rest of the
+      // stage: nobody looks at their sums.
+      const uint32_t block_step = __shfl_sync(0xffffffffu, block_size / 16, 0);
       for (int i = 0; i < stages && ok; ++i) {
         const uint32_t s = i & 1;
         ok = __all_sync(0xffffffffu, tc::mbar_wait(&ready[s], parity >> s & 1));
@@ -305,8 +315,8 @@ __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 
 #pragma unroll
             for (int ks = 0; ks < BLOCK / 16; ++ks) {
               const int at = b * BLOCK + ks * 16;
-              if (at % GROUP != 0) many_mma<true>(d + at / GROUP * NC, codes + b * 32 + ks * 8, x + b * (NC * 128 / 16) + ks * 2, IDESC);
-              else many_mma<false>(d + at / GROUP * NC, codes + b * 32 + ks * 8, x + b * (NC * 128 / 16) + ks * 2, IDESC);
+              if (at % GROUP != 0) many_mma<true>(d + at / GROUP * NC, codes + b * 32 + ks * 8, x + b * block_step + ks * 2, IDESC);
+              else many_mma<false>(d + at / GROUP * NC, codes + b * 32 + ks * 8, x + b * block_step + ks * 2, IDESC);
             }
           }
           if (here > 0) many_commit(&done[s]);
@@ -458,9 +468,9 @@ static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   const int64_t passes = a.pos != nullptr ? 1 : std::max<int64_t>(1, std::min({(a.rows + ROWS - 1) / ROWS, slots / tiles, (int64_t)65535}));
   a.shares_log = 0;
   while (a.shares_log < 3 && (2 << a.shares_log) <= a.batches && (tiles * passes << (a.shares_log + 1)) * a.experts <= slots) ++a.shares_log;
-  // All passes of all experts (arranged_at).
+  // All passes of all experts (arranged_at): the rows, up to 8 columns of the product more for each expert.
   PoolBuf arranged;
-  LAPIS_TRY(scratch(&arranged, (size_t)(a.rows / ROWS + a.experts + 1) * a.blocks * (NC * 128), st));
+  LAPIS_TRY(scratch(&arranged, (size_t)arranged_at<NC, ROWS>(a.rows, a.experts) * a.blocks * 1024, st));
   a.arranged = static_cast<uint8_t *>(arranged.p);
   const int64_t each = (a.rows + a.experts - 1) / a.experts * 2 * a.blocks;
   LAPIS_CUDA_TRY(launch_pdl(arrange_kernel<X, NC>, dim3((unsigned)std::min<int64_t>(4 * sm_count(), (each + 255) / 256), a.experts), 256, 0, st, a));

@@ -1,0 +1,34 @@
+"""Scratch memory of the products of experts: as much as the rows take, so that ordinary layers may be captured."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("tokens,k,experts,columns,group,dtype", [(513, 8, 256, 7168, 128, BF16), (1024, 8, 256, 7168, 128, BF16), (128, 8, 128, 16384, 64, F32)])
+def test_layers_of_many_experts_are_captured(tokens, k, experts, columns, group, dtype):
+    """Rows of 56, 112 and 96 MiB (three parts): a whole pass for every expert would be 281, 337 and 354 MiB, more than a graph can have."""
+    from lapis_b200 import experts as X
+    rng = np.random.default_rng(tokens)
+    outputs = 24
+    codes = torch.from_numpy(rng.integers(0, 256, (experts, outputs, columns // 2), dtype=np.uint8)).to(DEV)
+    scale = torch.from_numpy(rng.choice([0.25, 0.5, 1.0, 2.0], (experts, outputs, columns // group))).to(DEV, F32)
+    matrix = X.Int4Matrix(codes, scale, columns=columns, group=group)
+    lists = X.ExpertLists(torch.from_numpy(rng.integers(0, experts, (tokens, k))).to(DEV), experts)
+    x = torch.from_numpy(rng.integers(-3, 4, (tokens, columns))).to(DEV, dtype)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = matrix.matmul(x, lists, fetch=True)
+    y.zero_()
+    graph.replay()
+    token, pos = lists.crd.long() // k, lists.pos.tolist()
+    of = torch.arange(columns, device=DEV) // group
+    for e in range(experts):
+        # whole numbers times quarters, all sums below 16384 * 3 * 8 * 2 < 2^20 of them: exact in 32 bits, rounded once
+        code = torch.stack([codes[e] & 15, codes[e] >> 4], -1).flatten(-2).double() - 8
+        want = x[token[pos[e]:pos[e + 1]]].double() @ (code * scale[e].double()[:, of]).T
+        assert torch.equal(y[pos[e]:pos[e + 1]], want.to(dtype))

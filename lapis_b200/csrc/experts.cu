@@ -374,7 +374,7 @@ static int launch_lists_as(ListArgs &a, cudaStream_t st) {
   const int buckets = a.experts + 1;
   a.blocks = (int)((a.slots + LIST_THREADS * S - 1) / (LIST_THREADS * S));
   a.blocks = std::max(a.blocks, 1);
-  PoolBuf counts;
+  CallBuf counts;
   if (a.blocks > 1) {
     LAPIS_TRY(scratch(&counts, (size_t)a.blocks * buckets * sizeof(uint32_t), st));
     a.counts = static_cast<uint32_t *>(counts.p);

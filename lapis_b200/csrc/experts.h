@@ -21,9 +21,23 @@ int allow_smem(int bytes) {
   return LAPIS_OK;
 }
 
+// Memory of a call that is given back when it returns.  What the pool did not serve is freed in the mode in which another thread may capture a
+// stream meanwhile; in the others cudaFree fails and ends that capture.
+struct CallBuf : PoolBuf {
+  ~CallBuf() {
+    if (pooled || p == nullptr) return;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    p = nullptr;
+    pooled = true;
+  }
+};
+
 // Scratch memory of a call.  The first one of a process makes the pool that it comes from, which a stream that is captured allows in this mode
 // only.  What the pool does not serve is freed when the call returns, so a graph may not have it.
-inline int scratch(PoolBuf *buf, size_t bytes, cudaStream_t st) {
+inline int scratch(CallBuf *buf, size_t bytes, cudaStream_t st) {
   if (bytes > POOL_LARGEST) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     LAPIS_CUDA_TRY(cudaStreamIsCapturing(st, &capture));

@@ -469,7 +469,7 @@ static int launch_many_as(ProductArgs &a, int matrices, cudaStream_t st) {
   a.shares_log = 0;
   while (a.shares_log < 3 && (2 << a.shares_log) <= a.batches && (tiles * passes << (a.shares_log + 1)) * a.experts <= slots) ++a.shares_log;
   // All passes of all experts (arranged_at): the rows, up to 8 columns of the product more for each expert.
-  PoolBuf arranged;
+  CallBuf arranged;
   LAPIS_TRY(scratch(&arranged, (size_t)arranged_at<NC, ROWS>(a.rows, a.experts) * a.blocks * 1024, st));
   a.arranged = static_cast<uint8_t *>(arranged.p);
   const int64_t each = (a.rows + a.experts - 1) / a.experts * 2 * a.blocks;

@@ -1,10 +1,16 @@
-"""Scratch memory of the products of experts: as much as the rows take, so that ordinary layers may be captured."""
+"""Scratch memory of the products of experts: as much as the rows take, so that ordinary layers may be captured, and given back while
+another thread captures."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 F32, BF16 = torch.float32, torch.bfloat16
 DEV = "cuda"
 
@@ -32,3 +38,47 @@ def test_layers_of_many_experts_are_captured(tokens, k, experts, columns, group,
         code = torch.stack([codes[e] & 15, codes[e] >> 4], -1).flatten(-2).double() - 8
         want = x[token[pos[e]:pos[e + 1]]].double() @ (code * scale[e].double()[:, of]).T
         assert torch.equal(y[pos[e]:pos[e + 1]], want.to(dtype))
+
+
+TWO_THREADS = """
+import ctypes, threading
+import torch
+from lapis_b200 import _lib
+from lapis_b200 import experts as E
+codes = torch.full((16, 1024), 0x99, dtype=torch.uint8, device="cuda")
+matrix = E.Int4Matrix(codes, torch.ones(16, 16, device="cuda"), columns=2048)
+x, other = torch.ones(70_000, 2048, dtype=torch.bfloat16, device="cuda"), torch.ones(64, device="cuda")
+y = torch.zeros(70_000, 16, dtype=torch.bfloat16, device="cuda")
+lib, device, side = _lib.load(), torch.cuda.current_device(), torch.cuda.Stream()
+def product():
+    return lib.lapis_b200_int4_matmul(2, ctypes.byref(matrix._c), 70_000, x.data_ptr(), 2048, None, 0, y.data_ptr(), side.cuda_stream)
+assert product() == 0
+torch.cuda.synchronize()
+y.zero_()
+asked, done, got = threading.Event(), threading.Event(), []
+def worker():
+    torch.cuda.set_device(device)
+    asked.wait(60)
+    got.append(product())
+    done.set()
+thread = threading.Thread(target=worker)
+thread.start()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    other += 1
+    asked.set()
+    assert done.wait(60)
+    other *= 2
+thread.join()
+assert got == [0]
+graph.replay()
+torch.cuda.synchronize()
+assert bool((other == 4).all()) and bool((y == 2048).all())
+print("done")
+"""
+
+
+def test_large_scratch_while_another_thread_captures():
+    """273 MiB are cudaMalloc's; the other thread's capture is in the mode that forbids such calls everywhere."""
+    r = subprocess.run([sys.executable, "-c", TWO_THREADS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout == "done\n", r.stdout + r.stderr[-2000:]

@@ -170,7 +170,8 @@ class Int4Matrix:
     ``scale`` float32, float16 or bfloat16 [.., outputs, ceil(columns / group)]; ``zero`` uint8 of the same shape (0 to 15), or None:
     8 throughout.  ``group`` is 32, 64 or 128 columns.  ``gated``: the first half of the outputs are gates, and a product is
     silu(gate) * the other half.  The weights are laid out anew here, once; the call returns when that is done, and the tensors
-    are not needed any more."""
+    are not needed any more.  Products may run on any stream: the memory of weights that are dropped is kept until they have ended.  (Graphs
+    that were captured need their weights kept by the caller.)"""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor, zero: torch.Tensor | None = None, *, columns: int, group: int = 128, gated: bool = False):
         for name, t, dtypes in (("codes", codes, (torch.uint8,)), ("scale", scale, tuple(_TYPES)), ("zero", zero, (torch.uint8,))):
@@ -200,6 +201,7 @@ class Int4Matrix:
         check(lib.lapis_b200_int4_pack(ctypes.byref(self._c), _ptr(codes), _ptr(scale), _ptr(zero), _ptr(self._packed), _stream()))
         self._addr = ctypes.addressof(self._c)
         self._device = codes.device.index
+        self._streams = {_stream()}
 
     @classmethod
     def quantise(cls, w: torch.Tensor, group: int = 128, zeros: bool = False, scale_dtype: torch.dtype | None = None, gated: bool = False) -> "Int4Matrix":
@@ -216,6 +218,9 @@ class Int4Matrix:
         where they are float32."""
         if self._device != torch.cuda.current_device():
             raise TypeError("matmul: the weights must be on the current device")
+        if (stream := torch._C._cuda_getCurrentRawStream(self._device)) not in self._streams:  # nobody else has the weights' memory to say so
+            self._packed.record_stream(torch.cuda.current_stream())
+            self._streams.add(stream)
         if lists is None:
             if fetch:
                 raise ValueError("matmul: rows are fetched by lists")

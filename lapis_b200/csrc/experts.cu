@@ -254,6 +254,7 @@ struct ListArgs {
   const void *expert;
   int idx_bytes, experts, blocks;
   int64_t slots;
+  int rounds;        // of 512 S slots for each block, one behind the other
   uint32_t *counts;  // [blocks, experts + 1], or null for one block
   int32_t *pos, *crd, *place;
 };
@@ -272,116 +273,130 @@ __global__ void __launch_bounds__(LIST_THREADS) list_count_kernel(const __grid_c
   pdl_wait();
   pdl_release();
   __syncthreads();
-  const int64_t first = (int64_t)blockIdx.x * LIST_THREADS * S;
+  for (int round = 0; round < a.rounds; ++round) {
+    const int64_t first = ((int64_t)blockIdx.x * a.rounds + round) * LIST_THREADS * S;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int64_t slot = first + s * LIST_THREADS + threadIdx.x;
-    if (slot < a.slots) atomicAdd(&hist[bucket_of(a, slot)], 1u);
+    for (int s = 0; s < S; ++s) {
+      const int64_t slot = first + s * LIST_THREADS + threadIdx.x;
+      if (slot < a.slots) atomicAdd(&hist[bucket_of(a, slot)], 1u);
+    }
   }
   __syncthreads();
   for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) a.counts[(int64_t)blockIdx.x * buckets + b] = hist[b];
 }
 
 // Every warp numbers its slots within each list (peers in a step of 32 by match), the block adds up its warps and the blocks in
-// front of it, and the lists' beginnings are a scan over all lists' lengths.
+// front of it, and the lists' beginnings are a scan over all lists' lengths.  Further rounds go on where the one in front ended.
 template <int S>
 __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_constant__ ListArgs a) {
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t warp_sums[LIST_WARPS];
   const int buckets = a.experts + 1, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  uint32_t *const of_warp = smem, *const length = smem + LIST_WARPS * buckets, *const in_front = length + buckets;
+  uint32_t *const of_warp = smem, *const length = smem + LIST_WARPS * buckets, *const in_front = length + buckets, *const of_round = in_front + buckets;
   for (int i = threadIdx.x; i < (LIST_WARPS + 2) * buckets; i += LIST_THREADS) smem[i] = 0;
   pdl_wait();
   pdl_release();
-  const int64_t first = ((int64_t)blockIdx.x * LIST_WARPS + warp) * 32 * S;
-  int bucket[S];
-  uint32_t rank[S];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const int64_t slot = first + s * 32 + lane;
-    bucket[s] = slot < a.slots ? bucket_of(a, slot) : -1;
-  }
-  __syncthreads();
   uint32_t *const mine = of_warp + warp * buckets;
+  for (int round = 0; round < a.rounds; ++round) {
+    const int64_t first = (((int64_t)blockIdx.x * a.rounds + round) * LIST_WARPS + warp) * 32 * S;
+    int bucket[S];
+    uint32_t rank[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    const uint32_t peers = __match_any_sync(0xffffffffu, bucket[s]);
-    const uint32_t before = bucket[s] >= 0 ? mine[bucket[s]] : 0;
-    rank[s] = before + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (bucket[s] >= 0 && lane == __ffs(peers) - 1) mine[bucket[s]] = before + __popc(peers);
-    __syncwarp();
-  }
-  if (a.counts != nullptr) {
-    const int share = max(1, LIST_THREADS / buckets);  // threads that add up one list's counts
-    for (int i = threadIdx.x; i < share * buckets; i += LIST_THREADS) {
-      const int b = i % buckets;
-      uint32_t all = 0, before = 0;
+    for (int s = 0; s < S; ++s) {
+      const int64_t slot = first + s * 32 + lane;
+      bucket[s] = slot < a.slots ? bucket_of(a, slot) : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const uint32_t peers = __match_any_sync(0xffffffffu, bucket[s]);
+      const uint32_t before = bucket[s] >= 0 ? mine[bucket[s]] : 0;
+      rank[s] = before + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
+      if (bucket[s] >= 0 && lane == __ffs(peers) - 1) mine[bucket[s]] = before + __popc(peers);
+      __syncwarp();
+    }
+    if (round == 0 && a.counts != nullptr) {
+      const int share = max(1, LIST_THREADS / buckets);  // threads that add up one list's counts
+      for (int i = threadIdx.x; i < share * buckets; i += LIST_THREADS) {
+        const int b = i % buckets;
+        uint32_t all = 0, before = 0;
 #pragma unroll 8
-      for (int n = i / buckets; n < a.blocks; n += share) {
-        const uint32_t c = a.counts[(int64_t)n * buckets + b];
-        all += c;
-        before += n < (int)blockIdx.x ? c : 0;
+        for (int n = i / buckets; n < a.blocks; n += share) {
+          const uint32_t c = a.counts[(int64_t)n * buckets + b];
+          all += c;
+          before += n < (int)blockIdx.x ? c : 0;
+        }
+        atomicAdd(&length[b], all);
+        atomicAdd(&in_front[b], before);
       }
-      atomicAdd(&length[b], all);
-      atomicAdd(&in_front[b], before);
     }
-  }
-  __syncthreads();
-  for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) {
-    uint32_t upto = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) {
+      uint32_t upto = 0;
 #pragma unroll
-    for (int w = 0; w < LIST_WARPS; ++w) {
-      const uint32_t n = of_warp[w * buckets + b];
-      of_warp[w * buckets + b] = upto;
-      upto += n;
+      for (int w = 0; w < LIST_WARPS; ++w) {
+        const uint32_t n = of_warp[w * buckets + b];
+        of_warp[w * buckets + b] = upto;
+        upto += n;
+      }
+      of_round[b] = upto;
+      if (a.counts == nullptr) length[b] = upto;
     }
-    if (a.counts == nullptr) length[b] = upto;
-  }
-  __syncthreads();
-  // Where the lists begin: a thread takes `run` lists that lie next to one another.
-  const int run = (buckets + LIST_THREADS - 1) / LIST_THREADS, from = threadIdx.x * run;
-  uint32_t sum = 0;
-  for (int b = from; b < min(from + run, buckets); ++b) sum += length[b];
-  uint32_t upto = sum;
+    __syncthreads();
+    if (round == 0) {
+      // Where the lists begin: a thread takes `run` lists that lie next to one another.
+      const int run = (buckets + LIST_THREADS - 1) / LIST_THREADS, from = threadIdx.x * run;
+      uint32_t sum = 0;
+      for (int b = from; b < min(from + run, buckets); ++b) sum += length[b];
+      uint32_t upto = sum;
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += below;
-  }
-  if (lane == 31) warp_sums[warp] = upto;
-  __syncthreads();
-  uint32_t begin = upto - sum;
-  for (int w = 0; w < warp; ++w) begin += warp_sums[w];
-  for (int b = from; b < min(from + run, buckets); ++b) {
-    if (blockIdx.x == 0) a.pos[b] = (int32_t)begin;
-    in_front[b] += begin;
-    begin += length[b];
-  }
-  __syncthreads();
+      for (int d = 1; d < 32; d *= 2) {
+        const uint32_t below = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += below;
+      }
+      if (lane == 31) warp_sums[warp] = upto;
+      __syncthreads();
+      uint32_t begin = upto - sum;
+      for (int w = 0; w < warp; ++w) begin += warp_sums[w];
+      for (int b = from; b < min(from + run, buckets); ++b) {
+        if (blockIdx.x == 0) a.pos[b] = (int32_t)begin;
+        in_front[b] += begin;
+        begin += length[b];
+      }
+      __syncthreads();
+    }
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    if (bucket[s] < 0) continue;
-    const int64_t slot = first + s * 32 + lane;
-    const uint32_t at = in_front[bucket[s]] + mine[bucket[s]] + rank[s];
-    a.place[slot] = (int32_t)at;
-    if (at < a.slots) a.crd[at] = (int32_t)slot;  // not so only where somebody writes the experts meanwhile, which are read twice
+    for (int s = 0; s < S; ++s) {
+      if (bucket[s] < 0) continue;
+      const int64_t slot = first + s * 32 + lane;
+      const uint32_t at = in_front[bucket[s]] + mine[bucket[s]] + rank[s];
+      a.place[slot] = (int32_t)at;
+      if (at < a.slots) a.crd[at] = (int32_t)slot;  // not so only where somebody writes the experts meanwhile, which are read twice
+    }
+    if (round + 1 == a.rounds) break;
+    __syncthreads();
+    for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) in_front[b] += of_round[b];
+    for (int i = threadIdx.x; i < LIST_WARPS * buckets; i += LIST_THREADS) of_warp[i] = 0;
   }
 }
 
 template <int S>
 static int launch_lists_as(ListArgs &a, cudaStream_t st) {
   const int buckets = a.experts + 1;
-  a.blocks = (int)((a.slots + LIST_THREADS * S - 1) / (LIST_THREADS * S));
-  a.blocks = std::max(a.blocks, 1);
+  // Every block reads the counts of all, so there are not more of them than fill the GPU: 2^27 slots of 256 experts took 42.6 ms with a block
+  // for each 16,384, 4.2 ms like this.
+  const int64_t chunks = std::max<int64_t>(1, (a.slots + LIST_THREADS * S - 1) / (LIST_THREADS * S));
+  a.rounds = (int)((chunks + 2 * sm_count() - 1) / (2 * sm_count()));
+  a.blocks = (int)((chunks + a.rounds - 1) / a.rounds);
   CallBuf counts;
   if (a.blocks > 1) {
     LAPIS_TRY(scratch(&counts, (size_t)a.blocks * buckets * sizeof(uint32_t), st));
     a.counts = static_cast<uint32_t *>(counts.p);
     LAPIS_CUDA_TRY(launch_pdl(list_count_kernel<S>, dim3(a.blocks), LIST_THREADS, buckets * sizeof(uint32_t), st, a));
   }
-  const size_t smem = (LIST_WARPS + 2) * buckets * sizeof(uint32_t);
-  LAPIS_TRY(allow_smem<list_place_kernel<S>>((int)((LIST_WARPS + 2) * (MAX_EXPERTS + 1) * sizeof(uint32_t))));
+  const size_t smem = (LIST_WARPS + 3) * buckets * sizeof(uint32_t);
+  LAPIS_TRY(allow_smem<list_place_kernel<S>>((int)((LIST_WARPS + 3) * (MAX_EXPERTS + 1) * sizeof(uint32_t))));
   LAPIS_CUDA_TRY(launch_pdl(list_place_kernel<S>, dim3(a.blocks), LIST_THREADS, smem, st, a));
   return LAPIS_OK;
 }

@@ -8,6 +8,9 @@
 //
 // Everything is computed in 32 bits and rounded once, sums in a fixed order.  Places, offsets and experts are looked at before
 // they are followed.
+//
+// Kernels wait for the launch in front of them before anything else, and let the next one in as their blocks end: released at the top, the gradient of
+// 8191 x 130 logits takes 7.4 us in a stream of its like instead of 6.6, one row x 4096 x 4096 (int4_few.cu) 6.4 instead of 5.0; the others are within 1 %.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -105,7 +108,6 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_kernel(const __grid_const
   const int lane = threadIdx.x % 32;
   const int64_t token = (int64_t)blockIdx.x * (ROUTE_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
-  pdl_release();
   if (token >= a.tokens) return;
   const T *const logits = static_cast<const T *>(a.logits) + token * a.token_stride;
   T given[R];
@@ -171,7 +173,6 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_backward_kernel(const __g
   const int lane = threadIdx.x % 32;
   const int64_t token = (int64_t)blockIdx.x * (ROUTE_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
-  pdl_release();
   if (token >= a.tokens) return;
   const T *const logits = static_cast<const T *>(a.logits) + token * a.token_stride;
   T *const out = static_cast<T *>(a.dlogits) + token * a.experts;
@@ -271,7 +272,6 @@ __global__ void __launch_bounds__(LIST_THREADS) list_count_kernel(const __grid_c
   const int buckets = a.experts + 1;
   for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) hist[b] = 0;
   pdl_wait();
-  pdl_release();
   __syncthreads();
   for (int round = 0; round < a.rounds; ++round) {
     const int64_t first = ((int64_t)blockIdx.x * a.rounds + round) * LIST_THREADS * S;
@@ -295,7 +295,6 @@ __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_c
   uint32_t *const of_warp = smem, *const length = smem + LIST_WARPS * buckets, *const in_front = length + buckets, *const of_round = in_front + buckets;
   for (int i = threadIdx.x; i < (LIST_WARPS + 2) * buckets; i += LIST_THREADS) smem[i] = 0;
   pdl_wait();
-  pdl_release();
   uint32_t *const mine = of_warp + warp * buckets;
   for (int round = 0; round < a.rounds; ++round) {
     const int64_t first = (((int64_t)blockIdx.x * a.rounds + round) * LIST_WARPS + warp) * 32 * S;
@@ -458,7 +457,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) gather_kernel(const __grid_const
   const int lane = threadIdx.x % 32;
   const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
-  pdl_release();
   if (item >= a.items) return;
   const int64_t token = divided(item, a.chunks, a.items);
   const int64_t first = (item - token * a.chunks) * (32 * GATHER_PIECES) + lane, pieces = a.dim / V;
@@ -500,7 +498,6 @@ __global__ void __launch_bounds__(32 * RING_WARPS, 2) combine_ring_kernel(const 
   const int64_t step = (int64_t)gridDim.x * RING_WARPS;
   const int pieces = (int)(a.dim / V);
   pdl_wait();
-  pdl_release();
   const int32_t end = a.pos[a.experts];
 
   struct Unit {  // rows j0 to j0 + J - 1 of a token's chunk
@@ -603,7 +600,6 @@ __global__ void __launch_bounds__(ROWS_THREADS, 4) combine_kernel(const __grid_c
   const int lane = threadIdx.x % 32;
   const int64_t item = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
-  pdl_release();
   if (item >= a.items) return;
   const int64_t token = divided(item, a.chunks, a.items);
   const int chunk = (int)(item - token * a.chunks), dim = (int)a.dim;
@@ -660,7 +656,6 @@ __global__ void __launch_bounds__(ROWS_THREADS, BACK_BLOCKS) combine_backward_ke
   const int lane = threadIdx.x % 32;
   const int64_t slot = (int64_t)blockIdx.x * (ROWS_THREADS / 32) + threadIdx.x / 32;
   pdl_wait();
-  pdl_release();
   if (slot >= a.slots) return;
   const int64_t token = divided(slot, a.k, a.slots);
   const int pieces = (int)(a.dim / V);
@@ -733,7 +728,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) gather_narrow_kernel(const __gri
   using P = Piece<T, V>;
   const int64_t item = (int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x;
   pdl_wait();
-  pdl_release();
   if (item >= a.items) return;
   const int64_t slot = divided(item, a.chunks, a.items), token = divided(slot, a.k, a.slots);
   const int piece = (int)(item - slot * a.chunks);
@@ -750,7 +744,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) combine_narrow_kernel(const __gr
   constexpr int J = 4;  // rows asked for at a time
   const int64_t item = (int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x;
   pdl_wait();
-  pdl_release();
   if (item >= a.items) return;
   const int64_t token = divided(item, a.chunks, a.items);
   const int piece = (int)(item - token * a.chunks);
@@ -787,7 +780,6 @@ __global__ void __launch_bounds__(ROWS_THREADS) combine_backward_narrow_kernel(c
   const int64_t slot = ((int64_t)blockIdx.x * ROWS_THREADS + threadIdx.x) / a.run;
   const int piece = threadIdx.x & (a.run - 1);
   pdl_wait();
-  pdl_release();
   float dot = 0.0f;
   if (slot < a.slots) {
     const Place p = place_of(a, slot, a.pos[a.experts]);

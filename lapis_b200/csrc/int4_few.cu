@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(FEW_THREADS, FEW_BLOCKS) int4_few_kernel(const
   const bool early = a.pos == nullptr;
   if (early) way.begin(a, of_all, my_share, shares, lane);
   pdl_wait();
-  pdl_release();
   int64_t begin = 0, end = a.rows;
   if (a.pos != nullptr) {
     begin = min((int64_t)max(a.pos[expert], 0), a.rows);

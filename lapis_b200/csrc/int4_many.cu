@@ -113,7 +113,6 @@ __global__ void __launch_bounds__(256) arrange_kernel(const __grid_constant__ Pr
   constexpr bool PARTS = std::is_same<X, float>::value;
   constexpr int A_ROW = PARTS ? 3 : 1, ROWS = NC / A_ROW, V = 16 / sizeof(X);
   pdl_wait();
-  pdl_release();
   const int expert = blockIdx.y, columns = (int)a.columns;
   int64_t begin = 0, end = a.rows;
   if (a.pos != nullptr) {

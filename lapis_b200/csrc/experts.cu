@@ -818,17 +818,20 @@ static int launch_ring(RowsArgs &a, cudaStream_t st) {
 }
 template <typename T, int V>
 static int launch_combine(RowsArgs &a, cudaStream_t st) {
-  if constexpr (V > 1) return a.k <= 1 ? launch_ring<T, 1>(a, st) : a.k <= 2 ? launch_ring<T, 2>(a, st) : launch_ring<T, 4>(a, st);
-  constexpr int WARPS = ROWS_THREADS / 32, U = 8;
-  // A warp looks up a token's places once for several pieces, where there are warps enough for that.
-  const int64_t turns = (a.dim + 32 * U - 1) / (32 * U), warps = (int64_t)sm_count() * 128;
-  a.run = (int)std::min<int64_t>(turns, std::max<int64_t>(1, a.tokens * turns / warps));
-  a.chunks = (uint32_t)((turns + a.run - 1) / a.run);
-  a.items = a.tokens * a.chunks;
-  const int64_t blocks = (a.items + WARPS - 1) / WARPS;
-  if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
-  LAPIS_CUDA_TRY(launch_pdl(combine_kernel<T, U, 2>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
-  return LAPIS_OK;
+  if constexpr (V > 1) {
+    return a.k <= 1 ? launch_ring<T, 1>(a, st) : a.k <= 2 ? launch_ring<T, 2>(a, st) : launch_ring<T, 4>(a, st);
+  } else {
+    constexpr int WARPS = ROWS_THREADS / 32, U = 8;
+    // A warp looks up a token's places once for several pieces, where there are warps enough for that.
+    const int64_t turns = (a.dim + 32 * U - 1) / (32 * U), warps = (int64_t)sm_count() * 128;
+    a.run = (int)std::min<int64_t>(turns, std::max<int64_t>(1, a.tokens * turns / warps));
+    a.chunks = (uint32_t)((turns + a.run - 1) / a.run);
+    a.items = a.tokens * a.chunks;
+    const int64_t blocks = (a.items + WARPS - 1) / WARPS;
+    if (blocks > 0x7fffffff) return fail(LAPIS_ETOOBIG, "experts: rows beyond 2^31 blocks");
+    LAPIS_CUDA_TRY(launch_pdl(combine_kernel<T, U, 2>, dim3((unsigned)blocks), ROWS_THREADS, 0, st, a));
+    return LAPIS_OK;
+  }
 }
 template <typename T, int V>
 static int launch_narrow(RowsOp op, RowsArgs &a, cudaStream_t st) {

@@ -237,7 +237,8 @@ int lapis_b200_bgemm_f32(int64_t batch, int64_t M, int64_t N, int64_t K, const f
 /* Tile-aligned problems (M, N multiples of 128, K of 32) run on the tensor cores, whose kernel
  * bounds every internal wait and records a flag instead of hanging.  This reads and clears
  * that flag after synchronising `stream`: LAPIS_OK, or LAPIS_ECUDA when the last launches on
- * this device did not complete normally (their output is then invalid). */
+ * this device did not complete normally (their output is then invalid).  So do the products with 4-bit weights,
+ * lapis_b200_int4_matmul. */
 int lapis_b200_bgemm_status(void *stream);
 
 /* Vector kernels of examples/pcg_solve.py:22-48.  dot writes its result to *d_out. */
@@ -384,7 +385,7 @@ int lapis_b200_expert_gather(int type, int64_t dim, const void *d_x, int64_t x_s
 int lapis_b200_expert_combine(int type, int64_t dim, const void *d_rows, int64_t row_stride, const lapis_b200_expert_lists *lists, const float *d_weights,
                               void *d_out, void *stream);
 /* Its gradients: d_drows [tokens * k, dim] contiguous, zeros behind pos[experts], and d_dweights [tokens, k], zeros for the
- * slots that are there. */
+ * slots behind pos[experts]. */
 int lapis_b200_expert_combine_backward(int type, int64_t dim, const void *d_dout, int64_t dout_stride, const void *d_rows, int64_t row_stride,
                                        const lapis_b200_expert_lists *lists, const float *d_weights, void *d_drows, float *d_dweights, void *stream);
 
@@ -408,11 +409,13 @@ int lapis_b200_int4_pack(const lapis_b200_int4 *w, const void *d_codes, const vo
  * rounded to scale_type first (a number beyond that is infinite).  A group of zeros gets scale 0; one that is not finite a scale of NaN. */
 int lapis_b200_int4_quantise(int type, int64_t rows, int64_t columns, const void *d_w, int64_t w_stride, int group, int scale_type, void *d_codes,
                              void *d_scale, void *d_zero, void *stream);
-/* y = x w^T of `rows` rows [rows, columns], x_stride elements apart: codes and x are exact (x of 32 bits as three parts of bf16), sums
- * are in 32 bits, one rounding.  d_y [rows, outputs], or half as many if gated, contiguous.  With lists (may be null) the rows of
+/* y = x w^T of `rows` rows [rows, columns], x_stride elements apart.  Every product of a code and a value is exact (values of 32 bits go in three parts of
+ * bf16, which hold them whole from 2^-110 on; of smaller ones what lies below 2^-133 is lost).  Sums are in 32 bits; the tensor cores, which add up a
+ * group, cut where other additions round.  The result is rounded once.  d_y [rows, outputs], or half as many if gated, contiguous.  With lists (may be null) the rows of
  * y are the lists' slots, those of expert e times its matrix, zeros behind pos[experts]; row i of x is the slot's own, or, with
- * `fetch`, that of its token: x [tokens, columns].  Made for few rows, of each expert: up to 128 of them (64 with groups smaller than 128; one
- * of 32 bits counts three) share a pass over the weights.  Above 8 a copy of the rows (6 bytes a value where they are of 32 bits), and up
+ * `fetch`, that of its token: x [tokens, columns].  Made for few rows.  A pass over the weights serves 8, 32, 64 or, with groups of
+ * 128, 128 of them (a third of that where they are of 32 bits): as many as there are, with lists as twice the slots / experts (those of no expert counted).
+ * An expert that has more takes further passes, one after the other.  Above 8 a copy of the rows (6 bytes a value where they are of 32 bits), and up
  * to 8 columns of the product more for each expert, is laid out in memory of the library's pool, or, beyond 256 MiB, in memory of its own, which stream
  * capture refuses.  A failed wait of the kernel is reported by lapis_b200_bgemm_status. */
 int lapis_b200_int4_matmul(int type, const lapis_b200_int4 *w, int64_t rows, const void *d_x, int64_t x_stride, const lapis_b200_expert_lists *lists,

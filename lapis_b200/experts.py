@@ -210,12 +210,16 @@ class Int4Matrix:
         return cls(codes, scale, zero, columns=w.shape[-1], group=group, gated=gated)
 
     def matmul(self, x, lists: ExpertLists | None = None, fetch: bool = False):
-        """x w^T of rows ``x`` [rows, columns], of their type: every product is exact, sums are in 32 bits, one rounding.
+        """x w^T of rows ``x`` [rows, columns], of their type.  Every product of a code and a value is exact, but for what float32 values
+        below 2^-110 have below 2^-133; sums are in 32 bits, cut instead of rounded within a group, and rounded to the type once.
 
         With ``lists`` row i of the result is that of slot ``lists.crd[i]``, times its expert's weights, zeros for slots of no
-        expert; ``x`` holds the slots' rows in the same order, or with ``fetch`` those of the tokens [tokens, columns].  Made for
-        few rows (of each expert): up to 128 share a pass over the weights, 64 with groups smaller than 128, a third of that
-        where they are float32."""
+        expert; ``x`` holds the slots' rows in the same order, or with ``fetch`` those of the tokens [tokens, columns].
+
+        Made for few rows: a pass over the weights serves 8, 32, 64 or, with groups of 128, 128 of them (a third of that where they
+        are float32), as many as there are, or with ``lists`` as twice the slots / experts.  An expert with more rows takes
+        further passes, one after the other.  With more than 8 the kernel's waits are bounded: where one gave up, the result is not
+        valid and ``device.bgemm_status()`` raises."""
         if self._device != torch.cuda.current_device():
             raise TypeError("matmul: the weights must be on the current device")
         if (stream := torch._C._cuda_getCurrentRawStream(self._device)) not in self._streams:  # nobody else has the weights' memory to say so

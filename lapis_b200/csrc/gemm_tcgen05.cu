@@ -505,8 +505,8 @@ int bgemm_tcgen05_launch(int64_t batch, int64_t M, int64_t N, int64_t K, const f
 
 // Reads and clears the tensor-core kernel's error flag; synchronises `stream`.  A non-zero flag
 // means a bounded wait inside the kernel gave up (1 producer, 2 MMA issuer, 3 split warps,
-// 4 epilogue; of the product from split operands 5 producer, 6 MMA issuer, 7 epilogue) and the output of that launch is not
-// valid.
+// 4 epilogue; of the product from split operands 5 producer, 6 MMA issuer, 7 epilogue; 9 any of the product with 4-bit weights)
+// and the output of that launch is not valid.
 extern "C" int lapis_b200_bgemm_status(void *stream) {
   using namespace lapis_b200;
   clear_error();
@@ -519,7 +519,7 @@ extern "C" int lapis_b200_bgemm_status(void *stream) {
   LAPIS_CUDA_TRY(cudaMemcpy(&flag, at, sizeof(int), cudaMemcpyDeviceToHost));
   if (flag != 0) {
     cudaMemset(at, 0, sizeof(int));
-    return fail(LAPIS_ECUDA, "bgemm: tensor-core kernel gave up waiting (role %d)", flag);
+    return fail(LAPIS_ECUDA, "%s: tensor-core kernel gave up waiting (role %d)", flag == 9 ? "int4_matmul" : "bgemm", flag);
   }
   return LAPIS_OK;
 }

@@ -214,7 +214,7 @@ def bgemm(A: torch.Tensor, B: torch.Tensor, C: torch.Tensor) -> torch.Tensor:
 
 
 def bgemm_status() -> None:
-    """Synchronises and raises if the tensor-core matmul kernel reported a failed wait."""
+    """Synchronises and raises if a tensor-core kernel, of a matmul or a product with 4-bit weights, reported a failed wait."""
     check(load().lapis_b200_bgemm_status(_stream()))
 
 

@@ -31,7 +31,7 @@ struct ProductArgs {
 };
 
 // Columns of the product (rows, three for one of 32 bits) up to which it goes to int4_few_kernel, where a second product for the next eight
-// would do: 16 rows x 14,336 x 4096 took it 36 us, int4_many_kernel takes 23; 8 rows 18 and 23.
+// would do: 16 rows x 14,336 x 4096 took it 36 us, int4_many_kernel takes 21, as for 9; 8 rows take it 17.
 constexpr int FEW_COLUMNS = 8;
 int launch_few(int type, ProductArgs &a, int group, int matrices, cudaStream_t st);                     // int4_few.cu
 int launch_many(int type, ProductArgs &a, int group, int matrices, int64_t expected, cudaStream_t st);  // int4_many.cu
@@ -39,7 +39,7 @@ int launch_many(int type, ProductArgs &a, int group, int matrices, int64_t expec
 #ifdef __CUDACC__
 
 // Codes to whole numbers of 16 bits, exactly.  A code's bits behind those of a number 2^m are 2^m + code or, four places up, 2^m + 16
-// code; fp16 has room for both (1024), bf16 for one (128).  So of the four pairs of a word, fp16 takes two as they lie and two shifted
+// code (used for weights of 8 and 4 bits by Y. J. Kim et al., "Who Says Elephants Can't Run", 2022); fp16 has room for both (1024), bf16 for one (128).  So of the four pairs of a word, fp16 takes two as they lie and two shifted
 // once, and the zero is subtracted by the instruction that brings a code down.  What bounds the conversion are the instructions
 // on 32 bits, one every two cycles: five for eight codes, in bf16 seven.
 template <typename T>

@@ -2,9 +2,9 @@
 //
 // The weights go from memory to registers, a batch ahead, and need nothing but their own warp; the rows x, the B operand, are in shared
 // memory.  What bounds it are the instructions on 32 bits that make numbers of codes: of one every two cycles a batch of 16 x 256 takes 150 to
-// 190, its bytes as long as 170.  48 x 8 rows over 128 experts (2048 x 2048, groups of 32, gated) 79 us, 3.7 TB/s; one row times 14,336 x 4096 11.3 us,
-// 2.7 TB/s; 4096 x 4096 6.6 us, most of it launch and latency.  tcgen05 (int4_many.cu) with 8 columns would convert as many codes and add its
-// hand-overs: 16 rows take it 23 us where 8 take this 18.
+// 190, its bytes as long as 170.  48 x 8 rows over 128 experts (2048 x 2048, groups of 32, gated) 76 us, 3.8 TB/s; one row times 14,336 x 4096 10.9 us,
+// 2.8 TB/s; 4096 x 4096 5.0 us, most of it launch and latency.  tcgen05 (int4_many.cu) with 8 columns would convert as many codes and add its
+// hand-overs: 16 rows x 14,336 x 4096 take it 21 us where 8 take this 17.
 #include <algorithm>
 #include <cstdint>
 #include <type_traits>
@@ -81,7 +81,7 @@ constexpr int SUM_PITCH = STRIP + 1;
 
 constexpr int FEW_WARPS_LOG = 2, FEW_WARPS = 1 << FEW_WARPS_LOG, FEW_THREADS = 32 * FEW_WARPS;
 // Blocks of an SM, and the rows x of each in shared memory.  48 x 8 rows over 128 experts take 79 us with 5 blocks, 82 with 4, 78 with 6, for
-// which scales of 32 bits have to be spilled; with two of eight warps 87.
+// which scales of 32 bits have to be spilled (with 5 only where groups are of 32: 8 to 20 bytes); with two of eight warps 87.
 constexpr int FEW_BLOCKS = 5, FEW_ROOM = 40 << 10;
 
 // Bytes of a row of x in shared memory: neighbouring rows' pieces of a phase lie on different banks.

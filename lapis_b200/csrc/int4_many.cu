@@ -204,7 +204,8 @@ struct Record {
 // NC: columns of the product of a pass over the weights.  The tensor core's work comes in stages of 128 columns of x (64 where groups are of
 // 32).  A stage has half of the codes' room and of the sums' room in tensor memory, and one barrier says that its products are done and
 // both are free again: what bounds the kernel are the hand-overs between converting and issuing warps, 280 cycles for a wait and 100 for a
-// commit.  64 rows x 14,336 x 4096, gated, groups of 64: 30 us (1.1 TB/s, 250 TFLOP/s); with a commit for every block and group 38.
+// commit.  64 rows x 14,336 x 4096, gated, groups of 64: 30 us (1.1 TB/s, 250 TFLOP/s); with a commit for every block and group 38.  Two CTAs an SM have
+// 96 registers a thread: with 64 columns in groups of 128 a thread spills 68 to 120 bytes, with 32 up to 100.
 template <typename X, int GROUP, int NC, bool ZEROS>
 __global__ void __launch_bounds__(MANY_THREADS, many_tmem(GROUP, NC) == 256 ? 2 : 1) int4_many_kernel(const __grid_constant__ ProductArgs a) {
   using T = typename std::conditional<std::is_same<X, float>::value, __nv_bfloat16, X>::type;

@@ -9,8 +9,9 @@
 // Everything is computed in 32 bits and rounded once, sums in a fixed order.  Places, offsets and experts are looked at before
 // they are followed.
 //
-// Kernels wait for the launch in front of them before anything else, and let the next one in as their blocks end: released at the top, the gradient of
-// 8191 x 130 logits takes 7.4 us in a stream of its like instead of 6.6, one row x 4096 x 4096 (int4_few.cu) 6.4 instead of 5.0; the others are within 1 %.
+// Kernels wait for the launch in front of them before anything else, and let the next one in as their blocks end.  Released at the top, in a stream of
+// their like, the gradient of 8191 x 130 logits takes 7.4 us instead of 6.6, lists of 131,072 slots of 1024 experts 40 instead of 35, one row x 4096 x 4096
+// (int4_few.cu) 6.4 instead of 5.0; lists of 160 slots 1.85 instead of 2.05, of 16,384 5.8 instead of 6.05; the others are within 1 %.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -249,13 +250,15 @@ static int launch_route(int type, const RouteArgs &a, cudaStream_t st) {
 
 // ---- lists ----------------------------------------------------------------------
 
-constexpr int LIST_THREADS = 512, LIST_WARPS = LIST_THREADS / 32;
+constexpr int LIST_THREADS = 512, LIST_WARPS = LIST_THREADS / 32, LIST_MOST = 32;  // LIST_MOST: slots of a thread, where there are more rounds than one
 
 struct ListArgs {
   const void *expert;
   int idx_bytes, experts, blocks;
   int64_t slots;
   int rounds;        // of 512 S slots for each block, one behind the other
+  template <int S>
+  __device__ __forceinline__ int rounds_of() const { return S < LIST_MOST ? 1 : rounds; }
   uint32_t *counts;  // [blocks, experts + 1], or null for one block
   int32_t *pos, *crd, *place;
 };
@@ -273,8 +276,8 @@ __global__ void __launch_bounds__(LIST_THREADS) list_count_kernel(const __grid_c
   for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) hist[b] = 0;
   pdl_wait();
   __syncthreads();
-  for (int round = 0; round < a.rounds; ++round) {
-    const int64_t first = ((int64_t)blockIdx.x * a.rounds + round) * LIST_THREADS * S;
+  for (int round = 0; round < a.rounds_of<S>(); ++round) {
+    const int64_t first = ((int64_t)blockIdx.x * a.rounds_of<S>() + round) * LIST_THREADS * S;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int64_t slot = first + s * LIST_THREADS + threadIdx.x;
@@ -296,8 +299,8 @@ __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_c
   for (int i = threadIdx.x; i < (LIST_WARPS + 2) * buckets; i += LIST_THREADS) smem[i] = 0;
   pdl_wait();
   uint32_t *const mine = of_warp + warp * buckets;
-  for (int round = 0; round < a.rounds; ++round) {
-    const int64_t first = (((int64_t)blockIdx.x * a.rounds + round) * LIST_WARPS + warp) * 32 * S;
+  for (int round = 0; round < a.rounds_of<S>(); ++round) {
+    const int64_t first = (((int64_t)blockIdx.x * a.rounds_of<S>() + round) * LIST_WARPS + warp) * 32 * S;
     int bucket[S];
     uint32_t rank[S];
 #pragma unroll
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_c
         of_warp[w * buckets + b] = upto;
         upto += n;
       }
-      of_round[b] = upto;
+      if constexpr (S == LIST_MOST) of_round[b] = upto;
       if (a.counts == nullptr) length[b] = upto;
     }
     __syncthreads();
@@ -373,9 +376,10 @@ __global__ void __launch_bounds__(LIST_THREADS) list_place_kernel(const __grid_c
       a.place[slot] = (int32_t)at;
       if (at < a.slots) a.crd[at] = (int32_t)slot;  // not so only where somebody writes the experts meanwhile, which are read twice
     }
-    if (round + 1 == a.rounds) break;
+    if (round + 1 == a.rounds_of<S>()) break;
     __syncthreads();
-    for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) in_front[b] += of_round[b];
+    if constexpr (S == LIST_MOST)
+      for (int b = threadIdx.x; b < buckets; b += LIST_THREADS) in_front[b] += of_round[b];
     for (int i = threadIdx.x; i < LIST_WARPS * buckets; i += LIST_THREADS) of_warp[i] = 0;
   }
 }
@@ -386,7 +390,7 @@ static int launch_lists_as(ListArgs &a, cudaStream_t st) {
   // Every block reads the counts of all, so there are not more of them than fill the GPU: 2^27 slots of 256 experts took 42.6 ms with a block
   // for each 16,384, 4.2 ms like this.
   const int64_t chunks = std::max<int64_t>(1, (a.slots + LIST_THREADS * S - 1) / (LIST_THREADS * S));
-  a.rounds = (int)((chunks + 2 * sm_count() - 1) / (2 * sm_count()));
+  a.rounds = S < LIST_MOST ? 1 : (int)((chunks + 2 * sm_count() - 1) / (2 * sm_count()));
   a.blocks = (int)((chunks + a.rounds - 1) / a.rounds);
   CallBuf counts;
   if (a.blocks > 1) {
@@ -410,7 +414,7 @@ static int launch_lists(ListArgs &a, cudaStream_t st) {
   if (all <= 2 * LIST_THREADS) return launch_lists_as<2>(a, st);
   if (all <= 4 * LIST_THREADS) return launch_lists_as<4>(a, st);
   if (all <= 8 * LIST_THREADS) return launch_lists_as<8>(a, st);
-  return launch_lists_as<32>(a, st);
+  return launch_lists_as<LIST_MOST>(a, st);
 }
 
 // ---- rows there and back ----------------------------------------------------------

@@ -237,8 +237,8 @@ int lapis_b200_bgemm_f32(int64_t batch, int64_t M, int64_t N, int64_t K, const f
 /* Tile-aligned problems (M, N multiples of 128, K of 32) run on the tensor cores, whose kernel
  * bounds every internal wait and records a flag instead of hanging.  This reads and clears
  * that flag after synchronising `stream`: LAPIS_OK, or LAPIS_ECUDA when the last launches on
- * this device did not complete normally (their output is then invalid).  So do the products with 4-bit weights,
- * lapis_b200_int4_matmul. */
+ * this device did not complete normally (their output is then invalid).  Waits of
+ * lapis_b200_int4_matmul that gave up are recorded there too. */
 int lapis_b200_bgemm_status(void *stream);
 
 /* Vector kernels of examples/pcg_solve.py:22-48.  dot writes its result to *d_out. */
